@@ -449,6 +449,83 @@ int ns_paged_attention_noalloc(void* out, const void* query,
                                const void* decode_plan, size_t decode_plan_bytes, void* stream,
                                void* aux_stream, void* fork_event, void* join_event);
 
+/*
+ * The KV cache held in 4 bits.  K and V of a layer are one byte tensor each,
+ * [num_blocks, num_kv_heads, block_size, head_dim / 2 + 4], contiguous.  The
+ * bytes of a (block, head) are its codes (block_size * head_dim / 2), then one
+ * 32-bit word per token: scale << 16 | offset, both in the model's dtype.  A
+ * stored value is scale * code + offset.  K's codes lie token after token,
+ * dims 2i and 2i + 1 in the low and high nibble of byte i; V's in groups of
+ * four tokens, the byte of dims 2i and 2i + 1 of token t being byte
+ * 4 i + (0, 2, 1, 3)[t % 4] of group t / 4.  A row x becomes
+ *     offset = R(min x), scale = R((max x - min x) / 15),
+ *     code = clamp(rint((x - offset) / scale), 0, 15), 0 where scale is 0,
+ * in float32, R the rounding to the model's dtype.  A row with a NaN or an
+ * infinity, or whose scale or offset overflows the dtype, is stored with
+ * scale 0 and a NaN offset.  No counterpart in the reference, whose cache is
+ * 16 bits wide (nanoserve/kv_cache.py:30-85).
+ *
+ * For all of these dtype is the model's, NS_DTYPE_F16 or NS_DTYPE_BF16 (a
+ * cache is read in the dtype it was written in); head_dim is a multiple of 8
+ * and at most 256, block_size a multiple of 4; the caches are 16-byte
+ * aligned.  Slots and block ids may be int32 or int64.
+ *
+ * ns_reshape_and_cache_int4 -- ns_reshape_and_cache into such a cache.  Rows
+ * of any token and head stride (elements), unit head_dim stride; slots outside
+ * [0, num_blocks * block_size) are skipped.  The slots of one call must
+ * differ: a slot named twice holds a mixture of its rows.
+ *
+ * ns_rope_reshape_and_cache_int4 -- ns_rope_reshape_and_cache into such a
+ * cache.  cos and sin are [num_tokens, head_dim] rows in `dtype`; the rotation
+ * is evaluated in float32, the rotated query rounded once and the rotated key
+ * quantised unrounded.  q_out may equal query when query is contiguous.
+ *
+ * ns_gather_cache_int4 -- k_out, v_out [num_tokens, num_kv_heads, head_dim]
+ * (`dtype`, contiguous, 16-byte aligned) = the values stored in the given
+ * slots, zero for slots outside the cache.
+ */
+int ns_reshape_and_cache_int4(const void* key, const void* value,
+                              int64_t key_stride_token, int64_t key_stride_head,
+                              int64_t value_stride_token, int64_t value_stride_head,
+                              void* k_cache, void* v_cache,
+                              const void* slot_mapping, int slot_mapping_is_int64,
+                              int64_t num_tokens, int num_kv_heads, int head_dim,
+                              int block_size, int64_t num_blocks, int dtype, void* stream);
+int ns_rope_reshape_and_cache_int4(void* q_out, const void* query,
+                                   int64_t q_stride_token, int64_t q_stride_head,
+                                   const void* key, int64_t key_stride_token, int64_t key_stride_head,
+                                   const void* value, int64_t value_stride_token, int64_t value_stride_head,
+                                   const void* cos, const void* sin, int64_t cos_sin_stride_token,
+                                   void* k_cache, void* v_cache,
+                                   const void* slot_mapping, int slot_mapping_is_int64,
+                                   int64_t num_tokens, int num_heads, int num_kv_heads, int head_dim,
+                                   int block_size, int64_t num_blocks, int dtype, void* stream);
+int ns_gather_cache_int4(void* k_out, void* v_out, const void* k_cache, const void* v_cache,
+                         const void* slot_mapping, int slot_mapping_is_int64,
+                         int64_t num_tokens, int num_kv_heads, int head_dim,
+                         int block_size, int64_t num_blocks, int dtype, void* stream);
+
+/*
+ * ns_paged_attention_int4 -- ns_paged_attention over a cache held in 4 bits:
+ * the same rows, masks and metadata, for decode, prompts, chunks and mixed
+ * batches.  Each stored value enters as the exact scale * code + offset.
+ * query and out are [num_tokens, num_heads, head_dim] in `dtype`, 16-byte
+ * aligned.  A row without keys is zero; a row of no sequence is left as it
+ * is.  A block id outside [0, num_blocks) is never dereferenced and makes the
+ * rows that need it NaN.
+ */
+int ns_paged_attention_int4(void* out, const void* query,
+                            const void* k_cache, const void* v_cache,
+                            const void* block_tables, int64_t block_table_stride,
+                            int64_t block_table_width, int block_tables_is_int64,
+                            const void* seq_lens, int seq_lens_is_int64,
+                            const void* query_start_loc, int query_start_loc_is_int64,
+                            int num_seqs, int64_t num_tokens, int max_query_len, int max_seq_len,
+                            int is_decode_only,
+                            int num_heads, int num_kv_heads, int head_dim,
+                            int block_size, int64_t num_blocks,
+                            float scale, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

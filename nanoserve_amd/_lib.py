@@ -155,6 +155,41 @@ SIGNATURES = {
         c_void_p, c_size_t, c_void_p,            # decode plan (or None), bytes, stream
         c_void_p, c_void_p, c_void_p,            # aux stream, fork event, join event (all or none)
     ]),
+    "ns_reshape_and_cache_int4": (c_int, [
+        c_void_p, c_void_p,                      # key, value
+        c_int64, c_int64, c_int64, c_int64,      # key/value token and head strides
+        c_void_p, c_void_p,                      # k_cache, v_cache
+        c_void_p, c_int,                         # slot_mapping, is_int64
+        c_int64, c_int, c_int, c_int, c_int64,   # T, Hkv, D, block_size, num_blocks
+        c_int, c_void_p,                         # dtype, stream
+    ]),
+    "ns_rope_reshape_and_cache_int4": (c_int, [
+        c_void_p, c_void_p, c_int64, c_int64,    # q_out, query, query token / head strides
+        c_void_p, c_int64, c_int64,              # key, token / head strides
+        c_void_p, c_int64, c_int64,              # value, token / head strides
+        c_void_p, c_void_p, c_int64,             # cos, sin, token stride
+        c_void_p, c_void_p,                      # k_cache, v_cache
+        c_void_p, c_int,                         # slot_mapping, is_int64
+        c_int64, c_int, c_int, c_int,            # T, Hq, Hkv, D
+        c_int, c_int64,                          # block_size, num_blocks
+        c_int, c_void_p,                         # dtype, stream
+    ]),
+    "ns_gather_cache_int4": (c_int, [
+        c_void_p, c_void_p, c_void_p, c_void_p,  # k_out, v_out, k_cache, v_cache
+        c_void_p, c_int,                         # slot_mapping, is_int64
+        c_int64, c_int, c_int, c_int, c_int64,   # T, Hkv, D, block_size, num_blocks
+        c_int, c_void_p,                         # dtype, stream
+    ]),
+    "ns_paged_attention_int4": (c_int, [
+        c_void_p, c_void_p,                      # out, query
+        c_void_p, c_void_p,                      # k_cache, v_cache
+        c_void_p, c_int64, c_int64, c_int,       # block_tables, row stride, width, is_int64
+        c_void_p, c_int,                         # seq_lens, is_int64
+        c_void_p, c_int,                         # query_start_loc, is_int64
+        c_int, c_int64, c_int, c_int, c_int,     # S, T, max_query_len, max_seq_len, decode_only
+        c_int, c_int, c_int, c_int, c_int64,     # Hq, Hkv, D, block_size, num_blocks
+        c_float, c_int, c_void_p,                # scale, dtype, stream
+    ]),
 }
 
 _lock = threading.Lock()

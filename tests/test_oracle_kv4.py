@@ -1,0 +1,171 @@
+"""The 4-bit cache's oracle, pinned on the CPU, and what the product refuses
+without touching a GPU."""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import nanoserve_amd
+from nanoserve_amd import Int4PagedKVCache, _lib
+from nanoserve_amd.attention import AttentionMetadata
+from nanoserve_amd.kv4 import kv4_bytes_per_token, kv4_shape
+from oracle import kv4
+
+DTYPES = [torch.float16, torch.bfloat16]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("spread,shift", [(1.0, 0.0), (3.0, 20.0), (1e-3, -1.0)])
+def test_stored_rows_are_within_half_a_step(dtype, spread, shift):
+    x = (torch.randn(50, 2, 64, generator=torch.Generator().manual_seed(0)) * spread + shift).to(dtype).float()
+    codes, s, b = kv4.quantise_rows(x, dtype)
+    assert codes.max() <= 15 and codes.dtype == torch.uint8
+    err = (kv4.stored_values(codes, s, b) - x.double()).abs()
+    # Half a step; a scale rounded down leaves the top code short by 15 of its
+    # roundings, and a float32 quotient at a tie may fall on either side.
+    half = torch.finfo(dtype).eps / 2
+    tiny = torch.finfo(dtype).smallest_normal  # below it a scale rounds by an absolute step
+    assert (err <= s.double() * (0.5 + 15 * half + 1e-5) + 15 * tiny * half).all()
+    # The minimum is a value of the dtype, so it is stored exactly.
+    assert torch.equal(b.float(), x.amin(-1, keepdim=True))
+
+
+def test_constant_single_and_non_finite_rows():
+    x = torch.full((5, 1, 8), 2.5)
+    x[1, 0, 3] = float("nan")
+    x[2, 0, 0] = float("inf")
+    x[3, 0, 7] = -float("inf")
+    x[4] = 0.0
+    codes, s, b = kv4.quantise_rows(x, torch.float16)
+    assert (codes == 0).all() and (s == 0).all()
+    assert torch.equal(torch.isnan(b[:, 0, 0]), torch.tensor([False, True, True, True, False]))
+    assert b[0, 0, 0] == 2.5 and b[4, 0, 0] == 0
+
+
+@pytest.mark.parametrize("is_v", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_records_round_trip_and_rows_do_not_touch_each_other(dtype, is_v):
+    g = torch.Generator().manual_seed(1)
+    nb, heads, bs, d = 3, 2, 8, 24
+    cache = torch.zeros(nb, heads, bs, d // 2 + 4, dtype=torch.uint8)
+    slots = torch.randperm(nb * bs, generator=g).tolist()
+    rows = kv4.quantise_rows(torch.randn(nb * bs, heads, d, generator=g), dtype)
+    for i in range(0, nb * bs, 5):  # in several writes
+        kv4.put_rows(cache, slots[i:i + 5], *(x[i:i + 5] for x in rows), is_v)
+    for a, b in zip(kv4.get_rows(cache, slots, dtype, is_v), rows):
+        assert torch.equal(a, b)
+    before = cache.clone()
+    kv4.put_rows(cache, [-1, nb * bs], *(x[:2] for x in rows), is_v)
+    assert torch.equal(cache, before)
+
+
+def test_every_byte_of_a_record_belongs_to_one_row():
+    nb, heads, bs, d = 1, 1, 4, 16
+    for is_v in (False, True):
+        owner = np.zeros(bs * (d // 2 + 4), int)
+        for t in range(bs):
+            cache = torch.zeros(nb, heads, bs, d // 2 + 4, dtype=torch.uint8)
+            par = torch.full((1, 1, 1), -1, dtype=torch.int16).view(torch.float16)
+            kv4.put_rows(cache, [t], torch.full((1, 1, d), 15, dtype=torch.uint8), par, par, is_v)
+            owner += (cache.view(-1).numpy() != 0)
+        assert (owner == 1).all()
+
+
+def test_attention_closed_forms():
+    g = torch.Generator().manual_seed(2)
+    d, n = 16, 5
+    rows = kv4.quantise_rows(torch.randn(n, 1, d, generator=g), torch.float16)
+    q = torch.randn(n, 2, d, generator=g)
+    out, _, _ = kv4.attention_ref(q, [(rows, rows)], [n], [n], 0.3)
+    values = kv4.stored_values(*rows)[:, 0]
+    assert torch.allclose(out[0, 0], values[0], atol=1e-12)  # one key
+    zero, _, _ = kv4.attention_ref(torch.zeros_like(q), [(rows, rows)], [n], [n], 0.3)
+    assert torch.allclose(zero[4, 1], values.mean(0), atol=1e-12)  # equal weights
+    # A scalar softmax of the last row.
+    w = [math.exp(0.3 * sum(float(a) * float(b) for a, b in zip(q[4, 1], k))) for k in values]
+    want = sum(a * k for a, k in zip(w, values)) / sum(w)
+    assert torch.allclose(out[4, 1], want, atol=1e-12)
+    # More query rows than keys: the first rows see none.
+    short, _, _ = kv4.attention_ref(q, [(rows, rows)], [3], [n], 0.3)
+    assert (short[:2] == 0).all() and torch.allclose(short[2, 0], values[0], atol=1e-12)
+
+
+def test_the_cache_object_and_its_bytes():
+    c = Int4PagedKVCache(4, 16, 3, 2, 64, torch.bfloat16, "cpu")
+    assert len(c.k_cache) == 3 and c.k_cache[0].shape == (4, 2, 16, 36) and c.capacity_tokens == 64
+    assert kv4_shape(c.v_cache[1]) == (4, 2, 16, 64)
+    assert c.num_bytes == 64 * kv4_bytes_per_token(3, 2, 64)
+    for bad in (dict(head_dim=60), dict(head_dim=264), dict(block_size=6)):
+        with pytest.raises(ValueError):
+            Int4PagedKVCache(**{**dict(num_blocks=1, block_size=16, num_layers=1, num_kv_heads=1, head_dim=64,
+                                       dtype=torch.float16, device="cpu"), **bad})
+    with pytest.raises(TypeError):
+        Int4PagedKVCache(1, 16, 1, 1, 64, torch.float32, "cpu")
+
+
+def test_the_product_has_no_cpu_path():
+    c = Int4PagedKVCache(2, 16, 1, 2, 64, torch.float16, "cpu")
+    x, slots = torch.zeros(3, 2, 64, dtype=torch.float16), torch.arange(3)
+    md = AttentionMetadata(slots, None, torch.ones(3, dtype=torch.int64), torch.zeros(3, 1, dtype=torch.int64), 1, 1, 3,
+                           3, True)
+    with pytest.raises(ValueError, match="GPU"):
+        c.write(0, x, x, slots)
+    with pytest.raises(ValueError, match="GPU"):
+        c.read(0, slots)
+    with pytest.raises(ValueError, match="GPU"):
+        nanoserve_amd.rope_reshape_and_cache_int4(x, x, x, x[:, :1], x[:, :1], c.k_cache[0], c.v_cache[0], slots)
+    with pytest.raises(ValueError, match="GPU"):
+        nanoserve_amd.paged_attention_int4(x, c.k_cache[0], c.v_cache[0], md, 1.0)
+    with pytest.raises(ValueError, match="uint8"):
+        nanoserve_amd.paged_attention_int4(x, x[None], x[None], md, 1.0)
+
+
+OK, INV, UNS = _lib.NS_OK, _lib.NS_ERR_INVALID_ARG, _lib.NS_ERR_UNSUPPORTED
+
+
+def _write_args(**over):
+    a = dict(key=16, value=16, kst=128, ksh=64, vst=128, vsh=64, kc=16, vc=16, slots=16, s64=1,
+             T=4, Hkv=2, D=64, bs=16, nb=8, dtype=_lib.NS_DTYPE_F16, stream=None)
+    a.update(over)
+    return list(a.values())
+
+
+WRITE_BAD = [(dict(key=None), INV), (dict(vc=None), INV), (dict(slots=None), INV), (dict(T=-1), INV),
+             (dict(Hkv=0), INV), (dict(D=0), INV), (dict(nb=0), INV), (dict(D=60), UNS), (dict(D=264), UNS),
+             (dict(bs=6), UNS), (dict(dtype=_lib.NS_DTYPE_F32), UNS), (dict(kc=24), INV), (dict(key=17), INV),
+             (dict(slots=20), INV)]
+
+
+@pytest.mark.parametrize("over,code", WRITE_BAD)
+def test_write_rejects_bad_arguments(over, code):
+    assert _lib.load().ns_reshape_and_cache_int4(*_write_args(**over)) == code
+
+
+@pytest.mark.parametrize("over,code", WRITE_BAD + [
+    (dict(qo=None), INV), (dict(q=None), INV), (dict(cos=None), INV), (dict(sin=None), INV), (dict(Hq=0), INV),
+    (dict(cos=17), INV)])
+def test_rope_write_rejects_bad_arguments(over, code):
+    a = dict(qo=16, q=16, qst=896, qsh=64, key=16, kst=128, ksh=64, value=16, vst=128, vsh=64, cos=16, sin=16, cst=64,
+             kc=16, vc=16, slots=16, s64=1, T=4, Hq=14, Hkv=2, D=64, bs=16, nb=8, dtype=_lib.NS_DTYPE_F16, stream=None)
+    a.update(over)
+    assert _lib.load().ns_rope_reshape_and_cache_int4(*a.values()) == code
+
+
+@pytest.mark.parametrize("over,code", [
+    (dict(ko=None), INV), (dict(vo=24), INV), (dict(slots=None), INV), (dict(T=-1), INV), (dict(Hkv=0), INV),
+    (dict(D=60), UNS), (dict(bs=6), UNS), (dict(dtype=7), UNS), (dict(vc=8), INV)])
+def test_gather_rejects_bad_arguments(over, code):
+    a = dict(ko=16, vo=16, kc=16, vc=16, slots=16, s64=1, T=4, Hkv=2, D=64, bs=16, nb=8, dtype=_lib.NS_DTYPE_F16,
+             stream=None)
+    a.update(over)
+    assert _lib.load().ns_gather_cache_int4(*a.values()) == code
+
+
+def test_no_tokens_is_a_no_op():
+    lib = _lib.load()
+    assert lib.ns_reshape_and_cache_int4(*_write_args(T=0, key=None)) == OK
+    assert lib.ns_gather_cache_int4(None, None, None, None, None, 1, 0, 2, 64, 16, 8, _lib.NS_DTYPE_F16, None) == OK
