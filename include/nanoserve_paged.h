@@ -511,9 +511,21 @@ int ns_gather_cache_int4(void* k_out, void* v_out, const void* k_cache, const vo
  * batches.  Each stored value enters as the exact scale * code + offset.
  * query and out are [num_tokens, num_heads, head_dim] in `dtype`, 16-byte
  * aligned.  A row without keys is zero; a row of no sequence is left as it
- * is.  A block id outside [0, num_blocks) is never dereferenced and makes the
- * rows that need it NaN.
+ * is; no context is longer than max_seq_len, no query longer than
+ * max_query_len.  A block id outside [0, num_blocks) is never dereferenced and
+ * makes the rows that need it NaN.
+ *
+ * context_tokens is the sum of the context lengths where the caller knows it,
+ * else 0; it decides only how long contexts are cut for the device (and so the
+ * order of sums).  workspace: 256-byte aligned,
+ * ns_paged_attention_int4_workspace_size bytes for the same sizes (0: none is
+ * needed), not initialised, not read by later calls.  Calls that overlap in
+ * time need their own.  Head sizes 64 and 128 with blocks of whole 16-token
+ * tiles run on the matrix cores, every other shape a plain kernel.
  */
+size_t ns_paged_attention_int4_workspace_size(int num_seqs, int num_heads, int num_kv_heads, int head_dim,
+                                              int block_size, int max_seq_len, int max_query_len,
+                                              int64_t num_tokens, int64_t context_tokens, int is_decode_only);
 int ns_paged_attention_int4(void* out, const void* query,
                             const void* k_cache, const void* v_cache,
                             const void* block_tables, int64_t block_table_stride,
@@ -521,10 +533,11 @@ int ns_paged_attention_int4(void* out, const void* query,
                             const void* seq_lens, int seq_lens_is_int64,
                             const void* query_start_loc, int query_start_loc_is_int64,
                             int num_seqs, int64_t num_tokens, int max_query_len, int max_seq_len,
-                            int is_decode_only,
+                            int64_t context_tokens, int is_decode_only,
                             int num_heads, int num_kv_heads, int head_dim,
                             int block_size, int64_t num_blocks,
-                            float scale, int dtype, void* stream);
+                            float scale, int dtype,
+                            void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -180,15 +180,21 @@ SIGNATURES = {
         c_int64, c_int, c_int, c_int, c_int64,   # T, Hkv, D, block_size, num_blocks
         c_int, c_void_p,                         # dtype, stream
     ]),
+    "ns_paged_attention_int4_workspace_size": (c_size_t, [
+        c_int, c_int, c_int, c_int, c_int,       # S, Hq, Hkv, D, block_size
+        c_int, c_int, c_int64, c_int64, c_int,   # max_seq_len, max_query_len, T, context_tokens, decode_only
+    ]),
     "ns_paged_attention_int4": (c_int, [
         c_void_p, c_void_p,                      # out, query
         c_void_p, c_void_p,                      # k_cache, v_cache
         c_void_p, c_int64, c_int64, c_int,       # block_tables, row stride, width, is_int64
         c_void_p, c_int,                         # seq_lens, is_int64
         c_void_p, c_int,                         # query_start_loc, is_int64
-        c_int, c_int64, c_int, c_int, c_int,     # S, T, max_query_len, max_seq_len, decode_only
+        c_int, c_int64, c_int, c_int,            # S, T, max_query_len, max_seq_len
+        c_int64, c_int,                          # context_tokens, decode_only
         c_int, c_int, c_int, c_int, c_int64,     # Hq, Hkv, D, block_size, num_blocks
-        c_float, c_int, c_void_p,                # scale, dtype, stream
+        c_float, c_int,                          # scale, dtype
+        c_void_p, c_size_t, c_void_p,            # workspace, bytes, stream
     ]),
 }
 
