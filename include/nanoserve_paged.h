@@ -511,29 +511,31 @@ int ns_gather_cache_int4(void* k_out, void* v_out, const void* k_cache, const vo
  * batches.  Each stored value enters as the exact scale * code + offset.
  * query and out are [num_tokens, num_heads, head_dim] in `dtype`, 16-byte
  * aligned.  A row without keys is zero; a row of no sequence is left as it
- * is; no context is longer than max_seq_len, no query longer than
- * max_query_len.  A block id outside [0, num_blocks) is never dereferenced and
+ * is; no context is longer than max_seq_len (keys from there on are not seen).
+ * A block id outside [0, num_blocks) is never dereferenced and
  * makes the rows that need it NaN.
  *
  * context_tokens is the sum of the context lengths where the caller knows it,
  * else 0; it decides only how long contexts are cut for the device (and so the
- * order of sums).  workspace: 256-byte aligned,
+ * order of sums).  one_row_seqs is the number of sequences with one query row
+ * where the caller knows it (and the device's offsets say the same), else -1; a
+ * batch of none, or of nothing else, needs one launch less.  workspace: 256-byte aligned,
  * ns_paged_attention_int4_workspace_size bytes for the same sizes (0: none is
  * needed), not initialised, not read by later calls.  Calls that overlap in
  * time need their own.  Head sizes 64 and 128 with blocks of whole 16-token
  * tiles run on the matrix cores, every other shape a plain kernel.
  */
 size_t ns_paged_attention_int4_workspace_size(int num_seqs, int num_heads, int num_kv_heads, int head_dim,
-                                              int block_size, int max_seq_len, int max_query_len,
-                                              int64_t num_tokens, int64_t context_tokens, int is_decode_only);
+                                              int block_size, int max_seq_len, int64_t num_tokens,
+                                              int is_decode_only, int64_t context_tokens, int one_row_seqs);
 int ns_paged_attention_int4(void* out, const void* query,
                             const void* k_cache, const void* v_cache,
                             const void* block_tables, int64_t block_table_stride,
                             int64_t block_table_width, int block_tables_is_int64,
                             const void* seq_lens, int seq_lens_is_int64,
                             const void* query_start_loc, int query_start_loc_is_int64,
-                            int num_seqs, int64_t num_tokens, int max_query_len, int max_seq_len,
-                            int64_t context_tokens, int is_decode_only,
+                            int num_seqs, int64_t num_tokens, int max_seq_len, int is_decode_only,
+                            int64_t context_tokens, int one_row_seqs,
                             int num_heads, int num_kv_heads, int head_dim,
                             int block_size, int64_t num_blocks,
                             float scale, int dtype,

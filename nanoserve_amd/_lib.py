@@ -182,7 +182,7 @@ SIGNATURES = {
     ]),
     "ns_paged_attention_int4_workspace_size": (c_size_t, [
         c_int, c_int, c_int, c_int, c_int,       # S, Hq, Hkv, D, block_size
-        c_int, c_int, c_int64, c_int64, c_int,   # max_seq_len, max_query_len, T, context_tokens, decode_only
+        c_int, c_int64, c_int, c_int64, c_int,   # max_seq_len, T, decode_only, context_tokens, one_row_seqs
     ]),
     "ns_paged_attention_int4": (c_int, [
         c_void_p, c_void_p,                      # out, query
@@ -190,8 +190,8 @@ SIGNATURES = {
         c_void_p, c_int64, c_int64, c_int,       # block_tables, row stride, width, is_int64
         c_void_p, c_int,                         # seq_lens, is_int64
         c_void_p, c_int,                         # query_start_loc, is_int64
-        c_int, c_int64, c_int, c_int,            # S, T, max_query_len, max_seq_len
-        c_int64, c_int,                          # context_tokens, decode_only
+        c_int, c_int64, c_int, c_int,            # S, T, max_seq_len, decode_only
+        c_int64, c_int,                          # context_tokens, one_row_seqs
         c_int, c_int, c_int, c_int, c_int64,     # Hq, Hkv, D, block_size, num_blocks
         c_float, c_int,                          # scale, dtype
         c_void_p, c_size_t, c_void_p,            # workspace, bytes, stream

@@ -199,66 +199,120 @@ hipError_t launch_generic(const Kv4AttnParams& p, hipStream_t stream) {
 
 // ---- head sizes 64 and 128, blocks of whole 16-token tiles --------------------
 //
-// S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_f16, straight from the
-// cache: a lane's part of a 16-token tile is one load (8 or 16 bytes), a mask
-// turns its words into operands (kv4.h), and nothing passes through LDS.  Both
+// S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_f16.  A wave keeps a ring
+// of steps of 32 tokens in LDS, its own (no wave waits for another): codes and
+// parameter words arrive there by LDS-DMA, which holds no registers in flight,
+// several steps ahead.  A lane's part of a tile is one LDS read (8 or 16 bytes),
+// and a mask turns its words into operands (kv4.h).  Both
 // model dtypes run in float16: the codes are exact there, the query is brought
-// into its range by a power of two per column (exact but for elements 2^-29 of
-// the column's largest, whose error is below 2^-40 of it), and the probabilities
-// keep 11 bits where bfloat16 would keep 8.
+// into its range by a power of two for the wave's columns (exact but for
+// elements below 2^-25 of the largest, whose error is below 2^-36 of it), and
+// the probabilities keep 11 bits where bfloat16 would keep 8.
 //
-// A score is y = s_t (q.c_t) + b_t sum(q), its logarithm to base 2 is y times a
-// column's factor, which the exponential's own fused multiply-add applies.  The
-// operand of the second product is p s_t, rounded once to float16: p is kept
-// 2^14 times its value, s_t divided by a power of two above the largest scale
-// that the wave has met (the accumulators follow when that grows, exactly), so
-// a product lies below 2^14 and keeps its 11 bits down to 2^-28 of the largest.
-// sum p and sum p b_t are float32.
+// A score in log2 units is two fused multiply-adds, s_t (q.c_t) + (b_t sum(q) -
+// reference), with the softmax scale in s_t and b_t: the reference is the
+// maximum of an earlier step, and only when some score of a step passes it by
+// 2^8 is the column's maximum taken over its lanes and the reference moved.
+// The operand of the second product is p s_t, rounded once to float16: s_t is
+// divided by a power of two above the largest scale that the wave has met (the
+// accumulators follow when that grows, exactly), so a product lies below 2^14
+// and keeps its 11 bits down to 2^-20 of the largest.  sum p and sum p (b_t +
+// 8 s_t) are float32, and one more product, with a tile of eights, gives 8 times
+// the sum of the rounded p s_t to take off again: a rounding then acts on a code's
+// distance from the middle, half as far as its distance from 0.
 //
 // The result layout of the first product, tokens 4 g + r of column lane % 16 in
 // lane group g, is the operand layout of the second.
 
-// The operands of one step of 32 tokens: a lane's words of the two tiles.
+// A step's place in the ring: codes of two tiles of K, of V, then the parameter
+// words of both tiles of K and of V.
 template <int D>
-struct Step {
-  uint32_t k[2][D / 32], v[2][D / 32];
-  u32x4 kp[2], vp[2];  // parameter words of tokens 4 g .. 4 g + 3 of each tile
+struct Slot {
+  static constexpr int v = 16 * D, par = 32 * D, bytes = 32 * D + 256;
+  static constexpr int loads = D == 128 ? 5 : 3;  // vector memory operations that fill it
 };
 
-template <int N>
-__device__ __forceinline__ void load_words(uint32_t (&w)[N], const char* p) {
-  if constexpr (N == 2) {
-    const u32x2 x = *reinterpret_cast<const u32x2*>(p);
-    w[0] = x[0];
-    w[1] = x[1];
-  } else {
-    static_assert(N == 4, "head sizes 64 and 128");
-    const u32x4 x = *reinterpret_cast<const u32x4*>(p);
+// A lane's words of the two tiles of K or V, and the parameter words of tokens
+// 4 g .. 4 g + 3 of each.
+template <int D>
+struct Tiles {
+  uint32_t w[2][D / 32];
+  u32x4 par[2];
+
+  __device__ __forceinline__ void read_params(const char* params, int g) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = x[i];
+    for (int j = 0; j < 2; ++j) par[j] = *reinterpret_cast<const u32x4*>(params + j * 64 + g * 16);
   }
-}
+  // code_off: the lane's bytes in a tile.
+  __device__ __forceinline__ void read_codes(const char* codes, int code_off) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const char* at = codes + j * (8 * D) + code_off;
+      if constexpr (D == 64) {
+        const u32x2 x = *reinterpret_cast<const u32x2*>(at);
+        w[j][0] = x[0];
+        w[j][1] = x[1];
+      } else {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(at);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[j][i] = x[i];
+      }
+    }
+  }
+};
 
 // Where the wave's tiles lie: lane l holds tile l & 1 of step l / 2 of a window
-// of 32 steps, as the byte offset of its codes and, from there, of its
-// parameter words (bit 0 of which marks a block id outside the cache).
+// of 32 steps, as the addresses of its codes in K and V and, from there, the
+// distance to its parameter words.
 struct Window {
-  uint32_t lo, hi;
+  uint32_t k_lo, k_hi, v_lo, v_hi;
   int par;
 };
 
 __device__ __forceinline__ int lane_value(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+__device__ __forceinline__ const char* lane_pointer(uint32_t lo, uint32_t hi, int lane) {
+  return reinterpret_cast<const char*>(
+      (static_cast<uint64_t>(static_cast<uint32_t>(lane_value(static_cast<int>(hi), lane))) << 32) |
+      static_cast<uint32_t>(lane_value(static_cast<int>(lo), lane)));
+}
+// Until at most N of the wave's vector memory operations are pending.
+template <int N>
+__device__ __forceinline__ void vector_wait() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// What a block id outside the cache reads instead: rows of K that are NaN (an
+// offset of NaN, so every score with them is), rows of V without any.
+constexpr int kPageWords = 512;  // a tile's codes at head size 128 are 1 KiB, parameters start at 0
+struct Page {
+  uint32_t w[kPageWords];
+};
+constexpr Page page_of(uint32_t x) {
+  Page p = {};
+  for (int i = 0; i < kPageWords; ++i) p.w[i] = x;
+  return p;
+}
+__device__ const Page kNanF16 = page_of(Half<F16>::nan);
+__device__ const Page kNanBF16 = page_of(Half<BF16>::nan);
+__device__ const Page kZeros = page_of(0);
 
 constexpr float kCodeUnit = 16777216.f;  // 2^24: an even dim's code as a half's bits is code / 2^24
-constexpr float kLift = 14.f;            // p is kept 2^14 times its value
+// p is kept relative to a reference that is at most kSlack binades below the
+// column's running maximum and lifted by kLift, so that the largest lies in
+// [2^kLift, 2^(kLift + kSlack)] and fits a half: the reference (and with it the
+// accumulators) moves only when a score passes it by that much.
+constexpr float kLift = 6.f, kSlack = 8.f;
 
 // One wave's state: NT tiles of 16 columns, D output dims each.
 template <class DT, int D, int NT>
 struct Wave {
   half8 q[NT][D / 32];
-  float cf[NT], qs[NT];       // log2 units per score unit; sum(q) in score units
-  float m[NT], l[NT], b[NT];  // maximum (log2), sum p (this lane's tokens), sum p b_t (likewise)
+  float cf;                   // log2 units per score unit
+  float qs[NT];               // sum(q) in score units
+  float m[NT], ref[NT];       // reference (log2 units); kLift - reference
+  float l[NT], b[NT];         // sum p (this lane's tokens), sum p (b_t + 8 s_t) (likewise)
   floatx4 acc[NT][D / 16];
+  floatx4 mid[NT];            // the same of a dim whose every code is 8
   float sigma, inv_sigma;     // the scales' power of two
   uint32_t top;               // largest parameter word that needs no larger sigma
 
@@ -266,7 +320,9 @@ struct Wave {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       m[n] = -INFINITY;
+      ref[n] = INFINITY;
       l[n] = b[n] = 0.f;
+      mid[n] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) acc[n][i] = floatx4{0.f, 0.f, 0.f, 0.f};
     }
@@ -274,45 +330,53 @@ struct Wave {
     top = 0xFFFFu;
   }
 
-  // Column n's query row, as the operand that meets the codes: lane group g
+  // The columns' query rows, as the operands that meet the codes: lane group g
   // holds dims (D / 4) g .. + D / 4, eight of them per 32-dim step in the order
   // of a word's masked nibbles, odd dims a sixteenth of their value.
-  __device__ __forceinline__ void load_query(int n, const char* row, int g, float scale) {
-    float x[D / 4], big = 0.f;
+  __device__ __forceinline__ void load_queries(const char* const (&row)[NT], int g, float scale) {
+    uint32_t x[NT][D / 8];
+    float big = 0.f;
 #pragma unroll
-    for (int w = 0; w < D / 32; ++w) {
-      const u32x4 r = *reinterpret_cast<const u32x4*>(row + (g * (D / 4) + 8 * w) * 2);
+    for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[8 * w + 2 * e] = Half<DT>::to_f32(r[e] & 0xFFFFu);
-        x[8 * w + 2 * e + 1] = Half<DT>::to_f32(r[e] >> 16);
-        big = fmaxf(big, fmaxf(fabsf(x[8 * w + 2 * e]), fabsf(x[8 * w + 2 * e + 1])));
+      for (int w = 0; w < D / 32; ++w) {
+        const u32x4 r = *reinterpret_cast<const u32x4*>(row[n] + (g * (D / 4) + 8 * w) * 2);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[n][4 * w + e] = r[e];
+          const float lo = fabsf(Half<DT>::to_f32(r[e] & 0xFFFFu)), hi = fabsf(Half<DT>::to_f32(r[e] >> 16));
+          big = fmaxf(big, fmaxf(lo < INFINITY ? lo : 0.f, hi < INFINITY ? hi : 0.f));
+        }
       }
     }
-    big = group4_max(big);
-    // The largest becomes 2^14 .. 2^15 (a column of zeros or non-finite values as it comes).
-    int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;
-    e = 14 - e;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor(big, off));
+    // The wave's largest finite element becomes 2^14 .. 2^15.
+    int e = 14 - (static_cast<int>(__float_as_uint(big) >> 23) - 127);
     e = e < -113 ? -113 : e > 100 ? 100 : e;
-    if (!(big > 0.f) || !(big < INFINITY)) e = 0;
     float f = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
-    cf[n] = fabsf(scale) * 1.4426950408889634f * (kCodeUnit / f);
+    cf = fabsf(scale) * 1.4426950408889634f * (kCodeUnit / f);
     if (scale < 0.f) f = -f;  // a negative scale turns the query around, exactly
-    float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < D / 4; ++i) {
-      x[i] *= f;
-      sum += x[i];
-    }
-    qs[n] = group4_sum(sum) * (1.f / kCodeUnit);
+    for (int n = 0; n < NT; ++n) {
+      float sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < D / 32; ++w) {
+      for (int w = 0; w < D / 32; ++w) {
+        float v[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float unit = (i & 1) ? 0.0625f : 1.f;
-        q[n][w][2 * i] = static_cast<_Float16>(x[8 * w + i] * unit);
-        q[n][w][2 * i + 1] = static_cast<_Float16>(x[8 * w + i + 4] * unit);
+        for (int i = 0; i < 4; ++i) {
+          v[2 * i] = Half<DT>::to_f32(x[n][4 * w + i] & 0xFFFFu) * f;
+          v[2 * i + 1] = Half<DT>::to_f32(x[n][4 * w + i] >> 16) * f;
+          sum += v[2 * i] + v[2 * i + 1];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float unit = (i & 1) ? 0.0625f : 1.f;
+          q[n][w][2 * i] = static_cast<_Float16>(v[i] * unit);
+          q[n][w][2 * i + 1] = static_cast<_Float16>(v[i + 4] * unit);
+        }
       }
+      qs[n] = group4_sum(sum) * (1.f / kCodeUnit);
     }
   }
 
@@ -341,15 +405,22 @@ struct Wave {
     sigma = next;
     inv_sigma = 1.f / next;
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n) {
+      mid[n] *= ratio;
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) acc[n][i] *= ratio;
+    }
   }
 
   // One step over tokens tok .. tok + 31.  MASK: some column does not see all of
   // them; column n sees tokens up to limit[n], none of the wave's sees past last.
   template <bool MASK>
-  __device__ __forceinline__ void step(const Step<D>& d, int tok, int g, const int (&limit)[NT], int last) {
+  __device__ __forceinline__ void step(const char* slot, int lane, int tok, int g, const int (&limit)[NT], int last) {
+    Tiles<D> k, v;
+    // K for D = 128 and V lie in lane order; a tile of K at D = 64 row after row.
+    k.read_codes(slot, D == 128 ? lane * 16 : (lane & 15) * 32 + g * 8);
+    k.read_params(slot + Slot<D>::par, g);
+    v.read_params(slot + Slot<D>::par + 128, g);
     floatx4 s[NT][2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -357,9 +428,18 @@ struct Wave {
       for (int n = 0; n < NT; ++n) s[n][j] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < D / 32; ++w) {
-        const half8 a = k_operand(d.k[j][w]);
+        const half8 a = k_operand(k.w[j][w]);
 #pragma unroll
         for (int n = 0; n < NT; ++n) s[n][j] = mfma16x16x32(F16{}, a, q[n][w], s[n][j]);
+      }
+    }
+    float ks[2][4], kb[2][4];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        ks[j][r] = kv4_scale<DT>(k.par[j][r]) * cf;
+        kb[j][r] = kv4_offset<DT>(k.par[j][r]) * cf;
       }
     }
     float vs[2][4], vb[2][4];
@@ -368,14 +448,14 @@ struct Wave {
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        uint32_t w = d.vp[j][r];
+        uint32_t w = v.par[j][r];
         if (MASK && tok + 16 * j + 4 * g + r > last) w = 0;  // what lies there is nobody's
         big = max(big, w);
         vs[j][r] = kv4_scale<DT>(w);
-        vb[j][r] = kv4_offset<DT>(w);
+        vb[j][r] = __builtin_fmaf(8.f, vs[j][r], kv4_offset<DT>(w));
       }
     }
-    if (__builtin_amdgcn_ballot_w64(big > top)) raise_sigma(big);
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(big > top) != 0, 0)) raise_sigma(big);
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -384,54 +464,63 @@ struct Wave {
     half8 pv[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      float top_y = -INFINITY;
+      auto seen = [&](int j, int r) { return !MASK || tok + 16 * j + 4 * g + r <= limit[n]; };
+      float x[2][4], most = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const uint32_t w = d.kp[j][r];
-          const float y = __builtin_fmaf(kv4_scale<DT>(w), s[n][j][r], kv4_offset<DT>(w) * qs[n]);
-          s[n][j][r] = y;
-          if (MASK) top_y = fmaxf(top_y, tok + 16 * j + 4 * g + r <= limit[n] ? y : -INFINITY);
-          else top_y = fmaxf(top_y, y);
+          x[j][r] = __builtin_fmaf(ks[j][r], s[n][j][r], __builtin_fmaf(kb[j][r], qs[n], ref[n]));
+          most = fmaxf(most, seen(j, r) ? x[j][r] : -INFINITY);
         }
       }
-      float x = top_y * cf[n];
-      if (MASK && top_y == -INFINITY) x = -INFINITY;  // a factor of zero
-      const float m_new = fmaxf(m[n], group4_max_swap(x));
-      const float m_use = m_new == -INFINITY ? 0.f : m_new;
-      if (__builtin_amdgcn_ballot_w64(m_new > m[n])) {
-        const float alpha = fast_exp2(m[n] - m_use);
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(most > kLift + kSlack) != 0, 0)) {
+        most = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            x[j][r] = __builtin_fmaf(ks[j][r], s[n][j][r], kb[j][r] * qs[n]);
+            most = fmaxf(most, seen(j, r) ? x[j][r] : -INFINITY);
+          }
+        }
+        const float m_new = fmaxf(m[n], group4_max_swap(most));
+        const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m[n] - m_new);
         l[n] *= alpha;
         b[n] *= alpha;
+        mid[n] *= alpha;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) acc[n][i] *= alpha;
         m[n] = m_new;
+        ref[n] = kLift - m_new;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[j][r] += ref[n];
       }
-      const float shift = kLift - m_use;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          float p = fast_exp2(__builtin_fmaf(s[n][j][r], cf[n], shift));
-          float off = vb[j][r];
-          if (MASK) {
-            // A masked place may hold anything: neither its score nor its row enters.
-            const bool seen = tok + 16 * j + 4 * g + r <= limit[n];
-            p = seen ? p : 0.f;
-            off = seen ? off : 0.f;
-          }
+          // A masked place may hold anything: neither its score nor its row enters.
+          const float p = seen(j, r) ? fast_exp2(x[j][r]) : 0.f;
           l[n] += p;
-          b[n] = __builtin_fmaf(p, off, b[n]);
-          pv[n][4 * j + r] = static_cast<_Float16>(p * vs[j][r]);
+          b[n] = __builtin_fmaf(p, seen(j, r) ? vb[j][r] : 0.f, b[n]);
+          pv[n][4 * j + r] = static_cast<_Float16>(p * (seen(j, r) ? vs[j][r] : 0.f));
         }
       }
+    }
+    v.read_codes(slot + Slot<D>::v, lane * (D / 8));
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const half8 eights = __builtin_bit_cast(half8, u32x4{0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u});
+      mid[n] = mfma16x16x32(F16{}, eights, pv[n], mid[n]);
     }
 #pragma unroll
     for (int w = 0; w < D / 32; ++w) {
 #pragma unroll
       for (int odd = 0; odd < 2; ++odd) {
-        const half8 a = v_operand(d.v[0][w], d.v[1][w], odd ? 0x00F000F0u : 0x000F000Fu);
+        const half8 a = v_operand(v.w[0][w], v.w[1][w], odd ? 0x00F000F0u : 0x000F000Fu);
 #pragma unroll
         for (int n = 0; n < NT; ++n) acc[n][2 * w + odd] = mfma16x16x32(F16{}, a, pv[n], acc[n][2 * w + odd]);
       }
@@ -440,74 +529,92 @@ struct Wave {
 
   // Unnormalised output dim (D / 4) g + (D / 16) r + i of column n.
   __device__ __forceinline__ float value(int n, int r, int i, float b_sum) const {
-    return acc[n][i][r] * (sigma * ((i & 1) ? kCodeUnit / 16.f : kCodeUnit)) + b_sum;
+    const float code = (i & 1) ? acc[n][i][r] * 0.0625f : acc[n][i][r];
+    return __builtin_fmaf(code - mid[n][r], sigma * kCodeUnit, b_sum);
   }
 };
 
 // Tokens [first, end) of sequence s in steps `stride` tokens apart, into w.
 // Tokens from end on and past a column's limit are masked; tiles past the
-// wave's last token are never looked up.
-template <class DT, int D, int NT>
-__device__ __forceinline__ void run_keys(Wave<DT, D, NT>& w, const Kv4AttnParams& p, int s, int kvh, int lane,
-                                         int first, int end, int stride, const int (&limit)[NT], int all_see,
+// wave's last token are never looked up.  ring: R slots of this wave's.
+template <int R, class DT, int D, int NT>
+__device__ __forceinline__ void run_keys(Wave<DT, D, NT>& w, const Kv4AttnParams& p, char* ring, int s, int kvh,
+                                         int lane, int first, int end, int stride, const int (&limit)[NT], int all_see,
                                          int last) {
   if (first >= end) return;
+  static_assert((R & (R - 1)) == 0, "a power of two");
   const int g = lane >> 4, col = lane & 15;
   const int steps = (end - first + stride - 1) / stride;
   const int tpb = p.block_size >> 4;
   const int tile_last = last >> 4;
   const int64_t bt_row = static_cast<int64_t>(s) * p.bt_stride;
   const int code_bytes = p.block_size * (D / 2);
-  const int k_off = col * (D / 2) + g * (D / 8), v_off = g * (2 * D) + col * (D / 8), p_off = g * 16;
   Window win;
   auto fill = [&](int i) {
     int tile = (first + (i + (lane >> 1)) * stride) / 16 + (lane & 1);
     tile = tile < tile_last ? tile : tile_last;
     const int at = tile / tpb, in = tile - at * tpb;
-    int64_t id = load_index(p.bt, bt_row + at, p.bt64);
+    const int64_t id = load_index(p.bt, bt_row + at, p.bt64);
     const bool bad = id < 0 || id >= p.num_blocks;
-    id = bad ? 0 : id;
-    const int64_t off = (id * p.num_kv_heads + kvh) * p.record + in * (8 * D);
-    win.lo = static_cast<uint32_t>(off);
-    win.hi = static_cast<uint32_t>(off >> 32);
-    win.par = (code_bytes + in * (64 - 8 * D)) | (bad ? 1 : 0);
+    const int64_t off = bad ? 0 : (id * p.num_kv_heads + kvh) * p.record + in * (8 * D);
+    const char* nan_page = reinterpret_cast<const char*>(DT::code == NS_DTYPE_F16 ? &kNanF16 : &kNanBF16);
+    const uint64_t k = reinterpret_cast<uintptr_t>(bad ? nan_page : p.k_cache) + off;
+    const uint64_t v = reinterpret_cast<uintptr_t>(bad ? reinterpret_cast<const char*>(&kZeros) : p.v_cache) + off;
+    win.k_lo = static_cast<uint32_t>(k);
+    win.k_hi = static_cast<uint32_t>(k >> 32);
+    win.v_lo = static_cast<uint32_t>(v);
+    win.v_hi = static_cast<uint32_t>(v >> 32);
+    win.par = bad ? 0 : code_bytes + in * (64 - 8 * D);
   };
-  auto load = [&](Step<D>& d, int i) {
-    if ((i & 31) == 0) fill(i);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int from = 2 * (i & 31) + j;
-      const uint64_t off = (static_cast<uint64_t>(static_cast<uint32_t>(lane_value(static_cast<int>(win.hi), from))) << 32) |
-                           static_cast<uint32_t>(lane_value(static_cast<int>(win.lo), from));
-      const int par = lane_value(win.par, from);
-      const char* kb = p.k_cache + off;
-      const char* vb = p.v_cache + off;
-      load_words(d.k[j], kb + k_off);
-      load_words(d.v[j], vb + v_off);
-      d.kp[j] = *reinterpret_cast<const u32x4*>(kb + (par & ~1) + p_off);
-      d.vp[j] = *reinterpret_cast<const u32x4*>(vb + (par & ~1) + p_off);
-      if (par & 1) {  // a block outside the cache: every row of it is NaN
-        const uint32_t nan = Half<DT>::nan;
-        d.kp[j] = u32x4{nan, nan, nan, nan};
-        d.vp[j] = u32x4{0u, 0u, 0u, 0u};
-      }
+  // Fills the slot of step i; behind the last step the last one's again, so that
+  // the count of loads in flight stays what the waits expect.
+  auto issue = [&](int i) {
+    char* slot = ring + (i & (R - 1)) * Slot<D>::bytes;
+    if (i < steps) {
+      if ((i & 31) == 0) fill(i);
+    } else {
+      i = steps - 1;
     }
-  };
-  auto compute = [&](const Step<D>& d, int i) {
-    const int tok = first + i * stride;
-    if (tok + 31 <= all_see && tok + 32 <= end) w.template step<false>(d, tok, g, limit, last);
-    else w.template step<true>(d, tok, g, limit, last);
-  };
-  Step<D> a, b;
-  load(a, 0);
-  for (int i = 0; i < steps; i += 2) {
-    if (i + 1 < steps) load(b, i + 1);
-    compute(a, i);
-    if (i + 1 < steps) {
-      if (i + 2 < steps) load(a, i + 2);
-      compute(b, i + 1);
+    const int from = 2 * (i & 31);
+    const char* k0 = lane_pointer(win.k_lo, win.k_hi, from);
+    const char* k1 = lane_pointer(win.k_lo, win.k_hi, from + 1);
+    const char* v0 = lane_pointer(win.v_lo, win.v_hi, from);
+    const char* v1 = lane_pointer(win.v_lo, win.v_hi, from + 1);
+    const int par0 = lane_value(win.par, from), par1 = lane_value(win.par, from + 1);
+    if constexpr (D == 128) {
+      // Every lane brings the 16 bytes that it reads: tokens of K lie 64 bytes apart.
+      const uint32_t k_off = col * 64 + g * 16, v_off = lane * 16;
+      dma_lds16_off(k0, k_off, slot);
+      dma_lds16_off(k1, k_off, slot + 1024);
+      dma_lds16_off(v0, v_off, slot + Slot<D>::v);
+      dma_lds16_off(v1, v_off, slot + Slot<D>::v + 1024);
+    } else {
+      // Both tiles of 512 bytes in one operation, half a wave each.
+      const uint32_t off = (lane & 31) * 16;
+      dma_lds16((lane < 32 ? k0 : k1) + off, slot);
+      dma_lds16((lane < 32 ? v0 : v1) + off, slot + Slot<D>::v);
     }
+    // Lanes 0 .. 15 the first tile's words of K, then the second's, then V's.
+    const char* kp = (lane & 16) ? k1 + par1 : k0 + par0;
+    const char* vp = (lane & 16) ? v1 + par1 : v0 + par0;
+    dma_lds4((lane < 32 ? kp : vp) + col * 4, slot + Slot<D>::par);
+  };
+#pragma unroll 1
+  for (int i = 0; i < R; ++i) issue(i);
+  // Steps that every column sees whole, then the others.
+  const int whole = all_see + 1 < end ? all_see + 1 : end;
+  int i = 0, tok = first;
+  for (; tok + 32 <= whole; tok += stride, ++i) {
+    vector_wait<(R - 1) * Slot<D>::loads>();
+    w.template step<false>(ring + (i & (R - 1)) * Slot<D>::bytes, lane, tok, g, limit, last);
+    issue(i + R);
   }
+  for (; tok < end; tok += stride, ++i) {
+    vector_wait<(R - 1) * Slot<D>::loads>();
+    w.template step<true>(ring + (i & (R - 1)) * Slot<D>::bytes, lane, tok, g, limit, last);
+    issue(i + R);
+  }
+  vector_wait<0>();  // nothing lands in the ring behind its use
 }
 
 // A column's D / 4 consecutive results of this lane, as the output's dtype.
@@ -523,103 +630,172 @@ __device__ __forceinline__ void store_row(char* dst, const float (&x)[D / 4]) {
   }
 }
 
+// One sequence's part of a launch: index of count(rows) work items.
+struct Part {
+  int seq, row, ql, len, index;
+  bool more;  // there may be work items of later sequences, or of this one's
+};
+
+// The index-th work item of all sequences', count(rows) each; false behind the
+// last.  next: the index asked for afterwards.  Every wave counts for itself, 64
+// sequences at a time.
+template <class Count>
+__device__ __forceinline__ bool find_part(const Kv4AttnParams& p, int lane, int index, int next, Count count,
+                                          Part& out) {
+  int before = 0;
+  for (int s0 = 0; s0 < p.num_seqs; s0 += 64) {
+    Rows r = {0, 0, 0};
+    if (s0 + lane < p.num_seqs) r = rows_of(p, s0 + lane);
+    const int len = static_cast<int>(r.len), ql = static_cast<int>(r.ql);
+    const int mine = count(ql, len);
+    int upto = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int v = __shfl_up(upto, off);
+      upto += lane >= off ? v : 0;
+    }
+    const int all = lane_value(upto, 63);
+    if (index < before + all) {
+      const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before + upto > index));
+      out.seq = s0 + at;
+      out.row = lane_value(static_cast<int>(r.row0), at);
+      out.ql = lane_value(ql, at);
+      out.len = lane_value(len, at);
+      out.index = index - before - (lane_value(upto, at) - lane_value(mine, at));
+      out.more = s0 + 64 < p.num_seqs || next < before + all;
+      return true;
+    }
+    before += all;
+  }
+  return false;
+}
+// Ranges of a context: one where it is empty or nothing is split.
+__device__ __forceinline__ int ranges_of(const Kv4AttnParams& p, int len) {
+  return p.nsplit == 1 || len <= p.split ? 1 : (len + p.split - 1) / p.split;
+}
+
 // Rows of one-row sequences: a workgroup takes a range of one (sequence, KV
 // head)'s keys for the group's query heads (up to 16 columns), its four waves
-// every fourth step of it, and merges the four states through LDS.
+// every fourth step of it, and merges the four states through LDS.  The grid is
+// what the device holds at once at most; a workgroup goes from range to range,
+// gridDim apart in the list of all that there are, so a batch of unequal
+// contexts costs no empty workgroups and ends evenly.
+// Three workgroups of four waves on a compute unit (with four the 128 registers
+// left for a wave spill), so up to 53 KiB of LDS each.
+constexpr int kDecodeGroups = 3;
+template <int D>
+constexpr int kDecodeRing = D == 64 ? 4 : 2;
 template <class DT, int D>
-__global__ __launch_bounds__(256) void kv4_decode_kernel(Kv4AttnParams p) {
+__global__ __launch_bounds__(256, kDecodeGroups) void kv4_decode_kernel(Kv4AttnParams p) {
+  constexpr int R = kDecodeRing<D>;
   __shared__ float sm[4][16], sl[4][16];
-  __shared__ float so[4][16][D + 4];  // the four floats keep the 16 columns' stores on different banks
+  // A wave's ring, and behind its keys its unnormalised outputs: 16 columns,
+  // whose stores the four floats keep on different banks.
+  __shared__ __align__(16) char rings[4][R * Slot<D>::bytes];
+  static_assert(R * Slot<D>::bytes >= 16 * (D + 4) * 4, "the outputs lie in the ring");
+  auto so = [&](int wv, int c, int d) { return reinterpret_cast<float*>(rings[wv]) + c * (D + 4) + d; };
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
-  const int pairs = p.num_seqs * p.num_kv_heads;
-  const int range = blockIdx.x / pairs, pair = blockIdx.x - range * pairs;
-  const int s = pair / p.num_kv_heads, kvh = pair - s * p.num_kv_heads;
-  const Rows rows = rows_of(p, s);
-  if (rows.ql != 1) return;
-  const int len = static_cast<int>(rows.len);
-  const int t0 = range * p.split;
-  if (t0 >= len && range > 0) return;  // the merge reads ranges that hold keys
-  const int t1 = p.nsplit > 1 && len - t0 > p.split ? t0 + p.split : len;
+  Part found;
+  found.more = true;
+  for (int item = blockIdx.x; found.more; item += gridDim.x) {
+    const int kvh = item % p.num_kv_heads;
+    auto ranges = [&](int ql, int len) { return ql == 1 ? ranges_of(p, len) : 0; };
+    // The same for every wave.
+    if (!find_part(p, lane, item / p.num_kv_heads, (item + static_cast<int>(gridDim.x)) / p.num_kv_heads, ranges, found))
+      break;
+    const int s = found.seq, len = found.len, range = found.index;
+    const int64_t row0 = found.row;
+    const int t0 = range * p.split;
+    const int t1 = p.nsplit > 1 && len - t0 > p.split ? t0 + p.split : len;
 
-  Wave<DT, D, 1> w;
-  w.init();
-  const int head = kvh * p.group + (col < p.group ? col : p.group - 1);
-  w.load_query(0, p.query + (rows.row0 * p.num_heads + head) * (D * 2), g, p.scale);
-  const int limit[1] = {t1 - 1};
-  run_keys(w, p, s, kvh, lane, t0 + 32 * wave, t1, 128, limit, t1 - 1, len - 1);
-  const float l = group4_sum(w.l[0]), b = group4_sum(w.b[0]);
-  if (g == 0) {
-    sm[wave][col] = w.m[0];
-    sl[wave][col] = l;
-  }
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-#pragma unroll
-    for (int i = 0; i < D / 16; i += 4) {
-      floatx4 v;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = w.value(0, r, i + e, b);
-      *reinterpret_cast<floatx4*>(&so[wave][col][(D / 4) * g + (D / 16) * r + i]) = v;
-    }
-  }
-  __syncthreads();
-
-  // Column threadIdx.x / 16, D / 16 dims of it.
-  const int c = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (D / 16);
-  if (c >= p.group) return;
-  float m = fmaxf(fmaxf(sm[0][c], sm[1][c]), fmaxf(sm[2][c], sm[3][c]));
-  const float m_use = m == -INFINITY ? 0.f : m;
-  float sum = 0.f, o[D / 16];
-#pragma unroll
-  for (int e = 0; e < D / 16; ++e) o[e] = 0.f;
-#pragma unroll
-  for (int v = 0; v < 4; ++v) {
-    const float f = fast_exp2(sm[v][c] - m_use);
-    sum = __builtin_fmaf(f, sl[v][c], sum);
-#pragma unroll
-    for (int e = 0; e < D / 16; ++e) o[e] = __builtin_fmaf(f, so[v][c][d0 + e], o[e]);
-  }
-  const int64_t h = kvh * p.group + c;
-  if (p.nsplit > 1) {
-    const int64_t at = (static_cast<int64_t>(s) * p.num_heads + h) * p.nsplit + range;
-    if (d0 == 0) {
-      p.part_m[at] = m;
-      p.part_l[at] = sum;
+    Wave<DT, D, 1> w;
+    w.init();
+    const int head = kvh * p.group + (col < p.group ? col : p.group - 1);
+    const char* const query[1] = {p.query + (row0 * p.num_heads + head) * (D * 2)};
+    w.load_queries(query, g, p.scale);
+    const int limit[1] = {t1 - 1};
+    run_keys<R>(w, p, rings[wave], s, kvh, lane, t0 + 32 * wave, t1, 128, limit, t1 - 1, len - 1);
+    const float l = group4_sum(w.l[0]), b = group4_sum(w.b[0]);
+    if (g == 0) {
+      sm[wave][col] = w.m[0];
+      sl[wave][col] = l;
     }
 #pragma unroll
-    for (int e = 0; e < D / 16; ++e) p.part_o[at * D + d0 + e] = o[e];
-  } else {
-    const float inv = sum > 0.f ? 1.f / sum : sum;  // no key: zero; a NaN stays one
-    uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + (rows.row0 * p.num_heads + h) * D + d0;
+    for (int r = 0; r < 4; ++r) {
 #pragma unroll
-    for (int e = 0; e < D / 16; e += 2)
-      *reinterpret_cast<uint32_t*>(dst + e) =
-          Half<DT>::from_f32(o[e] * inv) | (Half<DT>::from_f32(o[e + 1] * inv) << 16);
+      for (int i = 0; i < D / 16; i += 4) {
+        floatx4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = w.value(0, r, i + e, b);
+        *reinterpret_cast<floatx4*>(so(wave, col, (D / 4) * g + (D / 16) * r + i)) = v;
+      }
+    }
+    __syncthreads();
+
+    // Column threadIdx.x / 16, D / 16 dims of it.
+    const int c = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (D / 16);
+    if (c < p.group) {
+      float m = fmaxf(fmaxf(sm[0][c], sm[1][c]), fmaxf(sm[2][c], sm[3][c]));
+      const float m_use = m == -INFINITY ? 0.f : m;
+      float sum = 0.f, o[D / 16];
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) o[e] = 0.f;
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const float f = fast_exp2(sm[v][c] - m_use);
+        sum = __builtin_fmaf(f, sl[v][c], sum);
+#pragma unroll
+        for (int e = 0; e < D / 16; ++e) o[e] = __builtin_fmaf(f, *so(v, c, d0 + e), o[e]);
+      }
+      const int64_t h = kvh * p.group + c;
+      if (p.nsplit > 1) {
+        const int64_t at = (static_cast<int64_t>(s) * p.num_heads + h) * p.nsplit + range;
+        if (d0 == 0) {
+          p.part_m[at] = m;
+          p.part_l[at] = sum;
+        }
+#pragma unroll
+        for (int e = 0; e < D / 16; ++e) p.part_o[at * D + d0 + e] = o[e];
+      } else {
+        const float inv = sum > 0.f ? 1.f / sum : sum;  // no key: zero; a NaN stays one
+        uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + (row0 * p.num_heads + h) * D + d0;
+#pragma unroll
+        for (int e = 0; e < D / 16; e += 2)
+          *reinterpret_cast<uint32_t*>(dst + e) =
+              Half<DT>::from_f32(o[e] * inv) | (Half<DT>::from_f32(o[e + 1] * inv) << 16);
+      }
+    }
+    __syncthreads();  // the next range's states go where these are read
   }
 }
+
+constexpr int kColumnRing = 4, kColumnTiles = 2;
 
 // Rows of longer queries: a wave takes 16 NT flattened (query row, head) columns
 // of one (sequence, KV head) over a range of its keys; the workgroup's four
 // waves lie side by side and walk the same keys, which the first of them to
 // come brings into the cache.  No wave waits for another.
 template <class DT, int D, int NT>
-__global__ __launch_bounds__(256) void kv4_columns_kernel(Kv4AttnParams p) {
+__global__ __launch_bounds__(256, 2) void kv4_columns_kernel(Kv4AttnParams p) {
+  __shared__ __align__(16) char rings[4][kColumnRing * Slot<D>::bytes];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
-  const int pairs = p.num_seqs * p.num_kv_heads;
-  const int part = blockIdx.x / pairs, pair = blockIdx.x - part * pairs;
-  const int block = part / p.nsplit, range = part - block * p.nsplit;
-  const int s = pair / p.num_kv_heads, kvh = pair - s * p.num_kv_heads;
-  const Rows rows = rows_of(p, s);
-  const int ql = static_cast<int>(rows.ql), len = static_cast<int>(rows.len);
-  if (ql < (p.every_row ? 1 : 2)) return;
+  const int kvh = blockIdx.x % p.num_kv_heads;
+  auto blocks_of = [&](int ql) { return (ql * p.group + 64 * NT - 1) / (64 * NT); };
+  auto items = [&](int ql, int len) {
+    return ql < (p.every_row ? 1 : 2) ? 0 : blocks_of(ql) * ranges_of(p, len);
+  };
+  Part found;
+  if (!find_part(p, lane, blockIdx.x / p.num_kv_heads, 0, items, found)) return;
+  const int s = found.seq, ql = found.ql, len = found.len;
+  const int64_t row0 = found.row;
   const int cols = ql * p.group;
   // The last columns, which see the most keys, first.
-  const int blocks = (cols + 64 * NT - 1) / (64 * NT);
-  if (block >= blocks) return;
+  const int blocks = blocks_of(ql), ranges = ranges_of(p, len);
+  const int block = found.index / ranges, range = found.index - block * ranges;
   const int base = ((blocks - 1 - block) * 4 + wave) * (16 * NT);
   if (base >= cols) return;
   const int end_col = base + 16 * NT < cols ? base + 16 * NT : cols;
@@ -635,17 +811,19 @@ __global__ __launch_bounds__(256) void kv4_columns_kernel(Kv4AttnParams p) {
   int limit[NT];
   int64_t row[NT];
   int head[NT];
+  const char* query[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     int f = base + 16 * n + col;
     f = f < cols ? f : cols - 1;  // a column past the last repeats it and is not stored
     const int j = f / p.group;
-    row[n] = rows.row0 + j;
+    row[n] = row0 + j;
     head[n] = kvh * p.group + (f - j * p.group);
     limit[n] = len - ql + j;
-    w.load_query(n, p.query + (row[n] * p.num_heads + head[n]) * (D * 2), g, p.scale);
+    query[n] = p.query + (row[n] * p.num_heads + head[n]) * (D * 2);
   }
-  run_keys(w, p, s, kvh, lane, t0, t1, 32, limit, all_see, last);
+  w.load_queries(query, g, p.scale);
+  run_keys<kColumnRing>(w, p, rings[wave], s, kvh, lane, t0, t1, 32, limit, all_see, last);
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const float l = group4_sum(w.l[n]), b = group4_sum(w.b[n]);
@@ -732,50 +910,59 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnParams p) {
   }
 }
 
+constexpr int kCUs = 256;
+
 // How a call is cut.  Host arithmetic on sizes only.
 struct Cut {
-  bool fast, decode, columns;     // matrix-core kernels; which of them
-  bool every_row;
-  int nt;                         // column tiles per wave
-  int dec_split, dec_n;           // tokens per range and ranges of one-row sequences
-  int col_split, col_n;           // ... of longer queries
-  int64_t col_blocks;             // column blocks of the longest query
-  size_t dec_bytes, col_bytes;    // partials
+  bool fast, decode, columns;   // matrix-core kernels; which of them
+  bool every_row;               // the column kernel takes one-row sequences too
+  int dec_split, dec_n;         // tokens per range and ranges of one-row sequences
+  int64_t dec_items;            // ranges of all of them, about
+  int col_split, col_n;         // the same of longer queries
+  int64_t col_blocks;           // column blocks of all queries, at most
+  size_t dec_bytes, col_bytes;  // partials
 };
 
-int round_up(int64_t x, int to) { return static_cast<int>((x + to - 1) / to * to); }
+int64_t round_up(int64_t x, int to) { return (x + to - 1) / to * to; }
 
-Cut cut_of(int num_seqs, int64_t num_tokens, int max_query_len, int max_seq_len, int64_t context, int decode_only,
+Cut cut_of(int num_seqs, int64_t num_tokens, int max_seq_len, int64_t context, int one_row, int decode_only,
            int num_heads, int num_kv_heads, int head_dim, int block_size) {
   Cut c = {};
   c.fast = (head_dim == 64 || head_dim == 128) && block_size % 16 == 0;
   if (!c.fast) return c;
   const int group = num_heads / num_kv_heads;
   c.every_row = group > 16;
-  c.decode = !c.every_row;
-  c.columns = !decode_only || c.every_row;
-  c.nt = 2;
-  const int longest = max_seq_len > 0 ? max_seq_len : 1;
-  const int64_t all = static_cast<int64_t>(num_seqs) * longest;
-  const int64_t tokens = (context > 0 && context < all ? context : all) * num_kv_heads;
-  const int row_bytes = (head_dim + 2) * 4;
+  c.decode = !c.every_row && (decode_only || one_row != 0);
+  c.columns = c.every_row || !(decode_only || one_row == num_seqs);
+  const int64_t longest = max_seq_len > 0 ? max_seq_len : 1;
+  const int64_t all = num_seqs * longest;
+  const int64_t tokens = context > 0 && context < all ? context : all;  // of K, and of V, that a KV head reads
+  const size_t row_bytes = (head_dim + 2) * sizeof(float);
   if (c.decode) {
-    c.dec_split = round_up(tokens / 1024, 128);
-    c.dec_split = c.dec_split < 256 ? 256 : c.dec_split;
-    c.dec_n = (longest + c.dec_split - 1) / c.dec_split;
+    // About one range for each workgroup that the device holds, but not under
+    // 384 tokens: a range costs its workgroup ~7 us of its own (the search, three
+    // dependent loads, the merge of the waves).  32 contexts around 1K (two KV
+    // heads of 64): 128 / 256 / 384 / 512 / 768 tokens 12.0 / 10.9 / 9.9 / 10.6 /
+    // 11.7 us; 64 around 4K (four of 128): 512 / 1024 / 2048 tokens 70.5 / 64.6 /
+    // 64.6 us.  Contexts of up to 1024 stay whole: one of 750 takes 9.7 us, in two
+    // ranges 8.6 and 3.0 for the second launch.
+    c.dec_split = static_cast<int>(round_up(tokens * num_kv_heads / (4 * kCUs), 128));
+    c.dec_split = c.dec_split < 384 ? 384 : c.dec_split;
+    if (longest <= 1024) c.dec_split = 1024;
+    c.dec_n = static_cast<int>((longest + c.dec_split - 1) / c.dec_split);
     c.dec_bytes = c.dec_n > 1 ? static_cast<size_t>(num_seqs) * num_heads * c.dec_n * row_bytes : 0;
+    c.dec_items = (tokens / c.dec_split + num_seqs) * num_kv_heads;
   }
   if (c.columns) {
-    const int ql = decode_only ? 1 : max_query_len;
-    c.col_blocks = (static_cast<int64_t>(ql) * group + 64 * c.nt - 1) / (64 * c.nt);
-    // Workgroups that there are at most, by the rows of the batch.
-    int64_t groups = num_tokens * group / (64 * c.nt);
-    groups = (groups < 1 ? 1 : groups) * num_kv_heads;
-    int64_t want = 512 / groups;
-    want = want < 1 ? 1 : want;
-    c.col_split = round_up((longest + want - 1) / want, 32);
-    c.col_split = c.col_split < 256 ? 256 : c.col_split;
-    c.col_n = (longest + c.col_split - 1) / c.col_split;
+    // Keys are split only where the column blocks leave half of the device idle:
+    // the joining launch reads every row's partials back.  Four chunks of 512
+    // rows (227 blocks) 54 us whole, 45 + 15 in ranges of 512 keys.
+    const int64_t blocks = (num_tokens * group + 64 * kColumnTiles - 1) / (64 * kColumnTiles) * num_kv_heads;
+    const int64_t want = kCUs / blocks < 1 ? 1 : kCUs / blocks;
+    const int64_t split = round_up((longest + want - 1) / want, 32);
+    c.col_split = static_cast<int>(split < 256 ? 256 : split);
+    c.col_n = static_cast<int>((longest + c.col_split - 1) / c.col_split);
+    c.col_blocks = num_tokens * group / (64 * kColumnTiles) + num_seqs;
     c.col_bytes = c.col_n > 1 ? static_cast<size_t>(num_tokens) * num_heads * c.col_n * row_bytes : 0;
   }
   return c;
@@ -805,7 +992,8 @@ hipError_t launch_fast(Kv4AttnParams p, const Cut& c, char* workspace, hipStream
     p.split = c.col_split;
     p.every_row = c.every_row ? 1 : 0;
     partials(workspace + align256(c.dec_bytes), p.num_tokens, c.col_n);
-    e = launch(reinterpret_cast<const void*>(&kv4_columns_kernel<DT, D, 2>), pairs * c.col_blocks * c.col_n, p, st);
+    const void* fn = reinterpret_cast<const void*>(&kv4_columns_kernel<DT, D, kColumnTiles>);
+    e = launch(fn, c.col_blocks * p.num_kv_heads * c.col_n, p, st);
     if (e == hipSuccess && c.col_n > 1)
       e = launch(reinterpret_cast<const void*>(&kv4_merge_kernel<DT, D, false>), (p.num_tokens * p.num_heads + 3) / 4, p, st);
     if (e != hipSuccess) return e;
@@ -814,7 +1002,9 @@ hipError_t launch_fast(Kv4AttnParams p, const Cut& c, char* workspace, hipStream
     p.nsplit = c.dec_n;
     p.split = c.dec_split;
     partials(workspace, p.num_seqs, c.dec_n);
-    e = launch(reinterpret_cast<const void*>(&kv4_decode_kernel<DT, D>), pairs * c.dec_n, p, st);
+    const int64_t held = static_cast<int64_t>(kCUs) * kDecodeGroups;
+    const int64_t most = pairs * c.dec_n < c.dec_items ? pairs * c.dec_n : c.dec_items;
+    e = launch(reinterpret_cast<const void*>(&kv4_decode_kernel<DT, D>), most < held ? most : held, p, st);
     if (e == hipSuccess && c.dec_n > 1)
       e = launch(reinterpret_cast<const void*>(&kv4_merge_kernel<DT, D, true>),
                  (static_cast<int64_t>(p.num_seqs) * p.num_heads + 3) / 4, p, st);
@@ -828,15 +1018,15 @@ bool misaligned(const void* p, unsigned n) { return reinterpret_cast<uintptr_t>(
 }  // namespace ns
 
 extern "C" size_t ns_paged_attention_int4_workspace_size(int num_seqs, int num_heads, int num_kv_heads, int head_dim,
-                                                        int block_size, int max_seq_len, int max_query_len,
-                                                        int64_t num_tokens, int64_t context_tokens,
-                                                        int is_decode_only) {
+                                                        int block_size, int max_seq_len,
+                                                        int64_t num_tokens, int is_decode_only,
+                                                        int64_t context_tokens, int one_row_seqs) {
   using namespace ns;
   if (num_seqs <= 0 || num_tokens <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 ||
       max_seq_len < 0 || !kv4_shape_ok(head_dim, block_size))
     return 0;
-  const Cut c = cut_of(num_seqs, num_tokens, max_query_len, max_seq_len, context_tokens, is_decode_only, num_heads,
-                       num_kv_heads, head_dim, block_size);
+  const Cut c = cut_of(num_seqs, num_tokens, max_seq_len, context_tokens, one_row_seqs, is_decode_only, num_heads, num_kv_heads,
+                       head_dim, block_size);
   return align256(c.dec_bytes) + align256(c.col_bytes);
 }
 
@@ -846,8 +1036,8 @@ extern "C" int ns_paged_attention_int4(void* out, const void* query,
                                        int64_t block_table_width, int block_tables_is_int64,
                                        const void* seq_lens, int seq_lens_is_int64,
                                        const void* query_start_loc, int query_start_loc_is_int64,
-                                       int num_seqs, int64_t num_tokens, int max_query_len, int max_seq_len,
-                                       int64_t context_tokens, int is_decode_only,
+                                       int num_seqs, int64_t num_tokens, int max_seq_len, int is_decode_only,
+                                       int64_t context_tokens, int one_row_seqs,
                                        int num_heads, int num_kv_heads, int head_dim,
                                        int block_size, int64_t num_blocks,
                                        float scale, int dtype,
@@ -861,7 +1051,7 @@ extern "C" int ns_paged_attention_int4(void* out, const void* query,
   if (num_seqs == 0 || num_tokens == 0) return NS_OK;
   if (!out || !query || !k_cache || !v_cache || !block_tables || !seq_lens) return NS_ERR_INVALID_ARG;
   if (is_decode_only ? num_tokens != num_seqs : !query_start_loc) return NS_ERR_INVALID_ARG;
-  if (!is_decode_only && max_query_len <= 0) return NS_ERR_INVALID_ARG;
+  if (context_tokens < 0 || one_row_seqs < -1 || one_row_seqs > num_seqs) return NS_ERR_INVALID_ARG;
   if (block_table_width <= 0 || block_table_stride < block_table_width) return NS_ERR_INVALID_ARG;
   if (misaligned(out, 16) || misaligned(query, 16) || misaligned(k_cache, 16) || misaligned(v_cache, 16) ||
       misaligned(block_tables, block_tables_is_int64 ? 8 : 4) || misaligned(seq_lens, seq_lens_is_int64 ? 8 : 4) ||
@@ -870,8 +1060,8 @@ extern "C" int ns_paged_attention_int4(void* out, const void* query,
   // Rows, heads and columns are counted in 32 bits.
   if (num_heads > 65535 || num_tokens > 0x7FFFFFFF / num_heads || num_seqs > 0x7FFFFFFF / num_heads)
     return NS_ERR_UNSUPPORTED;
-  const Cut cut = cut_of(num_seqs, num_tokens, max_query_len, max_seq_len, context_tokens, is_decode_only, num_heads,
-                         num_kv_heads, head_dim, block_size);
+  const Cut cut = cut_of(num_seqs, num_tokens, max_seq_len, context_tokens, one_row_seqs, is_decode_only, num_heads, num_kv_heads,
+                         head_dim, block_size);
   const size_t need = align256(cut.dec_bytes) + align256(cut.col_bytes);
   if (need > 0 && (!workspace || workspace_bytes < need || misaligned(workspace, 256))) return NS_ERR_WORKSPACE;
   Kv4AttnParams p;

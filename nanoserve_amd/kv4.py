@@ -216,7 +216,7 @@ def paged_attention_int4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     sl = _index(md.seq_lens, "seq_lens", device).contiguous()
     if sl.shape[0] < md.num_seqs:
         raise ValueError("seq_lens is shorter than num_seqs")
-    decode_only = bool(md.is_decode_only)
+    decode_only = int(bool(md.is_decode_only))
     qsl_ptr, qsl64 = None, 0
     if decode_only:
         if T != md.num_seqs:
@@ -232,19 +232,20 @@ def paged_attention_int4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: to
         host = md.query_start_loc_cpu
         full = host is not None and len(host) > md.num_seqs and host[0] == 0 and host[md.num_seqs] == T
         out = torch.empty_like(q) if full else torch.zeros_like(q)
-    # The context lengths' sum, where the host has them, sizes the split.  The
-    # partial results live in a tensor of this call's: captured graphs hold
+    # The context lengths' sum and the number of decode rows, where the host
+    # has them, shape the launches.  The partial results live in a tensor of this call's: captured graphs hold
     # their own, and calls on different streams share nothing.
     context = 0 if md.seq_lens_cpu is None else sum(md.seq_lens_cpu[:md.num_seqs])
+    ones = -1 if md.query_lens_cpu is None else md.query_lens_cpu[:md.num_seqs].count(1)
     nbytes = lib.ns_paged_attention_int4_workspace_size(md.num_seqs, Hq, heads, head_dim, block_size, md.max_seq_len,
-                                                        md.max_query_len, T, context, int(decode_only))
+                                                        T, decode_only, context, ones)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     with _on(device):
         rc = lib.ns_paged_attention_int4(
             out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
             bt.data_ptr(), bt.stride(0), bt.shape[1], int(bt.dtype == torch.int64),
             sl.data_ptr(), int(sl.dtype == torch.int64), qsl_ptr, qsl64,
-            md.num_seqs, T, md.max_query_len, md.max_seq_len, context, int(decode_only),
+            md.num_seqs, T, md.max_seq_len, decode_only, context, ones,
             Hq, heads, head_dim, block_size, num_blocks, float(scale), code,
             None if ws is None else ws.data_ptr(), nbytes, torch.cuda.current_stream(device).cuda_stream)
     _lib.check(rc, "ns_paged_attention_int4")

@@ -89,7 +89,8 @@ def attention_ref(query, kv, seq_lens, query_lens, scale: float):
 
     kv[i] = ((codes, scale, offset) of K, of V), each over seq_lens[i] tokens.
     Returns (out [T, Hq, D], scaled [T, Hq, D], whole [T, Hq, D]): the result,
-    sum p s c and sum p |v| of each element (what roundings of p s and of p act on).
+    sum p s |c - 8| and sum p |v| of each element (what roundings of p s act on
+    where codes count from the middle, and roundings of p).
     """
     T, hq, d = query.shape
     out, scaled, whole = (torch.zeros(T, hq, d, dtype=torch.float64) for _ in range(3))
@@ -110,7 +111,7 @@ def attention_ref(query, kv, seq_lens, query_lens, scale: float):
                 holds = torch.isnan(vb)[:, 0]
                 reached = (seen[some] & holds).any(-1)[:, None, None]
                 at = torch.arange(row, row + ql)[some]
-                for dst, x in ((out, vs * vc + vb), (scaled, vs * vc), (whole, (vs * vc + vb).abs())):
+                for dst, x in ((out, vs * vc + vb), (scaled, vs * (vc - 8).abs()), (whole, (vs * vc + vb).abs())):
                     o = (p @ torch.where(holds[:, None], 0.0, x)).view(-1, group, d)
                     dst[at, g * group:(g + 1) * group] = torch.where(reached, torch.nan, o)
         row += ql

@@ -5,7 +5,9 @@ and attention against the oracle's float64.
 Attention's tolerance, per element, from the roundings that the kernels make:
   the output's own, eps(dtype) / 2 of the result;
   every product p * scale rounded once to float16, 2^-11 relative (half a unit
-  of 2^-10), so at most 2^-11 of sum p s c;
+  of 2^-10).  With w the product and r its rounded value, the kernel forms
+  sum r c - 8 sum r + sum (w (8) + p b) = sum p v + sum (r - w) (c - 8), so the
+  roundings come to at most 2^-11 of sum p s |c - 8|;
   scores in float32: a dot product of up to 256 terms and the exponential are
   within 2^-13 of sum p |v| together for the scores drawn here (|score| < 64:
   64 * 2^-22 from the argument's rounding, as much again from the sum's order,
@@ -326,6 +328,36 @@ def test_one_long_context(hq, hkv, d, dtype):
 @pytest.mark.parametrize("host", [True, False])
 def test_a_short_chunk_behind_a_long_context(hq, hkv, d, dtype, host):
     c = _case([3000, 900, 1], [4, 300, 1], hq, hkv, d, 16, dtype, host=host)
+    _check(_run(c), c)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("host", [True, False])
+def test_many_sequences(d, host):
+    """More sequences than a wave has lanes, contexts of one and of several ranges, empty ones among them."""
+    rng = np.random.default_rng(3)
+    n = 150
+    seqs = [int(x) for x in rng.integers(0, 60, n)]
+    for i, long in ((5, 1500), (63, 1200), (64, 1100), (149, 1300)):
+        seqs[i] = long
+    c = _case(seqs, [1] * n, 4, 2, d, 16, torch.float16, host=host)
+    _check(_run(c), c)
+    ql = [1] * n
+    for i in range(0, n, 7):
+        ql[i] = min(40, seqs[i])
+    c = _case(seqs, ql, 4, 2, d, 16, torch.bfloat16, host=host, seed=1)
+    _check(_run(c), c)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_one_row_of_a_longer_query_layout(d):
+    """One-row sequences given by offsets, with no decode-only flag, and none of them."""
+    c = _case([700, 40, 1], [1, 1, 1], 6, 2, d, 16, torch.float16)
+    want = _run(c)
+    c.md.is_decode_only = False
+    assert torch.equal(_run(c), want)
+    _check(want, c)
+    c = _case([700, 40], [2, 40], 6, 2, d, 16, torch.float16)
     _check(_run(c), c)
 
 

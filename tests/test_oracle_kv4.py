@@ -165,7 +165,43 @@ def test_gather_rejects_bad_arguments(over, code):
     assert _lib.load().ns_gather_cache_int4(*a.values()) == code
 
 
+def _attend_args(**over):
+    a = dict(out=16, query=16, kc=16, vc=16, bt=16, bt_stride=4, bt_width=4, bt64=0, sl=16, sl64=0, qsl=16, qsl64=0,
+             S=2, T=2, maxs=64, decode_only=1, context=0, ones=-1, Hq=14, Hkv=2, D=64, bs=16, nb=32, scale=0.125,
+             dtype=_lib.NS_DTYPE_F16, ws=None, ws_bytes=0, stream=None)
+    a.update(over)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("over,code", [
+    (dict(out=None), INV), (dict(query=None), INV), (dict(kc=None), INV), (dict(bt=None), INV), (dict(sl=None), INV),
+    (dict(decode_only=0, qsl=None), INV), (dict(T=3), INV), (dict(Hq=15), INV), (dict(Hkv=0), INV), (dict(nb=0), INV),
+    (dict(S=-1), INV), (dict(maxs=-1), INV), (dict(bt_stride=3), INV), (dict(bt_width=0), INV), (dict(out=24), INV),
+    (dict(vc=20), INV), (dict(sl=18), INV), (dict(bt=20, bt64=1), INV), (dict(scale=float("nan")), INV),
+    (dict(scale=float("inf")), INV), (dict(context=-1), INV), (dict(ones=3), INV), (dict(ones=-2), INV),
+    (dict(D=60), UNS), (dict(D=264), UNS), (dict(bs=18), UNS), (dict(dtype=_lib.NS_DTYPE_F32), UNS),
+    (dict(T=1 << 28, S=1 << 28), UNS),
+    (dict(maxs=4096, bt_width=256, bt_stride=256), _lib.NS_ERR_WORKSPACE),
+    (dict(maxs=4096, bt_width=256, bt_stride=256, ws=256, ws_bytes=1000), _lib.NS_ERR_WORKSPACE),
+    (dict(maxs=4096, bt_width=256, bt_stride=256, ws=128, ws_bytes=1 << 30), _lib.NS_ERR_WORKSPACE),
+])
+def test_attention_rejects_bad_arguments(over, code):
+    assert _lib.load().ns_paged_attention_int4(*_attend_args(**over)) == code
+
+
+def test_workspace_is_needed_only_where_keys_are_split():
+    size = _lib.load().ns_paged_attention_int4_workspace_size
+    assert size(32, 14, 2, 64, 16, 1024, 32, 1, 0, -1) == 0
+    assert size(32, 14, 2, 64, 16, 8192, 32, 1, 0, -1) > 0
+    assert size(32, 14, 2, 24, 16, 8192, 32, 1, 0, -1) == 0       # the plain kernel
+    assert size(2, 28, 4, 128, 16, 4000, 8000, 0, 0, -1) == size(2, 28, 4, 128, 16, 4000, 2, 1, 0, -1)
+    assert size(2, 28, 4, 128, 16, 4000, 8000, 0, 0, 0) == 0      # whole prompts fill the device
+    assert size(1, 28, 4, 128, 16, 16000, 16, 0, 0, 0) > 0        # a short chunk behind a long context
+    assert size(2, 13, 2, 64, 16, 4000, 2, 1, 0, -1) == 0 and size(0, 14, 2, 64, 16, 4000, 2, 1, 0, -1) == 0
+
+
 def test_no_tokens_is_a_no_op():
     lib = _lib.load()
     assert lib.ns_reshape_and_cache_int4(*_write_args(T=0, key=None)) == OK
+    assert lib.ns_paged_attention_int4(*_attend_args(S=0, T=0, out=None)) == OK
     assert lib.ns_gather_cache_int4(None, None, None, None, None, 1, 0, 2, 64, 16, 8, _lib.NS_DTYPE_F16, None) == OK
