@@ -273,6 +273,35 @@ int ns_argmax_rows(int64_t* out, const void* x, int64_t x_stride_row, int64_t M,
                    int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * ns_sample_rows -- out[m] = a token of row m of x ([M, N], row stride
+ * x_stride_row elements) drawn with the row's uniform number: the reference's
+ * sampler (nanoserve/sampler.py:24-77: temperature, top-k, top-p, one draw) with
+ * min-p beside it and the random numbers given.  uniform, temperature, top_p and
+ * min_p are float32 [M], top_k int32 or int64 [M]; the last three may be NULL
+ * (off).  With z the row in float32 and w_i = exp((z_i - max z) / temperature),
+ * the tokens are ordered by z descending, then index ascending, and every
+ * filter keeps a prefix of that order:
+ *   top_k  the first top_k (off for a row with top_k <= 0 or >= N);
+ *   top_p  those with the sum of w before them below top_p times the sum of w
+ *          over the first top_k, and always the first (off for top_p >= 1);
+ *   min_p  those with w >= min_p, and always the first (off for min_p <= 0).
+ * out[m] is the first of the kept tokens whose running sum of w exceeds
+ * uniform[m] times the sum over all of them; uniform numbers are taken into
+ * [0, 1).  A row with a temperature that is not positive, with a NaN, or whose
+ * largest element is not finite takes its largest element by ns_argmax_rows'
+ * rules.  Weights are float64, rounded to 2^-45 of the largest at N of 150K;
+ * their sums are exact, so a result depends on nothing else.
+ * x need only be aligned to its element; M <= 65535, N < 2^31.  workspace:
+ * ns_sample_rows_workspace_size bytes, 8-byte aligned, not initialised; calls
+ * that overlap in time need their own.
+ */
+size_t ns_sample_rows_workspace_size(int64_t M, int64_t N);
+int ns_sample_rows(int64_t* out, const void* x, int64_t x_stride_row, int64_t M, int64_t N, int dtype,
+                   const float* uniform, const float* temperature,
+                   const void* top_k, int top_k_is_int64, const float* top_p, const float* min_p,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * ns_paged_attention_workspace_size -- bytes of device workspace that
  * ns_paged_attention needs for these sizes: arrival counters, a region for
  * the call's own decode plan, the decode split-K slots and, without

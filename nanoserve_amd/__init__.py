@@ -10,7 +10,8 @@ write with hand-written gfx950 HIP kernels behind a C ABI
   rotary.apply + PagedKVCache.write fused              (rope_reshape_and_cache)
 
 Beside the reference's: the same write and attention over a cache held in 4
-bits (kv4.py).
+bits (kv4.py), and the draw of a token from given uniform numbers
+(sampling.sample_rows).
 """
 
 from .attention import AttentionMetadata, get_attention_backend, paged_attention_hip
@@ -19,6 +20,7 @@ from .kv_cache import PagedKVCache, kv_bytes_per_token, reshape_and_cache
 from .kv4 import (Int4PagedKVCache, gather_cache_int4, paged_attention_int4, reshape_and_cache_int4,
                   rope_reshape_and_cache_int4)
 from .rotary import RotaryEmbedding, rope_reshape_and_cache
+from .sampling import argmax_rows, sample_rows
 
 __version__ = "0.1.0"
 
@@ -27,6 +29,7 @@ __all__ = [
     "BlockSpaceManager",
     "Int4PagedKVCache",
     "PagedKVCache",
+    "argmax_rows",
     "gather_cache_int4",
     "get_attention_backend",
     "kv_bytes_per_token",
@@ -37,4 +40,5 @@ __all__ = [
     "RotaryEmbedding",
     "rope_reshape_and_cache",
     "rope_reshape_and_cache_int4",
+    "sample_rows",
 ]

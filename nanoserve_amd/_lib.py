@@ -111,6 +111,14 @@ SIGNATURES = {
         c_int64, c_int64, c_int,                 # M, N, dtype
         c_void_p, c_size_t, c_void_p,            # workspace, bytes, stream
     ]),
+    "ns_sample_rows_workspace_size": (c_size_t, [c_int64, c_int64]),  # M, N
+    "ns_sample_rows": (c_int, [
+        c_void_p, c_void_p, c_int64,             # out (int64), x, x row stride
+        c_int64, c_int64, c_int,                 # M, N, dtype
+        c_void_p, c_void_p,                      # uniform, temperature
+        c_void_p, c_int, c_void_p, c_void_p,     # top_k (or None), is_int64, top_p, min_p (or None)
+        c_void_p, c_size_t, c_void_p,            # workspace, bytes, stream
+    ]),
     "ns_paged_attention_workspace_size": (c_size_t, [
         c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int64, c_int,
     ]),

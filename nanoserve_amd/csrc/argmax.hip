@@ -6,47 +6,14 @@
 // is cut into slices of 4096 elements scanned by separate workgroups (38 per
 // row, over 1200 for a batch of 32) and a second small launch combines the
 // slices.
-//
-// torch's rules -- the first index among equal maxima, the first NaN if the
-// row holds one -- are folded into one 64-bit key per candidate:
-//     key = order(value) << 32 | (2^32 - 1 - index)
-// where order() maps floats to unsigned integers in value order (+0 and -0
-// equal, every NaN above +inf), so the largest key is the answer.
-#include "ns_convert.h"
+// torch's rules are folded into one 64-bit key per candidate (row_keys.h).
+#include "row_keys.h"
 
 namespace ns {
 namespace {
 
 constexpr int kSliceThreads = 256;
 constexpr int kSliceElems = 4096;  // elements per workgroup slice
-
-__device__ __forceinline__ uint64_t key_of(float v, uint32_t idx) {
-  uint32_t u = __float_as_uint(v);
-  uint32_t ord;
-  if ((u & 0x7FFFFFFFu) > 0x7F800000u) {
-    ord = 0xFFFFFFFFu;                   // NaN
-  } else {
-    if (u == 0x80000000u) u = 0u;        // -0 == +0
-    ord = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-  }
-  return (static_cast<uint64_t>(ord) << 32) | static_cast<uint64_t>(0xFFFFFFFFu - idx);
-}
-
-__device__ __forceinline__ uint64_t max_u64(uint64_t a, uint64_t b) { return a > b ? a : b; }
-
-__device__ __forceinline__ uint64_t wave_max(uint64_t k) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) k = max_u64(k, __shfl_xor(k, off));
-  return k;
-}
-
-template <int DT>
-__device__ __forceinline__ float elem_f32(const char* row, int64_t i) {
-  if constexpr (DT == NS_DTYPE_F32) return reinterpret_cast<const float*>(row)[i];
-  const uint16_t h = reinterpret_cast<const uint16_t*>(row)[i];
-  if constexpr (DT == NS_DTYPE_F16) return static_cast<float>(__builtin_bit_cast(_Float16, h));
-  return __uint_as_float(static_cast<uint32_t>(h) << 16);
-}
 
 // Stage 1: grid (slices, rows).  Writes each slice's best key to keys[row * slices + slice].
 template <int DT>
@@ -65,15 +32,7 @@ __global__ __launch_bounds__(kSliceThreads) void argmax_slices_kernel(uint64_t* 
     const u32x4 w = reinterpret_cast<const u32x4*>(row)[j];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      float v;
-      if constexpr (DT == NS_DTYPE_F32) {
-        v = __uint_as_float(w[e]);
-      } else {
-        const uint16_t h = static_cast<uint16_t>((w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu);
-        v = DT == NS_DTYPE_F16 ? static_cast<float>(__builtin_bit_cast(_Float16, h))
-                               : __uint_as_float(static_cast<uint32_t>(h) << 16);
-      }
-      best = max_u64(best, key_of(v, static_cast<uint32_t>(VEC * j + e)));
+      best = max_u64(best, key_of(vec_elem_f32<DT>(w, e), static_cast<uint32_t>(VEC * j + e)));
     }
   }
   for (int64_t i = VEC * v1 + threadIdx.x; i < s1; i += kSliceThreads)

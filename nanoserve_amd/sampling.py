@@ -1,8 +1,11 @@
-"""Greedy token selection on the GPU (ns_argmax_rows).
+"""Token selection on the GPU (ns_argmax_rows, ns_sample_rows).
 
 The reference's sampler takes logits.argmax(dim=-1) for greedy requests
 (nanoserve/sampler.py:24-27); `argmax_rows` is the same selection -- first
 index among equal maxima, first NaN if any -- in one HIP launch per batch.
+For the others it filters by temperature, top-k and top-p and draws once
+(sampler.py:28-77); `sample_rows` does so, with min-p beside them, from uniform
+numbers that the caller gives, without a sort and without leaving the GPU.
 """
 
 from __future__ import annotations
@@ -10,6 +13,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
+from .kv4 import _on
 
 # One slice-key workspace per (device, stream), grown on demand; graph capture
 # records its pointer, so it is allocated by the warm-up call before capture.
@@ -62,4 +66,73 @@ def argmax_rows(logits: torch.Tensor, out: torch.Tensor | None = None) -> torch.
     rc = lib.ns_argmax_rows(out.data_ptr(), x.data_ptr(), x.stride(0), M, N, _lib.DTYPE_CODES[x.dtype],
                             ws.data_ptr(), ws.numel(), stream)
     _lib.check(rc, "ns_argmax_rows")
+    return out
+
+
+def _per_row(x, rows: int, dtypes: tuple, device: torch.device, name: str) -> torch.Tensor | None:
+    """A per-row setting as a contiguous [M] tensor on the device (a number is every row's)."""
+    if x is None:
+        return None
+    if not isinstance(x, torch.Tensor):
+        return torch.full((rows,), x, dtype=dtypes[0], device=device)
+    if x.device != device:
+        raise ValueError(f"{name} is on {x.device}, expected {device}")
+    if x.dim() != 1 or x.shape[0] != rows:
+        raise ValueError(f"{name} must be [{rows}], got {tuple(x.shape)}")
+    if x.dtype not in dtypes:
+        raise TypeError(f"{name} must be one of {dtypes}, got {x.dtype}")
+    return x.contiguous()
+
+
+@torch.inference_mode()
+def sample_rows(logits: torch.Tensor, uniform: torch.Tensor, temperature, top_k=None, top_p=None, min_p=None,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """[M, N] logits (f32/f16/bf16) and [M] float32 uniform numbers in [0, 1) -> [M] int64 tokens.
+
+    temperature, top_p, min_p (float32) and top_k (int32 or int64) are [M]
+    tensors on the logits' device, or one number for all rows.  Tokens are
+    ordered by logit descending, then index ascending; every filter keeps a
+    prefix of that order:
+
+      top_k  the first top_k                     (off for a row with top_k <= 0 or >= N)
+      top_p  while the probability before a token, among the first top_k, is
+             below top_p; always the first       (off with top_p >= 1)
+      min_p  probabilities of at least min_p times the largest (off with min_p <= 0)
+
+    The token is the first kept one whose running probability, renormalised
+    over the kept ones, exceeds the row's uniform number.  A row with a
+    temperature that is not positive, with a NaN, or whose largest logit is not
+    finite takes argmax_rows' token.  `out`: a contiguous int64 [M] tensor."""
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be [M, N], got {tuple(logits.shape)}")
+    if not logits.is_cuda:
+        raise ValueError("sample_rows needs a GPU tensor (the HIP path has no CPU fallback)")
+    if logits.dtype not in _lib.DTYPE_CODES:
+        raise TypeError(f"unsupported dtype {logits.dtype}")
+    M, N = logits.shape
+    device = logits.device
+    x = logits if logits.stride(1) == 1 and (M < 2 or logits.stride(0) >= N) else logits.contiguous()
+    f32 = (torch.float32,)
+    if uniform is None or temperature is None:
+        raise ValueError("uniform and temperature are needed")
+    u = _per_row(uniform, M, f32, device, "uniform")
+    t = _per_row(temperature, M, f32, device, "temperature")
+    k = _per_row(top_k, M, (torch.int64, torch.int32), device, "top_k")
+    p = _per_row(top_p, M, f32, device, "top_p")
+    mp = _per_row(min_p, M, f32, device, "min_p")
+    if out is None:
+        out = torch.empty(M, dtype=torch.int64, device=device)
+    elif out.shape != (M,) or out.dtype != torch.int64 or out.device != device or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous int64 [{M}] tensor on {device}")
+    if M == 0:
+        return out
+    lib = _lib.load()
+    nbytes = lib.ns_sample_rows_workspace_size(M, N)
+    ws = torch.empty(max(nbytes, 8), dtype=torch.uint8, device=device)  # this call's own
+    ptr = lambda a: None if a is None else a.data_ptr()  # noqa: E731
+    with _on(device):
+        rc = lib.ns_sample_rows(out.data_ptr(), x.data_ptr(), max(x.stride(0), N), M, N, _lib.DTYPE_CODES[x.dtype],
+                                u.data_ptr(), t.data_ptr(), ptr(k), int(k is not None and k.dtype == torch.int64),
+                                ptr(p), ptr(mp), ws.data_ptr(), nbytes, torch.cuda.current_stream(device).cuda_stream)
+    _lib.check(rc, "ns_sample_rows")
     return out
