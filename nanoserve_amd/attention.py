@@ -351,16 +351,23 @@ def _attention(query, k_cache, v_cache, md: AttentionMetadata, scale: float, sha
 paged_attention_hip.prepare = prepare_decode_plan
 
 
-def get_attention_backend(name: str = "auto"):
+def get_attention_backend(name: str = "auto", kv_bits: int = 16):
     """Resolve a backend name to (callable, name) with attn_fn's signature.
 
     Mirrors reference attention.py:193-206, with one backend: "auto" and "hip"
-    return the HIP path and raise if its library cannot be loaded.  The
+    return the HIP path and raise if its library cannot be loaded; kv_bits 4
+    is the same op over a cache held in 4 bits (kv4.Int4PagedKVCache).  The
     reference's "torch" (gather+SDPA) and "triton" backends are not product
     paths here and are rejected rather than silently substituted.
     """
+    if kv_bits not in (4, 16):
+        raise ValueError(f"kv_bits must be 16 or 4, got {kv_bits}")
     if name in ("auto", "hip"):
         _lib.load()
+        if kv_bits == 4:
+            from .kv4 import paged_attention_int4
+
+            return paged_attention_int4, "hip-int4"
         return paged_attention_hip, "hip"
     if name in ("torch", "triton"):
         raise ValueError(

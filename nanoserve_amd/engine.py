@@ -5,8 +5,9 @@ metrics.py) to run the end-to-end serving benchmark with the kernels inside
 the model: requests join and leave the batch every step, prefill and decode
 share one token budget, long prompts are prefilled in chunks, and when
 blocks run out sequences are evicted and later recomputed (the scheduling
-rules live in `scheduling.py`).  Sampling is greedy (the benchmark's
-setting).  A step's metadata is built in scheduler order with int64 indices
+rules live in `scheduling.py`).  Tokens are greedy (the benchmark's setting) or
+drawn as each request's SamplingParams say; the cache is 16 bits wide or held
+in 4 (`kv_bits`).  A step's metadata is built in scheduler order with int64 indices
 in one host-to-device copy (model_runner.py:52-147); a sequence yields a
 token only in the step that computes its last uncomputed token.
 """
@@ -22,8 +23,9 @@ import torch
 from .attention import AttentionMetadata, get_attention_backend
 from .block_manager import BlockSpaceManager
 from .capture import no_cycle_collection
+from .kv4 import Int4PagedKVCache
 from .kv_cache import PagedKVCache
-from .sampling import argmax_rows
+from .sampling import SamplerInputs, argmax_rows, sample_rows
 from .scheduling import RequestMetrics, SamplingParams, Scheduler, SchedulerConfig, Sequence, SeqState
 
 __all__ = ["DecodeGraphs", "LLMEngine", "ModelRunner", "RequestMetrics", "SamplingParams", "Scheduler",
@@ -31,7 +33,7 @@ __all__ = ["DecodeGraphs", "LLMEngine", "ModelRunner", "RequestMetrics", "Sampli
 
 
 class ModelRunner:
-    """Scheduler decision -> metadata -> forward -> greedy tokens.
+    """Scheduler decision -> metadata -> forward -> tokens, greedy or drawn.
 
     With `use_graphs`, decode-only steps replay a HIP graph of the whole
     forward (embedding to greedy token) captured once per batch-size bucket;
@@ -46,9 +48,10 @@ class ModelRunner:
         self.block_manager = block_manager
         self.device = torch.device(device)
         self.block_size = kv_cache.block_size
-        self.attn_fn, self.backend_name = get_attention_backend(backend)
+        self.attn_fn, self.backend_name = get_attention_backend(backend, getattr(kv_cache, "bits", 16))
         self._host: torch.Tensor | None = None
         self._dev: torch.Tensor | None = None
+        self._draw: SamplerInputs | None = None
         self.graphs = DecodeGraphs(self, graph_batch_sizes, max_model_len) if use_graphs else None
 
     def _stage(self, chunks: list[list[int]]) -> list[torch.Tensor]:
@@ -113,7 +116,13 @@ class ModelRunner:
         if sample_idx is None:
             return []
         logits = self.model.compute_logits(hidden, sample_idx)
-        tokens = argmax_rows(logits).tolist()  # greedy; the step's one device-to-host sync
+        if any(seq.sampling.draws for seq in sample_seqs):
+            if self._draw is None:
+                self._draw = SamplerInputs(self.device)
+            chosen = sample_rows(logits, **self._draw.stage(sample_seqs))
+        else:
+            chosen = argmax_rows(logits)
+        tokens = chosen.tolist()  # the step's one device-to-host sync
         return list(zip(sample_seqs, tokens))
 
 
@@ -136,7 +145,9 @@ class DecodeGraphs:
 
     `launch` and `tokens` split a step so that the engine can plan and launch
     the next step before reading this one's tokens back: the next step's input
-    ids are then gathered on the device from this step's greedy output.  Two
+    ids are then gathered on the device from this step's output.  A batch with
+    a request that draws its tokens runs sample_rows on the graph's logits
+    behind the replay, over the same output.  Two
     pinned staging buffers alternate, so filling step N+1 never overwrites the
     buffer step N's copy may still be reading.
 
@@ -168,6 +179,7 @@ class DecodeGraphs:
         self._host = [torch.zeros(self._per, dtype=torch.int64, pin_memory=pin) for _ in range(2)]
         self._host_np = [h.numpy() for h in self._host]
         self._tok = [torch.zeros(n, dtype=torch.int64, pin_memory=pin) for _ in range(2)]
+        self._draw: list[SamplerInputs] = []  # per staging buffer, once a request draws
         self._next = 0  # staging buffer of the next launch
         self._dev = torch.zeros(self._per, dtype=torch.int64, device=runner.device)
         # What each table row of a staging buffer holds: (table width, and per
@@ -296,7 +308,7 @@ class DecodeGraphs:
     @torch.inference_mode()
     def launch(self, scheduled, after: "GraphLaunch | None" = None) -> "GraphLaunch":
         """Replay the step's graph; with `after`, every row's token comes from
-        that earlier launch's greedy output (gathered on the device)."""
+        that earlier launch's output (gathered on the device)."""
         b = next(x for x in self.sizes if x >= len(scheduled))
         longest = max(seq.num_computed_tokens + 1 for seq, _ in scheduled)
         ctx = next(c for c in self.ctx_sizes if c >= longest)
@@ -315,6 +327,12 @@ class DecodeGraphs:
             torch.index_select(after.out, 0, self._dev[4 * n:4 * n + k], out=self._dev[0:k])
         g.replay()
         self.last_logits = logits[:k]
+        if any(seq.sampling.draws for seq, _ in scheduled):
+            if not self._draw:
+                self._draw = [SamplerInputs(self.device, max(self.sizes)) for _ in range(2)]
+            # The output token's index counts the placeholder of a step in flight.
+            sample_rows(logits[:k], **self._draw[slot_i].stage([s for s, _ in scheduled], non_blocking=True),
+                        out=out[:k])
         # The tokens leave the graph's output before a later replay of the
         # same graph can overwrite it.
         tok = self._tok[slot_i]
@@ -341,7 +359,7 @@ class CapturedStep:
     metadata (with the decode-plan buffer) its kernels were captured with."""
 
     graph: torch.cuda.CUDAGraph
-    out: torch.Tensor        # greedy token per row
+    out: torch.Tensor        # greedy token per row (drawn ones are written over it)
     logits: torch.Tensor     # [bucket, vocab]
     md: AttentionMetadata    # keeps md.decode_plan's buffer allocated
 
@@ -351,7 +369,7 @@ class GraphLaunch:
     """A replayed decode step whose tokens may not have been read back yet."""
 
     scheduled: list
-    out: torch.Tensor          # the graph's greedy output (device)
+    out: torch.Tensor          # the graph's output (device)
     tokens_host: torch.Tensor  # pinned copy of it, valid once `done` has completed
     done: torch.cuda.Event
 
@@ -361,12 +379,16 @@ class LLMEngine:
 
     def __init__(self, model, num_blocks: int, block_size: int = 16, device="cuda",
                  scheduler_config: SchedulerConfig | None = None, eos_token_id: int | None = None,
-                 max_model_len: int = 4096, use_graphs: bool = False, pipeline_decode: bool = True) -> None:
+                 max_model_len: int = 4096, use_graphs: bool = False, pipeline_decode: bool = True,
+                 kv_bits: int = 16) -> None:
+        if kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits must be 16 or 4, got {kv_bits}")
         self.model = model.eval().requires_grad_(False)
         self.device = torch.device(device)
         dtype = model.model.embed_tokens.weight.dtype
-        self.kv_cache = PagedKVCache(num_blocks, block_size, model.num_layers, model.num_kv_heads,
-                                     model.head_dim, dtype, device)
+        cache = Int4PagedKVCache if kv_bits == 4 else PagedKVCache
+        self.kv_cache = cache(num_blocks, block_size, model.num_layers, model.num_kv_heads, model.head_dim, dtype,
+                              device)
         self.block_manager = BlockSpaceManager(block_size, num_blocks, watermark=0.0)
         self.scheduler = Scheduler(scheduler_config or SchedulerConfig(), self.block_manager)
         self.runner = ModelRunner(model, self.kv_cache, self.block_manager, device,

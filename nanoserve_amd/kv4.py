@@ -257,6 +257,8 @@ class Int4PagedKVCache:
     model's, float16 or bfloat16: the dtype of the rows written and of every
     row's scale and offset."""
 
+    bits = 4
+
     def __init__(self, num_blocks: int, block_size: int, num_layers: int, num_kv_heads: int, head_dim: int,
                  dtype: torch.dtype, device: str) -> None:
         _model_dtype(dtype, "Int4PagedKVCache")

@@ -74,6 +74,8 @@ def reshape_and_cache(key: torch.Tensor, value: torch.Tensor,
 class PagedKVCache:
     """Per-layer K and V cache tensors (reference kv_cache.py:30-85)."""
 
+    bits = 16  # of a stored element, besides kv4.Int4PagedKVCache's 4
+
     def __init__(
         self,
         num_blocks: int,

@@ -18,6 +18,9 @@ fused INT4 q|k|v projection keeps each head's rows in rotary-pair order and
 runs rotary and the cache write in its own epilogue
 (ns_int4_linear_rope_cache), so projection, rotary and cache write are one
 launch.
+
+With a cache held in 4 bits (kv4.Int4PagedKVCache) rotary and the quantising
+write are one launch behind the projection, and attn_fn is paged_attention_int4.
 """
 
 from __future__ import annotations
@@ -28,6 +31,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .kv4 import rope_reshape_and_cache_int4
 from .quant import Int4Linear, int4_qkv_rope_cache
 from .rotary import RotaryEmbedding, rope_reshape_and_cache
 
@@ -112,9 +116,9 @@ class Qwen2Attention(nn.Module):
         self.o_proj = linear_cls(self.num_heads * hd, cfg.hidden_size, bias=False)
         self.qkv_proj: nn.Module | None = None
 
-    def fuse(self) -> None:
+    def fuse(self, kv_bits: int = 16) -> None:
         qkv = _concat_linears([self.q_proj, self.k_proj, self.v_proj])
-        if isinstance(qkv, Int4Linear) and self.head_dim % 16 == 0:
+        if isinstance(qkv, Int4Linear) and self.head_dim % 16 == 0 and kv_bits == 16:
             # Rows in rotary-pair order: rotary and the cache write run in the
             # projection's epilogue (ns_int4_linear_rope_cache).
             qkv = Int4Linear.rope_pairs(qkv, self.num_heads, self.num_kv_heads, self.head_dim)
@@ -129,7 +133,8 @@ class Qwen2Attention(nn.Module):
         if norm is not None and not (isinstance(self.qkv_proj, Int4Linear) and self.qkv_proj.fuses_norm):
             hidden, norm = norm(hidden), None
         kc, vc = kv_cache.k_cache[self.layer_idx], kv_cache.v_cache[self.layer_idx]
-        if isinstance(self.qkv_proj, Int4Linear) and self.qkv_proj.rope_heads is not None:
+        held_in_4 = getattr(kv_cache, "bits", 16) == 4
+        if isinstance(self.qkv_proj, Int4Linear) and self.qkv_proj.rope_heads is not None and not held_in_4:
             q = int4_qkv_rope_cache(hidden, self.qkv_proj, cos, sin, kc, vc, md.slot_mapping, norm=norm)
             out = attn_fn(q, kc, vc, md, self.scale)
             return _linear(self.o_proj, out.view(T, Hq * D), residual)
@@ -144,7 +149,8 @@ class Qwen2Attention(nn.Module):
             v = self.v_proj(hidden).view(T, Hkv, D)
         # Rotary on q and k, then k and v into the cache before attention reads
         # it (a prefill chunk attends to the keys it just produced).
-        q = rope_reshape_and_cache(q, k, v, cos, sin, kc, vc, md.slot_mapping)
+        write = rope_reshape_and_cache_int4 if held_in_4 else rope_reshape_and_cache
+        q = write(q, k, v, cos, sin, kc, vc, md.slot_mapping)
         out = attn_fn(q, kc, vc, md, self.scale)
         return _linear(self.o_proj, out.view(T, Hq * D), residual)
 
@@ -242,9 +248,11 @@ class Qwen2ForCausalLM(nn.Module):
             hidden = hidden.index_select(0, indices)
         return self.lm_head(hidden)
 
-    def fuse_projections(self) -> "Qwen2ForCausalLM":
+    def fuse_projections(self, kv_bits: int = 16) -> "Qwen2ForCausalLM":
+        """kv_bits 4: for a cache held in 4 bits, whose write is no epilogue of the
+        projection (one fused for 16 bits works with either cache, at a launch more)."""
         for layer in self.model.layers:
-            layer.self_attn.fuse()
+            layer.self_attn.fuse(kv_bits)
             layer.mlp.fuse()
         return self
 

@@ -10,6 +10,7 @@ numbers that the caller gives, without a sort and without leaving the GPU.
 
 from __future__ import annotations
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -136,3 +137,38 @@ def sample_rows(logits: torch.Tensor, uniform: torch.Tensor, temperature, top_k=
                                 ptr(p), ptr(mp), ws.data_ptr(), nbytes, torch.cuda.current_stream(device).cuda_stream)
     _lib.check(rc, "ns_sample_rows")
     return out
+
+
+class SamplerInputs:
+    """Per-row settings of a step's draw: one pinned host buffer, one device
+    buffer, one copy.  Rows: uniform, temperature, top_p, min_p (float32) and
+    top_k (int32)."""
+
+    def __init__(self, device: torch.device, rows: int = 64) -> None:
+        self.device = device
+        self._reserve(rows)
+
+    def _reserve(self, rows: int) -> None:
+        self._host = torch.zeros(5, rows, dtype=torch.float32, pin_memory=self.device.type == "cuda")
+        self._np = self._host.numpy()
+        self._dev = torch.zeros(5, rows, dtype=torch.float32, device=self.device)
+
+    def stage(self, seqs, non_blocking: bool = False) -> dict:
+        """sample_rows' arguments for the next token of each sequence
+        (scheduling.Sequence).  With non_blocking the host buffer is still being
+        read on return: a caller that stages again before the copy is done
+        needs another object."""
+        n = len(seqs)
+        if self._host.shape[1] < n:
+            self._reserve(2 * n)
+        h = self._np
+        p = [s.sampling for s in seqs]
+        h[0, :n] = [s.uniform(len(s.output_token_ids)) for s in seqs]
+        h[1, :n] = [x.temperature for x in p]
+        h[2, :n] = [x.top_p for x in p]
+        h[3, :n] = [x.min_p for x in p]
+        h[4].view(np.int32)[:n] = [min(x.top_k, 0x7FFFFFFF) for x in p]
+        self._dev.copy_(self._host, non_blocking=non_blocking)
+        d = self._dev
+        return dict(uniform=d[0, :n], temperature=d[1, :n], top_p=d[2, :n], min_p=d[3, :n],
+                    top_k=d[4].view(torch.int32)[:n])

@@ -27,17 +27,48 @@ as part of their next prefill.
 from __future__ import annotations
 
 import enum
+import math
 import time
 from collections import deque
 from dataclasses import dataclass, field
+
+import numpy as np
 
 from .block_manager import BlockSpaceManager
 
 
 @dataclass
 class SamplingParams:
+    """How a request ends and how its tokens are chosen (the reference's
+    sampler's settings, sampler.py:24-77, and min-p).  Temperature 0 takes the largest logit; else
+    the token is drawn after top_k (0: off), top_p (1: off) and min_p (0: off)
+    as sampling.sample_rows describes, with uniform numbers of the request's
+    own: `seed` (None: the request's id) and the token's index decide them, not
+    the batch it runs in."""
+
     max_new_tokens: int = 16
     ignore_eos: bool = False
+    temperature: float = 0.0
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+    seed: int | None = None
+
+    def __post_init__(self) -> None:
+        if not 0.0 <= self.temperature < math.inf:
+            raise ValueError(f"temperature must be finite and not negative, got {self.temperature}")
+        if self.top_k < 0:
+            raise ValueError(f"top_k must not be negative, got {self.top_k}")
+        if not 0.0 < self.top_p <= 1.0:
+            raise ValueError(f"top_p must be in (0, 1], got {self.top_p}")
+        if not 0.0 <= self.min_p <= 1.0:
+            raise ValueError(f"min_p must be in [0, 1], got {self.min_p}")
+        if self.seed is not None and self.seed < 0:
+            raise ValueError(f"seed must not be negative, got {self.seed}")
+
+    @property
+    def draws(self) -> bool:
+        return self.temperature > 0.0
 
 
 PREEMPTION_MODES = ("recompute", "none")
@@ -112,7 +143,7 @@ class Sequence:
     """
 
     __slots__ = ("seq_id", "prompt_token_ids", "output_token_ids", "sampling", "state", "block_table",
-                 "num_computed_tokens", "num_evictions", "metrics")
+                 "num_computed_tokens", "num_evictions", "metrics", "_uniform")
 
     def __init__(self, seq_id: int, prompt_token_ids: list[int], sampling: SamplingParams,
                  arrival: float | None = None) -> None:
@@ -126,6 +157,15 @@ class Sequence:
         self.num_evictions = 0
         t = time.perf_counter() if arrival is None else arrival
         self.metrics = RequestMetrics(seq_id, len(prompt_token_ids), t)
+        self._uniform: np.ndarray | None = None
+
+    def uniform(self, index: int) -> float:
+        """The uniform number in [0, 1) that draws output token `index`."""
+        if self._uniform is None or len(self._uniform) <= index:
+            seed = self.seq_id if self.sampling.seed is None else self.sampling.seed
+            n = max(self.sampling.max_new_tokens, index + 1)
+            self._uniform = np.random.default_rng(seed).random(n, dtype=np.float32)
+        return self._uniform[index]
 
     def __repr__(self) -> str:
         return (f"Sequence({self.seq_id}, {self.state.value}, prompt={len(self.prompt_token_ids)}, "
