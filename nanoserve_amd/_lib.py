@@ -239,6 +239,21 @@ def check(rc: int, what: str) -> None:
         raise RuntimeError(f"{what} failed: {msg} (status {rc})")
 
 
+def launch(device: torch.device, what: str, fn, *args) -> None:
+    """fn(*args, current stream of `device`) on that device, whichever is current;
+    raises as `check` does.  The stream handle comes from torch's raw accessor:
+    building a torch.cuda.Stream object costs as much as the call itself."""
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, stream)
+    if rc != NS_OK:
+        check(rc, what)
+
+
 def stream_capture_id(stream: int) -> int:
     """The id of the graph capture under way on `stream` (a hipStream_t as an
     int), or 0 when the stream is not capturing.

@@ -22,12 +22,10 @@ attention.py:99-190); the reference has no such cache.
 
 from __future__ import annotations
 
-import contextlib
-
 import torch
 
 from . import _lib
-from .attention import AttentionMetadata, _index
+from .attention import AttentionMetadata
 
 _CODES = {torch.float16: _lib.NS_DTYPE_F16, torch.bfloat16: _lib.NS_DTYPE_BF16}
 
@@ -45,39 +43,60 @@ def kv4_bytes_per_token(num_layers: int, num_kv_heads: int, head_dim: int) -> in
     return 2 * num_layers * num_kv_heads * (head_dim // 2 + 4)
 
 
+# These wrappers run once per layer and step and hold no launch back by more
+# than a few microseconds: every tensor attribute is read once, and no context
+# manager stands around a call.  None of the ops is differentiable; what they
+# return has no history.
+
+
 def _caches(k_cache: torch.Tensor, v_cache: torch.Tensor, what: str) -> tuple[int, int, int, int]:
-    shape = kv4_shape(k_cache)
-    if v_cache.shape != k_cache.shape or v_cache.dtype != torch.uint8:
-        raise ValueError(f"{what}: K and V caches must have one shape, got {tuple(k_cache.shape)} and "
+    shape = k_cache.shape
+    if len(shape) != 4 or k_cache.dtype is not torch.uint8 or shape[3] < 8:
+        kv4_shape(k_cache)
+    if v_cache.shape != shape or v_cache.dtype is not torch.uint8:
+        raise ValueError(f"{what}: K and V caches must have one shape, got {tuple(shape)} and "
                          f"{v_cache.dtype} {tuple(v_cache.shape)}")
-    if not (k_cache.is_cuda and v_cache.device == k_cache.device):
+    if not k_cache.is_cuda or v_cache.device != k_cache.device:
         raise ValueError(f"{what} needs GPU tensors on one device (the HIP path has no CPU fallback)")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError(f"{what}: caches must be contiguous")
-    return shape
+    return shape[0], shape[1], shape[2], 2 * (shape[3] - 4)
+
+
+def _indices(t: torch.Tensor, name: str, device: torch.device) -> torch.Tensor:
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if t.dtype is not torch.int64 and t.dtype is not torch.int32:
+        t = t.to(torch.int64)
+    return t
+
+
+def _vector(t: torch.Tensor, name: str, least: int, device: torch.device) -> torch.Tensor:
+    t = _indices(t, name, device)
+    if t.dim() != 1 or t.shape[0] < least:
+        raise ValueError(f"{name} must hold at least {least} entries, got {tuple(t.shape)}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _slots(slot_mapping: torch.Tensor, tokens: int, device: torch.device) -> torch.Tensor:
     if slot_mapping.dim() != 1 or slot_mapping.shape[0] != tokens:
         raise ValueError(f"slot_mapping must hold {tokens} slots, got {tuple(slot_mapping.shape)}")
-    return _index(slot_mapping, "slot_mapping", device).contiguous()
+    return _vector(slot_mapping, "slot_mapping", tokens, device)
 
 
-def _rows(x: torch.Tensor, shape: tuple, dtype: torch.dtype, device: torch.device, name: str) -> torch.Tensor:
-    if tuple(x.shape) != shape:
+def _rows(x: torch.Tensor, shape: tuple, dtype: torch.dtype, device: torch.device, name: str):
+    """(x with a unit stride in its last dimension, its strides)."""
+    if x.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {tuple(x.shape)}")
-    if x.dtype != dtype:
+    if x.dtype is not dtype:
         raise TypeError(f"{name} is {x.dtype}, expected {dtype}")
     if x.device != device:
         raise ValueError(f"{name} is on {x.device}, expected {device}")
-    return x if x.stride(-1) == 1 else x.contiguous()
-
-
-def _on(device: torch.device):
-    """A launch goes to the tensors' device whichever is current."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+    stride = x.stride()
+    if stride[-1] != 1:
+        x = x.contiguous()
+        stride = x.stride()
+    return x, stride
 
 
 def _model_dtype(dtype: torch.dtype, what: str) -> int:
@@ -87,31 +106,26 @@ def _model_dtype(dtype: torch.dtype, what: str) -> int:
     return code
 
 
-@torch.inference_mode()
 def reshape_and_cache_int4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                            slot_mapping: torch.Tensor) -> None:
     """Quantise the rows of key and value ([T, Hkv, D], any token and head
     strides) into their slots.  Slots outside the cache (e.g. -1 padding) are
     skipped; the others must differ."""
-    lib = _lib.load()
-    num_blocks, heads, block_size, head_dim = _caches(k_cache, v_cache, "reshape_and_cache_int4")
-    code = _model_dtype(key.dtype, "reshape_and_cache_int4")
-    device = k_cache.device
+    what = "reshape_and_cache_int4"
+    num_blocks, heads, block_size, head_dim = _caches(k_cache, v_cache, what)
+    dtype, device = key.dtype, k_cache.device
+    code = _model_dtype(dtype, what)
     T = key.shape[0] if key.dim() else 0
-    key = _rows(key, (T, heads, head_dim), key.dtype, device, "key")
-    value = _rows(value, (T, heads, head_dim), key.dtype, device, "value")
+    key, ks = _rows(key, (T, heads, head_dim), dtype, device, "key")
+    value, vs = _rows(value, (T, heads, head_dim), dtype, device, "value")
     slots = _slots(slot_mapping, T, device)
     if T == 0:
         return
-    with _on(device):
-        rc = lib.ns_reshape_and_cache_int4(
-            key.data_ptr(), value.data_ptr(), key.stride(0), key.stride(1), value.stride(0), value.stride(1),
-            k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(), int(slots.dtype == torch.int64),
-            T, heads, head_dim, block_size, num_blocks, code, torch.cuda.current_stream(device).cuda_stream)
-    _lib.check(rc, "ns_reshape_and_cache_int4")
+    _lib.launch(device, what, _lib.load().ns_reshape_and_cache_int4,
+                key.data_ptr(), value.data_ptr(), ks[0], ks[1], vs[0], vs[1], k_cache.data_ptr(), v_cache.data_ptr(),
+                slots.data_ptr(), slots.dtype is torch.int64, T, heads, head_dim, block_size, num_blocks, code)
 
 
-@torch.inference_mode()
 def rope_reshape_and_cache_int4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                                 cos: torch.Tensor, sin: torch.Tensor,
                                 k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -123,132 +137,121 @@ def rope_reshape_and_cache_int4(q: torch.Tensor, k: torch.Tensor, v: torch.Tenso
     cos, sin: [T, 1, D] or [T, D] in q's dtype.  The rotation is evaluated in
     float32 and rounded once (q) or not at all before the codes are taken (k);
     rope_reshape_and_cache rounds after every product and sum instead."""
-    lib = _lib.load()
-    num_blocks, heads, block_size, head_dim = _caches(k_cache, v_cache, "rope_reshape_and_cache_int4")
-    code = _model_dtype(q.dtype, "rope_reshape_and_cache_int4")
-    device = k_cache.device
+    what = "rope_reshape_and_cache_int4"
+    num_blocks, heads, block_size, head_dim = _caches(k_cache, v_cache, what)
+    dtype, device = q.dtype, k_cache.device
+    code = _model_dtype(dtype, what)
     if q.dim() != 3:
         raise ValueError(f"q must be [T, Hq, {head_dim}], got {tuple(q.shape)}")
-    T, Hq = q.shape[0], q.shape[1]
-    q = _rows(q, (T, Hq, head_dim), q.dtype, device, "q")
-    k = _rows(k, (T, heads, head_dim), q.dtype, device, "k")
-    v = _rows(v, (T, heads, head_dim), q.dtype, device, "v")
-    if cos.dim() == 3 and cos.shape[1] == 1:
-        cos = cos[:, 0]
-    if sin.dim() == 3 and sin.shape[1] == 1:
-        sin = sin[:, 0]
-    cos = _rows(cos, (T, head_dim), q.dtype, device, "cos")
-    sin = _rows(sin, (T, head_dim), q.dtype, device, "sin")
-    if cos.stride(0) != sin.stride(0):
+    T, Hq, _ = q.shape
+    q, qs = _rows(q, (T, Hq, head_dim), dtype, device, "q")
+    k, ks = _rows(k, (T, heads, head_dim), dtype, device, "k")
+    v, vs = _rows(v, (T, heads, head_dim), dtype, device, "v")
+    tables = (T, head_dim), (T, 1, head_dim)
+    cos, cs = _rows(cos, tables[cos.dim() == 3], dtype, device, "cos")
+    sin, ss = _rows(sin, tables[sin.dim() == 3], dtype, device, "sin")
+    if cs[0] != ss[0]:
         cos, sin = cos.contiguous(), sin.contiguous()
+        cs = cos.stride()
     slots = _slots(slot_mapping, T, device)
     if out is None:
-        out = torch.empty((T, Hq, head_dim), dtype=q.dtype, device=device)
-    elif out.shape != (T, Hq, head_dim) or out.dtype != q.dtype or out.device != device or not out.is_contiguous():
-        raise ValueError(f"out must be a contiguous [{T}, {Hq}, {head_dim}] {q.dtype} tensor on {device}")
+        out = torch.empty((T, Hq, head_dim), dtype=dtype, device=device)
+    elif out.shape != (T, Hq, head_dim) or out.dtype != dtype or out.device != device or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous [{T}, {Hq}, {head_dim}] {dtype} tensor on {device}")
     elif out.data_ptr() == q.data_ptr() and not q.is_contiguous():
         raise ValueError("out may alias q only when q is contiguous")
     if T == 0 or Hq == 0:
         return out
-    with _on(device):
-        rc = lib.ns_rope_reshape_and_cache_int4(
-            out.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-            v.data_ptr(), v.stride(0), v.stride(1), cos.data_ptr(), sin.data_ptr(), cos.stride(0),
-            k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(), int(slots.dtype == torch.int64),
-            T, Hq, heads, head_dim, block_size, num_blocks, code, torch.cuda.current_stream(device).cuda_stream)
-    _lib.check(rc, "ns_rope_reshape_and_cache_int4")
+    _lib.launch(device, what, _lib.load().ns_rope_reshape_and_cache_int4,
+                out.data_ptr(), q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+                cos.data_ptr(), sin.data_ptr(), cs[0], k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(),
+                slots.dtype is torch.int64, T, Hq, heads, head_dim, block_size, num_blocks, code)
     return out
 
 
-@torch.inference_mode()
 def gather_cache_int4(k_cache: torch.Tensor, v_cache: torch.Tensor, slot_mapping: torch.Tensor,
                       dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
     """The values stored in the given slots, (K, V) as [T, Hkv, D] tensors of
     `dtype`, the dtype the cache was written in; zero rows for slots outside
     the cache.  For moving a cached prefix, and for looking at a cache."""
-    lib = _lib.load()
-    num_blocks, heads, block_size, head_dim = _caches(k_cache, v_cache, "gather_cache_int4")
-    code = _model_dtype(dtype, "gather_cache_int4")
+    what = "gather_cache_int4"
+    num_blocks, heads, block_size, head_dim = _caches(k_cache, v_cache, what)
+    code = _model_dtype(dtype, what)
     device = k_cache.device
     T = slot_mapping.shape[0] if slot_mapping.dim() else 0
     slots = _slots(slot_mapping, T, device)
-    k, v = (torch.empty((T, heads, head_dim), dtype=dtype, device=device) for _ in range(2))
+    k, v = torch.empty((2, T, heads, head_dim), dtype=dtype, device=device).unbind()
     if T:
-        with _on(device):
-            rc = lib.ns_gather_cache_int4(
-                k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(),
-                int(slots.dtype == torch.int64), T, heads, head_dim, block_size, num_blocks, code,
-                torch.cuda.current_stream(device).cuda_stream)
-        _lib.check(rc, "ns_gather_cache_int4")
+        _lib.launch(device, what, _lib.load().ns_gather_cache_int4,
+                    k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(),
+                    slots.dtype is torch.int64, T, heads, head_dim, block_size, num_blocks, code)
     return k, v
 
 
-@torch.inference_mode()
 def paged_attention_int4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                          md: AttentionMetadata, scale: float) -> torch.Tensor:
     """Paged attention over a cache held in 4 bits: attn_fn's contract
     (attention.paged_attention_hip) with the caches of Int4PagedKVCache, in the
     dtype they were written in.  Returns [num_tokens, num_heads, head_dim]."""
-    lib = _lib.load()
-    num_blocks, heads, block_size, head_dim = _caches(k_cache, v_cache, "paged_attention_int4")
-    code = _model_dtype(query.dtype, "paged_attention_int4")
+    what = "paged_attention_int4"
+    num_blocks, heads, block_size, head_dim = _caches(k_cache, v_cache, what)
+    code = _model_dtype(query.dtype, what)
     device = k_cache.device
-    if query.dim() != 3 or query.shape[2] != head_dim:
-        raise ValueError(f"query must be [T, Hq, {head_dim}], got {tuple(query.shape)}")
+    shape = query.shape
+    if len(shape) != 3 or shape[2] != head_dim:
+        raise ValueError(f"query must be [T, Hq, {head_dim}], got {tuple(shape)}")
     if query.device != device:
         raise ValueError(f"query is on {query.device}, expected {device}")
-    T, Hq, _ = query.shape
+    T, Hq, _ = shape
+    n, longest = md.num_seqs, md.max_seq_len
     if md.num_tokens != T:
         raise ValueError(f"metadata has {md.num_tokens} tokens, query has {T}")
     if Hq % heads:
         raise ValueError(f"{Hq} query heads over {heads} KV heads")
-    q = query.contiguous()
-    if T == 0 or md.num_seqs == 0:
+    q = query if query.is_contiguous() else query.contiguous()
+    if T == 0 or n == 0:
         return torch.zeros_like(q)
-    bt = _index(md.block_tables, "block_tables", device)
-    if bt.dim() != 2 or bt.shape[0] < md.num_seqs:
+    bt = _indices(md.block_tables, "block_tables", device)
+    if bt.dim() != 2 or bt.shape[0] < n:
         raise ValueError(f"block_tables must be [num_seqs, max_blocks], got {tuple(bt.shape)}")
-    if bt.shape[1] * block_size < md.max_seq_len:
-        raise ValueError(f"block_tables has {bt.shape[1]} columns but max_seq_len={md.max_seq_len} needs "
-                         f"{-(-md.max_seq_len // block_size)}")
-    if bt.stride(1) != 1:
+    width = bt.shape[1]
+    if width * block_size < longest:
+        raise ValueError(f"block_tables has {width} columns but max_seq_len={longest} needs {-(-longest // block_size)}")
+    bs = bt.stride()
+    if bs[1] != 1 or bs[0] < width:
         bt = bt.contiguous()
-    sl = _index(md.seq_lens, "seq_lens", device).contiguous()
-    if sl.shape[0] < md.num_seqs:
-        raise ValueError("seq_lens is shorter than num_seqs")
-    decode_only = int(bool(md.is_decode_only))
+        bs = bt.stride()
+    sl = _vector(md.seq_lens, "seq_lens", n, device)
+    decode_only = bool(md.is_decode_only)
     qsl_ptr, qsl64 = None, 0
     if decode_only:
-        if T != md.num_seqs:
+        if T != n:
             raise ValueError("is_decode_only needs one query token per sequence")
         out = torch.empty_like(q)
     else:
-        qsl = _index(md.query_start_loc, "query_start_loc", device).contiguous()
-        if qsl.shape[0] < md.num_seqs + 1:
-            raise ValueError("query_start_loc is shorter than num_seqs + 1")
-        qsl_ptr, qsl64 = qsl.data_ptr(), int(qsl.dtype == torch.int64)
+        qsl = _vector(md.query_start_loc, "query_start_loc", n + 1, device)
+        qsl_ptr, qsl64 = qsl.data_ptr(), qsl.dtype is torch.int64
         # Rows behind the last sequence are not written: zero unless the host
         # offsets show that there are none.
         host = md.query_start_loc_cpu
-        full = host is not None and len(host) > md.num_seqs and host[0] == 0 and host[md.num_seqs] == T
+        full = host is not None and len(host) > n and host[0] == 0 and host[n] == T
         out = torch.empty_like(q) if full else torch.zeros_like(q)
     # The context lengths' sum and the number of decode rows, where the host
-    # has them, shape the launches.  The partial results live in a tensor of this call's: captured graphs hold
-    # their own, and calls on different streams share nothing.
-    context = 0 if md.seq_lens_cpu is None else sum(md.seq_lens_cpu[:md.num_seqs])
-    ones = -1 if md.query_lens_cpu is None else md.query_lens_cpu[:md.num_seqs].count(1)
-    nbytes = lib.ns_paged_attention_int4_workspace_size(md.num_seqs, Hq, heads, head_dim, block_size, md.max_seq_len,
-                                                        T, decode_only, context, ones)
+    # has them, shape the launches.  The partial results live in a tensor of
+    # this call's: captured graphs hold their own, and calls on different
+    # streams share nothing.
+    lens, rows = md.seq_lens_cpu, md.query_lens_cpu
+    context = 0 if lens is None else sum(lens if len(lens) == n else lens[:n])
+    ones = n if decode_only else -1 if rows is None else rows[:n].count(1)
+    lib = _lib.load()
+    nbytes = lib.ns_paged_attention_int4_workspace_size(n, Hq, heads, head_dim, block_size, longest, T, decode_only,
+                                                        context, ones)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    with _on(device):
-        rc = lib.ns_paged_attention_int4(
-            out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-            bt.data_ptr(), bt.stride(0), bt.shape[1], int(bt.dtype == torch.int64),
-            sl.data_ptr(), int(sl.dtype == torch.int64), qsl_ptr, qsl64,
-            md.num_seqs, T, md.max_seq_len, decode_only, context, ones,
-            Hq, heads, head_dim, block_size, num_blocks, float(scale), code,
-            None if ws is None else ws.data_ptr(), nbytes, torch.cuda.current_stream(device).cuda_stream)
-    _lib.check(rc, "ns_paged_attention_int4")
+    _lib.launch(device, what, lib.ns_paged_attention_int4,
+                out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                bt.data_ptr(), bs[0], width, bt.dtype is torch.int64, sl.data_ptr(), sl.dtype is torch.int64,
+                qsl_ptr, qsl64, n, T, longest, decode_only, context, ones, Hq, heads, head_dim, block_size, num_blocks,
+                float(scale), code, None if ws is None else ws.data_ptr(), nbytes)
     return out
 
 

@@ -14,7 +14,6 @@ import numpy as np
 import torch
 
 from . import _lib
-from .kv4 import _on
 
 # One slice-key workspace per (device, stream), grown on demand; graph capture
 # records its pointer, so it is allocated by the warm-up call before capture.
@@ -85,7 +84,6 @@ def _per_row(x, rows: int, dtypes: tuple, device: torch.device, name: str) -> to
     return x.contiguous()
 
 
-@torch.inference_mode()
 def sample_rows(logits: torch.Tensor, uniform: torch.Tensor, temperature, top_k=None, top_p=None, min_p=None,
                 out: torch.Tensor | None = None) -> torch.Tensor:
     """[M, N] logits (f32/f16/bf16) and [M] float32 uniform numbers in [0, 1) -> [M] int64 tokens.
@@ -131,11 +129,10 @@ def sample_rows(logits: torch.Tensor, uniform: torch.Tensor, temperature, top_k=
     nbytes = lib.ns_sample_rows_workspace_size(M, N)
     ws = torch.empty(max(nbytes, 8), dtype=torch.uint8, device=device)  # this call's own
     ptr = lambda a: None if a is None else a.data_ptr()  # noqa: E731
-    with _on(device):
-        rc = lib.ns_sample_rows(out.data_ptr(), x.data_ptr(), max(x.stride(0), N), M, N, _lib.DTYPE_CODES[x.dtype],
-                                u.data_ptr(), t.data_ptr(), ptr(k), int(k is not None and k.dtype == torch.int64),
-                                ptr(p), ptr(mp), ws.data_ptr(), nbytes, torch.cuda.current_stream(device).cuda_stream)
-    _lib.check(rc, "ns_sample_rows")
+    _lib.launch(device, "sample_rows", lib.ns_sample_rows,
+                out.data_ptr(), x.data_ptr(), max(x.stride(0), N), M, N, _lib.DTYPE_CODES[x.dtype],
+                u.data_ptr(), t.data_ptr(), ptr(k), k is not None and k.dtype is torch.int64, ptr(p), ptr(mp),
+                ws.data_ptr(), nbytes)
     return out
 
 
