@@ -96,7 +96,6 @@ __device__ __forceinline__ void each_element(const char* row, int64_t s0, int64_
   v0 = v0 < s1 ? v0 : s1;
   const int64_t vecs = (s1 - v0) / VEC;
   const int tid = threadIdx.x;
-  if (tid < v0 - s0) f(elem_f32<DT>(row, s0 + tid), static_cast<uint32_t>(s0 + tid));
   const u32x4* v = reinterpret_cast<const u32x4*>(row + v0 * ESZ);
   int64_t j = tid;
   // Four loads in flight.
@@ -115,8 +114,11 @@ __device__ __forceinline__ void each_element(const char* row, int64_t s0, int64_
 #pragma unroll
     for (int e = 0; e < VEC; ++e) f(vec_elem_f32<DT>(w, e), static_cast<uint32_t>(v0 + j * VEC + e));
   }
-  const int64_t t0 = v0 + vecs * VEC;
-  if (tid < s1 - t0) f(elem_f32<DT>(row, t0 + tid), static_cast<uint32_t>(t0 + tid));
+  const int64_t head = v0 - s0, t0 = v0 + vecs * VEC;
+  if (tid < head + (s1 - t0)) {
+    const int64_t i = tid < head ? s0 + tid : t0 + (tid - head);
+    f(elem_f32<DT>(row, i), static_cast<uint32_t>(i));
+  }
 }
 
 // A row's constants.
@@ -346,16 +348,21 @@ __device__ __forceinline__ void scan(ScanScratch& s, uint32_t& c, uint64_t& w) {
   __syncthreads();
 }
 
-// The first i in [0, n) with cum[i] >= goal; cum ascends and cum[n - 1] >= goal.
+// The first i in [0, n) with cum[i] >= goal; cum ascends, cum[n - 1] >= goal and
+// n <= 4096.  A wave looks at 64 places at a time: two reads deep, where a
+// bisection of 4096 would be twelve.
 template <class T>
 __device__ __forceinline__ int first_reaching(const T* cum, int n, uint64_t goal) {
-  int lo = 0, hi = n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (cum[mid] >= goal) hi = mid;
-    else lo = mid + 1;
-  }
-  return lo;
+  const int lane = threadIdx.x & 63;
+  const int step = (n + 63) >> 6;
+  int at = (lane + 1) * step - 1;
+  at = at < n ? at : n - 1;
+  uint64_t hit = __builtin_amdgcn_ballot_w64(cum[at] >= goal);
+  const int from = hit ? __builtin_ctzll(hit) * step : n - 1;
+  at = from + lane < n ? from + lane : n - 1;
+  hit = __builtin_amdgcn_ballot_w64(lane < step && cum[at] >= goal);
+  at = from + (hit ? __builtin_ctzll(hit) : 0);
+  return at < n ? at : n - 1;
 }
 
 // A prefix of the row's order.
@@ -393,15 +400,9 @@ __global__ __launch_bounds__(kRowThreads) void sample_plan_kernel(SampleParams p
   __shared__ ScanScratch scratch;
   const int tid = threadIdx.x;
   const int64_t r = blockIdx.x;
-  const Ends ends = row_ends(p, r);
-  if (takes_largest(ends.top, p.temperature[r])) {
-    if (tid == 0) {
-      p.out[r] = index_of(ends.top);
-      p.plan[r].mode = kDone;
-    }
-    return;
-  }
   static_assert(kBins == kRowThreads, "one bin per thread");
+  // Everything that is read, at once: each of these is a round trip past this
+  // XCD's cache.  (A greedy row has no histograms; its sums go nowhere.)
   uint32_t c = 0;
   uint64_t w = 0;
 #pragma unroll 8
@@ -409,6 +410,17 @@ __global__ __launch_bounds__(kRowThreads) void sample_plan_kernel(SampleParams p
     const int64_t at = (r * p.slices + i) * kBins + tid;
     c += p.hist_c[at];
     w += p.hist_w[at];
+  }
+  const float u = p.u[r], temperature = p.temperature[r], tp = top_p_of(p, r);
+  const int64_t k = top_k_of(p, r);
+  const bool has_min = p.min_p && p.min_p[r] > 0.f;
+  const Ends ends = row_ends(p, r);
+  if (takes_largest(ends.top, temperature)) {
+    if (tid == 0) {
+      p.out[r] = index_of(ends.top);
+      p.plan[r].mode = kDone;
+    }
+    return;
   }
   scan(scratch, c, w);
   cum_c[tid + 1] = c;
@@ -423,7 +435,6 @@ __global__ __launch_bounds__(kRowThreads) void sample_plan_kernel(SampleParams p
   if (tid >= 64) return;  // the rest is one thread's work, which a wave does alike
 
   Prefix least = {0, 0};
-  const bool has_min = p.min_p && p.min_p[r] > 0.f;
   if (has_min) {
     for (int i = tid; i < p.slices; i += 64) {
       least.count += p.min_c[r * p.slices + i];
@@ -443,7 +454,6 @@ __global__ __launch_bounds__(kRowThreads) void sample_plan_kernel(SampleParams p
   auto bin_w = [&](uint64_t goal) { return first_reaching(cum_w + 1, kBins, goal < all ? goal : all); };
   uint64_t lo_w = all, hi_w = all;
   int lo[3] = {1, 1, 1}, hi[3] = {0, 0, 0};
-  const int64_t k = top_k_of(p, r);
   if (k > 0) {
     const int b = first_reaching(cum_c + 1, kBins, static_cast<uint64_t>(k));
     hi_w = lo_w = cum_w[b + 1];
@@ -452,7 +462,6 @@ __global__ __launch_bounds__(kRowThreads) void sample_plan_kernel(SampleParams p
       lo_w = cum_w[b] > one ? cum_w[b] : one;
     }
   }
-  const float tp = top_p_of(p, r);
   if (tp < 1.f) {
     lo[1] = bin_w(top_p_goal(tp, lo_w));
     hi[1] = bin_w(top_p_goal(tp, hi_w));
@@ -463,8 +472,8 @@ __global__ __launch_bounds__(kRowThreads) void sample_plan_kernel(SampleParams p
   lo_w = least.weight < lo_w ? least.weight : lo_w;
   hi_w = least.weight < hi_w ? least.weight : hi_w;
   if (least.count > 0) {
-    lo[2] = bin_w(draw_goal(p.u[r], lo_w));
-    hi[2] = bin_w(draw_goal(p.u[r], hi_w));
+    lo[2] = bin_w(draw_goal(u, lo_w));
+    hi[2] = bin_w(draw_goal(u, hi_w));
   }
   // Overlapping ranges become one.
   auto join = [&](int a, int b) {
@@ -536,19 +545,54 @@ __global__ __launch_bounds__(kSliceThreads) void sample_collect_kernel(SamplePar
     if (base + i < static_cast<uint32_t>(p.list_cap)) list[base + i] = local[i];
 }
 
-// Sorts the first `size` (a power of two) of list, ascending: a bitonic network.
-__device__ __forceinline__ void sort_list(uint64_t* list, uint32_t size) {
+// Sorts E elements per thread (element e of thread t is number t * E + e),
+// ascending, by a bitonic network over the first `size` (a power of two, a
+// multiple of E; the others stay apart).  Partners within a thread are compared
+// in place, within a wave by a lane exchange, further ones through `swap`; only
+// the latter need the workgroup to wait.
+template <int E>
+__device__ __forceinline__ void sort_registers(uint64_t (&v)[E], uint64_t* swap, uint32_t size) {
+  const uint32_t tid = threadIdx.x;
+  // Waves without any of the elements only wait with the others.
+  const bool here = __builtin_amdgcn_readfirstlane(tid) * E < size;
   for (uint32_t k = 2; k <= size; k <<= 1) {
     for (uint32_t j = k >> 1; j > 0; j >>= 1) {
-      for (uint32_t q = threadIdx.x; q < size / 2; q += kRowThreads) {
-        const uint32_t a = 2 * q - (q & (j - 1)), b = a + j;  // q with a zero put in at j's bit
-        const uint64_t x = list[a], y = list[b];
-        if ((x > y) == ((a & k) == 0)) {
-          list[a] = y;
-          list[b] = x;
+      if (j < E) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+#pragma unroll
+          for (int bit = 1; bit < E; bit <<= 1) {
+            if (j == static_cast<uint32_t>(bit) && (e & bit) == 0) {
+              const bool up = ((tid * E + e) & k) == 0;
+              const uint64_t x = v[e], y = v[e + bit];
+              if ((x > y) == up) {
+                v[e] = y;
+                v[e + bit] = x;
+              }
+            }
+          }
         }
+        continue;
       }
-      __syncthreads();
+      const uint32_t lanes = j / E;
+      uint64_t other[E];
+      if (lanes < 64) {
+        if (!here) continue;
+#pragma unroll
+        for (int e = 0; e < E; ++e) other[e] = __shfl_xor(v[e], static_cast<int>(lanes));
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) swap[e * kRowThreads + tid] = v[e];
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < E; ++e) other[e] = swap[e * kRowThreads + (tid ^ lanes)];
+        __syncthreads();
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const bool up = ((tid * E + e) & k) == 0, lower = (tid & lanes) == 0;
+        v[e] = (up == lower) == (other[e] < v[e]) ? other[e] : v[e];
+      }
     }
   }
 }
@@ -558,7 +602,7 @@ struct Pick {
   uint64_t cum_w[kBins + 1];
   uint32_t cum_c[kBins + 1];
   uint64_t list[kList];
-  uint64_t run[kList];       // running weights of the sorted list
+  uint64_t run[kList];       // running weights of the sorted list (before: the sort's exchange)
   ScanScratch scratch;
   uint64_t sub_w[kSub];      // the long way's
   uint32_t sub_c[kSub];
@@ -604,15 +648,16 @@ __device__ __forceinline__ End end_in_list(const Pick& s, const Plan& plan, uint
 }
 
 // The shortest prefix of the row's order with at least `goal` elements
-// (BY_COUNT) or weight; the row has that much, and goal > 0.
-template <int DT, bool BY_COUNT>
-__device__ __noinline__ End end_by_passes(const SampleParams& p, Pick& s, const Row& row, const char* x, uint64_t goal) {
+// (by_count) or weight; the row has that much, and goal > 0.
+template <int DT>
+__device__ __forceinline__ End end_by_passes(const SampleParams& p, Pick& s, const Row& row, const char* x,
+                                             bool by_count, uint64_t goal) {
   const int tid = threadIdx.x;
   if (tid == 0) s.found = kBins - 1;
   __syncthreads();
   {
-    const uint64_t before = BY_COUNT ? s.cum_c[tid] : s.cum_w[tid];
-    const uint64_t upto = BY_COUNT ? s.cum_c[tid + 1] : s.cum_w[tid + 1];
+    const uint64_t before = by_count ? s.cum_c[tid] : s.cum_w[tid];
+    const uint64_t upto = by_count ? s.cum_c[tid + 1] : s.cum_w[tid + 1];
     if (before < goal && goal <= upto) s.found = tid;
   }
   __syncthreads();
@@ -670,7 +715,7 @@ __device__ __noinline__ End end_by_passes(const SampleParams& p, Pick& s, const 
       const uint32_t own_c = c;
       const uint64_t own_w = w;
       scan(s.scratch, c, w);
-      const uint64_t upto = BY_COUNT ? base_c + c : base_w + w, mine = BY_COUNT ? own_c : own_w;
+      const uint64_t upto = by_count ? base_c + c : base_w + w, mine = by_count ? own_c : own_w;
       if (tid < kSub && upto - mine < goal && goal <= upto) {
         s.found = tid;
         s.n = own_c;
@@ -696,7 +741,7 @@ __device__ __noinline__ End end_by_passes(const SampleParams& p, Pick& s, const 
   }
   uint32_t size = 1;
   while (size < n) size <<= 1;
-  if (tid < size) s.list[tid] = ~0ull;
+  s.list[tid] = ~0ull;
   __syncthreads();
   each_element<DT, kRowThreads>(x, 0, p.n, [&](float z, uint32_t i) {
     if (by_bin && bin_of(row, z) != bin) return;
@@ -706,14 +751,16 @@ __device__ __noinline__ End end_by_passes(const SampleParams& p, Pick& s, const 
     if (at < kSort) s.list[at] = k;
   });
   __syncthreads();
-  sort_list(s.list, size);
-  const uint64_t key = tid < static_cast<int>(n) ? s.list[tid] : 0;
+  uint64_t place[1] = {s.list[tid]};
+  __syncthreads();
+  sort_registers(place, s.run, size);
+  const uint64_t key = tid < static_cast<int>(n) ? place[0] : 0;
   uint32_t c = tid < static_cast<int>(n) ? 1 : 0;
   uint64_t w = c ? weight_of(row, value_of(~static_cast<uint32_t>(key >> 32))) : 0;
   const uint64_t own_w = w;
   scan(s.scratch, c, w);
   if (tid < static_cast<int>(n)) {
-    const uint64_t upto = BY_COUNT ? base_c + c : base_w + w, mine = BY_COUNT ? 1 : own_w;
+    const uint64_t upto = by_count ? base_c + c : base_w + w, mine = by_count ? 1 : own_w;
     if (upto - mine < goal && goal <= upto) {
       s.found = tid;
       s.lo = base_w + w;
@@ -729,64 +776,91 @@ __device__ __noinline__ End end_by_passes(const SampleParams& p, Pick& s, const 
   return e;
 }
 
-template <int DT>
-__global__ __launch_bounds__(kRowThreads) void sample_pick_kernel(SampleParams p) {
-  __shared__ Pick s;
-  const int tid = threadIdx.x;
-  const int64_t r = blockIdx.x;
-  const Plan plan = p.plan[r];
-  if (plan.mode == kDone) return;
-  const Row row = row_of(p, row_ends(p, r), p.temperature[r]);
-  s.cum_c[tid + 1] = p.cum_c[r * (kBins + 1) + tid + 1];
-  s.cum_w[tid + 1] = p.cum_w[r * (kBins + 1) + tid + 1];
-  if (tid == 0) {
-    s.cum_c[0] = 0;
-    s.cum_w[0] = 0;
+// list's n keys into s.list, ascending, and the running sums of their weights
+// into s.run.  early: the thread's one of the first kRowThreads.
+template <int E>
+__device__ __forceinline__ void sort_and_sum(Pick& s, const Row& row, const uint64_t* list, uint64_t early,
+                                             uint32_t n) {
+  const uint32_t first = threadIdx.x * E;
+  uint64_t v[E], sum[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    // Which thread starts with which key does not matter.
+    const uint32_t i = e * kRowThreads + threadIdx.x;
+    v[e] = i >= n ? ~0ull : e == 0 ? early : list[i];
   }
-  const int64_t k = top_k_of(p, r);
-  const float tp = top_p_of(p, r);
-  const Prefix least = {p.kept_c[r], p.kept_w[r]};  // the min-p prefix
-  if (plan.mode == kLong) {
-    __syncthreads();
-    const char* x = p.x + r * p.row_bytes;
-    Prefix kept = least;
-    Prefix first = {static_cast<uint32_t>(p.n), s.cum_w[kBins]};
-    if (k > 0) {
-      const End e = end_by_passes<DT, true>(p, s, row, x, static_cast<uint64_t>(k));
-      first = Prefix{e.count, e.weight};
-    }
-    if (first.count < kept.count) kept = first;
-    if (tp < 1.f) {
-      const End e = end_by_passes<DT, false>(p, s, row, x, top_p_goal(tp, first.weight));
-      if (e.count < kept.count) kept = Prefix{e.count, e.weight};
-    }
-    const End e = end_by_passes<DT, false>(p, s, row, x, draw_goal(p.u[r], kept.weight));
-    if (tid == 0) p.out[r] = e.index;
-    return;
-  }
-
-  // The collected elements: sorted, and their weights' running sums.
-  const uint32_t n = p.list_n[r] < static_cast<uint32_t>(p.list_cap) ? p.list_n[r] : p.list_cap;
-  uint32_t size = 1;
+  uint32_t size = E;
   while (size < n) size <<= 1;
-  for (uint32_t i = tid; i < size; i += kRowThreads) s.list[i] = i < n ? p.list[r * p.list_cap + i] : ~0ull;
-  __syncthreads();
-  sort_list(s.list, size);
-  const uint32_t each = size > kRowThreads ? size / kRowThreads : 1;
-  uint64_t own[kList / kRowThreads];
+  if (E > 1) size = E * kRowThreads;  // the keys start in all threads
+  sort_registers(v, s.run, size);
   uint64_t w = 0;
 #pragma unroll
-  for (uint32_t e = 0; e < kList / kRowThreads; ++e) {
-    const uint32_t i = tid * each + e;
-    if (e < each && i < n) w += weight_of(row, value_of(~static_cast<uint32_t>(s.list[i] >> 32)));
-    own[e] = w;
+  for (int e = 0; e < E; ++e) {
+    if (first + e < n) w += weight_of(row, value_of(~static_cast<uint32_t>(v[e] >> 32)));
+    sum[e] = w;
   }
   uint32_t none = 0;
   const uint64_t mine = w;
   scan(s.scratch, none, w);
 #pragma unroll
-  for (uint32_t e = 0; e < kList / kRowThreads; ++e)
-    if (e < each && tid * each + e < n) s.run[tid * each + e] = w - mine + own[e];
+  for (int e = 0; e < E; ++e) {
+    if (first + e < n) {
+      s.list[first + e] = v[e];
+      s.run[first + e] = w - mine + sum[e];
+    }
+  }
+}
+
+template <int DT>
+__global__ __launch_bounds__(kRowThreads) void sample_pick_kernel(SampleParams p) {
+  __shared__ Pick s;
+  const int tid = threadIdx.x;
+  const int64_t r = blockIdx.x;
+  // Everything that is read, at once, the first collected keys among it.
+  const Plan plan = p.plan[r];
+  const uint32_t cc = p.cum_c[r * (kBins + 1) + tid + 1];
+  const uint64_t cw = p.cum_w[r * (kBins + 1) + tid + 1];
+  const uint64_t* list = p.list + r * p.list_cap;
+  const uint64_t early = tid < p.list_cap ? list[tid] : 0;
+  const uint32_t listed = p.list_n[r];
+  const float u = p.u[r], temperature = p.temperature[r], tp = top_p_of(p, r);
+  const int64_t k = top_k_of(p, r);
+  const Prefix least = {p.kept_c[r], p.kept_w[r]};  // the min-p prefix
+  const Ends ends = row_ends(p, r);
+  if (plan.mode == kDone) return;
+  const Row row = row_of(p, ends, temperature);
+  s.cum_c[tid + 1] = cc;
+  s.cum_w[tid + 1] = cw;
+  if (tid == 0) {
+    s.cum_c[0] = 0;
+    s.cum_w[0] = 0;
+  }
+  if (plan.mode == kLong) {
+    __syncthreads();
+    const char* x = p.x + r * p.row_bytes;
+    Prefix first = {static_cast<uint32_t>(p.n), s.cum_w[kBins]};
+    Prefix kept = least.count < first.count ? least : first;
+    // One inlined copy for the three ends: calls would give the kernel a stack,
+    // which costs every launch of it 11 us.
+#pragma unroll 1
+    for (int step = 0; step < 3; ++step) {
+      if ((step == 0 && k == 0) || (step == 1 && !(tp < 1.f))) continue;
+      const uint64_t goal = step == 0   ? static_cast<uint64_t>(k)
+                            : step == 1 ? top_p_goal(tp, first.weight)
+                                        : draw_goal(u, kept.weight);
+      const End e = end_by_passes<DT>(p, s, row, x, step == 0, goal);
+      if (step == 0) first = Prefix{e.count, e.weight};
+      if (step < 2 && e.count < kept.count) kept = Prefix{e.count, e.weight};
+      if (step == 2 && tid == 0) p.out[r] = e.index;
+    }
+    return;
+  }
+
+  // The collected elements: sorted, and their weights' running sums.
+  const uint32_t n = listed < static_cast<uint32_t>(p.list_cap) ? listed : p.list_cap;
+  if (n <= kRowThreads) sort_and_sum<1>(s, row, list, early, n);
+  else if (n <= 2 * kRowThreads) sort_and_sum<2>(s, row, list, early, n);
+  else sort_and_sum<4>(s, row, list, early, n);
   __syncthreads();
   if (tid >= 64) return;
   Prefix kept = least;
@@ -800,7 +874,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_pick_kernel(SampleParams p
     const End e = end_in_list<false>(s, plan, top_p_goal(tp, first.weight));
     if (e.count < kept.count) kept = Prefix{e.count, e.weight};
   }
-  const End e = end_in_list<false>(s, plan, draw_goal(p.u[r], kept.weight));
+  const End e = end_in_list<false>(s, plan, draw_goal(u, kept.weight));
   if (tid == 0) p.out[r] = e.index;
 }
 
@@ -813,9 +887,9 @@ struct Layout {
 
 Layout layout_of(int64_t M, int64_t N) {
   Layout l;
-  // About four workgroups for each compute unit, up to 32 slices of at least 2048 elements.
+  // About four workgroups for each compute unit, up to 16 slices of at least 2048 elements.
   int64_t slices = 1024 / M < 1 ? 1 : 1024 / M;
-  slices = slices > 32 ? 32 : slices;
+  slices = slices > 16 ? 16 : slices;
   const int64_t most = (N + 2047) / 2048;
   slices = slices > most ? most : slices;
   l.slice_elems = ((N + slices - 1) / slices + 7) / 8 * 8;
