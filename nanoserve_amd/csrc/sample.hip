@@ -130,31 +130,40 @@ struct Row {
   int shift;
 };
 
+// Taylor coefficients 1 / 2! .. 1 / 12!, held in scalar registers: as literals
+// each would take two moves in front of its multiply-add.
+struct Series {
+  double c[11];
+  __device__ __forceinline__ void load() {
+    constexpr double k[11] = {1.0 / 2,     1.0 / 6,      1.0 / 24,      1.0 / 120,      1.0 / 720,      1.0 / 5040,
+                              1.0 / 40320, 1.0 / 362880, 1.0 / 3628800, 1.0 / 39916800, 1.0 / 479001600};
+#pragma unroll
+    for (int i = 0; i < 11; ++i) {
+      c[i] = k[i];
+      asm volatile("" : "+s"(c[i]));
+    }
+  }
+};
+
 // exp((z - z_max) / T) * 2^shift as an integer.  exp(a) = 2^n exp(r) with
 // n = rint(a / ln 2), r = a - n ln 2 in [-0.347, 0.347], and exp(r) by its
-// Taylor series to r^12 / 12! (the rest is below 2^-52).
-__device__ __forceinline__ uint64_t weight_of(const Row& r, float z) {
+// Taylor series to r^12 / 12! (the rest is below 2^-52).  No branches, so that
+// the steps of several elements interleave.
+__device__ __forceinline__ uint64_t weight_of(const Row& r, const Series& t, float z) {
 #pragma clang fp contract(off)
   const double a = (static_cast<double>(z) - static_cast<double>(r.top)) * r.inv_t;
-  if (!(a > r.zero_below)) return 0;  // and a z of -inf whatever the temperature
   const double n = __builtin_rint(a * 1.4426950408889634);
   const double x = __builtin_fma(n, -0.6931471805599453, a);
-  double e = 1.0 / 479001600.0;
-  e = __builtin_fma(e, x, 1.0 / 39916800.0);
-  e = __builtin_fma(e, x, 1.0 / 3628800.0);
-  e = __builtin_fma(e, x, 1.0 / 362880.0);
-  e = __builtin_fma(e, x, 1.0 / 40320.0);
-  e = __builtin_fma(e, x, 1.0 / 5040.0);
-  e = __builtin_fma(e, x, 1.0 / 720.0);
-  e = __builtin_fma(e, x, 1.0 / 120.0);
-  e = __builtin_fma(e, x, 1.0 / 24.0);
-  e = __builtin_fma(e, x, 1.0 / 6.0);
-  e = __builtin_fma(e, x, 0.5);
+  double e = t.c[10];
+#pragma unroll
+  for (int i = 9; i >= 0; --i) e = __builtin_fma(e, x, t.c[i]);
   e = __builtin_fma(e, x, 1.0);
   e = __builtin_fma(e, x, 1.0);
   // Below 2^52 a sum with 2^52 holds the rounded integer in its mantissa.
   const double v = __builtin_ldexp(e, static_cast<int>(n) + r.shift) + 4503599627370496.0;
-  return __builtin_bit_cast(uint64_t, v) & 0xFFFFFFFFFFFFFull;
+  const uint64_t w = __builtin_bit_cast(uint64_t, v) & 0xFFFFFFFFFFFFFull;
+  // Far below, and for a z of -inf whatever the temperature: nothing.
+  return a > r.zero_below ? w : 0;
 }
 
 // Monotone in z: a larger z never has a larger bin.
@@ -259,16 +268,19 @@ __global__ __launch_bounds__(kSliceThreads) void sample_ends_kernel(SampleParams
 
 template <int DT>
 __global__ __launch_bounds__(kSliceThreads) void sample_hist_kernel(SampleParams p) {
-  __shared__ uint64_t hw[kBins];
-  __shared__ uint32_t hc[kBins];
+  // The last bin, which may hold most of a row, has a place for every lane:
+  // atomics on one address wait for each other.
+  __shared__ uint64_t hw[kBins + 64];
+  __shared__ uint32_t hc[kBins + 64];
   __shared__ uint64_t mw;
   __shared__ uint32_t mc;
   const int tid = threadIdx.x;
   const int64_t r = blockIdx.y;
   const Ends ends = row_ends(p, r);
   const float t = p.temperature[r];
+  const float mp = p.min_p ? p.min_p[r] : 0.f;
   if (takes_largest(ends.top, t)) return;
-  for (int b = tid; b < kBins; b += kSliceThreads) {
+  for (int b = tid; b < kBins + 64; b += kSliceThreads) {
     hw[b] = 0;
     hc[b] = 0;
   }
@@ -278,25 +290,23 @@ __global__ __launch_bounds__(kSliceThreads) void sample_hist_kernel(SampleParams
   }
   __syncthreads();
   const Row row = row_of(p, ends, t);
-  // The prefix of w >= min_p, as integers.
-  const float mp = p.min_p ? p.min_p[r] : 0.f;
-  const uint64_t enough =
-      mp < 4.f ? static_cast<uint64_t>(ceil(static_cast<double>(mp) * __builtin_ldexp(1.0, p.shift))) : ~0ull;
-  uint32_t tail_c = 0, min_c = 0;
-  uint64_t tail_w = 0, min_w = 0;
+  Series series;
+  series.load();
+  const int last = kBins - 1 + (tid & 63);
   auto count = [&](float z, uint64_t w) {
-    const int b = bin_of(row, z);
-    if (b == kBins - 1) {  // far below: most of many rows, so not by atomics
-      ++tail_c;
-      tail_w += w;
-    } else {
-      atomicAdd(&hc[b], 1u);
-      atomicAdd(reinterpret_cast<unsigned long long*>(&hw[b]), static_cast<unsigned long long>(w));
-    }
+    int b = bin_of(row, z);
+    b = b == kBins - 1 ? last : b;
+    atomicAdd(&hc[b], 1u);
+    atomicAdd(reinterpret_cast<unsigned long long*>(&hw[b]), static_cast<unsigned long long>(w));
   };
   if (mp > 0.f) {
+    // The prefix of w >= min_p, as integers.
+    const uint64_t enough =
+        mp < 4.f ? static_cast<uint64_t>(ceil(static_cast<double>(mp) * __builtin_ldexp(1.0, p.shift))) : ~0ull;
+    uint32_t min_c = 0;
+    uint64_t min_w = 0;
     each_of_slice<DT>(p, [&](float z, uint32_t) {
-      const uint64_t w = weight_of(row, z);
+      const uint64_t w = weight_of(row, series, z);
       min_c += w >= enough ? 1 : 0;
       min_w += w >= enough ? w : 0;
       count(z, w);
@@ -304,10 +314,13 @@ __global__ __launch_bounds__(kSliceThreads) void sample_hist_kernel(SampleParams
     atomicAdd(&mc, min_c);
     atomicAdd(reinterpret_cast<unsigned long long*>(&mw), static_cast<unsigned long long>(min_w));
   } else {
-    each_of_slice<DT>(p, [&](float z, uint32_t) { count(z, weight_of(row, z)); });
+    each_of_slice<DT>(p, [&](float z, uint32_t) { count(z, weight_of(row, series, z)); });
   }
-  atomicAdd(&hc[kBins - 1], tail_c);
-  atomicAdd(reinterpret_cast<unsigned long long*>(&hw[kBins - 1]), static_cast<unsigned long long>(tail_w));
+  __syncthreads();
+  if (tid > 0 && tid < 64) {
+    atomicAdd(&hc[kBins - 1], hc[last]);
+    atomicAdd(reinterpret_cast<unsigned long long*>(&hw[kBins - 1]), static_cast<unsigned long long>(hw[last]));
+  }
   __syncthreads();
   const int64_t at = r * p.slices + blockIdx.x;
   for (int b = tid; b < kBins; b += kSliceThreads) {
@@ -650,8 +663,8 @@ __device__ __forceinline__ End end_in_list(const Pick& s, const Plan& plan, uint
 // The shortest prefix of the row's order with at least `goal` elements
 // (by_count) or weight; the row has that much, and goal > 0.
 template <int DT>
-__device__ __forceinline__ End end_by_passes(const SampleParams& p, Pick& s, const Row& row, const char* x,
-                                             bool by_count, uint64_t goal) {
+__device__ __forceinline__ End end_by_passes(const SampleParams& p, Pick& s, const Row& row, const Series& series,
+                                             const char* x, bool by_count, uint64_t goal) {
   const int tid = threadIdx.x;
   if (tid == 0) s.found = kBins - 1;
   __syncthreads();
@@ -707,7 +720,7 @@ __device__ __forceinline__ End end_by_passes(const SampleParams& p, Pick& s, con
         const int b = static_cast<int>((k - lo) >> cut);
         atomicAdd(&s.sub_c[b], 1u);
         atomicAdd(reinterpret_cast<unsigned long long*>(&s.sub_w[b]),
-                  static_cast<unsigned long long>(weight_of(row, z)));
+                  static_cast<unsigned long long>(weight_of(row, series, z)));
       });
       __syncthreads();
       uint32_t c = tid < kSub ? s.sub_c[tid] : 0;
@@ -756,7 +769,7 @@ __device__ __forceinline__ End end_by_passes(const SampleParams& p, Pick& s, con
   sort_registers(place, s.run, size);
   const uint64_t key = tid < static_cast<int>(n) ? place[0] : 0;
   uint32_t c = tid < static_cast<int>(n) ? 1 : 0;
-  uint64_t w = c ? weight_of(row, value_of(~static_cast<uint32_t>(key >> 32))) : 0;
+  uint64_t w = c ? weight_of(row, series, value_of(~static_cast<uint32_t>(key >> 32))) : 0;
   const uint64_t own_w = w;
   scan(s.scratch, c, w);
   if (tid < static_cast<int>(n)) {
@@ -779,8 +792,8 @@ __device__ __forceinline__ End end_by_passes(const SampleParams& p, Pick& s, con
 // list's n keys into s.list, ascending, and the running sums of their weights
 // into s.run.  early: the thread's one of the first kRowThreads.
 template <int E>
-__device__ __forceinline__ void sort_and_sum(Pick& s, const Row& row, const uint64_t* list, uint64_t early,
-                                             uint32_t n) {
+__device__ __forceinline__ void sort_and_sum(Pick& s, const Row& row, const Series& series, const uint64_t* list,
+                                             uint64_t early, uint32_t n) {
   const uint32_t first = threadIdx.x * E;
   uint64_t v[E], sum[E];
 #pragma unroll
@@ -796,7 +809,7 @@ __device__ __forceinline__ void sort_and_sum(Pick& s, const Row& row, const uint
   uint64_t w = 0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    if (first + e < n) w += weight_of(row, value_of(~static_cast<uint32_t>(v[e] >> 32)));
+    if (first + e < n) w += weight_of(row, series, value_of(~static_cast<uint32_t>(v[e] >> 32)));
     sum[e] = w;
   }
   uint32_t none = 0;
@@ -829,6 +842,8 @@ __global__ __launch_bounds__(kRowThreads) void sample_pick_kernel(SampleParams p
   const Ends ends = row_ends(p, r);
   if (plan.mode == kDone) return;
   const Row row = row_of(p, ends, temperature);
+  Series series;
+  series.load();
   s.cum_c[tid + 1] = cc;
   s.cum_w[tid + 1] = cw;
   if (tid == 0) {
@@ -848,7 +863,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_pick_kernel(SampleParams p
       const uint64_t goal = step == 0   ? static_cast<uint64_t>(k)
                             : step == 1 ? top_p_goal(tp, first.weight)
                                         : draw_goal(u, kept.weight);
-      const End e = end_by_passes<DT>(p, s, row, x, step == 0, goal);
+      const End e = end_by_passes<DT>(p, s, row, series, x, step == 0, goal);
       if (step == 0) first = Prefix{e.count, e.weight};
       if (step < 2 && e.count < kept.count) kept = Prefix{e.count, e.weight};
       if (step == 2 && tid == 0) p.out[r] = e.index;
@@ -858,9 +873,9 @@ __global__ __launch_bounds__(kRowThreads) void sample_pick_kernel(SampleParams p
 
   // The collected elements: sorted, and their weights' running sums.
   const uint32_t n = listed < static_cast<uint32_t>(p.list_cap) ? listed : p.list_cap;
-  if (n <= kRowThreads) sort_and_sum<1>(s, row, list, early, n);
-  else if (n <= 2 * kRowThreads) sort_and_sum<2>(s, row, list, early, n);
-  else sort_and_sum<4>(s, row, list, early, n);
+  if (n <= kRowThreads) sort_and_sum<1>(s, row, series, list, early, n);
+  else if (n <= 2 * kRowThreads) sort_and_sum<2>(s, row, series, list, early, n);
+  else sort_and_sum<4>(s, row, series, list, early, n);
   __syncthreads();
   if (tid >= 64) return;
   Prefix kept = least;
