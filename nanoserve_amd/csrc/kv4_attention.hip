@@ -232,17 +232,19 @@ struct Slot {
   static constexpr int loads = D == 128 ? 5 : 3;  // vector memory operations that fill it
 };
 
-// A lane's words of the two tiles of K or V, and the parameter words of tokens
-// 4 g .. 4 g + 3 of each.
+// A step's parameters as float32: lane l makes the two of token l % 32 of K
+// (l < 32) or V, and each lane reads back those of tokens 4 g .. 4 g + 3 of both
+// tiles.  (Each lane converting the eight words that it needs itself was 72 of
+// the ~330 vector instructions of a step of 32 columns.)
+struct Params {
+  float first[64], second[64];  // K: s_t, b_t in log2 units; V: s_t, b_t + 8 s_t
+};
+
+// A lane's words of the two tiles of K or V.
 template <int D>
 struct Tiles {
   uint32_t w[2][D / 32];
-  u32x4 par[2];
 
-  __device__ __forceinline__ void read_params(const char* params, int g) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) par[j] = *reinterpret_cast<const u32x4*>(params + j * 64 + g * 16);
-  }
   // code_off: the lane's bytes in a tile.
   __device__ __forceinline__ void read_codes(const char* codes, int code_off) {
 #pragma unroll
@@ -296,6 +298,13 @@ __device__ const Page kNanF16 = page_of(Half<F16>::nan);
 __device__ const Page kNanBF16 = page_of(Half<BF16>::nan);
 __device__ const Page kZeros = page_of(0);
 
+// The wave's largest, on every lane.
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t w) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) w = max(w, static_cast<uint32_t>(__shfl_xor(static_cast<int>(w), off)));
+  return w;
+}
+
 constexpr float kCodeUnit = 16777216.f;  // 2^24: an even dim's code as a half's bits is code / 2^24
 // p is kept relative to a reference that is at most kSlack binades below the
 // column's running maximum and lifted by kLift, so that the largest lies in
@@ -333,7 +342,9 @@ struct Wave {
   // The columns' query rows, as the operands that meet the codes: lane group g
   // holds dims (D / 4) g .. + D / 4, eight of them per 32-dim step in the order
   // of a word's masked nibbles, odd dims a sixteenth of their value.
-  __device__ __forceinline__ void load_queries(const char* const (&row)[NT], int g, float scale) {
+  // all: the largest of those who share parameters, from this wave's.
+  template <class All>
+  __device__ __forceinline__ void load_queries(const char* const (&row)[NT], int g, float scale, All all) {
     uint32_t x[NT][D / 8];
     float big = 0.f;
 #pragma unroll
@@ -351,7 +362,8 @@ struct Wave {
     }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor(big, off));
-    // The wave's largest finite element becomes 2^14 .. 2^15.
+    big = all(big);
+    // The largest finite element becomes 2^14 .. 2^15.
     int e = 14 - (static_cast<int>(__float_as_uint(big) >> 23) - 127);
     e = e < -113 ? -113 : e > 100 ? 100 : e;
     float f = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
@@ -391,8 +403,7 @@ struct Wave {
 
   // A larger scale has come: the next power of two above it, the accumulators along.
   __device__ __forceinline__ void raise_sigma(uint32_t w) {
-    w = max(w, static_cast<uint32_t>(__shfl_xor(static_cast<int>(w), 16)));
-    w = max(w, static_cast<uint32_t>(__shfl_xor(static_cast<int>(w), 32)));
+    w = wave_max_u32(w);
     const uint32_t bits = __float_as_uint(kv4_scale<DT>(w));
     float next = __uint_as_float((bits & 0x7F800000u) + 0x00800000u);
     if constexpr (DT::code == NS_DTYPE_F16) {
@@ -412,15 +423,28 @@ struct Wave {
     }
   }
 
+  // Makes a slot's parameters; its tokens from `valid` on are nobody's.  Gives
+  // this lane's word of V, the scale in the upper half, or 0.
+  __device__ __forceinline__ uint32_t convert(const char* slot, Params& params, int lane, int valid) const {
+    uint32_t word = *reinterpret_cast<const uint32_t*>(slot + Slot<D>::par + lane * 4);
+    const bool of_v = lane >= 32;
+    if ((lane & 31) >= valid) word = 0;
+    const float sc = kv4_scale<DT>(word), of = kv4_offset<DT>(word);
+    params.first[lane] = of_v ? sc : sc * cf;
+    params.second[lane] = of_v ? __builtin_fmaf(8.f, sc, of) : of * cf;
+    return of_v ? word : 0;
+  }
+
   // One step over tokens tok .. tok + 31.  MASK: some column does not see all of
-  // them; column n sees tokens up to limit[n], none of the wave's sees past last.
+  // them; column n sees tokens up to limit[n].  big: at least the largest of the
+  // step's parameter words of V, on some lane.
   template <bool MASK>
-  __device__ __forceinline__ void step(const char* slot, int lane, int tok, int g, const int (&limit)[NT], int last) {
+  __device__ __forceinline__ void step(const char* slot, const Params& params, uint32_t big, int lane, int tok, int g,
+                                       const int (&limit)[NT]) {
     Tiles<D> k, v;
     // K for D = 128 and V lie in lane order; a tile of K at D = 64 row after row.
     k.read_codes(slot, D == 128 ? lane * 16 : (lane & 15) * 32 + g * 8);
-    k.read_params(slot + Slot<D>::par, g);
-    v.read_params(slot + Slot<D>::par + 128, g);
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(big > top) != 0, 0)) raise_sigma(big);
     floatx4 s[NT][2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -433,45 +457,25 @@ struct Wave {
         for (int n = 0; n < NT; ++n) s[n][j] = mfma16x16x32(F16{}, a, q[n][w], s[n][j]);
       }
     }
-    float ks[2][4], kb[2][4];
+    floatx4 ks[2], kb[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        ks[j][r] = kv4_scale<DT>(k.par[j][r]) * cf;
-        kb[j][r] = kv4_offset<DT>(k.par[j][r]) * cf;
-      }
+      const int at = 16 * j + 4 * g;
+      ks[j] = *reinterpret_cast<const floatx4*>(params.first + at);
+      kb[j] = *reinterpret_cast<const floatx4*>(params.second + at);
     }
-    float vs[2][4], vb[2][4];
-    uint32_t big = 0;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        uint32_t w = v.par[j][r];
-        if (MASK && tok + 16 * j + 4 * g + r > last) w = 0;  // what lies there is nobody's
-        big = max(big, w);
-        vs[j][r] = kv4_scale<DT>(w);
-        vb[j][r] = __builtin_fmaf(8.f, vs[j][r], kv4_offset<DT>(w));
-      }
-    }
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(big > top) != 0, 0)) raise_sigma(big);
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) vs[j][r] *= inv_sigma;
 
-    half8 pv[NT];
+    float x[NT][2][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       auto seen = [&](int j, int r) { return !MASK || tok + 16 * j + 4 * g + r <= limit[n]; };
-      float x[2][4], most = -INFINITY;
+      float most = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          x[j][r] = __builtin_fmaf(ks[j][r], s[n][j][r], __builtin_fmaf(kb[j][r], qs[n], ref[n]));
-          most = fmaxf(most, seen(j, r) ? x[j][r] : -INFINITY);
+          x[n][j][r] = __builtin_fmaf(ks[j][r], s[n][j][r], __builtin_fmaf(kb[j][r], qs[n], ref[n]));
+          most = fmaxf(most, seen(j, r) ? x[n][j][r] : -INFINITY);
         }
       }
       if (__builtin_expect(__builtin_amdgcn_ballot_w64(most > kLift + kSlack) != 0, 0)) {
@@ -480,8 +484,8 @@ struct Wave {
         for (int j = 0; j < 2; ++j) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            x[j][r] = __builtin_fmaf(ks[j][r], s[n][j][r], kb[j][r] * qs[n]);
-            most = fmaxf(most, seen(j, r) ? x[j][r] : -INFINITY);
+            x[n][j][r] = __builtin_fmaf(ks[j][r], s[n][j][r], kb[j][r] * qs[n]);
+            most = fmaxf(most, seen(j, r) ? x[n][j][r] : -INFINITY);
           }
         }
         const float m_new = fmaxf(m[n], group4_max_swap(most));
@@ -496,14 +500,26 @@ struct Wave {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) x[j][r] += ref[n];
+          for (int r = 0; r < 4; ++r) x[n][j][r] += ref[n];
       }
+    }
+    floatx4 vs[2], vb[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int at = 32 + 16 * j + 4 * g;
+      vs[j] = *reinterpret_cast<const floatx4*>(params.first + at) * inv_sigma;
+      vb[j] = *reinterpret_cast<const floatx4*>(params.second + at);
+    }
+    half8 pv[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      auto seen = [&](int j, int r) { return !MASK || tok + 16 * j + 4 * g + r <= limit[n]; };
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           // A masked place may hold anything: neither its score nor its row enters.
-          const float p = seen(j, r) ? fast_exp2(x[j][r]) : 0.f;
+          const float p = seen(j, r) ? fast_exp2(x[n][j][r]) : 0.f;
           l[n] += p;
           b[n] = __builtin_fmaf(p, seen(j, r) ? vb[j][r] : 0.f, b[n]);
           pv[n][4 * j + r] = static_cast<_Float16>(p * (seen(j, r) ? vs[j][r] : 0.f));
@@ -534,27 +550,20 @@ struct Wave {
   }
 };
 
-// Tokens [first, end) of sequence s in steps `stride` tokens apart, into w.
-// Tokens from end on and past a column's limit are masked; tiles past the
-// wave's last token are never looked up.  ring: R slots of this wave's.
-template <int R, class DT, int D, int NT>
-__device__ __forceinline__ void run_keys(Wave<DT, D, NT>& w, const Kv4AttnParams& p, char* ring, int s, int kvh,
-                                         int lane, int first, int end, int stride, const int (&limit)[NT], int all_see,
-                                         int last) {
-  if (first >= end) return;
-  static_assert((R & (R - 1)) == 0, "a power of two");
-  const int g = lane >> 4, col = lane & 15;
-  const int steps = (end - first + stride - 1) / stride;
-  const int tpb = p.block_size >> 4;
-  const int tile_last = last >> 4;
-  const int64_t bt_row = static_cast<int64_t>(s) * p.bt_stride;
-  const int code_bytes = p.block_size * (D / 2);
+// Brings the steps first, first + stride, ... of one (sequence, KV head) into LDS.
+template <class DT, int D>
+struct Feed {
+  const Kv4AttnParams& p;
+  int s, kvh, lane, first, stride, steps, tile_last;
   Window win;
-  auto fill = [&](int i) {
+
+  // Tiles past tile_last are never looked up.
+  __device__ __forceinline__ void fill(int i) {
+    const int tpb = p.block_size >> 4;
     int tile = (first + (i + (lane >> 1)) * stride) / 16 + (lane & 1);
     tile = tile < tile_last ? tile : tile_last;
     const int at = tile / tpb, in = tile - at * tpb;
-    const int64_t id = load_index(p.bt, bt_row + at, p.bt64);
+    const int64_t id = load_index(p.bt, static_cast<int64_t>(s) * p.bt_stride + at, p.bt64);
     const bool bad = id < 0 || id >= p.num_blocks;
     const int64_t off = bad ? 0 : (id * p.num_kv_heads + kvh) * p.record + in * (8 * D);
     const char* nan_page = reinterpret_cast<const char*>(DT::code == NS_DTYPE_F16 ? &kNanF16 : &kNanBF16);
@@ -564,17 +573,18 @@ __device__ __forceinline__ void run_keys(Wave<DT, D, NT>& w, const Kv4AttnParams
     win.k_hi = static_cast<uint32_t>(k >> 32);
     win.v_lo = static_cast<uint32_t>(v);
     win.v_hi = static_cast<uint32_t>(v >> 32);
-    win.par = bad ? 0 : code_bytes + in * (64 - 8 * D);
-  };
-  // Fills the slot of step i; behind the last step the last one's again, so that
-  // the count of loads in flight stays what the waits expect.
-  auto issue = [&](int i) {
-    char* slot = ring + (i & (R - 1)) * Slot<D>::bytes;
+    win.par = bad ? 0 : p.block_size * (D / 2) + in * (64 - 8 * D);
+  }
+  // Fills a slot with step i; behind the last step with the last one again, so
+  // that the count of loads in flight stays what the waits expect.  Steps are
+  // asked for in order.
+  __device__ __forceinline__ void issue(int i, char* slot) {
     if (i < steps) {
       if ((i & 31) == 0) fill(i);
     } else {
       i = steps - 1;
     }
+    const int col = lane & 15, g = lane >> 4;
     const int from = 2 * (i & 31);
     const char* k0 = lane_pointer(win.k_lo, win.k_hi, from);
     const char* k1 = lane_pointer(win.k_lo, win.k_hi, from + 1);
@@ -598,21 +608,42 @@ __device__ __forceinline__ void run_keys(Wave<DT, D, NT>& w, const Kv4AttnParams
     const char* kp = (lane & 16) ? k1 + par1 : k0 + par0;
     const char* vp = (lane & 16) ? v1 + par1 : v0 + par0;
     dma_lds4((lane < 32 ? kp : vp) + col * 4, slot + Slot<D>::par);
-  };
+  }
+};
+
+// A wave by itself: tokens [first, end) of sequence s in steps `stride` tokens
+// apart, into w.  Tokens from end on are masked; last is the wave's last token.
+// ring: R slots of this wave's.
+template <int R, class DT, int D>
+__device__ __forceinline__ void run_keys(Wave<DT, D, 1>& w, const Kv4AttnParams& p, char* ring, Params& params, int s,
+                                         int kvh, int lane, int first, int end, int stride, int last) {
+  if (first >= end) return;
+  static_assert((R & (R - 1)) == 0, "a power of two");
+  const int g = lane >> 4;
+  Feed<DT, D> feed = {p, s, kvh, lane, first, stride, (end - first + stride - 1) / stride, last >> 4, {}};
 #pragma unroll 1
-  for (int i = 0; i < R; ++i) issue(i);
-  // Steps that every column sees whole, then the others.
-  const int whole = all_see + 1 < end ? all_see + 1 : end;
+  for (int i = 0; i < R; ++i) feed.issue(i, ring + i * Slot<D>::bytes);
+  const int limit[1] = {end - 1};
   int i = 0, tok = first;
-  for (; tok + 32 <= whole; tok += stride, ++i) {
+  // The parameters of the step before have been read when these are written: a
+  // wave's LDS operations are done in order.
+  for (; tok + 32 <= end; tok += stride, ++i) {
+    char* slot = ring + (i & (R - 1)) * Slot<D>::bytes;
     vector_wait<(R - 1) * Slot<D>::loads>();
-    w.template step<false>(ring + (i & (R - 1)) * Slot<D>::bytes, lane, tok, g, limit, last);
-    issue(i + R);
+    const uint32_t big = w.convert(slot, params, lane, 32);
+    __builtin_amdgcn_wave_barrier();
+    w.template step<false>(slot, params, big, lane, tok, g, limit);
+    __builtin_amdgcn_wave_barrier();
+    feed.issue(i + R, slot);
   }
   for (; tok < end; tok += stride, ++i) {
+    char* slot = ring + (i & (R - 1)) * Slot<D>::bytes;
     vector_wait<(R - 1) * Slot<D>::loads>();
-    w.template step<true>(ring + (i & (R - 1)) * Slot<D>::bytes, lane, tok, g, limit, last);
-    issue(i + R);
+    const uint32_t big = w.convert(slot, params, lane, last + 1 - tok);
+    __builtin_amdgcn_wave_barrier();
+    w.template step<true>(slot, params, big, lane, tok, g, limit);
+    __builtin_amdgcn_wave_barrier();
+    feed.issue(i + R, slot);
   }
   vector_wait<0>();  // nothing lands in the ring behind its use
 }
@@ -692,6 +723,7 @@ __global__ __launch_bounds__(256, kDecodeGroups) void kv4_decode_kernel(Kv4AttnP
   // A wave's ring, and behind its keys its unnormalised outputs: 16 columns,
   // whose stores the four floats keep on different banks.
   __shared__ __align__(16) char rings[4][R * Slot<D>::bytes];
+  __shared__ __align__(16) Params params[4];
   static_assert(R * Slot<D>::bytes >= 16 * (D + 4) * 4, "the outputs lie in the ring");
   auto so = [&](int wv, int c, int d) { return reinterpret_cast<float*>(rings[wv]) + c * (D + 4) + d; };
   const int lane = threadIdx.x & 63;
@@ -714,9 +746,8 @@ __global__ __launch_bounds__(256, kDecodeGroups) void kv4_decode_kernel(Kv4AttnP
     w.init();
     const int head = kvh * p.group + (col < p.group ? col : p.group - 1);
     const char* const query[1] = {p.query + (row0 * p.num_heads + head) * (D * 2)};
-    w.load_queries(query, g, p.scale);
-    const int limit[1] = {t1 - 1};
-    run_keys<R>(w, p, rings[wave], s, kvh, lane, t0 + 32 * wave, t1, 128, limit, t1 - 1, len - 1);
+    w.load_queries(query, g, p.scale, [](float big) { return big; });
+    run_keys<R>(w, p, rings[wave], params[wave], s, kvh, lane, t0 + 32 * wave, t1, 128, len - 1);
     const float l = group4_sum(w.l[0]), b = group4_sum(w.b[0]);
     if (g == 0) {
       sm[wave][col] = w.m[0];
@@ -771,15 +802,27 @@ __global__ __launch_bounds__(256, kDecodeGroups) void kv4_decode_kernel(Kv4AttnP
   }
 }
 
-constexpr int kColumnRing = 4, kColumnTiles = 2;
+constexpr int kColumnTiles = 2;
 
-// Rows of longer queries: a wave takes 16 NT flattened (query row, head) columns
-// of one (sequence, KV head) over a range of its keys; the workgroup's four
-// waves lie side by side and walk the same keys, which the first of them to
-// come brings into the cache.  No wave waits for another.
-template <class DT, int D, int NT>
-__global__ __launch_bounds__(256, 2) void kv4_columns_kernel(Kv4AttnParams p) {
-  __shared__ __align__(16) char rings[4][kColumnRing * Slot<D>::bytes];
+// Rows of longer queries: four waves of 16 NT flattened (query row, head) columns
+// each of one (sequence, KV head), side by side over a range of its keys.  They
+// walk the keys in chunks of W steps of 32 tokens, each of the W waves bringing
+// and converting one step of the next chunk while all work on this one.  W = 8:
+// four more waves take the second half of each chunk's steps for the same
+// columns, and the two states are joined through LDS at the end.
+template <class DT, int D, int NT, int W>
+__global__ __launch_bounds__(64 * W, 2) void kv4_columns_kernel(Kv4AttnParams p) {
+  constexpr int kCells = NT * (D / 4 + 2);  // floats a lane hands over where W = 8
+  struct Buffer {
+    char slots[W][Slot<D>::bytes];
+    Params params[W];
+    uint32_t big[W];
+  };
+  constexpr int kBytes = W == 8 && 4 * kCells * 256 > static_cast<int>(2 * sizeof(Buffer))
+                             ? 4 * kCells * 256
+                             : static_cast<int>(2 * sizeof(Buffer));
+  __shared__ __align__(16) char lds[kBytes];
+  Buffer* const buffers = reinterpret_cast<Buffer*>(lds);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
@@ -796,15 +839,18 @@ __global__ __launch_bounds__(256, 2) void kv4_columns_kernel(Kv4AttnParams p) {
   // The last columns, which see the most keys, first.
   const int blocks = blocks_of(ql), ranges = ranges_of(p, len);
   const int block = found.index / ranges, range = found.index - block * ranges;
-  const int base = ((blocks - 1 - block) * 4 + wave) * (16 * NT);
-  if (base >= cols) return;
-  const int end_col = base + 16 * NT < cols ? base + 16 * NT : cols;
-  const int all_see = len - ql + base / p.group;               // the first column's last key
-  const int last = len - ql + (end_col - 1) / p.group;         // the last column's
+  const int block_base = (blocks - 1 - block) * (64 * NT);
+  auto last_of = [&](int end_col) { return len - ql + ((end_col < cols ? end_col : cols) - 1) / p.group; };
   const int t0 = range * p.split;
-  if (t0 > last && range > 0) return;  // the merge reads ranges that hold keys
-  int t1 = last + 1;
-  if (p.nsplit > 1 && t1 - t0 > p.split) t1 = t0 + p.split;
+  const int block_last = last_of(block_base + 64 * NT);  // the workgroup's last key
+  if (t0 > block_last && range > 0) return;              // the merge reads ranges that hold keys
+  auto end_of = [&](int last) { return p.nsplit > 1 && last + 1 - t0 > p.split ? t0 + p.split : last + 1; };
+  const int block_end = end_of(block_last);
+  const int base = block_base + (wave & 3) * (16 * NT);
+  const bool idle = base >= cols;  // brings keys for the others
+  const int all_see = len - ql + base / p.group;  // the first column's last key
+  const int last = last_of(base + 16 * NT);
+  const int end = idle ? t0 : end_of(last);
 
   Wave<DT, D, NT> w;
   w.init();
@@ -822,32 +868,97 @@ __global__ __launch_bounds__(256, 2) void kv4_columns_kernel(Kv4AttnParams p) {
     limit[n] = len - ql + j;
     query[n] = p.query + (row[n] * p.num_heads + head[n]) * (D * 2);
   }
-  w.load_queries(query, g, p.scale);
-  run_keys<kColumnRing>(w, p, rings[wave], s, kvh, lane, t0, t1, 32, limit, all_see, last);
+  w.load_queries(query, g, p.scale, [&](float big) {
+    uint32_t* const each = buffers[1].big;
+    if (lane == 0) each[wave] = __float_as_uint(big);  // not negative: ordered as its bits
+    __syncthreads();
+    for (int i = 0; i < W; ++i) big = fmaxf(big, __uint_as_float(each[i]));
+    return big;
+  });
+
+  if (t0 < block_end) {
+    const int chunks = (block_end - t0 + 32 * W - 1) / (32 * W);
+    const int whole = all_see + 1 < end ? all_see + 1 : end;
+    const int mine = t0 + 32 * wave;
+    Feed<DT, D> feed = {p, s, kvh, lane, mine, 32 * W, chunks, block_last >> 4, {}};
+    feed.issue(0, buffers[0].slots[wave]);
+    for (int c = 0; c < chunks; ++c) {
+      Buffer& now = buffers[c & 1];
+      vector_wait<0>();
+      const uint32_t word = w.convert(now.slots[wave], now.params[wave], lane, block_last + 1 - (mine + c * 32 * W));
+      const uint32_t most = wave_max_u32(word);
+      if (lane == 0) now.big[wave] = most;
+      __syncthreads();  // this chunk is there, and the one before is done with
+      if (c + 1 < chunks) feed.issue(c + 1, buffers[(c + 1) & 1].slots[wave]);
+      int i = W == 8 ? (wave >> 2) * 4 : 0;
+      const int to = i + 4;
+      int tok = t0 + (c * W + i) * 32;
+      // Steps that every column sees whole, then the others.
+      for (; i < to && tok + 32 <= whole; ++i, tok += 32)
+        w.template step<false>(now.slots[i], now.params[i], now.big[i], lane, tok, g, limit);
+      for (; i < to && tok < end; ++i, tok += 32)
+        w.template step<true>(now.slots[i], now.params[i], now.big[i], lane, tok, g, limit);
+    }
+  }
+
+  // A column's outputs and sum, not yet divided.
+  float x[NT][D / 4], l[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const float l = group4_sum(w.l[n]), b = group4_sum(w.b[n]);
-    if (base + 16 * n + col >= cols) continue;
-    float x[D / 4];
+    l[n] = group4_sum(w.l[n]);
+    const float b = group4_sum(w.b[n]);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) x[(D / 16) * r + i] = w.value(n, r, i, b);
+      for (int i = 0; i < D / 16; ++i) x[n][(D / 16) * r + i] = w.value(n, r, i, b);
+  }
+  if constexpr (W == 8) {
+    float* const other = reinterpret_cast<float*>(lds) + (wave & 3) * (kCells * 64) + lane;
+    __syncthreads();
+    if (wave >= 4) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float* at = other + n * (D / 4 + 2) * 64;
+        at[0] = w.m[n];
+        at[64] = l[n];
+#pragma unroll
+        for (int i = 0; i < D / 4; ++i) at[(2 + i) * 64] = x[n][i];
+      }
+    }
+    __syncthreads();
+    if (wave >= 4) return;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float* at = other + n * (D / 4 + 2) * 64;
+      const float m = fmaxf(w.m[n], at[0]);
+      const float m_use = m == -INFINITY ? 0.f : m;
+      const float f0 = fast_exp2(w.m[n] - m_use), f1 = fast_exp2(at[0] - m_use);
+      w.m[n] = m;
+      l[n] = __builtin_fmaf(f1, at[64], f0 * l[n]);
+#pragma unroll
+      for (int i = 0; i < D / 4; ++i) x[n][i] = __builtin_fmaf(f1, at[(2 + i) * 64], f0 * x[n][i]);
+    }
+  }
+  if (idle) return;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    // A range that none of the columns of this wave sees was left out by the merge.
+    if (base + 16 * n + col >= cols || (range > 0 && t0 >= end)) continue;
     const int64_t at = row[n] * p.num_heads + head[n];
     if (p.nsplit > 1) {
       if (g == 0) {
         p.part_m[at * p.nsplit + range] = w.m[n];
-        p.part_l[at * p.nsplit + range] = l;
+        p.part_l[at * p.nsplit + range] = l[n];
       }
       float* dst = p.part_o + (at * p.nsplit + range) * D + g * (D / 4);
 #pragma unroll
       for (int i = 0; i < D / 4; i += 4)
-        *reinterpret_cast<floatx4*>(dst + i) = floatx4{x[i], x[i + 1], x[i + 2], x[i + 3]};
+        *reinterpret_cast<floatx4*>(dst + i) = floatx4{x[n][i], x[n][i + 1], x[n][i + 2], x[n][i + 3]};
     } else {
-      const float inv = l > 0.f ? 1.f / l : l;
+      const float inv = l[n] > 0.f ? 1.f / l[n] : l[n];  // no key: zero; a NaN stays one
 #pragma unroll
-      for (int i = 0; i < D / 4; ++i) x[i] *= inv;
-      store_row<DT, D>(p.out + (at * D + g * (D / 4)) * 2, x);
+      for (int i = 0; i < D / 4; ++i) x[n][i] *= inv;
+      store_row<DT, D>(p.out + (at * D + g * (D / 4)) * 2, x[n]);
     }
   }
 }
@@ -919,6 +1030,7 @@ struct Cut {
   int dec_split, dec_n;         // tokens per range and ranges of one-row sequences
   int64_t dec_items;            // ranges of all of them, about
   int col_split, col_n;         // the same of longer queries
+  int col_waves;                // waves of a workgroup of the column kernel
   int64_t col_blocks;           // column blocks of all queries, at most
   size_t dec_bytes, col_bytes;  // partials
 };
@@ -962,6 +1074,7 @@ Cut cut_of(int num_seqs, int64_t num_tokens, int max_seq_len, int64_t context, i
     const int64_t split = round_up((longest + want - 1) / want, 32);
     c.col_split = static_cast<int>(split < 256 ? 256 : split);
     c.col_n = static_cast<int>((longest + c.col_split - 1) / c.col_split);
+    c.col_waves = blocks * c.col_n <= kCUs ? 8 : 4;
     c.col_blocks = num_tokens * group / (64 * kColumnTiles) + num_seqs;
     c.col_bytes = c.col_n > 1 ? static_cast<size_t>(num_tokens) * num_heads * c.col_n * row_bytes : 0;
   }
@@ -970,11 +1083,11 @@ Cut cut_of(int num_seqs, int64_t num_tokens, int max_seq_len, int64_t context, i
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
-hipError_t launch(const void* fn, int64_t blocks, Kv4AttnParams& p, hipStream_t st) {
+hipError_t launch(const void* fn, int64_t blocks, Kv4AttnParams& p, hipStream_t st, int threads = 256) {
   if (blocks <= 0) return hipSuccess;
   if (blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
   void* args[] = {&p};
-  return hipLaunchKernel(fn, dim3(static_cast<unsigned>(blocks)), dim3(256), args, 0, st);
+  return hipLaunchKernel(fn, dim3(static_cast<unsigned>(blocks)), dim3(static_cast<unsigned>(threads)), args, 0, st);
 }
 
 template <class DT, int D>
@@ -992,8 +1105,9 @@ hipError_t launch_fast(Kv4AttnParams p, const Cut& c, char* workspace, hipStream
     p.split = c.col_split;
     p.every_row = c.every_row ? 1 : 0;
     partials(workspace + align256(c.dec_bytes), p.num_tokens, c.col_n);
-    const void* fn = reinterpret_cast<const void*>(&kv4_columns_kernel<DT, D, kColumnTiles>);
-    e = launch(fn, c.col_blocks * p.num_kv_heads * c.col_n, p, st);
+    const void* fn = c.col_waves == 8 ? reinterpret_cast<const void*>(&kv4_columns_kernel<DT, D, kColumnTiles, 8>)
+                                      : reinterpret_cast<const void*>(&kv4_columns_kernel<DT, D, kColumnTiles, 4>);
+    e = launch(fn, c.col_blocks * p.num_kv_heads * c.col_n, p, st, 64 * c.col_waves);
     if (e == hipSuccess && c.col_n > 1)
       e = launch(reinterpret_cast<const void*>(&kv4_merge_kernel<DT, D, false>), (p.num_tokens * p.num_heads + 3) / 4, p, st);
     if (e != hipSuccess) return e;
