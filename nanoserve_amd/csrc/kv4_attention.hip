@@ -16,6 +16,21 @@
 namespace ns {
 namespace {
 
+// A row's keys are cut into n ranges of `tokens` (a multiple of 32).  With more
+// than one, range i of row r and head h leaves its maximum (log2 units), sum and
+// unnormalised output at index (r * num_heads + h) * n + i of the three.
+struct Ranges {
+  int n, tokens;
+  float* maxima;
+  float* sums;
+  float* outputs;
+
+  // Ranges of a context: one where it is empty or nothing is split.
+  __device__ __forceinline__ int of(int len) const {
+    return n == 1 || len <= tokens ? 1 : (len + tokens - 1) / tokens;
+  }
+};
+
 struct Kv4AttnParams {
   char* out;
   const char* query;
@@ -30,15 +45,10 @@ struct Kv4AttnParams {
   int64_t num_tokens, num_blocks, record;
   int64_t max_ctx;        // keys a row may have: max_seq_len, within the table
   float scale;
-  // Matrix-core kernels: a row's keys are cut into nsplit ranges of split
-  // tokens (a multiple of 32).  With more than one, range i of row r and head h
-  // leaves its maximum (log2 units), sum and unnormalised output at index
-  // (r * num_heads + h) * nsplit + i of part_m, part_l and part_o.
-  int nsplit, split;
-  int every_row;          // the column kernel takes one-row sequences too
-  float* part_m;
-  float* part_l;
-  float* part_o;
+  // Matrix-core kernels.
+  Ranges one, more;       // of one-row sequences; of longer queries
+  int every_row;          // the column part takes one-row sequences too
+  int column_groups;      // workgroups of the column part, in front of the others
 };
 
 struct Rows {
@@ -700,58 +710,52 @@ __device__ __forceinline__ bool find_part(const Kv4AttnParams& p, int lane, int 
   }
   return false;
 }
-// Ranges of a context: one where it is empty or nothing is split.
-__device__ __forceinline__ int ranges_of(const Kv4AttnParams& p, int len) {
-  return p.nsplit == 1 || len <= p.split ? 1 : (len + p.split - 1) / p.split;
-}
 
-// Rows of one-row sequences: a workgroup takes a range of one (sequence, KV
-// head)'s keys for the group's query heads (up to 16 columns), its four waves
-// every fourth step of it, and merges the four states through LDS.  The grid is
-// what the device holds at once at most; a workgroup goes from range to range,
-// gridDim apart in the list of all that there are, so a batch of unequal
-// contexts costs no empty workgroups and ends evenly.
-// Three workgroups of four waves on a compute unit (with four the 128 registers
-// left for a wave spill), so up to 53 KiB of LDS each.
-constexpr int kDecodeGroups = 3;
-template <int D>
-constexpr int kDecodeRing = D == 64 ? 4 : 2;
-template <class DT, int D>
-__global__ __launch_bounds__(256, kDecodeGroups) void kv4_decode_kernel(Kv4AttnParams p) {
-  constexpr int R = kDecodeRing<D>;
-  __shared__ float sm[4][16], sl[4][16];
+// Rows of one-row sequences: a workgroup of W waves takes a range of one
+// (sequence, KV head)'s keys for the group's query heads (up to 16 columns), its
+// waves every W-th step of it, and merges their states through LDS.  It goes from
+// range to range, `groups` apart in the list of all that there are, so a batch of
+// unequal contexts costs no empty workgroups and ends evenly.
+template <int D, int W, int R>
+struct RowState {
+  static constexpr int ring = R * Slot<D>::bytes;
+  static_assert(ring >= 16 * (D + 4) * 4, "the outputs lie in the ring");
+  float m[W][16], l[W][16];
+  Params params[W];
   // A wave's ring, and behind its keys its unnormalised outputs: 16 columns,
   // whose stores the four floats keep on different banks.
-  __shared__ __align__(16) char rings[4][R * Slot<D>::bytes];
-  __shared__ __align__(16) Params params[4];
-  static_assert(R * Slot<D>::bytes >= 16 * (D + 4) * 4, "the outputs lie in the ring");
-  auto so = [&](int wv, int c, int d) { return reinterpret_cast<float*>(rings[wv]) + c * (D + 4) + d; };
+  char rings[W][ring];
+};
+
+template <class DT, int D, int W, int R>
+__device__ __forceinline__ void one_rows(const Kv4AttnParams& p, RowState<D, W, R>& lds, int first, int groups) {
+  const Ranges& rg = p.one;
+  auto so = [&](int wv, int c, int d) { return reinterpret_cast<float*>(lds.rings[wv]) + c * (D + 4) + d; };
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
   Part found;
   found.more = true;
-  for (int item = blockIdx.x; found.more; item += gridDim.x) {
+  for (int item = first; found.more; item += groups) {
     const int kvh = item % p.num_kv_heads;
-    auto ranges = [&](int ql, int len) { return ql == 1 ? ranges_of(p, len) : 0; };
+    auto ranges = [&](int ql, int len) { return ql == 1 ? rg.of(len) : 0; };
     // The same for every wave.
-    if (!find_part(p, lane, item / p.num_kv_heads, (item + static_cast<int>(gridDim.x)) / p.num_kv_heads, ranges, found))
-      break;
+    if (!find_part(p, lane, item / p.num_kv_heads, (item + groups) / p.num_kv_heads, ranges, found)) break;
     const int s = found.seq, len = found.len, range = found.index;
     const int64_t row0 = found.row;
-    const int t0 = range * p.split;
-    const int t1 = p.nsplit > 1 && len - t0 > p.split ? t0 + p.split : len;
+    const int t0 = range * rg.tokens;
+    const int t1 = rg.n > 1 && len - t0 > rg.tokens ? t0 + rg.tokens : len;
 
     Wave<DT, D, 1> w;
     w.init();
     const int head = kvh * p.group + (col < p.group ? col : p.group - 1);
     const char* const query[1] = {p.query + (row0 * p.num_heads + head) * (D * 2)};
     w.load_queries(query, g, p.scale, [](float big) { return big; });
-    run_keys<R>(w, p, rings[wave], params[wave], s, kvh, lane, t0 + 32 * wave, t1, 128, len - 1);
+    run_keys<R>(w, p, lds.rings[wave], lds.params[wave], s, kvh, lane, t0 + 32 * wave, t1, 32 * W, len - 1);
     const float l = group4_sum(w.l[0]), b = group4_sum(w.b[0]);
     if (g == 0) {
-      sm[wave][col] = w.m[0];
-      sl[wave][col] = l;
+      lds.m[wave][col] = w.m[0];
+      lds.l[wave][col] = l;
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -765,41 +769,56 @@ __global__ __launch_bounds__(256, kDecodeGroups) void kv4_decode_kernel(Kv4AttnP
     }
     __syncthreads();
 
-    // Column threadIdx.x / 16, D / 16 dims of it.
-    const int c = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (D / 16);
+    // E dims of a column for each thread.
+    constexpr int E = D / (4 * W);
+    const int c = threadIdx.x / (4 * W), d0 = threadIdx.x % (4 * W) * E;
     if (c < p.group) {
-      float m = fmaxf(fmaxf(sm[0][c], sm[1][c]), fmaxf(sm[2][c], sm[3][c]));
+      float m = -INFINITY;
+#pragma unroll
+      for (int v = 0; v < W; ++v) m = fmaxf(m, lds.m[v][c]);
       const float m_use = m == -INFINITY ? 0.f : m;
-      float sum = 0.f, o[D / 16];
+      float sum = 0.f, o[E];
 #pragma unroll
-      for (int e = 0; e < D / 16; ++e) o[e] = 0.f;
+      for (int e = 0; e < E; ++e) o[e] = 0.f;
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const float f = fast_exp2(sm[v][c] - m_use);
-        sum = __builtin_fmaf(f, sl[v][c], sum);
+      for (int v = 0; v < W; ++v) {
+        const float f = fast_exp2(lds.m[v][c] - m_use);
+        sum = __builtin_fmaf(f, lds.l[v][c], sum);
 #pragma unroll
-        for (int e = 0; e < D / 16; ++e) o[e] = __builtin_fmaf(f, *so(v, c, d0 + e), o[e]);
+        for (int e = 0; e < E; ++e) o[e] = __builtin_fmaf(f, *so(v, c, d0 + e), o[e]);
       }
       const int64_t h = kvh * p.group + c;
-      if (p.nsplit > 1) {
-        const int64_t at = (static_cast<int64_t>(s) * p.num_heads + h) * p.nsplit + range;
+      if (rg.n > 1) {
+        const int64_t at = (static_cast<int64_t>(s) * p.num_heads + h) * rg.n + range;
         if (d0 == 0) {
-          p.part_m[at] = m;
-          p.part_l[at] = sum;
+          rg.maxima[at] = m;
+          rg.sums[at] = sum;
         }
 #pragma unroll
-        for (int e = 0; e < D / 16; ++e) p.part_o[at * D + d0 + e] = o[e];
+        for (int e = 0; e < E; ++e) rg.outputs[at * D + d0 + e] = o[e];
       } else {
         const float inv = sum > 0.f ? 1.f / sum : sum;  // no key: zero; a NaN stays one
         uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + (row0 * p.num_heads + h) * D + d0;
 #pragma unroll
-        for (int e = 0; e < D / 16; e += 2)
+        for (int e = 0; e < E; e += 2)
           *reinterpret_cast<uint32_t*>(dst + e) =
               Half<DT>::from_f32(o[e] * inv) | (Half<DT>::from_f32(o[e + 1] * inv) << 16);
       }
     }
     __syncthreads();  // the next range's states go where these are read
   }
+}
+
+// A batch of one-row sequences.  Four waves: three workgroups on a compute unit
+// (with four the 128 registers left for a wave spill), so up to 53 KiB of LDS
+// each.  Eight where the ranges leave compute units idle.
+constexpr int kDecodeGroups = 3;
+template <int D>
+constexpr int kDecodeRing = D == 64 ? 4 : 2;
+template <class DT, int D, int W>
+__global__ __launch_bounds__(64 * W, W == 4 ? kDecodeGroups : 2) void kv4_decode_kernel(Kv4AttnParams p) {
+  __shared__ __align__(16) RowState<D, W, kDecodeRing<D>> lds;
+  one_rows<DT>(p, lds, blockIdx.x, gridDim.x);
 }
 
 constexpr int kColumnTiles = 2;
@@ -810,26 +829,31 @@ constexpr int kColumnTiles = 2;
 // and converting one step of the next chunk while all work on this one.  W = 8:
 // four more waves take the second half of each chunk's steps for the same
 // columns, and the two states are joined through LDS at the end.
-template <class DT, int D, int NT, int W>
-__global__ __launch_bounds__(64 * W, 2) void kv4_columns_kernel(Kv4AttnParams p) {
-  constexpr int kCells = NT * (D / 4 + 2);  // floats a lane hands over where W = 8
+template <int D, int NT, int W>
+struct ColumnState {
+  static constexpr int cells = NT * (D / 4 + 2);  // floats a lane hands over where W = 8
   struct Buffer {
     char slots[W][Slot<D>::bytes];
     Params params[W];
     uint32_t big[W];
   };
-  constexpr int kBytes = W == 8 && 4 * kCells * 256 > static_cast<int>(2 * sizeof(Buffer))
-                             ? 4 * kCells * 256
-                             : static_cast<int>(2 * sizeof(Buffer));
-  __shared__ __align__(16) char lds[kBytes];
-  Buffer* const buffers = reinterpret_cast<Buffer*>(lds);
+  union {
+    Buffer buffers[2];
+    float states[W == 8 ? 4 : 1][cells * 64];
+  };
+};
+
+template <class DT, int D, int NT, int W>
+__device__ __forceinline__ void columns(const Kv4AttnParams& p, ColumnState<D, NT, W>& lds) {
+  const Ranges& rg = p.more;
+  auto& buffers = lds.buffers;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
   const int kvh = blockIdx.x % p.num_kv_heads;
   auto blocks_of = [&](int ql) { return (ql * p.group + 64 * NT - 1) / (64 * NT); };
   auto items = [&](int ql, int len) {
-    return ql < (p.every_row ? 1 : 2) ? 0 : blocks_of(ql) * ranges_of(p, len);
+    return ql < (p.every_row ? 1 : 2) ? 0 : blocks_of(ql) * rg.of(len);
   };
   Part found;
   if (!find_part(p, lane, blockIdx.x / p.num_kv_heads, 0, items, found)) return;
@@ -837,14 +861,14 @@ __global__ __launch_bounds__(64 * W, 2) void kv4_columns_kernel(Kv4AttnParams p)
   const int64_t row0 = found.row;
   const int cols = ql * p.group;
   // The last columns, which see the most keys, first.
-  const int blocks = blocks_of(ql), ranges = ranges_of(p, len);
+  const int blocks = blocks_of(ql), ranges = rg.of(len);
   const int block = found.index / ranges, range = found.index - block * ranges;
   const int block_base = (blocks - 1 - block) * (64 * NT);
   auto last_of = [&](int end_col) { return len - ql + ((end_col < cols ? end_col : cols) - 1) / p.group; };
-  const int t0 = range * p.split;
+  const int t0 = range * rg.tokens;
   const int block_last = last_of(block_base + 64 * NT);  // the workgroup's last key
   if (t0 > block_last && range > 0) return;              // the merge reads ranges that hold keys
-  auto end_of = [&](int last) { return p.nsplit > 1 && last + 1 - t0 > p.split ? t0 + p.split : last + 1; };
+  auto end_of = [&](int last) { return rg.n > 1 && last + 1 - t0 > rg.tokens ? t0 + rg.tokens : last + 1; };
   const int block_end = end_of(block_last);
   const int base = block_base + (wave & 3) * (16 * NT);
   const bool idle = base >= cols;  // brings keys for the others
@@ -883,7 +907,7 @@ __global__ __launch_bounds__(64 * W, 2) void kv4_columns_kernel(Kv4AttnParams p)
     Feed<DT, D> feed = {p, s, kvh, lane, mine, 32 * W, chunks, block_last >> 4, {}};
     feed.issue(0, buffers[0].slots[wave]);
     for (int c = 0; c < chunks; ++c) {
-      Buffer& now = buffers[c & 1];
+      auto& now = buffers[c & 1];
       vector_wait<0>();
       const uint32_t word = w.convert(now.slots[wave], now.params[wave], lane, block_last + 1 - (mine + c * 32 * W));
       const uint32_t most = wave_max_u32(word);
@@ -913,7 +937,7 @@ __global__ __launch_bounds__(64 * W, 2) void kv4_columns_kernel(Kv4AttnParams p)
       for (int i = 0; i < D / 16; ++i) x[n][(D / 16) * r + i] = w.value(n, r, i, b);
   }
   if constexpr (W == 8) {
-    float* const other = reinterpret_cast<float*>(lds) + (wave & 3) * (kCells * 64) + lane;
+    float* const other = lds.states[W == 8 ? wave & 3 : 0] + lane;
     __syncthreads();
     if (wave >= 4) {
 #pragma unroll
@@ -945,12 +969,12 @@ __global__ __launch_bounds__(64 * W, 2) void kv4_columns_kernel(Kv4AttnParams p)
     // A range that none of the columns of this wave sees was left out by the merge.
     if (base + 16 * n + col >= cols || (range > 0 && t0 >= end)) continue;
     const int64_t at = row[n] * p.num_heads + head[n];
-    if (p.nsplit > 1) {
+    if (rg.n > 1) {
       if (g == 0) {
-        p.part_m[at * p.nsplit + range] = w.m[n];
-        p.part_l[at * p.nsplit + range] = l[n];
+        rg.maxima[at * rg.n + range] = w.m[n];
+        rg.sums[at * rg.n + range] = l[n];
       }
-      float* dst = p.part_o + (at * p.nsplit + range) * D + g * (D / 4);
+      float* dst = rg.outputs + (at * rg.n + range) * D + g * (D / 4);
 #pragma unroll
       for (int i = 0; i < D / 4; i += 4)
         *reinterpret_cast<floatx4*>(dst + i) = floatx4{x[n][i], x[n][i + 1], x[n][i + 2], x[n][i + 3]};
@@ -963,10 +987,27 @@ __global__ __launch_bounds__(64 * W, 2) void kv4_columns_kernel(Kv4AttnParams p)
   }
 }
 
+// Both kinds of rows in one launch: the column part's workgroups first, and where
+// those leave compute units idle, at the start or towards the end, workgroups of
+// one-row sequences.
+template <class DT, int D, int NT, int W>
+__global__ __launch_bounds__(64 * W, 2) void kv4_columns_kernel(Kv4AttnParams p) {
+  constexpr int R = W == 4 ? kDecodeRing<D> : 2;
+  union Lds {
+    ColumnState<D, NT, W> columns;
+    RowState<D, W, R> rows;
+  };
+  __shared__ __align__(16) Lds lds;
+  const int groups = p.column_groups;
+  if (static_cast<int>(blockIdx.x) < groups) columns<DT>(p, lds.columns);
+  else one_rows<DT>(p, lds.rows, blockIdx.x - groups, gridDim.x - groups);
+}
+
 // Joins the ranges of a row, in order: one wave per (row, query head).  DECODE:
 // row r of the partials is sequence r's only row; else it is query row r.
 template <class DT, int D, bool DECODE>
 __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnParams p) {
+  const Ranges& rg = DECODE ? p.one : p.more;
   const int lane = threadIdx.x & 63;
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t r = at / p.num_heads;
@@ -993,10 +1034,10 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnParams p) {
     row = r;
     keys = rows.len - rows.ql + (r - rows.row0) + 1;
   }
-  const int n = keys <= 0 ? 0 : static_cast<int>((keys + p.split - 1) / p.split);
-  const float* pm = p.part_m + at * p.nsplit;
-  const float* pl = p.part_l + at * p.nsplit;
-  const float* po = p.part_o + at * p.nsplit * D;
+  const int n = keys <= 0 ? 0 : static_cast<int>((keys + rg.tokens - 1) / rg.tokens);
+  const float* pm = rg.maxima + at * rg.n;
+  const float* pl = rg.sums + at * rg.n;
+  const float* po = rg.outputs + at * rg.n * D;
   float m = -INFINITY;
   for (int i = lane; i < n; i += 64) m = fmaxf(m, pm[i]);
 #pragma unroll
@@ -1093,36 +1134,37 @@ hipError_t launch(const void* fn, int64_t blocks, Kv4AttnParams& p, hipStream_t 
 template <class DT, int D>
 hipError_t launch_fast(Kv4AttnParams p, const Cut& c, char* workspace, hipStream_t st) {
   const int64_t pairs = static_cast<int64_t>(p.num_seqs) * p.num_kv_heads;
-  auto partials = [&](char* at, int64_t rows, int n) {
+  auto ranges = [&](char* at, int64_t rows, int n, int tokens) {
     const int64_t cells = rows * p.num_heads * n;
-    p.part_o = reinterpret_cast<float*>(at);
-    p.part_m = p.part_o + cells * D;
-    p.part_l = p.part_m + cells;
+    float* o = reinterpret_cast<float*>(at);
+    return Ranges{n, tokens, o + cells * D, o + cells * (D + 1), o};
   };
-  hipError_t e = hipSuccess;
+  int64_t row_groups = 0;
+  if (c.decode) {
+    p.one = ranges(workspace, p.num_seqs, c.dec_n, c.dec_split);
+    const int64_t most = pairs * c.dec_n < c.dec_items ? pairs * c.dec_n : c.dec_items;
+    const int64_t held = static_cast<int64_t>(kCUs) * kDecodeGroups;
+    row_groups = most < held ? most : held;
+  }
+  hipError_t e;
   if (c.columns) {
-    p.nsplit = c.col_n;
-    p.split = c.col_split;
+    p.more = ranges(workspace + align256(c.dec_bytes), p.num_tokens, c.col_n, c.col_split);
     p.every_row = c.every_row ? 1 : 0;
-    partials(workspace + align256(c.dec_bytes), p.num_tokens, c.col_n);
+    const int64_t groups = c.col_blocks * p.num_kv_heads * c.col_n;
+    if (groups > 0x7FFFFFFF) return hipErrorInvalidValue;
+    p.column_groups = static_cast<int>(groups);
     const void* fn = c.col_waves == 8 ? reinterpret_cast<const void*>(&kv4_columns_kernel<DT, D, kColumnTiles, 8>)
                                       : reinterpret_cast<const void*>(&kv4_columns_kernel<DT, D, kColumnTiles, 4>);
-    e = launch(fn, c.col_blocks * p.num_kv_heads * c.col_n, p, st, 64 * c.col_waves);
+    e = launch(fn, groups + row_groups, p, st, 64 * c.col_waves);
     if (e == hipSuccess && c.col_n > 1)
       e = launch(reinterpret_cast<const void*>(&kv4_merge_kernel<DT, D, false>), (p.num_tokens * p.num_heads + 3) / 4, p, st);
-    if (e != hipSuccess) return e;
+  } else {
+    e = row_groups <= kCUs ? launch(reinterpret_cast<const void*>(&kv4_decode_kernel<DT, D, 8>), row_groups, p, st, 512)
+                           : launch(reinterpret_cast<const void*>(&kv4_decode_kernel<DT, D, 4>), row_groups, p, st);
   }
-  if (c.decode) {
-    p.nsplit = c.dec_n;
-    p.split = c.dec_split;
-    partials(workspace, p.num_seqs, c.dec_n);
-    const int64_t held = static_cast<int64_t>(kCUs) * kDecodeGroups;
-    const int64_t most = pairs * c.dec_n < c.dec_items ? pairs * c.dec_n : c.dec_items;
-    e = launch(reinterpret_cast<const void*>(&kv4_decode_kernel<DT, D>), most < held ? most : held, p, st);
-    if (e == hipSuccess && c.dec_n > 1)
-      e = launch(reinterpret_cast<const void*>(&kv4_merge_kernel<DT, D, true>),
-                 (static_cast<int64_t>(p.num_seqs) * p.num_heads + 3) / 4, p, st);
-  }
+  if (e == hipSuccess && c.decode && c.dec_n > 1)
+    e = launch(reinterpret_cast<const void*>(&kv4_merge_kernel<DT, D, true>),
+               (static_cast<int64_t>(p.num_seqs) * p.num_heads + 3) / 4, p, st);
   return e;
 }
 
@@ -1203,10 +1245,9 @@ extern "C" int ns_paged_attention_int4(void* out, const void* query,
   const int64_t table = block_table_width * static_cast<int64_t>(block_size);
   p.max_ctx = max_seq_len < table ? max_seq_len : table;
   p.scale = scale;
-  p.nsplit = 1;
-  p.split = 0;
+  p.one = p.more = {1, 0, nullptr, nullptr, nullptr};
   p.every_row = 0;
-  p.part_m = p.part_l = p.part_o = nullptr;
+  p.column_groups = 0;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   hipError_t e;
   if (!cut.fast) {
