@@ -9,14 +9,18 @@
 // the shortest of these prefixes.
 //
 // No sort of the row, which is cut into slices:
-//   1. every slice's largest element and smallest finite one;
+//   1. every slice's largest element, smallest finite one, and the largest of each
+//      group of threads;
 //   2. every slice's histogram over z_max - z in 1024 steps, counts and sums of
-//      w, and its part of the min-p prefix;
+//      w, and its part of the min-p prefix.  Where k groups of threads had their
+//      largest in the first bins, the first k elements lie there too, and only
+//      those bins' elements are counted, and listed;
 //   3. one workgroup per row adds the slices' histograms and scans them.  Every
 //      prefix's end, and the token, then lie in known bins: the end of the first k
 //      in one, those that follow from its weight in one or two, since that weight
 //      is known to within a bin;
-//   4. the elements of these bins are collected from all slices;
+//   4. the elements of these bins are collected, from the list of the second
+//      stage or from all slices;
 //   5. one workgroup per row sorts them, sums their weights and decides.
 // Where the bins hold more than the list takes (nearly equal logits, temperatures
 // far from 1), the last workgroup finds each end by itself: it cuts the bin by
@@ -30,8 +34,12 @@
 // additions; the rounding, 2^-45 of the largest weight, moves a border by less
 // than 1e-9 of the row's sum even where all 150K roundings agree.
 //
-// Bound: for a few rows the five launches; for many the float64 exponentials of
-// the second (about 50 operations for each element).
+// Bound: for a few rows the five launches (one row of 152K float16: 4.7, 10, 7,
+// 3.7 and 6.2 us); for many the three passes over the logits, of which the second
+// evaluates a float64 exponential (about 40 operations) for every element of the
+// rows without a top-k.  256 rows of 152K float32, three quarters with a top-k of
+// 20 to 400: 31 (5.1 TB/s), 45, 8.6, 28 and 16 us; with every element counted and
+// collected from the slices 31, 58, 8.5, 35 and 16.
 #include <math.h>
 
 #include "row_keys.h"
@@ -52,7 +60,7 @@ struct Plan {
   uint32_t lo[3], hi[3];  // ranges of bins to collect, disjoint; empty where lo > hi
   uint32_t mode;          // one of the below
 };
-constexpr uint32_t kDone = 0, kCollect = 1, kLong = 2;
+constexpr uint32_t kDone = 0, kCollect = 1, kLong = 2, kListed = 3;
 
 struct SampleParams {
   int64_t* out;
@@ -71,6 +79,8 @@ struct SampleParams {
   double zero_below;       // ln w below which a weight rounds to 0
   uint64_t* keys;          // [rows, slices]: the largest element's
   uint32_t* least;         // [rows, slices]: the smallest finite element's order
+  uint32_t* parts;         // [rows, slices, kSliceThreads / part_lanes]: the largest order of a group of threads
+  int part_lanes;          // threads of a group: 1, 2 or 4
   uint64_t* hist_w;        // [rows, slices, kBins]
   uint32_t* hist_c;
   uint64_t* min_w;         // [rows, slices]
@@ -81,6 +91,8 @@ struct SampleParams {
   uint64_t* kept_w;        // [rows]: the min-p prefix
   uint32_t* kept_c;
   uint32_t* list_n;        // [rows]
+  uint32_t* cand_n;        // [rows]: elements in the first bins, where these alone were counted; or 0
+  uint64_t* cands;         // [rows, list_cap]: their keys
   uint64_t* list;          // [rows, list_cap]: collected keys
   int list_cap;
 };
@@ -223,6 +235,12 @@ __device__ __forceinline__ uint64_t place_of(float z, uint32_t i) {
   return (static_cast<uint64_t>(~order_of(z)) << 32) | i;
 }
 
+// A row's top-k, or 0 where it cuts nothing off.
+__device__ __forceinline__ int64_t top_k_of(const SampleParams& p, int64_t r) {
+  const int64_t k = p.top_k ? load_index(p.top_k, r, p.top_k64) : 0;
+  return k > 0 && k < p.n ? k : 0;
+}
+
 // f(value, index) for the workgroup's slice of row blockIdx.y.
 template <int DT, class F>
 __device__ __forceinline__ void each_of_slice(const SampleParams& p, F f) {
@@ -243,6 +261,16 @@ __global__ __launch_bounds__(kSliceThreads) void sample_ends_kernel(SampleParams
     const uint32_t ord = static_cast<uint32_t>(k >> 32);
     least = ord < least && v > -INFINITY ? ord : least;
   });
+  if (p.top_k) {
+    uint32_t part = static_cast<uint32_t>(best >> 32);
+    for (int off = 1; off < p.part_lanes; off <<= 1) {
+      const uint32_t v = __shfl_xor(part, off);
+      part = v > part ? v : part;
+    }
+    const int64_t at = static_cast<int64_t>(blockIdx.y) * p.slices + blockIdx.x;
+    if (threadIdx.x % p.part_lanes == 0)
+      p.parts[(at * kSliceThreads + threadIdx.x) / p.part_lanes] = part;
+  }
   best = wave_max(best);
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) {
@@ -262,16 +290,80 @@ __global__ __launch_bounds__(kSliceThreads) void sample_ends_kernel(SampleParams
     const int64_t at = static_cast<int64_t>(blockIdx.y) * p.slices + blockIdx.x;
     p.keys[at] = best;
     p.least[at] = least;
-    if (blockIdx.x == 0) p.list_n[blockIdx.y] = 0;
+    if (blockIdx.x == 0) p.list_n[blockIdx.y] = p.cand_n[blockIdx.y] = 0;
   }
 }
 
+// Keys on their way to a row's list: a workgroup's first kLocal go out together.
+constexpr uint32_t kLocal = 1024;
+struct Outbox {
+  uint64_t keys[kLocal];
+  uint32_t n, base;
+
+  __device__ __forceinline__ void add(uint64_t key, uint64_t* list, uint32_t* list_n, uint32_t cap) {
+    const uint32_t at = atomicAdd(&n, 1u);
+    if (at < kLocal) {
+      keys[at] = key;
+    } else {
+      const uint32_t to = atomicAdd(list_n, 1u);
+      if (to < cap) list[to] = key;
+    }
+  }
+  // By the whole workgroup.
+  __device__ __forceinline__ void send(uint64_t* list, uint32_t* list_n, uint32_t cap) {
+    __syncthreads();
+    const uint32_t here = n < kLocal ? n : kLocal;
+    if (threadIdx.x == 0 && here > 0) base = atomicAdd(list_n, here);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < here; i += kSliceThreads)
+      if (base + i < cap) list[base + i] = keys[i];
+  }
+};
+
+// A bin such that the first k elements lie in it and the bins before it: k groups
+// of threads had their largest there.  The last bin where there are not so many
+// groups.  count: kBins zeros, and zeros again afterwards.
+__device__ __forceinline__ int last_bin_for(const SampleParams& p, const Row& row, int64_t r, int64_t k,
+                                            uint32_t* count) {
+  __shared__ uint32_t upto[kSliceThreads / 64];
+  __shared__ int found;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int groups = p.slices * kSliceThreads / p.part_lanes;
+  if (k == 0 || k > groups) return kBins - 1;
+  for (int i = tid; i < groups; i += kSliceThreads)
+    atomicAdd(&count[bin_of(row, value_of(p.parts[r * groups + i]))], 1u);
+  __syncthreads();
+  static_assert(kBins == 4 * kSliceThreads, "four bins for each thread");
+  u32x4& mine = reinterpret_cast<u32x4*>(count)[tid];
+  const u32x4 c = mine;
+  mine = u32x4{0, 0, 0, 0};
+  const uint32_t all = c[0] + c[1] + c[2] + c[3];
+  uint32_t sum = all;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint32_t v = __shfl_up(sum, off);
+    sum += lane >= off ? v : 0;
+  }
+  if (lane == 63) upto[wave] = sum;
+  __syncthreads();
+  for (int i = 0; i < wave; ++i) sum += upto[i];
+  uint32_t before = sum - all;
+  if (before < k && sum >= k) {
+    int b = 0;
+    while (before + c[b] < k) before += c[b++];
+    found = 4 * tid + b;
+  }
+  __syncthreads();
+  return found;
+}
+
 template <int DT>
-__global__ __launch_bounds__(kSliceThreads) void sample_hist_kernel(SampleParams p) {
+__global__ __launch_bounds__(kSliceThreads, 4) void sample_hist_kernel(SampleParams p) {
   // The last bin, which may hold most of a row, has a place for every lane:
   // atomics on one address wait for each other.
   __shared__ uint64_t hw[kBins + 64];
-  __shared__ uint32_t hc[kBins + 64];
+  __shared__ __align__(16) uint32_t hc[kBins + 64];
+  __shared__ Outbox box;
   __shared__ uint64_t mw;
   __shared__ uint32_t mc;
   const int tid = threadIdx.x;
@@ -287,34 +379,53 @@ __global__ __launch_bounds__(kSliceThreads) void sample_hist_kernel(SampleParams
   if (tid == 0) {
     mw = 0;
     mc = 0;
+    box.n = 0;
   }
   __syncthreads();
   const Row row = row_of(p, ends, t);
   Series series;
   series.load();
   const int last = kBins - 1 + (tid & 63);
-  auto count = [&](float z, uint64_t w) {
-    int b = bin_of(row, z);
+  // Elements behind the first k decide nothing and are left out, where a bin that
+  // they cannot lie in is known: most of a row then needs no exponential, and the
+  // others can be listed at once.
+  const int most = last_bin_for(p, row, r, top_k_of(p, r), hc);
+  auto count = [&](int b, uint64_t w) {
     b = b == kBins - 1 ? last : b;
     atomicAdd(&hc[b], 1u);
     atomicAdd(reinterpret_cast<unsigned long long*>(&hw[b]), static_cast<unsigned long long>(w));
   };
-  if (mp > 0.f) {
-    // The prefix of w >= min_p, as integers.
-    const uint64_t enough =
-        mp < 4.f ? static_cast<uint64_t>(ceil(static_cast<double>(mp) * __builtin_ldexp(1.0, p.shift))) : ~0ull;
-    uint32_t min_c = 0;
-    uint64_t min_w = 0;
+  // The prefix of w >= min_p, as integers.
+  const uint64_t enough =
+      mp > 0.f && mp < 4.f ? static_cast<uint64_t>(ceil(static_cast<double>(mp) * __builtin_ldexp(1.0, p.shift))) : ~0ull;
+  uint32_t min_c = 0;
+  uint64_t min_w = 0;
+  auto count_min = [&](uint64_t w) {
+    min_c += w >= enough ? 1 : 0;
+    min_w += w >= enough ? w : 0;
+  };
+  if (most < kBins - 1) {
+    each_of_slice<DT>(p, [&](float z, uint32_t i) {
+      const int b = bin_of(row, z);
+      if (b > most) return;
+      const uint64_t w = weight_of(row, series, z);
+      count_min(w);
+      count(b, w);
+      box.add(place_of(z, i), p.cands + r * p.list_cap, &p.cand_n[r], p.list_cap);
+    });
+    box.send(p.cands + r * p.list_cap, &p.cand_n[r], p.list_cap);
+  } else if (mp > 0.f) {
     each_of_slice<DT>(p, [&](float z, uint32_t) {
       const uint64_t w = weight_of(row, series, z);
-      min_c += w >= enough ? 1 : 0;
-      min_w += w >= enough ? w : 0;
-      count(z, w);
+      count_min(w);
+      count(bin_of(row, z), w);
     });
+  } else {
+    each_of_slice<DT>(p, [&](float z, uint32_t) { count(bin_of(row, z), weight_of(row, series, z)); });
+  }
+  if (mp > 0.f) {
     atomicAdd(&mc, min_c);
     atomicAdd(reinterpret_cast<unsigned long long*>(&mw), static_cast<unsigned long long>(min_w));
-  } else {
-    each_of_slice<DT>(p, [&](float z, uint32_t) { count(z, weight_of(row, series, z)); });
   }
   __syncthreads();
   if (tid > 0 && tid < 64) {
@@ -397,11 +508,7 @@ __device__ __forceinline__ uint64_t draw_goal(float u, uint64_t weight) {
   const uint64_t goal = target < static_cast<double>(weight) ? static_cast<uint64_t>(target) + 1 : weight;
   return goal < weight ? goal : weight;
 }
-// Whether a row's top-k or top-p cuts anything off.
-__device__ __forceinline__ int64_t top_k_of(const SampleParams& p, int64_t r) {
-  const int64_t k = p.top_k ? load_index(p.top_k, r, p.top_k64) : 0;
-  return k > 0 && k < p.n ? k : 0;
-}
+// A row's top-p, or 1.
 __device__ __forceinline__ float top_p_of(const SampleParams& p, int64_t r) {
   const float v = p.top_p ? p.top_p[r] : 1.f;
   return v < 1.f ? v : 1.f;
@@ -427,6 +534,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_plan_kernel(SampleParams p
   const float u = p.u[r], temperature = p.temperature[r], tp = top_p_of(p, r);
   const int64_t k = top_k_of(p, r);
   const bool has_min = p.min_p && p.min_p[r] > 0.f;
+  const uint32_t listed = p.cand_n[r];
   const Ends ends = row_ends(p, r);
   if (takes_largest(ends.top, temperature)) {
     if (tid == 0) {
@@ -510,7 +618,8 @@ __global__ __launch_bounds__(kRowThreads) void sample_plan_kernel(SampleParams p
       plan.lo[i] = lo[i];
       plan.hi[i] = hi[i];
     }
-    plan.mode = count <= static_cast<uint32_t>(p.list_cap) ? kCollect : kLong;
+    const uint32_t cap = p.list_cap;
+    plan.mode = listed > 0 && listed <= cap ? kListed : count <= cap ? kCollect : kLong;
     if (least.count == 0) {  // min_p above 1: the largest alone
       plan.mode = kDone;
       p.out[r] = index_of(ends.top);
@@ -525,37 +634,32 @@ __global__ __launch_bounds__(kRowThreads) void sample_plan_kernel(SampleParams p
 
 template <int DT>
 __global__ __launch_bounds__(kSliceThreads) void sample_collect_kernel(SampleParams p) {
-  constexpr uint32_t kLocal = 1024;  // a workgroup's elements go out together
-  __shared__ uint64_t local[kLocal];
-  __shared__ uint32_t n, base;
+  __shared__ Outbox box;
   const int tid = threadIdx.x;
   const int64_t r = blockIdx.y;
   const Plan plan = p.plan[r];
-  if (plan.mode != kCollect) return;
+  if (plan.mode != kCollect && (plan.mode != kListed || blockIdx.x > 0)) return;
   const Row row = row_of(p, row_ends(p, r), p.temperature[r]);
-  if (tid == 0) n = 0;
+  if (tid == 0) box.n = 0;
   __syncthreads();
   uint64_t* list = p.list + r * p.list_cap;
-  each_of_slice<DT>(p, [&](float z, uint32_t i) {
+  auto collect = [&](float z, uint32_t i) {
     const uint32_t b = bin_of(row, z);
     bool in = false;
 #pragma unroll
     for (int q = 0; q < 3; ++q) in = in || (b >= plan.lo[q] && b <= plan.hi[q]);
-    if (!in) return;
-    const uint32_t at = atomicAdd(&n, 1u);
-    if (at < kLocal) {
-      local[at] = place_of(z, i);
-    } else {
-      const uint32_t to = atomicAdd(&p.list_n[r], 1u);
-      if (to < static_cast<uint32_t>(p.list_cap)) list[to] = place_of(z, i);
+    if (in) box.add(place_of(z, i), list, &p.list_n[r], p.list_cap);
+  };
+  if (plan.mode == kListed) {
+    const uint32_t n = p.cand_n[r];
+    for (uint32_t i = tid; i < n; i += kSliceThreads) {
+      const uint64_t place = p.cands[r * p.list_cap + i];
+      collect(value_of(~static_cast<uint32_t>(place >> 32)), static_cast<uint32_t>(place));
     }
-  });
-  __syncthreads();
-  const uint32_t here = n < kLocal ? n : kLocal;
-  if (tid == 0 && here > 0) base = atomicAdd(&p.list_n[r], here);
-  __syncthreads();
-  for (uint32_t i = tid; i < here; i += kSliceThreads)
-    if (base + i < static_cast<uint32_t>(p.list_cap)) list[base + i] = local[i];
+  } else {
+    each_of_slice<DT>(p, collect);
+  }
+  box.send(list, &p.list_n[r], p.list_cap);
 }
 
 // Sorts E elements per thread (element e of thread t is number t * E + e),
@@ -897,7 +1001,9 @@ __global__ __launch_bounds__(kRowThreads) void sample_pick_kernel(SampleParams p
 struct Layout {
   int slices, list_cap;
   int64_t slice_elems;
-  size_t keys, hist_w, min_w, cum_w, kept_w, list, least, hist_c, min_c, cum_c, kept_c, list_n, plan, total;
+  int part_lanes;
+  size_t keys, hist_w, min_w, cum_w, kept_w, list, cands, least, parts, hist_c, min_c, cum_c, kept_c,
+      list_n, cand_n, plan, total;
 };
 
 Layout layout_of(int64_t M, int64_t N) {
@@ -923,12 +1029,17 @@ Layout layout_of(int64_t M, int64_t N) {
   l.cum_w = take(m * (kBins + 1) * 8);
   l.kept_w = take(m * 8);
   l.list = take(m * l.list_cap * 8);
+  l.cands = take(m * l.list_cap * 8);
   l.least = take(cells * 4);
+  // Up to 1024 groups of a row.
+  l.part_lanes = l.slices > 8 ? 4 : l.slices > 4 ? 2 : 1;
+  l.parts = take(cells * (kSliceThreads / l.part_lanes) * 4);
   l.hist_c = take(cells * kBins * 4);
   l.min_c = take(cells * 4);
   l.cum_c = take(m * (kBins + 1) * 4);
   l.kept_c = take(m * 4);
   l.list_n = take(m * 4);
+  l.cand_n = take(m * 4);
   l.plan = take(m * sizeof(Plan));
   l.total = at;
   return l;
@@ -1000,12 +1111,16 @@ extern "C" int ns_sample_rows(int64_t* out, const void* x, int64_t x_stride_row,
   p.cum_w = u64(l.cum_w);
   p.kept_w = u64(l.kept_w);
   p.list = u64(l.list);
+  p.cands = u64(l.cands);
   p.least = u32(l.least);
+  p.parts = u32(l.parts);
+  p.part_lanes = l.part_lanes;
   p.hist_c = u32(l.hist_c);
   p.min_c = u32(l.min_c);
   p.cum_c = u32(l.cum_c);
   p.kept_c = u32(l.kept_c);
   p.list_n = u32(l.list_n);
+  p.cand_n = u32(l.cand_n);
   p.plan = reinterpret_cast<Plan*>(ws + l.plan);
   int log = 0;
   while ((1ll << log) < N) ++log;
