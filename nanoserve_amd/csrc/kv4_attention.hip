@@ -1107,15 +1107,22 @@ Cut cut_of(int num_seqs, int64_t num_tokens, int max_seq_len, int64_t context, i
     c.dec_items = (tokens / c.dec_split + num_seqs) * num_kv_heads;
   }
   if (c.columns) {
-    // Keys are split only where the column blocks leave half of the device idle:
-    // the joining launch reads every row's partials back.  Four chunks of 512
-    // rows (227 blocks) 54 us whole, 45 + 15 in ranges of 512 keys.
+    // Keys are split only where the column blocks leave half of the device idle,
+    // and not under 256 keys or in contexts of up to 768: the partials and the
+    // launch that joins them cost 5 us and more, 300 keys' worth.  One chunk of
+    // 512 rows (head size 64 / 128): without a context 16 / 20 us whole, 19 / 28
+    // in two ranges; behind 2048 tokens 26 / 48 us in four, 32 / 55 in two; four
+    // such chunks 45 / 78 us whole, 56 / 122 in ranges of 512 keys.
     const int64_t blocks = (num_tokens * group + 64 * kColumnTiles - 1) / (64 * kColumnTiles) * num_kv_heads;
-    const int64_t want = kCUs / blocks < 1 ? 1 : kCUs / blocks;
+    const int64_t want = kCUs / blocks < 1 || longest <= 768 ? 1 : kCUs / blocks;
     const int64_t split = round_up((longest + want - 1) / want, 32);
     c.col_split = static_cast<int>(split < 256 ? 256 : split);
     c.col_n = static_cast<int>((longest + c.col_split - 1) / c.col_split);
-    c.col_waves = blocks * c.col_n <= kCUs ? 8 : 4;
+    // Eight waves where the blocks are few, up to one on each compute unit (two at
+    // head size 64).  Two chunks (112 / 224 blocks) 38 / 58 us, with four waves
+    // 44 / 71; six (342 at size 64) 48 and 59; prompts of 2048 tokens, two of them
+    // 43 and 56 (448) and 103 / 84 (896 at size 128), four 88 / 71 (896 at 64).
+    c.col_waves = blocks * c.col_n <= (head_dim == 64 ? 2 : 1) * kCUs ? 8 : 4;
     c.col_blocks = num_tokens * group / (64 * kColumnTiles) + num_seqs;
     c.col_bytes = c.col_n > 1 ? static_cast<size_t>(num_tokens) * num_heads * c.col_n * row_bytes : 0;
   }
