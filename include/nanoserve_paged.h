@@ -547,8 +547,8 @@ int ns_gather_cache_int4(void* k_out, void* v_out, const void* k_cache, const vo
  * context_tokens is the sum of the context lengths where the caller knows it,
  * else 0; it decides only how long contexts are cut for the device (and so the
  * order of sums).  one_row_seqs is the number of sequences with one query row
- * where the caller knows it (and the device's offsets say the same), else -1; a
- * batch of none, or of nothing else, needs one launch less.  workspace: 256-byte aligned,
+ * where the caller knows it, else -1; it decides only which kernel takes such
+ * rows.  No context passes 2^30 tokens.  workspace: 256-byte aligned,
  * ns_paged_attention_int4_workspace_size bytes for the same sizes (0: none is
  * needed), not initialised, not read by later calls.  Calls that overlap in
  * time need their own.  Head sizes 64 and 128 with blocks of whole 16-token

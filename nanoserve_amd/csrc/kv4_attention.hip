@@ -1084,9 +1084,11 @@ Cut cut_of(int num_seqs, int64_t num_tokens, int max_seq_len, int64_t context, i
   c.fast = (head_dim == 64 || head_dim == 128) && block_size % 16 == 0;
   if (!c.fast) return c;
   const int group = num_heads / num_kv_heads;
-  c.every_row = group > 16;
-  c.decode = !c.every_row && (decode_only || one_row != 0);
-  c.columns = c.every_row || !(decode_only || one_row == num_seqs);
+  // The column part takes one-row sequences too where the caller expects none of
+  // them: expectations shape the launches and never decide what is computed.
+  c.every_row = group > 16 || (!decode_only && one_row == 0);
+  c.decode = !c.every_row;
+  c.columns = c.every_row || !decode_only;
   const int64_t longest = max_seq_len > 0 ? max_seq_len : 1;
   const int64_t all = num_seqs * longest;
   const int64_t tokens = context > 0 && context < all ? context : all;  // of K, and of V, that a KV head reads
@@ -1220,7 +1222,8 @@ extern "C" int ns_paged_attention_int4(void* out, const void* query,
       misaligned(block_tables, block_tables_is_int64 ? 8 : 4) || misaligned(seq_lens, seq_lens_is_int64 ? 8 : 4) ||
       misaligned(query_start_loc, query_start_loc_is_int64 ? 8 : 4))
     return NS_ERR_INVALID_ARG;
-  // Rows, heads and columns are counted in 32 bits.
+  // Rows, heads, columns and a context's tokens are counted in 32 bits.
+  if (max_seq_len > 1 << 30) return NS_ERR_UNSUPPORTED;
   if (num_heads > 65535 || num_tokens > 0x7FFFFFFF / num_heads || num_seqs > 0x7FFFFFFF / num_heads)
     return NS_ERR_UNSUPPORTED;
   const Cut cut = cut_of(num_seqs, num_tokens, max_seq_len, context_tokens, one_row_seqs, is_decode_only, num_heads, num_kv_heads,

@@ -361,6 +361,29 @@ def test_one_row_of_a_longer_query_layout(d):
     _check(_run(c), c)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,hkv,d,n", [(14, 2, 64, 60), (28, 4, 128, 16), (40, 2, 64, 24)])
+def test_enough_rows_to_fill_the_device(hq, hkv, d, n, dtype):
+    """Thousands of query rows, whole prompts and chunks, with decode rows among them."""
+    rng = np.random.default_rng(d)
+    ql = [int(x) for x in rng.integers(70, 130, n)]
+    seqs = [q + int(rng.integers(0, 60)) * int(i % 3 == 0) for i, q in enumerate(ql)]
+    for i, long in ((1, 400), (2, 33), (n - 1, 1)):
+        seqs[i], ql[i] = long, 1
+    c = _case(seqs, ql, hq, hkv, d, 16, dtype)
+    _check(_run(c), c)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (28, 4, 128), (4, 2, 24)])
+@pytest.mark.parametrize("told", [[1, 1, 1], [2, 2, 2], [34, 1, 40]])
+def test_lengths_that_the_host_did_not_expect(hq, hkv, d, told):
+    """The device's lengths decide what is computed: here the host's lists are of another step."""
+    c = _case([700, 33, 90], [1, 33, 41], hq, hkv, d, 16, torch.float16)
+    c.md.query_lens_cpu = told
+    c.md.seq_lens_cpu = [1, 1, 1]
+    _check(_run(c), c)
+
+
 @pytest.mark.parametrize("d", [64, 128, 24])
 def test_empty_contexts_are_zero(d):
     c = _case([0, 3, 0], [1, 1, 1], 4, 2, d, 16, torch.float16)
@@ -518,6 +541,39 @@ def test_graph_replays_with_eager_calls_between(seqs, query_lens):
         # Both are held to float64's tolerance of each other; the splits may differ.
         assert torch.allclose(out.float(), want.float(), atol=2e-3, rtol=2e-3)
         assert torch.equal(out2, want2)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_replay_with_longer_contexts_and_other_chunks(d):
+    """A graph captured at one step's lengths and replayed at another's."""
+    first = _case([20, 9, 30], [1, 1, 30], 6, 2, d, 16, torch.float16)
+    later = _case([1500, 60, 17], [1, 30, 1], 6, 2, d, 16, torch.float16, seed=5)
+    width = max(c.md.block_tables.shape[1] for c in (first, later))
+    blocks = max(c.kc.shape[0] for c in (first, later))
+
+    def padded(c):
+        grow = lambda x: torch.cat((x, torch.zeros(blocks - x.shape[0], *x.shape[1:], dtype=x.dtype)))  # noqa: E731
+        tables = torch.zeros(3, width, dtype=c.md.block_tables.dtype)
+        tables[:, :c.md.block_tables.shape[1]] = c.md.block_tables
+        return c.q.to(DEV), grow(c.kc).to(DEV), grow(c.vc).to(DEV), tables.to(DEV)
+
+    q, kc, vc, tables = padded(first)
+    md = dataclasses.replace(md_to(first.md, DEV), block_tables=tables, max_seq_len=1500)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        paged_attention_int4(q, kc, vc, md, first.scale)
+    stream.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with graph_capture(g, stream):
+        out = paged_attention_int4(q, kc, vc, md, first.scale)
+    for c in (later, first, later, later):
+        for dst, src in zip((q, kc, vc, tables), padded(c)):
+            dst.copy_(src)
+        md.seq_lens.copy_(c.md.seq_lens)
+        md.query_start_loc.copy_(c.md.query_start_loc)
+        g.replay()
+        _check(out, c)
 
 
 def test_streams_and_repeated_calls_agree():

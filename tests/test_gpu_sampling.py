@@ -52,6 +52,32 @@ def test_matches_float64(M, N, which, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,N", [(1024, 300), (300, 9001), (200, 20011), (110, 30000), (70, 4097)])
+def test_many_rows_with_a_top_k(M, N, dtype):
+    """Every way in which rows are cut, top-k on both sides of the number of groups of threads."""
+    z = (torch.randn(M, N, generator=_g(N)) * 2.5).to(dtype)
+    u, t, k, p, mp = _settings(M, M)
+    k = torch.tensor([1, 2, 40, 400, 768, 1000, 1023, 1024, 1025, 4096, 0])[torch.arange(M) % 11]
+    _check(z, u, t, k, p, mp)
+    _check(z, u, t, k.int())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M", [2, 200])
+def test_more_equal_largest_elements_than_are_listed(M, dtype):
+    """The first bin holds from half a workgroup's share of the list to more than the whole list."""
+    N = 20000
+    z = torch.randn(M, N, generator=_g(1))
+    for r in range(M):
+        n = (500, 1025, 3000, 4096, 4097, 20000)[r % 6]
+        z[r, r:r + n] = 9.0                                 # side by side: one slice's
+        z[r, torch.randperm(N, generator=_g(r))[:n // 2]] = 9.0
+    z[0, 5:9] = -torch.inf
+    u, t, _, p, mp = _settings(M, 3)
+    _check(z.to(dtype), u, t, torch.tensor([50, 3, 1000, 700])[torch.arange(M) % 4], p, mp)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_equal_logits_and_few_values(dtype):
     """Bins that hold far more elements than the last stage sorts at once."""
     N = 60000

@@ -180,7 +180,7 @@ def _attend_args(**over):
     (dict(vc=20), INV), (dict(sl=18), INV), (dict(bt=20, bt64=1), INV), (dict(scale=float("nan")), INV),
     (dict(scale=float("inf")), INV), (dict(context=-1), INV), (dict(ones=3), INV), (dict(ones=-2), INV),
     (dict(D=60), UNS), (dict(D=264), UNS), (dict(bs=18), UNS), (dict(dtype=_lib.NS_DTYPE_F32), UNS),
-    (dict(T=1 << 28, S=1 << 28), UNS),
+    (dict(T=1 << 28, S=1 << 28), UNS), (dict(maxs=(1 << 30) + 1), UNS),
     (dict(maxs=4096, bt_width=256, bt_stride=256), _lib.NS_ERR_WORKSPACE),
     (dict(maxs=4096, bt_width=256, bt_stride=256, ws=256, ws_bytes=1000), _lib.NS_ERR_WORKSPACE),
     (dict(maxs=4096, bt_width=256, bt_stride=256, ws=128, ws_bytes=1 << 30), _lib.NS_ERR_WORKSPACE),
