@@ -163,7 +163,8 @@ class Sequence:
         """The uniform number in [0, 1) that draws output token `index`."""
         if self._uniform is None or len(self._uniform) <= index:
             seed = self.seq_id if self.sampling.seed is None else self.sampling.seed
-            n = max(self.sampling.max_new_tokens, index + 1)
+            # A longer series starts with the shorter one's numbers.
+            n = max(64, 1 << index.bit_length())
             self._uniform = np.random.default_rng(seed).random(n, dtype=np.float32)
         return self._uniform[index]
 

@@ -33,6 +33,14 @@ def test_uniform_numbers_follow_the_seed_and_the_index_alone():
     assert a.uniform(20) < 1 and [a.uniform(i) for i in range(5)] == u  # past the length: the same start
 
 
+def test_a_request_without_an_end_holds_no_more_numbers_than_it_has_used():
+    a = Sequence(0, [1], SamplingParams(max_new_tokens=1 << 40, temperature=1.0, seed=2))
+    b = Sequence(1, [1], SamplingParams(temperature=1.0, seed=2))
+    b.uniform(5000)
+    assert [a.uniform(i) for i in range(300)] == [b.uniform(i) for i in range(300)]
+    assert len(a._uniform) < 1024
+
+
 def test_staged_settings_are_the_requests():
     inputs = SamplerInputs(torch.device("cpu"), rows=2)
     seqs = [Sequence(i, [1], SamplingParams(temperature=0.5 + i, top_k=1 << (8 * i), top_p=0.9, min_p=0.1 * i, seed=i))
