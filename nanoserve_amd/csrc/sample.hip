@@ -38,7 +38,7 @@
 // 3.7 and 6.2 us); for many the three passes over the logits, of which the second
 // evaluates a float64 exponential (about 40 operations) for every element of the
 // rows without a top-k.  256 rows of 152K float32, three quarters with a top-k of
-// 20 to 400: 31 (5.1 TB/s), 45, 8.6, 28 and 16 us; with every element counted and
+// 20 to 400: 31 (5.1 TB/s), 45, 8.6, 20 and 16 us; with every element counted and
 // collected from the slices 31, 58, 8.5, 35 and 16.
 #include <math.h>
 
@@ -75,6 +75,7 @@ struct SampleParams {
   const float* min_p;      // or null
   int slices;
   int64_t slice_elems;     // a multiple of 8
+  int64_t collect_elems;   // the same of the fourth stage's slices
   int shift;               // weights are w * 2^shift
   double zero_below;       // ln w below which a weight rounds to 0
   uint64_t* keys;          // [rows, slices]: the largest element's
@@ -243,9 +244,9 @@ __device__ __forceinline__ int64_t top_k_of(const SampleParams& p, int64_t r) {
 
 // f(value, index) for the workgroup's slice of row blockIdx.y.
 template <int DT, class F>
-__device__ __forceinline__ void each_of_slice(const SampleParams& p, F f) {
-  const int64_t s0 = static_cast<int64_t>(blockIdx.x) * p.slice_elems;
-  const int64_t s1 = s0 + p.slice_elems < p.n ? s0 + p.slice_elems : p.n;
+__device__ __forceinline__ void each_of_slice(const SampleParams& p, int64_t elems, F f) {
+  const int64_t s0 = static_cast<int64_t>(blockIdx.x) * elems;
+  const int64_t s1 = s0 + elems < p.n ? s0 + elems : p.n;
   each_element<DT, kSliceThreads>(p.x + static_cast<int64_t>(blockIdx.y) * p.row_bytes, s0, s1, f);
 }
 
@@ -255,7 +256,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_ends_kernel(SampleParams
   __shared__ uint32_t wl[kSliceThreads / 64];
   uint64_t best = 0;
   uint32_t least = kNanOrder;
-  each_of_slice<DT>(p, [&](float v, uint32_t i) {
+  each_of_slice<DT>(p, p.slice_elems, [&](float v, uint32_t i) {
     const uint64_t k = key_of(v, i);
     best = max_u64(best, k);
     const uint32_t ord = static_cast<uint32_t>(k >> 32);
@@ -405,7 +406,7 @@ __global__ __launch_bounds__(kSliceThreads, 4) void sample_hist_kernel(SamplePar
     min_w += w >= enough ? w : 0;
   };
   if (most < kBins - 1) {
-    each_of_slice<DT>(p, [&](float z, uint32_t i) {
+    each_of_slice<DT>(p, p.slice_elems, [&](float z, uint32_t i) {
       const int b = bin_of(row, z);
       if (b > most) return;
       const uint64_t w = weight_of(row, series, z);
@@ -415,13 +416,13 @@ __global__ __launch_bounds__(kSliceThreads, 4) void sample_hist_kernel(SamplePar
     });
     box.send(p.cands + r * p.list_cap, &p.cand_n[r], p.list_cap);
   } else if (mp > 0.f) {
-    each_of_slice<DT>(p, [&](float z, uint32_t) {
+    each_of_slice<DT>(p, p.slice_elems, [&](float z, uint32_t) {
       const uint64_t w = weight_of(row, series, z);
       count_min(w);
       count(bin_of(row, z), w);
     });
   } else {
-    each_of_slice<DT>(p, [&](float z, uint32_t) { count(bin_of(row, z), weight_of(row, series, z)); });
+    each_of_slice<DT>(p, p.slice_elems, [&](float z, uint32_t) { count(bin_of(row, z), weight_of(row, series, z)); });
   }
   if (mp > 0.f) {
     atomicAdd(&mc, min_c);
@@ -657,7 +658,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_collect_kernel(SamplePar
       collect(value_of(~static_cast<uint32_t>(place >> 32)), static_cast<uint32_t>(place));
     }
   } else {
-    each_of_slice<DT>(p, collect);
+    each_of_slice<DT>(p, p.collect_elems, collect);
   }
   box.send(list, &p.list_n[r], p.list_cap);
 }
@@ -999,8 +1000,8 @@ __global__ __launch_bounds__(kRowThreads) void sample_pick_kernel(SampleParams p
 
 // How the rows are cut, and where the workspace's parts lie (byte offsets).
 struct Layout {
-  int slices, list_cap;
-  int64_t slice_elems;
+  int slices, collect_slices, list_cap;
+  int64_t slice_elems, collect_elems;
   int part_lanes;
   size_t keys, hist_w, min_w, cum_w, kept_w, list, cands, least, parts, hist_c, min_c, cum_c, kept_c,
       list_n, cand_n, plan, total;
@@ -1008,13 +1009,19 @@ struct Layout {
 
 Layout layout_of(int64_t M, int64_t N) {
   Layout l;
-  // About four workgroups for each compute unit, up to 16 slices of at least 2048 elements.
-  int64_t slices = 1024 / M < 1 ? 1 : 1024 / M;
-  slices = slices > 16 ? 16 : slices;
-  const int64_t most = (N + 2047) / 2048;
-  slices = slices > most ? most : slices;
-  l.slice_elems = ((N + slices - 1) / slices + 7) / 8 * 8;
-  l.slices = static_cast<int>((N + l.slice_elems - 1) / l.slice_elems);
+  // About four workgroups for each compute unit, up to 16 slices of at least 2048
+  // elements.  Twice as many where only some rows are read (256 rows: 20 us, 27 with
+  // four).
+  auto cut = [&](int64_t groups, int& slices, int64_t& elems) {
+    int64_t n = groups / M < 1 ? 1 : groups / M;
+    n = n > 16 ? 16 : n;
+    const int64_t most = (N + 2047) / 2048;
+    n = n > most ? most : n;
+    elems = ((N + n - 1) / n + 7) / 8 * 8;
+    slices = static_cast<int>((N + elems - 1) / elems);
+  };
+  cut(1024, l.slices, l.slice_elems);
+  cut(2048, l.collect_slices, l.collect_elems);
   l.list_cap = N < kList ? static_cast<int>(N) : kList;
   size_t at = 0;
   const size_t m = static_cast<size_t>(M), cells = m * l.slices;
@@ -1048,16 +1055,16 @@ Layout layout_of(int64_t M, int64_t N) {
 bool misaligned(const void* p, unsigned n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }
 
 template <int DT>
-hipError_t launch(SampleParams& p, int64_t M, hipStream_t st) {
+hipError_t launch(SampleParams& p, int64_t M, int collect_slices, hipStream_t st) {
   void* args[] = {&p};
   const unsigned m = static_cast<unsigned>(M);
-  const dim3 slices(static_cast<unsigned>(p.slices), m);
   const void* by_slice[] = {reinterpret_cast<const void*>(&sample_ends_kernel<DT>),
                             reinterpret_cast<const void*>(&sample_hist_kernel<DT>), nullptr,
                             reinterpret_cast<const void*>(&sample_collect_kernel<DT>), nullptr};
   const void* by_row[] = {nullptr, nullptr, reinterpret_cast<const void*>(&sample_plan_kernel), nullptr,
                           reinterpret_cast<const void*>(&sample_pick_kernel<DT>)};
   for (int i = 0; i < 5; ++i) {
+    const dim3 slices(static_cast<unsigned>(i == 3 ? collect_slices : p.slices), m);
     const hipError_t e = by_slice[i] ? hipLaunchKernel(by_slice[i], slices, dim3(kSliceThreads), args, 0, st)
                                      : hipLaunchKernel(by_row[i], dim3(m), dim3(kRowThreads), args, 0, st);
     if (e != hipSuccess) return e;
@@ -1104,6 +1111,7 @@ extern "C" int ns_sample_rows(int64_t* out, const void* x, int64_t x_stride_row,
   auto u32 = [&](size_t at) { return reinterpret_cast<uint32_t*>(ws + at); };
   p.slices = l.slices;
   p.slice_elems = l.slice_elems;
+  p.collect_elems = l.collect_elems;
   p.list_cap = l.list_cap;
   p.keys = u64(l.keys);
   p.hist_w = u64(l.hist_w);
@@ -1127,8 +1135,8 @@ extern "C" int ns_sample_rows(int64_t* out, const void* x, int64_t x_stride_row,
   p.shift = 62 - log < 51 ? 62 - log : 51;
   p.zero_below = -(p.shift + 1) * 0.6931471805599453;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  const hipError_t e = dtype == NS_DTYPE_F32   ? launch<NS_DTYPE_F32>(p, M, st)
-                       : dtype == NS_DTYPE_F16 ? launch<NS_DTYPE_F16>(p, M, st)
-                                               : launch<NS_DTYPE_BF16>(p, M, st);
+  const hipError_t e = dtype == NS_DTYPE_F32   ? launch<NS_DTYPE_F32>(p, M, l.collect_slices, st)
+                       : dtype == NS_DTYPE_F16 ? launch<NS_DTYPE_F16>(p, M, l.collect_slices, st)
+                                               : launch<NS_DTYPE_BF16>(p, M, l.collect_slices, st);
   return e == hipSuccess ? NS_OK : NS_ERR_HIP;
 }
