@@ -433,25 +433,27 @@ struct Wave {
     }
   }
 
-  // Makes a slot's parameters; its tokens from `valid` on are nobody's.  Gives
-  // this lane's word of V, the scale in the upper half, or 0.
-  __device__ __forceinline__ uint32_t convert(const char* slot, Params& params, int lane, int valid) const {
-    uint32_t word = *reinterpret_cast<const uint32_t*>(slot + Slot<D>::par + lane * 4);
+  // Makes a slot's parameters; its tokens from `valid` on are nobody's.
+  __device__ __forceinline__ void convert(char* slot, Params& params, int lane, int valid) const {
+    uint32_t& at = *reinterpret_cast<uint32_t*>(slot + Slot<D>::par + lane * 4);
+    uint32_t word = at;
     const bool of_v = lane >= 32;
-    if ((lane & 31) >= valid) word = 0;
+    if (valid < 32) {
+      if ((lane & 31) >= valid) word = 0;
+      at = word;
+    }
     const float sc = kv4_scale<DT>(word), of = kv4_offset<DT>(word);
     params.first[lane] = of_v ? sc : sc * cf;
     params.second[lane] = of_v ? __builtin_fmaf(8.f, sc, of) : of * cf;
-    return of_v ? word : 0;
   }
 
   // One step over tokens tok .. tok + 31.  MASK: some column does not see all of
-  // them; column n sees tokens up to limit[n].  big: at least the largest of the
-  // step's parameter words of V, on some lane.
+  // them; column n sees tokens up to limit[n].
   template <bool MASK>
-  __device__ __forceinline__ void step(const char* slot, const Params& params, uint32_t big, int lane, int tok, int g,
+  __device__ __forceinline__ void step(const char* slot, const Params& params, int lane, int tok, int g,
                                        const int (&limit)[NT]) {
     Tiles<D> k, v;
+    const uint32_t big = *reinterpret_cast<const uint32_t*>(slot + Slot<D>::par + 128 + (lane & 31) * 4);
     // K for D = 128 and V lie in lane order; a tile of K at D = 64 row after row.
     k.read_codes(slot, D == 128 ? lane * 16 : (lane & 15) * 32 + g * 8);
     if (__builtin_expect(__builtin_amdgcn_ballot_w64(big > top) != 0, 0)) raise_sigma(big);
@@ -640,18 +642,18 @@ __device__ __forceinline__ void run_keys(Wave<DT, D, 1>& w, const Kv4AttnParams&
   for (; tok + 32 <= end; tok += stride, ++i) {
     char* slot = ring + (i & (R - 1)) * Slot<D>::bytes;
     vector_wait<(R - 1) * Slot<D>::loads>();
-    const uint32_t big = w.convert(slot, params, lane, 32);
+    w.convert(slot, params, lane, 32);
     __builtin_amdgcn_wave_barrier();
-    w.template step<false>(slot, params, big, lane, tok, g, limit);
+    w.template step<false>(slot, params, lane, tok, g, limit);
     __builtin_amdgcn_wave_barrier();
     feed.issue(i + R, slot);
   }
   for (; tok < end; tok += stride, ++i) {
     char* slot = ring + (i & (R - 1)) * Slot<D>::bytes;
     vector_wait<(R - 1) * Slot<D>::loads>();
-    const uint32_t big = w.convert(slot, params, lane, last + 1 - tok);
+    w.convert(slot, params, lane, last + 1 - tok);
     __builtin_amdgcn_wave_barrier();
-    w.template step<true>(slot, params, big, lane, tok, g, limit);
+    w.template step<true>(slot, params, lane, tok, g, limit);
     __builtin_amdgcn_wave_barrier();
     feed.issue(i + R, slot);
   }
@@ -821,7 +823,7 @@ __global__ __launch_bounds__(64 * W, W == 4 ? kDecodeGroups : 2) void kv4_decode
   one_rows<DT>(p, lds, blockIdx.x, gridDim.x);
 }
 
-constexpr int kColumnTiles = 2;
+constexpr int kColumnBuffers = 2;  // of chunks; three or four are no faster
 
 // Rows of longer queries: four waves of 16 NT flattened (query row, head) columns
 // each of one (sequence, KV head), side by side over a range of its keys.  They
@@ -835,10 +837,9 @@ struct ColumnState {
   struct Buffer {
     char slots[W][Slot<D>::bytes];
     Params params[W];
-    uint32_t big[W];
   };
   union {
-    Buffer buffers[2];
+    Buffer buffers[kColumnBuffers];
     float states[W == 8 ? 4 : 1][cells * 64];
   };
 };
@@ -893,7 +894,7 @@ __device__ __forceinline__ void columns(const Kv4AttnParams& p, ColumnState<D, N
     query[n] = p.query + (row[n] * p.num_heads + head[n]) * (D * 2);
   }
   w.load_queries(query, g, p.scale, [&](float big) {
-    uint32_t* const each = buffers[1].big;
+    uint32_t* const each = reinterpret_cast<uint32_t*>(&buffers[1].params);
     if (lane == 0) each[wave] = __float_as_uint(big);  // not negative: ordered as its bits
     __syncthreads();
     for (int i = 0; i < W; ++i) big = fmaxf(big, __uint_as_float(each[i]));
@@ -905,24 +906,27 @@ __device__ __forceinline__ void columns(const Kv4AttnParams& p, ColumnState<D, N
     const int whole = all_see + 1 < end ? all_see + 1 : end;
     const int mine = t0 + 32 * wave;
     Feed<DT, D> feed = {p, s, kvh, lane, mine, 32 * W, chunks, block_last >> 4, {}};
-    feed.issue(0, buffers[0].slots[wave]);
+    constexpr int kAhead = kColumnBuffers - 1;  // chunks on their way
+#pragma unroll
+    for (int c = 0; c < kAhead; ++c) feed.issue(c, buffers[c].slots[wave]);
+    int at = 0;
     for (int c = 0; c < chunks; ++c) {
-      auto& now = buffers[c & 1];
-      vector_wait<0>();
-      const uint32_t word = w.convert(now.slots[wave], now.params[wave], lane, block_last + 1 - (mine + c * 32 * W));
-      const uint32_t most = wave_max_u32(word);
-      if (lane == 0) now.big[wave] = most;
+      auto& now = buffers[at];
+      vector_wait<(kAhead - 1) * Slot<D>::loads>();
+      w.convert(now.slots[wave], now.params[wave], lane, block_last + 1 - (mine + c * 32 * W));
       __syncthreads();  // this chunk is there, and the one before is done with
-      if (c + 1 < chunks) feed.issue(c + 1, buffers[(c + 1) & 1].slots[wave]);
+      feed.issue(c + kAhead, buffers[at == 0 ? kAhead : at - 1].slots[wave]);
+      at = at == kAhead ? 0 : at + 1;
       int i = W == 8 ? (wave >> 2) * 4 : 0;
       const int to = i + 4;
       int tok = t0 + (c * W + i) * 32;
       // Steps that every column sees whole, then the others.
       for (; i < to && tok + 32 <= whole; ++i, tok += 32)
-        w.template step<false>(now.slots[i], now.params[i], now.big[i], lane, tok, g, limit);
+        w.template step<false>(now.slots[i], now.params[i], lane, tok, g, limit);
       for (; i < to && tok < end; ++i, tok += 32)
-        w.template step<true>(now.slots[i], now.params[i], now.big[i], lane, tok, g, limit);
+        w.template step<true>(now.slots[i], now.params[i], lane, tok, g, limit);
     }
+    vector_wait<0>();  // nothing lands in the buffers behind their use
   }
 
   // A column's outputs and sum, not yet divided.
@@ -991,7 +995,7 @@ __device__ __forceinline__ void columns(const Kv4AttnParams& p, ColumnState<D, N
 // those leave compute units idle, at the start or towards the end, workgroups of
 // one-row sequences.
 template <class DT, int D, int NT, int W>
-__global__ __launch_bounds__(64 * W, 2) void kv4_columns_kernel(Kv4AttnParams p) {
+__global__ __launch_bounds__(64 * W, D == 64 ? (NT == 1 ? 4 : W == 4 ? 3 : 2) : 2) void kv4_columns_kernel(Kv4AttnParams p) {
   constexpr int R = W == 4 ? kDecodeRing<D> : 2;
   union Lds {
     ColumnState<D, NT, W> columns;
@@ -1075,7 +1079,7 @@ struct Cut {
   int dec_split, dec_n;         // tokens per range and ranges of one-row sequences
   int64_t dec_items;            // ranges of all of them, about
   int col_split, col_n;         // the same of longer queries
-  int col_waves;                // waves of a workgroup of the column kernel
+  int col_waves, col_tiles;     // waves of a workgroup of the column kernel, column tiles of a wave
   int64_t col_blocks;           // column blocks of all queries, at most
   size_t dec_bytes, col_bytes;  // partials
 };
@@ -1113,23 +1117,31 @@ Cut cut_of(int num_seqs, int64_t num_tokens, int max_seq_len, int64_t context, i
     c.dec_items = (tokens / c.dec_split + num_seqs) * num_kv_heads;
   }
   if (c.columns) {
-    // Keys are split only where the column blocks leave half of the device idle,
-    // and not under 256 keys or in contexts of up to 768: the partials and the
-    // launch that joins them cost 5 us and more, 300 keys' worth.  One chunk of
-    // 512 rows (head size 64 / 128): without a context 16 / 20 us whole, 19 / 28
-    // in two ranges; behind 2048 tokens 26 / 48 us in four, 32 / 55 in two; four
-    // such chunks 45 / 78 us whole, 56 / 122 in ranges of 512 keys.
-    const int64_t blocks = (num_tokens * group + 64 * kColumnTiles - 1) / (64 * kColumnTiles) * num_kv_heads;
+    // Column tiles of a wave: one needs a fifth more vector operations than two
+    // (a step's codes are unpacked for half as many columns) and gives twice the
+    // blocks.  Waves: eight, four on either half of the keys, or four.  Vector
+    // issue bounds all of them once a SIMD has two waves, so few rows want many
+    // blocks of eight waves, up to one on each compute unit (two at head size 64,
+    // where two fit).  Head size 64 / 128, us, one tile and two: a chunk of 512 rows
+    // 12.6 / 15.3 and 16.3 / 20.3, behind 2100 tokens 27 / 40 and 27 / 48, two such
+    // chunks 34 and 39 (size 64), four 40 and 44.  Two tiles, eight waves and four:
+    // six chunks (342 blocks, size 64) 47 and 59, two prompts of 2048 (448 blocks,
+    // size 64) 43 and 56, but (896, size 128) 103 and 84, four (896, size 64) 88 and 71.
+    auto count = [&](int tiles) { return (num_tokens * group + 64 * tiles - 1) / (64 * tiles) * num_kv_heads; };
+    const int64_t few = (head_dim == 64 ? 2 : 1) * kCUs;
+    c.col_tiles = count(1) <= few ? 1 : 2;
+    const int64_t blocks = count(c.col_tiles);
+    c.col_waves = blocks <= few ? 8 : 4;
+    // Keys are split only where the blocks leave half of the device idle, and not
+    // under 256 keys or in contexts of up to 768: the partials and the launch that
+    // joins them cost 5 us and more, 300 keys' worth.  Four chunks of 512 rows
+    // (size 64 / 128) 45 / 78 us whole, 56 / 122 in ranges of 512 keys; ranges of
+    // the longer half of such contexts alone make a second round, 62 to 76 / 87 to 104.
     const int64_t want = kCUs / blocks < 1 || longest <= 768 ? 1 : kCUs / blocks;
     const int64_t split = round_up((longest + want - 1) / want, 32);
     c.col_split = static_cast<int>(split < 256 ? 256 : split);
     c.col_n = static_cast<int>((longest + c.col_split - 1) / c.col_split);
-    // Eight waves where the blocks are few, up to one on each compute unit (two at
-    // head size 64).  Two chunks (112 / 224 blocks) 38 / 58 us, with four waves
-    // 44 / 71; six (342 at size 64) 48 and 59; prompts of 2048 tokens, two of them
-    // 43 and 56 (448) and 103 / 84 (896 at size 128), four 88 / 71 (896 at 64).
-    c.col_waves = blocks <= (head_dim == 64 ? 2 : 1) * kCUs ? 8 : 4;
-    c.col_blocks = num_tokens * group / (64 * kColumnTiles) + num_seqs;
+    c.col_blocks = num_tokens * group / (64 * c.col_tiles) + num_seqs;
     c.col_bytes = c.col_n > 1 ? static_cast<size_t>(num_tokens) * num_heads * c.col_n * row_bytes : 0;
   }
   return c;
@@ -1166,8 +1178,9 @@ hipError_t launch_fast(Kv4AttnParams p, const Cut& c, char* workspace, hipStream
     const int64_t groups = c.col_blocks * p.num_kv_heads * c.col_n;
     if (groups > 0x7FFFFFFF) return hipErrorInvalidValue;
     p.column_groups = static_cast<int>(groups);
-    const void* fn = c.col_waves == 8 ? reinterpret_cast<const void*>(&kv4_columns_kernel<DT, D, kColumnTiles, 8>)
-                                      : reinterpret_cast<const void*>(&kv4_columns_kernel<DT, D, kColumnTiles, 4>);
+    const void* fn = c.col_tiles == 1   ? reinterpret_cast<const void*>(&kv4_columns_kernel<DT, D, 1, 8>)
+                     : c.col_waves == 8 ? reinterpret_cast<const void*>(&kv4_columns_kernel<DT, D, 2, 8>)
+                                        : reinterpret_cast<const void*>(&kv4_columns_kernel<DT, D, 2, 4>);
     e = launch(fn, groups + row_groups, p, st, 64 * c.col_waves);
     if (e == hipSuccess && c.col_n > 1)
       e = launch(reinterpret_cast<const void*>(&kv4_merge_kernel<DT, D, false>), (p.num_tokens * p.num_heads + 3) / 4, p, st);

@@ -362,7 +362,7 @@ def test_one_row_of_a_longer_query_layout(d):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("hq,hkv,d,n", [(14, 2, 64, 60), (28, 4, 128, 16), (40, 2, 64, 24)])
+@pytest.mark.parametrize("hq,hkv,d,n", [(14, 2, 64, 60), (14, 2, 64, 30), (28, 4, 128, 16), (28, 4, 128, 8), (40, 2, 64, 24)])
 def test_enough_rows_to_fill_the_device(hq, hkv, d, n, dtype):
     """Thousands of query rows, whole prompts and chunks, with decode rows among them."""
     rng = np.random.default_rng(d)
