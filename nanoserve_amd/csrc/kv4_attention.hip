@@ -355,8 +355,10 @@ struct Wave {
   // all: the largest of those who share parameters, from this wave's.
   template <class All>
   __device__ __forceinline__ void load_queries(const char* const (&row)[NT], int g, float scale, All all) {
+    // Without their signs, halves are ordered as their bits are.
+    using u16x2 = unsigned short __attribute__((ext_vector_type(2)));
     uint32_t x[NT][D / 8];
-    float big = 0.f;
+    u16x2 bits = {0, 0};
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -365,11 +367,24 @@ struct Wave {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           x[n][4 * w + e] = r[e];
-          const float lo = fabsf(Half<DT>::to_f32(r[e] & 0xFFFFu)), hi = fabsf(Half<DT>::to_f32(r[e] >> 16));
-          big = fmaxf(big, fmaxf(lo < INFINITY ? lo : 0.f, hi < INFINITY ? hi : 0.f));
+          bits = __builtin_elementwise_max(bits, __builtin_bit_cast(u16x2, r[e] & 0x7FFF7FFFu));
         }
       }
     }
+    uint32_t most = max(static_cast<uint32_t>(bits[0]), static_cast<uint32_t>(bits[1]));
+    const uint32_t inf = DT::code == NS_DTYPE_F16 ? 0x7C00u : 0x7F80u;
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(most >= inf) != 0, 0)) {
+      most = 0;  // of the finite elements
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const uint32_t lo = x[n][i] & 0x7FFFu, hi = (x[n][i] >> 16) & 0x7FFFu;
+          most = max(most, max(lo < inf ? lo : 0u, hi < inf ? hi : 0u));
+        }
+      }
+    }
+    float big = Half<DT>::to_f32(most);
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor(big, off));
     big = all(big);
