@@ -215,9 +215,10 @@ hipError_t launch_generic(const Kv4AttnParams& p, hipStream_t stream) {
 // several steps ahead.  A lane's part of a tile is one LDS read (8 or 16 bytes),
 // and a mask turns its words into operands (kv4.h).  Both
 // model dtypes run in float16: the codes are exact there, the query is brought
-// into its range by a power of two for the wave's columns (exact but for
-// elements below 2^-25 of the largest, whose error is below 2^-36 of it), and
-// the probabilities keep 11 bits where bfloat16 would keep 8.
+// into its range by a power of two for the columns that share a workgroup (exact
+// but for elements below 2^-25 of the largest, whose error is below 2^-36 of it;
+// bfloat16 rows beyond 2^16 by a power of their own besides), and the
+// probabilities keep 11 bits where bfloat16 would keep 8.
 //
 // A score in log2 units is two fused multiply-adds, s_t (q.c_t) + (b_t sum(q) -
 // reference), with the softmax scale in s_t and b_t: the reference is the
@@ -321,6 +322,7 @@ constexpr float kCodeUnit = 16777216.f;  // 2^24: an even dim's code as a half's
 // [2^kLift, 2^(kLift + kSlack)] and fits a half: the reference (and with it the
 // accumulators) moves only when a score passes it by that much.
 constexpr float kLift = 6.f, kSlack = 8.f;
+constexpr float kEven = 65536.f;  // more than any float16
 
 // One wave's state: NT tiles of 16 columns, D output dims each.
 template <class DT, int D, int NT>
@@ -332,6 +334,8 @@ struct Wave {
   float l[NT], b[NT];         // sum p (this lane's tokens), sum p (b_t + 8 s_t) (likewise)
   floatx4 acc[NT][D / 16];
   floatx4 mid[NT];            // the same of a dim whose every code is 8
+  bool uneven;                // some column's q was divided by far[column], in LDS, beforehand
+  const float* far;
   float sigma, inv_sigma;     // the scales' power of two
   uint32_t top;               // largest parameter word that needs no larger sigma
 
@@ -352,9 +356,11 @@ struct Wave {
   // The columns' query rows, as the operands that meet the codes: lane group g
   // holds dims (D / 4) g .. + D / 4, eight of them per 32-dim step in the order
   // of a word's masked nibbles, odd dims a sixteenth of their value.
-  // all: the largest of those who share parameters, from this wave's.
+  // all: the largest of those who share parameters, from this wave's.  spare: 16 NT
+  // floats of LDS, this wave's.
   template <class All>
-  __device__ __forceinline__ void load_queries(const char* const (&row)[NT], int g, float scale, All all) {
+  __device__ __forceinline__ void load_queries(const char* const (&row)[NT], int g, float scale, float* spare,
+                                               All all) {
     // Without their signs, halves are ordered as their bits are.
     using u16x2 = unsigned short __attribute__((ext_vector_type(2)));
     uint32_t x[NT][D / 8];
@@ -385,10 +391,40 @@ struct Wave {
       }
     }
     float big = Half<DT>::to_f32(most);
+    // A bfloat16 query may hold a row so large that the others would vanish beside
+    // it in float16: columns past kEven are divided by a power of two of their own,
+    // which their scores are given back.
+    uneven = false;
+    far = spare;
+    if constexpr (DT::code != NS_DTYPE_F16) {
+      uneven = __builtin_amdgcn_ballot_w64(big > kEven) != 0;
+      if (__builtin_expect(uneven, 0)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          uint32_t top = 0;
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            const uint32_t lo = x[n][i] & 0x7FFFu, hi = (x[n][i] >> 16) & 0x7FFFu;
+            top = max(top, max(lo < inf ? lo : 0u, hi < inf ? hi : 0u));
+          }
+          top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
+          top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
+          const float above = Half<DT>::to_f32(top) * (2.f / kEven);
+          const float by = above > 2.f ? __uint_as_float(__float_as_uint(above) & 0x7F800000u) : 1.f;
+          spare[16 * n + (threadIdx.x & 15)] = by;  // the same from a column's four lanes
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            const float lo = Half<DT>::to_f32(x[n][i] & 0xFFFFu) / by, hi = Half<DT>::to_f32(x[n][i] >> 16) / by;
+            x[n][i] = Half<DT>::from_f32(lo) | (Half<DT>::from_f32(hi) << 16);
+          }
+        }
+        big = fminf(big, kEven);
+      }
+    }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) big = fmaxf(big, __shfl_xor(big, off));
     big = all(big);
-    // The largest finite element becomes 2^14 .. 2^15.
+    // The largest finite element (or kEven) becomes 2^14 .. 2^15.
     int e = 14 - (static_cast<int>(__float_as_uint(big) >> 23) - 127);
     e = e < -113 ? -113 : e > 100 ? 100 : e;
     float f = __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
@@ -414,6 +450,7 @@ struct Wave {
         }
       }
       qs[n] = group4_sum(sum) * (1.f / kCodeUnit);
+      if (DT::code != NS_DTYPE_F16 && __builtin_expect(uneven, 0)) qs[n] *= far[16 * n + (threadIdx.x & 15)];
     }
   }
 
@@ -505,13 +542,16 @@ struct Wave {
           most = fmaxf(most, seen(j, r) ? x[n][j][r] : -INFINITY);
         }
       }
-      if (__builtin_expect(__builtin_amdgcn_ballot_w64(most > kLift + kSlack) != 0, 0)) {
+      const bool anew = __builtin_amdgcn_ballot_w64(most > kLift + kSlack) != 0 ||
+                        (DT::code != NS_DTYPE_F16 && uneven);  // whose scores are made here alone
+      if (__builtin_expect(anew, 0)) {
+        const float by = DT::code != NS_DTYPE_F16 && uneven ? far[16 * n + (lane & 15)] : 1.f;
         most = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            x[n][j][r] = __builtin_fmaf(ks[j][r], s[n][j][r], kb[j][r] * qs[n]);
+            x[n][j][r] = __builtin_fmaf(ks[j][r], s[n][j][r] * by, kb[j][r] * qs[n]);
             most = fmaxf(most, seen(j, r) ? x[n][j][r] : -INFINITY);
           }
         }
@@ -737,7 +777,7 @@ template <int D, int W, int R>
 struct RowState {
   static constexpr int ring = R * Slot<D>::bytes;
   static_assert(ring >= 16 * (D + 4) * 4, "the outputs lie in the ring");
-  float m[W][16], l[W][16];
+  float m[W][16], l[W][16], far[W][16];
   Params params[W];
   // A wave's ring, and behind its keys its unnormalised outputs: 16 columns,
   // whose stores the four floats keep on different banks.
@@ -767,7 +807,7 @@ __device__ __forceinline__ void one_rows(const Kv4AttnParams& p, RowState<D, W, 
     w.init();
     const int head = kvh * p.group + (col < p.group ? col : p.group - 1);
     const char* const query[1] = {p.query + (row0 * p.num_heads + head) * (D * 2)};
-    w.load_queries(query, g, p.scale, [](float big) { return big; });
+    w.load_queries(query, g, p.scale, lds.far[wave], [](float big) { return big; });
     run_keys<R>(w, p, lds.rings[wave], lds.params[wave], s, kvh, lane, t0 + 32 * wave, t1, 32 * W, len - 1);
     const float l = group4_sum(w.l[0]), b = group4_sum(w.b[0]);
     if (g == 0) {
@@ -853,6 +893,7 @@ struct ColumnState {
     char slots[W][Slot<D>::bytes];
     Params params[W];
   };
+  float far[W][16 * NT];
   union {
     Buffer buffers[kColumnBuffers];
     float states[W == 8 ? 4 : 1][cells * 64];
@@ -908,7 +949,7 @@ __device__ __forceinline__ void columns(const Kv4AttnParams& p, ColumnState<D, N
     limit[n] = len - ql + j;
     query[n] = p.query + (row[n] * p.num_heads + head[n]) * (D * 2);
   }
-  w.load_queries(query, g, p.scale, [&](float big) {
+  w.load_queries(query, g, p.scale, lds.far[wave], [&](float big) {
     uint32_t* const each = reinterpret_cast<uint32_t*>(&buffers[1].params);
     if (lane == 0) each[wave] = __float_as_uint(big);  // not negative: ordered as its bits
     __syncthreads();

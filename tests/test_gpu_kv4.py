@@ -453,6 +453,31 @@ def test_query_sizes(size):
         _check(_run(c), c)
 
 
+@pytest.mark.parametrize("d", [64, 128, 24])
+@pytest.mark.parametrize("dtype,size", [(torch.float16, 6e4), (torch.bfloat16, 6e4), (torch.bfloat16, 3e7),
+                                        (torch.bfloat16, 1e25)])
+def test_query_rows_of_very_different_sizes(d, dtype, size):
+    """A row up to 10^25 times its neighbours leaves them their precision."""
+    for seqs, ql in (([120], [40]), ([90, 50], [1, 1]), ([400], [200])):
+        c = _case(seqs, ql, 4, 2, d, 16, dtype, spread=0.05)
+        c.q[0, 1] *= size
+        c.q[-1, 2] = torch.sign(c.q[-1, 2]) * size
+        _check(_run(c), c)
+
+
+@pytest.mark.parametrize("d", [64, 128, 24])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_non_finite_query_rows_spoil_no_others(d, dtype):
+    for seqs, ql in (([120], [40]), ([90, 50], [1, 1])):
+        c = _case(seqs, ql, 4, 2, d, 16, dtype)
+        want = _run(c)
+        c.q[0, 1, 3], c.q[-1, 2, 7] = float("nan"), float("inf")
+        got = _run(c)
+        assert torch.isnan(got[0, 1]).all() and torch.isnan(got[-1, 2]).all()
+        got[0, 1], got[-1, 2] = want[0, 1], want[-1, 2]
+        assert torch.equal(got, want)
+
+
 def test_rows_of_no_sequence_are_zero():
     c = _case([40, 20], [30, 1], 4, 2, 64, 16, torch.float16, host=False)
     q = torch.cat((c.q, torch.ones(5, 4, 64, dtype=torch.float16)))
