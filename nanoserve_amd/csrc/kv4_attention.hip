@@ -209,12 +209,12 @@ hipError_t launch_generic(const Kv4AttnParams& p, hipStream_t stream) {
 
 // ---- head sizes 64 and 128, blocks of whole 16-token tiles --------------------
 //
-// S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_f16.  A wave keeps a ring
-// of steps of 32 tokens in LDS, its own (no wave waits for another): codes and
-// parameter words arrive there by LDS-DMA, which holds no registers in flight,
-// several steps ahead.  A lane's part of a tile is one LDS read (8 or 16 bytes),
-// and a mask turns its words into operands (kv4.h).  Both
-// model dtypes run in float16: the codes are exact there, the query is brought
+// S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_f16, 32 tokens a step.  Codes
+// and parameter words arrive in LDS by LDS-DMA, which holds no registers in
+// flight: into a ring of each wave's own (one-row sequences; no wave waits for
+// another) or into chunks that a workgroup shares (longer queries).  A lane's part
+// of a tile is one LDS read (8 or 16 bytes), and a mask turns its words into
+// operands (kv4.h).  Both model dtypes run in float16: the codes are exact there, the query is brought
 // into its range by a power of two for the columns that share a workgroup (exact
 // but for elements below 2^-25 of the largest, whose error is below 2^-36 of it;
 // bfloat16 rows beyond 2^16 by a power of their own besides), and the
@@ -231,6 +231,12 @@ hipError_t launch_generic(const Kv4AttnParams& p, hipStream_t stream) {
 // 8 s_t) are float32, and one more product, with a tile of eights, gives 8 times
 // the sum of the rounded p s_t to take off again: a rounding then acts on a code's
 // distance from the middle, half as far as its distance from 0.
+//
+// Bound: one-row sequences by the cache's stream (64 contexts around 4K, four KV
+// heads of 128: 53 us, 4.0 TB/s of codes and parameters) or, where that is short, by
+// the chain of lengths, block ids and tiles; longer queries by vector issue, 80% of
+// the cycles at head size 128: ~205 operations and 16 exponentials a step of 32
+// columns, 80 of them unpacking, beside 34 matrix products (35%).
 //
 // The result layout of the first product, tokens 4 g + r of column lane % 16 in
 // lane group g, is the operand layout of the second.
