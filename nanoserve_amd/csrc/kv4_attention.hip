@@ -249,12 +249,14 @@ struct Slot {
   static constexpr int loads = D == 128 ? 5 : 3;  // vector memory operations that fill it
 };
 
+using floatx2 = float __attribute__((ext_vector_type(2)));
+
 // A step's parameters as float32: lane l makes the two of token l % 32 of K
 // (l < 32) or V, and each lane reads back those of tokens 4 g .. 4 g + 3 of both
 // tiles.  (Each lane converting the eight words that it needs itself was 72 of
 // the ~330 vector instructions of a step of 32 columns.)
-struct Params {
-  float first[64], second[64];  // K: s_t, b_t in log2 units; V: s_t, b_t + 8 s_t
+struct alignas(16) Params {
+  float of[64][2];  // K: s_t, b_t in log2 units; V (from 32 on): s_t, b_t + 8 s_t
 };
 
 // A lane's words of the two tiles of K or V.
@@ -501,8 +503,8 @@ struct Wave {
       at = word;
     }
     const float sc = kv4_scale<DT>(word), of = kv4_offset<DT>(word);
-    params.first[lane] = of_v ? sc : sc * cf;
-    params.second[lane] = of_v ? __builtin_fmaf(8.f, sc, of) : of * cf;
+    *reinterpret_cast<floatx2*>(params.of[lane]) =
+        floatx2{of_v ? sc : sc * cf, of_v ? __builtin_fmaf(8.f, sc, of) : of * cf};
   }
 
   // One step over tokens tok .. tok + 31.  MASK: some column does not see all of
@@ -531,8 +533,10 @@ struct Wave {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int at = 16 * j + 4 * g;
-      ks[j] = *reinterpret_cast<const floatx4*>(params.first + at);
-      kb[j] = *reinterpret_cast<const floatx4*>(params.second + at);
+      const floatx4 a = *reinterpret_cast<const floatx4*>(params.of[at]);
+      const floatx4 b = *reinterpret_cast<const floatx4*>(params.of[at + 2]);
+      ks[j] = floatx4{a[0], a[2], b[0], b[2]};
+      kb[j] = floatx4{a[1], a[3], b[1], b[3]};
     }
 
     float x[NT][2][4];
@@ -580,8 +584,10 @@ struct Wave {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int at = 32 + 16 * j + 4 * g;
-      vs[j] = *reinterpret_cast<const floatx4*>(params.first + at) * inv_sigma;
-      vb[j] = *reinterpret_cast<const floatx4*>(params.second + at);
+      const floatx4 a = *reinterpret_cast<const floatx4*>(params.of[at]);
+      const floatx4 b = *reinterpret_cast<const floatx4*>(params.of[at + 2]);
+      vs[j] = floatx4{a[0], a[2], b[0], b[2]} * inv_sigma;
+      vb[j] = floatx4{a[1], a[3], b[1], b[3]};
     }
     half8 pv[NT];
 #pragma unroll
@@ -737,42 +743,65 @@ __device__ __forceinline__ void store_row(char* dst, const float (&x)[D / 4]) {
 // One sequence's part of a launch: index of count(rows) work items.
 struct Part {
   int seq, row, ql, len, index;
-  bool more;  // there may be work items of later sequences, or of this one's
 };
 
-// The index-th work item of all sequences', count(rows) each; false behind the
-// last.  next: the index asked for afterwards.  Every wave counts for itself, 64
-// sequences at a time.
+// The work items of all sequences, count(rows) each, in order.  Every wave keeps
+// the list for itself: lane l the sequences from l * per on, and the items up to
+// and with theirs, so that an item costs one look at its lane's sequences (and,
+// up to 64 sequences, none).
 template <class Count>
-__device__ __forceinline__ bool find_part(const Kv4AttnParams& p, int lane, int index, int next, Count count,
-                                          Part& out) {
-  int before = 0;
-  for (int s0 = 0; s0 < p.num_seqs; s0 += 64) {
-    Rows r = {0, 0, 0};
-    if (s0 + lane < p.num_seqs) r = rows_of(p, s0 + lane);
-    const int len = static_cast<int>(r.len), ql = static_cast<int>(r.ql);
-    const int mine = count(ql, len);
-    int upto = mine;
+struct PartList {
+  const Kv4AttnParams& p;
+  Count count;
+  int per, upto, mine;
+  int row, ql, len;  // of the lane's first sequence
+
+  __device__ __forceinline__ PartList(const Kv4AttnParams& params, int lane, Count c)
+      : p(params), count(c), per((params.num_seqs + 63) >> 6), mine(0), row(0), ql(0), len(0) {
+    for (int i = per - 1; i >= 0; --i) {
+      const int s = lane * per + i;
+      Rows r = {0, 0, 0};
+      if (s < p.num_seqs) r = rows_of(p, s);
+      row = static_cast<int>(r.row0);
+      ql = static_cast<int>(r.ql);
+      len = static_cast<int>(r.len);
+      mine += s < p.num_seqs ? count(ql, len) : 0;
+    }
+    upto = scan(mine, lane);
+  }
+  static __device__ __forceinline__ int scan(int v, int lane) {
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
-      const int v = __shfl_up(upto, off);
-      upto += lane >= off ? v : 0;
+      const int u = __shfl_up(v, off);
+      v += lane >= off ? u : 0;
     }
-    const int all = lane_value(upto, 63);
-    if (index < before + all) {
-      const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before + upto > index));
-      out.seq = s0 + at;
-      out.row = lane_value(static_cast<int>(r.row0), at);
-      out.ql = lane_value(ql, at);
-      out.len = lane_value(len, at);
-      out.index = index - before - (lane_value(upto, at) - lane_value(mine, at));
-      out.more = s0 + 64 < p.num_seqs || next < before + all;
-      return true;
-    }
-    before += all;
+    return v;
   }
-  return false;
-}
+  __device__ __forceinline__ int size() const { return lane_value(upto, 63); }
+  // index < size().
+  __device__ __forceinline__ Part find(int index, int lane) const {
+    const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > index));
+    index -= lane_value(upto, at) - lane_value(mine, at);
+    if (per == 1) return {at, lane_value(row, at), lane_value(ql, at), lane_value(len, at), index};
+    for (int i = 0;; i += 64) {
+      const int s = at * per + i + lane;
+      const bool one = i + lane < per && s < p.num_seqs;
+      Rows r = {0, 0, 0};
+      if (one) r = rows_of(p, s);
+      const int q = static_cast<int>(r.ql), n = static_cast<int>(r.len);
+      const int own = one ? count(q, n) : 0;
+      const int sum = scan(own, lane);
+      const uint64_t hit = __builtin_amdgcn_ballot_w64(sum > index);
+      if (hit) {
+        const int l = __builtin_ctzll(hit);
+        return {at * per + i + l, lane_value(static_cast<int>(r.row0), l), lane_value(q, l), lane_value(n, l),
+                index - (lane_value(sum, l) - lane_value(own, l))};
+      }
+      if (i + 64 >= per) return {0, 0, 0, 0, 0};  // not reached: the lane has the item
+      index -= lane_value(sum, 63);
+    }
+  }
+};
 
 // Rows of one-row sequences: a workgroup of W waves takes a range of one
 // (sequence, KV head)'s keys for the group's query heads (up to 16 columns), its
@@ -797,13 +826,12 @@ __device__ __forceinline__ void one_rows(const Kv4AttnParams& p, RowState<D, W, 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
-  Part found;
-  found.more = true;
-  for (int item = first; found.more; item += groups) {
+  auto ranges = [&](int ql, int len) { return ql == 1 ? rg.of(len) : 0; };
+  const PartList<decltype(ranges)> parts(p, lane, ranges);
+  const int items = parts.size() * p.num_kv_heads;  // the same for every wave
+  for (int item = first; item < items; item += groups) {
     const int kvh = item % p.num_kv_heads;
-    auto ranges = [&](int ql, int len) { return ql == 1 ? rg.of(len) : 0; };
-    // The same for every wave.
-    if (!find_part(p, lane, item / p.num_kv_heads, (item + groups) / p.num_kv_heads, ranges, found)) break;
+    const Part found = parts.find(item / p.num_kv_heads, lane);
     const int s = found.seq, len = found.len, range = found.index;
     const int64_t row0 = found.row;
     const int t0 = range * rg.tokens;
@@ -895,7 +923,7 @@ constexpr int kColumnBuffers = 2;  // of chunks; three or four are no faster
 template <int D, int NT, int W>
 struct ColumnState {
   static constexpr int cells = NT * (D / 4 + 2);  // floats a lane hands over where W = 8
-  struct Buffer {
+  struct alignas(16) Buffer {
     char slots[W][Slot<D>::bytes];
     Params params[W];
   };
@@ -906,25 +934,25 @@ struct ColumnState {
   };
 };
 
-template <class DT, int D, int NT, int W>
-__device__ __forceinline__ void columns(const Kv4AttnParams& p, ColumnState<D, NT, W>& lds) {
+template <int NT>
+__device__ __forceinline__ int column_blocks(const Kv4AttnParams& p, int ql) {
+  return (ql * p.group + 64 * NT - 1) / (64 * NT);
+}
+template <class DT, bool LOOP, int D, int NT, int W>
+__device__ __forceinline__ void column_block(const Kv4AttnParams& p, ColumnState<D, NT, W>& lds, const Part& found,
+                                             int kvh) {
   const Ranges& rg = p.more;
   auto& buffers = lds.buffers;
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int thread = threadIdx.x;
+  if (LOOP) asm volatile("" : "+v"(thread));  // nothing made of it is kept from one block to the next
+  const int lane = thread & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(thread >> 6);
   const int g = lane >> 4, col = lane & 15;
-  const int kvh = blockIdx.x % p.num_kv_heads;
-  auto blocks_of = [&](int ql) { return (ql * p.group + 64 * NT - 1) / (64 * NT); };
-  auto items = [&](int ql, int len) {
-    return ql < (p.every_row ? 1 : 2) ? 0 : blocks_of(ql) * rg.of(len);
-  };
-  Part found;
-  if (!find_part(p, lane, blockIdx.x / p.num_kv_heads, 0, items, found)) return;
   const int s = found.seq, ql = found.ql, len = found.len;
   const int64_t row0 = found.row;
   const int cols = ql * p.group;
   // The last columns, which see the most keys, first.
-  const int blocks = blocks_of(ql), ranges = rg.of(len);
+  const int blocks = column_blocks<NT>(p, ql), ranges = rg.of(len);
   const int block = found.index / ranges, range = found.index - block * ranges;
   const int block_base = (blocks - 1 - block) * (64 * NT);
   auto last_of = [&](int end_col) { return len - ql + ((end_col < cols ? end_col : cols) - 1) / p.group; };
@@ -1053,10 +1081,39 @@ __device__ __forceinline__ void columns(const Kv4AttnParams& p, ColumnState<D, N
   }
 }
 
+// LOOP: the workgroup goes from block to block, `groups` apart; else there are as
+// many workgroups as blocks at most.  (The loop alone costs long prompts 5%: values
+// that outlive a block hold registers.)
+template <class DT, int D, int NT, int W, bool LOOP>
+__device__ __forceinline__ void columns(const Kv4AttnParams& p, ColumnState<D, NT, W>& lds, int first, int groups) {
+  const int lane = threadIdx.x & 63;
+  auto blocks = [&](int ql, int len) {
+    return ql < (p.every_row ? 1 : 2) ? 0 : column_blocks<NT>(p, ql) * p.more.of(len);
+  };
+  // Mostly one round: for another the list is made anew, and holds no registers meanwhile.
+  int item = first;
+#pragma unroll 1
+  for (;;) {
+    int items;  // the same for every wave
+    Part found;
+    {
+      const PartList<decltype(blocks)> parts(p, lane, blocks);
+      items = parts.size() * p.num_kv_heads;
+      if (item >= items) return;
+      found = parts.find(item / p.num_kv_heads, lane);
+    }
+    column_block<DT, LOOP>(p, lds, found, item % p.num_kv_heads);
+    if (!LOOP) return;
+    item += groups;
+    if (item >= items) return;
+    __syncthreads();  // the next block's keys go where this one's states are read
+  }
+}
+
 // Both kinds of rows in one launch: the column part's workgroups first, and where
 // those leave compute units idle, at the start or towards the end, workgroups of
 // one-row sequences.
-template <class DT, int D, int NT, int W>
+template <class DT, int D, int NT, int W, bool LOOP>
 __global__ __launch_bounds__(64 * W, D == 64 ? (NT == 1 ? 4 : W == 4 ? 3 : 2) : 2) void kv4_columns_kernel(Kv4AttnParams p) {
   constexpr int R = W == 4 ? kDecodeRing<D> : 2;
   union Lds {
@@ -1065,7 +1122,7 @@ __global__ __launch_bounds__(64 * W, D == 64 ? (NT == 1 ? 4 : W == 4 ? 3 : 2) : 
   };
   __shared__ __align__(16) Lds lds;
   const int groups = p.column_groups;
-  if (static_cast<int>(blockIdx.x) < groups) columns<DT>(p, lds.columns);
+  if (static_cast<int>(blockIdx.x) < groups) columns<DT, D, NT, W, LOOP>(p, lds.columns, blockIdx.x, groups);
   else one_rows<DT>(p, lds.rows, blockIdx.x - groups, gridDim.x - groups);
 }
 
@@ -1142,7 +1199,7 @@ struct Cut {
   int64_t dec_items;            // ranges of all of them, about
   int col_split, col_n;         // the same of longer queries
   int col_waves, col_tiles;     // waves of a workgroup of the column kernel, column tiles of a wave
-  int64_t col_blocks;           // column blocks of all queries, at most
+  int64_t col_blocks, col_most; // column blocks of all queries, expected and at most
   size_t dec_bytes, col_bytes;  // partials
 };
 
@@ -1189,7 +1246,10 @@ Cut cut_of(int num_seqs, int64_t num_tokens, int max_seq_len, int64_t context, i
     // chunks 34 and 39 (size 64), four 40 and 44.  Two tiles, eight waves and four:
     // six chunks (342 blocks, size 64) 47 and 59, two prompts of 2048 (448 blocks,
     // size 64) 43 and 56, but (896, size 128) 103 and 84, four (896, size 64) 88 and 71.
-    auto count = [&](int tiles) { return (num_tokens * group + 64 * tiles - 1) / (64 * tiles) * num_kv_heads; };
+    // Without the one-row sequences, where the caller knows them.
+    const int64_t ones = c.decode && one_row > 0 && one_row < num_tokens ? one_row : 0;
+    const int64_t rows = num_tokens - ones;
+    auto count = [&](int tiles) { return (rows * group + 64 * tiles - 1) / (64 * tiles) * num_kv_heads; };
     const int64_t few = (head_dim == 64 ? 2 : 1) * kCUs;
     c.col_tiles = count(1) <= few ? 1 : 2;
     const int64_t blocks = count(c.col_tiles);
@@ -1203,7 +1263,9 @@ Cut cut_of(int num_seqs, int64_t num_tokens, int max_seq_len, int64_t context, i
     const int64_t split = round_up((longest + want - 1) / want, 32);
     c.col_split = static_cast<int>(split < 256 ? 256 : split);
     c.col_n = static_cast<int>((longest + c.col_split - 1) / c.col_split);
-    c.col_blocks = num_tokens * group / (64 * c.col_tiles) + num_seqs;
+    // A sequence's last block may hold a single column.
+    c.col_blocks = rows * group / (64 * c.col_tiles) + (num_seqs - ones > 0 ? num_seqs - ones : 1);
+    c.col_most = num_tokens * group / (64 * c.col_tiles) + num_seqs;
     c.col_bytes = c.col_n > 1 ? static_cast<size_t>(num_tokens) * num_heads * c.col_n * row_bytes : 0;
   }
   return c;
@@ -1226,27 +1288,38 @@ hipError_t launch_fast(Kv4AttnParams p, const Cut& c, char* workspace, hipStream
     float* o = reinterpret_cast<float*>(at);
     return Ranges{n, tokens, o + cells * D, o + cells * (D + 1), o};
   };
+  const int64_t held = static_cast<int64_t>(kCUs) * kDecodeGroups;
   int64_t row_groups = 0;
   if (c.decode) {
     p.one = ranges(workspace, p.num_seqs, c.dec_n, c.dec_split);
     const int64_t most = pairs * c.dec_n < c.dec_items ? pairs * c.dec_n : c.dec_items;
-    const int64_t held = static_cast<int64_t>(kCUs) * kDecodeGroups;
     row_groups = most < held ? most : held;
   }
-  hipError_t e;
+  // One launch for both kinds of rows where those of one row fit the device beside;
+  // else the decode kernel's workgroups of four waves are worth a launch of their own.
+  // A chunk of 300 rows beside 32 / 128 / 512 contexts around 400, us: four KV heads of
+  // 128 together 23 / 47 / 109, apart 26 / 40 / 78; two of 64 18 / 25 / 54 and 23 / 31 / 54.
+  const bool together = c.columns && row_groups < held;
+  hipError_t e = hipSuccess;
   if (c.columns) {
     p.more = ranges(workspace + align256(c.dec_bytes), p.num_tokens, c.col_n, c.col_split);
     p.every_row = c.every_row ? 1 : 0;
-    const int64_t groups = c.col_blocks * p.num_kv_heads * c.col_n;
-    if (groups > 0x7FFFFFFF) return hipErrorInvalidValue;
+    // Where the caller's count of one-row sequences leaves far fewer blocks than the
+    // rows could make, as many workgroups as blocks are expected, and a loop.
+    const int64_t each = static_cast<int64_t>(p.num_kv_heads) * c.col_n;
+    const bool loop = c.col_waves == 8 || c.col_most > c.col_blocks + c.col_blocks / 2;
+    const int64_t groups = (loop ? c.col_blocks : c.col_most) * each;
+    if (groups > 0x3FFFFFFF) return hipErrorInvalidValue;
     p.column_groups = static_cast<int>(groups);
-    const void* fn = c.col_tiles == 1   ? reinterpret_cast<const void*>(&kv4_columns_kernel<DT, D, 1, 8>)
-                     : c.col_waves == 8 ? reinterpret_cast<const void*>(&kv4_columns_kernel<DT, D, 2, 8>)
-                                        : reinterpret_cast<const void*>(&kv4_columns_kernel<DT, D, 2, 4>);
-    e = launch(fn, groups + row_groups, p, st, 64 * c.col_waves);
+    const void* fn = c.col_tiles == 1   ? reinterpret_cast<const void*>(&kv4_columns_kernel<DT, D, 1, 8, true>)
+                     : c.col_waves == 8 ? reinterpret_cast<const void*>(&kv4_columns_kernel<DT, D, 2, 8, true>)
+                     : loop             ? reinterpret_cast<const void*>(&kv4_columns_kernel<DT, D, 2, 4, true>)
+                                        : reinterpret_cast<const void*>(&kv4_columns_kernel<DT, D, 2, 4, false>);
+    e = launch(fn, groups + (together ? row_groups : 0), p, st, 64 * c.col_waves);
     if (e == hipSuccess && c.col_n > 1)
       e = launch(reinterpret_cast<const void*>(&kv4_merge_kernel<DT, D, false>), (p.num_tokens * p.num_heads + 3) / 4, p, st);
-  } else {
+  }
+  if (e == hipSuccess && c.decode && !together) {
     e = row_groups <= kCUs ? launch(reinterpret_cast<const void*>(&kv4_decode_kernel<DT, D, 8>), row_groups, p, st, 512)
                            : launch(reinterpret_cast<const void*>(&kv4_decode_kernel<DT, D, 4>), row_groups, p, st);
   }

@@ -349,6 +349,24 @@ def test_many_sequences(d, host):
     _check(_run(c), c)
 
 
+@pytest.mark.parametrize("host", [True, False])
+@pytest.mark.parametrize("n", [4200, 700])
+def test_thousands_of_sequences(n, host):
+    rng = np.random.default_rng(n)
+    seqs = [int(x) for x in rng.integers(0, 5, n)]
+    seqs[0] = seqs[n // 2] = seqs[-1] = 40
+    c = _case(seqs, [1] * n, 2, 1, 64, 16, torch.float16, host=host, extra=0)
+    _check(_run(c), c)
+    ql = [1 + int(x) for x in rng.integers(0, 2, n)]
+    ql[5], ql[-1] = 0, 40
+    c = _case(seqs, ql, 2, 1, 64, 16, torch.bfloat16, host=host, extra=0, seed=1)
+    _check(_run(c), c)
+    ql = [1] * n
+    ql[n // 2], ql[-2] = 30, 3
+    c = _case(seqs, ql, 2, 1, 64, 16, torch.float16, host=host, extra=0, seed=2)
+    _check(_run(c), c)
+
+
 @pytest.mark.parametrize("d", [64, 128])
 def test_one_row_of_a_longer_query_layout(d):
     """One-row sequences given by offsets, with no decode-only flag, and none of them."""
