@@ -38,7 +38,7 @@
 // 3.7 and 6.2 us); for many the three passes over the logits, of which the second
 // evaluates a float64 exponential (about 40 operations) for every element of the
 // rows without a top-k.  256 rows of 152K float32, three quarters with a top-k of
-// 20 to 400: 31 (5.1 TB/s), 45, 8.6, 20 and 16 us; with every element counted and
+// 20 to 400: 31 (5.1 TB/s), 42, 8.9, 19 and 16 us; with every element counted and
 // collected from the slices 31, 58, 8.5, 35 and 16.
 #include <math.h>
 
@@ -84,6 +84,7 @@ struct SampleParams {
   int part_lanes;          // threads of a group: 1, 2 or 4
   uint64_t* hist_w;        // [rows, slices, kBins]
   uint32_t* hist_c;
+  int* last_bin;           // [rows]: the bins behind it were not counted, nor written
   uint64_t* min_w;         // [rows, slices]
   uint32_t* min_c;
   uint64_t* cum_w;         // [rows, kBins + 1]: weight and count before each bin
@@ -98,9 +99,11 @@ struct SampleParams {
   int list_cap;
 };
 
-// f(value, index) for the elements [s0, s1) of a row, over the workgroup.
-template <int DT, int THREADS, class F>
-__device__ __forceinline__ void each_element(const char* row, int64_t s0, int64_t s1, F f) {
+// f(value, index) for the elements [s0, s1) of a row, over the workgroup.  SOME:
+// elements below `least` may be left out, and are where a whole wave's vector has
+// no other: a test and a branch for every element would cost as much as the rest.
+template <int DT, int THREADS, bool SOME = false, class F>
+__device__ __forceinline__ void each_element(const char* row, int64_t s0, int64_t s1, F f, float least = 0.f) {
   constexpr int ESZ = DT == NS_DTYPE_F32 ? 4 : 2;
   constexpr int VEC = 16 / ESZ;
   // Elements up to the first 16-byte boundary, whole vectors, the rest.
@@ -111,22 +114,25 @@ __device__ __forceinline__ void each_element(const char* row, int64_t s0, int64_
   const int tid = threadIdx.x;
   const u32x4* v = reinterpret_cast<const u32x4*>(row + v0 * ESZ);
   int64_t j = tid;
+  auto vector = [&](const u32x4& w, int64_t at) {
+    if (SOME) {
+      float most = vec_elem_f32<DT>(w, 0);
+#pragma unroll
+      for (int e = 1; e < VEC; ++e) most = fmaxf(most, vec_elem_f32<DT>(w, e));
+      if (!(most >= least)) return;
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f(vec_elem_f32<DT>(w, e), static_cast<uint32_t>(v0 + at * VEC + e));
+  };
   // Four loads in flight.
   for (; j + 3 * THREADS < vecs; j += 4 * THREADS) {
     u32x4 w[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) w[q] = v[j + q * THREADS];
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        f(vec_elem_f32<DT>(w[q], e), static_cast<uint32_t>(v0 + (j + q * THREADS) * VEC + e));
+    for (int q = 0; q < 4; ++q) vector(w[q], j + q * THREADS);
   }
-  for (; j < vecs; j += THREADS) {
-    const u32x4 w = v[j];
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) f(vec_elem_f32<DT>(w, e), static_cast<uint32_t>(v0 + j * VEC + e));
-  }
+  for (; j < vecs; j += THREADS) vector(v[j], j);
   const int64_t head = v0 - s0, t0 = v0 + vecs * VEC;
   if (tid < head + (s1 - t0)) {
     const int64_t i = tid < head ? s0 + tid : t0 + (tid - head);
@@ -243,11 +249,11 @@ __device__ __forceinline__ int64_t top_k_of(const SampleParams& p, int64_t r) {
 }
 
 // f(value, index) for the workgroup's slice of row blockIdx.y.
-template <int DT, class F>
-__device__ __forceinline__ void each_of_slice(const SampleParams& p, int64_t elems, F f) {
+template <int DT, bool SOME = false, class F>
+__device__ __forceinline__ void each_of_slice(const SampleParams& p, int64_t elems, F f, float least = 0.f) {
   const int64_t s0 = static_cast<int64_t>(blockIdx.x) * elems;
   const int64_t s1 = s0 + elems < p.n ? s0 + elems : p.n;
-  each_element<DT, kSliceThreads>(p.x + static_cast<int64_t>(blockIdx.y) * p.row_bytes, s0, s1, f);
+  each_element<DT, kSliceThreads, SOME>(p.x + static_cast<int64_t>(blockIdx.y) * p.row_bytes, s0, s1, f, least);
 }
 
 template <int DT>
@@ -301,14 +307,16 @@ struct Outbox {
   uint64_t keys[kLocal];
   uint32_t n, base;
 
-  __device__ __forceinline__ void add(uint64_t key, uint64_t* list, uint32_t* list_n, uint32_t cap) {
+  // Whether the key is among those.
+  __device__ __forceinline__ bool add(uint64_t key, uint64_t* list, uint32_t* list_n, uint32_t cap) {
     const uint32_t at = atomicAdd(&n, 1u);
     if (at < kLocal) {
       keys[at] = key;
-    } else {
-      const uint32_t to = atomicAdd(list_n, 1u);
-      if (to < cap) list[to] = key;
+      return true;
     }
+    const uint32_t to = atomicAdd(list_n, 1u);
+    if (to < cap) list[to] = key;
+    return false;
   }
   // By the whole workgroup.
   __device__ __forceinline__ void send(uint64_t* list, uint32_t* list_n, uint32_t cap) {
@@ -406,15 +414,27 @@ __global__ __launch_bounds__(kSliceThreads, 4) void sample_hist_kernel(SamplePar
     min_w += w >= enough ? w : 0;
   };
   if (most < kBins - 1) {
-    each_of_slice<DT>(p, p.slice_elems, [&](float z, uint32_t i) {
-      const int b = bin_of(row, z);
-      if (b > most) return;
+    uint64_t* const cands = p.cands + r * p.list_cap;
+    auto weigh = [&](float z) {
       const uint64_t w = weight_of(row, series, z);
       count_min(w);
-      count(b, w);
-      box.add(place_of(z, i), p.cands + r * p.list_cap, &p.cand_n[r], p.list_cap);
-    });
-    box.send(p.cands + r * p.list_cap, &p.cand_n[r], p.list_cap);
+      count(bin_of(row, z), w);
+    };
+    // Nothing below this lies in the bins up to `most` (a bin's width, and a
+    // rounding of the result, to be sure).
+    const double edge = static_cast<double>(row.top) - (most + 2) / static_cast<double>(row.bin_scale);
+    const float least = static_cast<float>(edge) - fabsf(static_cast<float>(edge)) * 2.4e-7f;
+    each_of_slice<DT, true>(
+        p, p.slice_elems,
+        [&](float z, uint32_t i) {
+          if (bin_of(row, z) > most) return;
+          if (!box.add(place_of(z, i), cands, &p.cand_n[r], p.list_cap)) weigh(z);
+        },
+        least);
+    __syncthreads();
+    const uint32_t here = box.n < kLocal ? box.n : kLocal;
+    for (uint32_t i = tid; i < here; i += kSliceThreads) weigh(value_of(~static_cast<uint32_t>(box.keys[i] >> 32)));
+    box.send(cands, &p.cand_n[r], p.list_cap);
   } else if (mp > 0.f) {
     each_of_slice<DT>(p, p.slice_elems, [&](float z, uint32_t) {
       const uint64_t w = weight_of(row, series, z);
@@ -435,11 +455,12 @@ __global__ __launch_bounds__(kSliceThreads, 4) void sample_hist_kernel(SamplePar
   }
   __syncthreads();
   const int64_t at = r * p.slices + blockIdx.x;
-  for (int b = tid; b < kBins; b += kSliceThreads) {
+  for (int b = tid; b <= most; b += kSliceThreads) {
     p.hist_w[at * kBins + b] = hw[b];
     p.hist_c[at * kBins + b] = hc[b];
   }
   if (tid == 0) {
+    if (blockIdx.x == 0) p.last_bin[r] = most;
     p.min_c[at] = mc;
     p.min_w[at] = mw;
   }
@@ -536,6 +557,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_plan_kernel(SampleParams p
   const int64_t k = top_k_of(p, r);
   const bool has_min = p.min_p && p.min_p[r] > 0.f;
   const uint32_t listed = p.cand_n[r];
+  const int last_bin = p.last_bin[r];
   const Ends ends = row_ends(p, r);
   if (takes_largest(ends.top, temperature)) {
     if (tid == 0) {
@@ -543,6 +565,10 @@ __global__ __launch_bounds__(kRowThreads) void sample_plan_kernel(SampleParams p
       p.plan[r].mode = kDone;
     }
     return;
+  }
+  if (tid > last_bin) {
+    c = 0;
+    w = 0;
   }
   scan(scratch, c, w);
   cum_c[tid + 1] = c;
@@ -1004,14 +1030,16 @@ struct Layout {
   int64_t slice_elems, collect_elems;
   int part_lanes;
   size_t keys, hist_w, min_w, cum_w, kept_w, list, cands, least, parts, hist_c, min_c, cum_c, kept_c,
-      list_n, cand_n, plan, total;
+      list_n, cand_n, last_bin, plan, total;
 };
 
 Layout layout_of(int64_t M, int64_t N) {
   Layout l;
   // About four workgroups for each compute unit, up to 16 slices of at least 2048
-  // elements.  Twice as many where only some rows are read (256 rows: 20 us, 27 with
-  // four).
+  // elements; eight for many rows, whose work is unequal (rows with and without a
+  // top-k; 512 rows of 152K 172 us, 198 with four, 1024 314 and 412, but 256 and 128
+  // rows 4 and 6 us more).  The fourth stage, where most rows are done with, takes
+  // more still (256 rows: 28, 21, 19 us with 4, 8, 16 slices).
   auto cut = [&](int64_t groups, int& slices, int64_t& elems) {
     int64_t n = groups / M < 1 ? 1 : groups / M;
     n = n > 16 ? 16 : n;
@@ -1020,8 +1048,8 @@ Layout layout_of(int64_t M, int64_t N) {
     elems = ((N + n - 1) / n + 7) / 8 * 8;
     slices = static_cast<int>((N + elems - 1) / elems);
   };
-  cut(1024, l.slices, l.slice_elems);
-  cut(2048, l.collect_slices, l.collect_elems);
+  cut(M > 256 ? 2048 : 1024, l.slices, l.slice_elems);
+  cut(4096, l.collect_slices, l.collect_elems);
   l.list_cap = N < kList ? static_cast<int>(N) : kList;
   size_t at = 0;
   const size_t m = static_cast<size_t>(M), cells = m * l.slices;
@@ -1047,6 +1075,7 @@ Layout layout_of(int64_t M, int64_t N) {
   l.kept_c = take(m * 4);
   l.list_n = take(m * 4);
   l.cand_n = take(m * 4);
+  l.last_bin = take(m * 4);
   l.plan = take(m * sizeof(Plan));
   l.total = at;
   return l;
@@ -1129,6 +1158,7 @@ extern "C" int ns_sample_rows(int64_t* out, const void* x, int64_t x_stride_row,
   p.kept_c = u32(l.kept_c);
   p.list_n = u32(l.list_n);
   p.cand_n = u32(l.cand_n);
+  p.last_bin = reinterpret_cast<int*>(ws + l.last_bin);
   p.plan = reinterpret_cast<Plan*>(ws + l.plan);
   int log = 0;
   while ((1ll << log) < N) ++log;
