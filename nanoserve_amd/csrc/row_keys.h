@@ -31,11 +31,40 @@ __device__ __forceinline__ uint64_t key_of(float v, uint32_t idx) {
 
 __device__ __forceinline__ uint64_t max_u64(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
-__device__ __forceinline__ uint64_t wave_max(uint64_t k) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) k = max_u64(k, __shfl_xor(k, off));
-  return k;
+// Another lane of the same 16 by a data-parallel move, which costs a register
+// move where a shuffle is a trip through LDS.
+template <int CTRL>
+__device__ __forceinline__ uint32_t moved(uint32_t v) {
+  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xF, 0xF, false));
 }
+template <int CTRL>
+__device__ __forceinline__ uint64_t moved(uint64_t v) {
+  return (static_cast<uint64_t>(moved<CTRL>(static_cast<uint32_t>(v >> 32))) << 32) |
+         moved<CTRL>(static_cast<uint32_t>(v));
+}
+// The 16 lanes' best, on each of them: neighbours, pairs, fours and eights
+// exchange (the two mirrors meet lanes that hold the same by then).
+template <class T, class Best>
+__device__ __forceinline__ T row_best(T v, Best best) {
+  v = best(v, moved<0xB1>(v));   // lane ^ 1
+  v = best(v, moved<0x4E>(v));   // lane ^ 2
+  v = best(v, moved<0x141>(v));  // 7 - lane, of eight
+  return best(v, moved<0x140>(v));  // 15 - lane
+}
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) {
+  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
+}
+__device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
+  return (static_cast<uint64_t>(lane_of(static_cast<uint32_t>(v >> 32), lane)) << 32) |
+         lane_of(static_cast<uint32_t>(v), lane);
+}
+template <class T, class Best>
+__device__ __forceinline__ T wave_best(T v, Best best) {
+  v = row_best(v, best);
+  return best(best(lane_of(v, 0), lane_of(v, 16)), best(lane_of(v, 32), lane_of(v, 48)));
+}
+__device__ __forceinline__ uint32_t min_u32(uint32_t a, uint32_t b) { return a < b ? a : b; }
+__device__ __forceinline__ uint64_t wave_max(uint64_t k) { return wave_best(k, max_u64); }
 
 template <int DT>
 __device__ __forceinline__ float elem_f32(const char* row, int64_t i) {

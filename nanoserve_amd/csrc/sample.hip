@@ -34,13 +34,15 @@
 // additions; the rounding, 2^-45 of the largest weight, moves a border by less
 // than 1e-9 of the row's sum even where all 150K roundings agree.
 //
-// Bound: for a few rows the five launches (one row of 152K float16: 4.7, 10, 7,
-// 3.7 and 6.2 us); for many the three passes over the logits, of which the second
+// Bound: for a few rows the five launches (one row of 152K float16: 4.5, 8, 7,
+// 3.5 and 5.5 us); for many the three passes over the logits, of which the second
 // evaluates a float64 exponential (about 40 operations) for every element of the
 // rows without a top-k.  256 rows of 152K float32, three quarters with a top-k of
 // 20 to 400: 31 (5.1 TB/s), 42, 8.9, 19 and 16 us; with every element counted and
 // collected from the slices 31, 58, 8.5, 35 and 16.
 #include <math.h>
+
+#include <type_traits>
 
 #include "row_keys.h"
 
@@ -54,6 +56,7 @@ constexpr float kReach = 36.f;         // the bins span this much of (z_max - z)
 constexpr int kList = 4096;            // collected elements of a row
 constexpr int kSort = 1024;            // elements that the long way sorts at once
 constexpr int kSub = 256;              // sub-bins of its histograms
+constexpr int kMostSlices = 16;        // of a row
 
 // What the third stage decides about a row.
 struct Plan {
@@ -200,17 +203,12 @@ struct Ends {
 __device__ __forceinline__ Ends row_ends(const SampleParams& p, int64_t row) {
   const int lane = threadIdx.x & 63;
   Ends e = {0, kNanOrder};
-  for (int i = lane; i < p.slices; i += 64) {
-    e.top = max_u64(e.top, p.keys[row * p.slices + i]);
-    const uint32_t v = p.least[row * p.slices + i];
-    e.least = v < e.least ? v : e.least;
+  if (lane < p.slices) {  // 16 at most
+    e.top = p.keys[row * p.slices + lane];
+    e.least = p.least[row * p.slices + lane];
   }
-  e.top = wave_max(e.top);
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    const uint32_t v = __shfl_xor(e.least, off);
-    e.least = v < e.least ? v : e.least;
-  }
+  e.top = lane_of(row_best(e.top, max_u64), 0);
+  e.least = lane_of(row_best(e.least, min_u32), 0);
   return e;
 }
 
@@ -279,11 +277,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_ends_kernel(SampleParams
       p.parts[(at * kSliceThreads + threadIdx.x) / p.part_lanes] = part;
   }
   best = wave_max(best);
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    const uint32_t v = __shfl_xor(least, off);
-    least = v < least ? v : least;
-  }
+  least = wave_best(least, min_u32);
   if ((threadIdx.x & 63) == 0) {
     wk[threadIdx.x >> 6] = best;
     wl[threadIdx.x >> 6] = least;
@@ -329,18 +323,24 @@ struct Outbox {
   }
 };
 
+// Groups of threads of a row.
+__device__ __forceinline__ int groups_of(const SampleParams& p) {
+  return p.slices * kSliceThreads / p.part_lanes;  // 1024 at most
+}
+
 // A bin such that the first k elements lie in it and the bins before it: k groups
 // of threads had their largest there.  The last bin where there are not so many
 // groups.  count: kBins zeros, and zeros again afterwards.
-__device__ __forceinline__ int last_bin_for(const SampleParams& p, const Row& row, int64_t r, int64_t k,
-                                            uint32_t* count) {
+__device__ __forceinline__ int last_bin_for(const SampleParams& p, const Row& row, int64_t k,
+                                            const uint32_t (&part)[4], uint32_t* count) {
   __shared__ uint32_t upto[kSliceThreads / 64];
   __shared__ int found;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int groups = p.slices * kSliceThreads / p.part_lanes;
+  const int groups = groups_of(p);
   if (k == 0 || k > groups) return kBins - 1;
-  for (int i = tid; i < groups; i += kSliceThreads)
-    atomicAdd(&count[bin_of(row, value_of(p.parts[r * groups + i]))], 1u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i * kSliceThreads + tid < groups) atomicAdd(&count[bin_of(row, value_of(part[i]))], 1u);
   __syncthreads();
   static_assert(kBins == 4 * kSliceThreads, "four bins for each thread");
   u32x4& mine = reinterpret_cast<u32x4*>(count)[tid];
@@ -377,9 +377,18 @@ __global__ __launch_bounds__(kSliceThreads, 4) void sample_hist_kernel(SamplePar
   __shared__ uint32_t mc;
   const int tid = threadIdx.x;
   const int64_t r = blockIdx.y;
-  const Ends ends = row_ends(p, r);
+  // Everything that is read besides the row, at once.
+  const int64_t k = top_k_of(p, r);
   const float t = p.temperature[r];
   const float mp = p.min_p ? p.min_p[r] : 0.f;
+  uint32_t part[4] = {0, 0, 0, 0};
+  if (p.top_k) {
+    const int groups = groups_of(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i * kSliceThreads + tid < groups) part[i] = p.parts[r * groups + i * kSliceThreads + tid];
+  }
+  const Ends ends = row_ends(p, r);
   if (takes_largest(ends.top, t)) return;
   for (int b = tid; b < kBins + 64; b += kSliceThreads) {
     hw[b] = 0;
@@ -398,7 +407,7 @@ __global__ __launch_bounds__(kSliceThreads, 4) void sample_hist_kernel(SamplePar
   // Elements behind the first k decide nothing and are left out, where a bin that
   // they cannot lie in is known: most of a row then needs no exponential, and the
   // others can be listed at once.
-  const int most = last_bin_for(p, row, r, top_k_of(p, r), hc);
+  const int most = last_bin_for(p, row, k, part, hc);
   auto count = [&](int b, uint64_t w) {
     b = b == kBins - 1 ? last : b;
     atomicAdd(&hc[b], 1u);
@@ -487,9 +496,10 @@ __device__ __forceinline__ void scan(ScanScratch& s, uint32_t& c, uint64_t& w) {
     s.w[wave] = w;
   }
   __syncthreads();
-  for (int i = 0; i < wave; ++i) {
-    c += s.c[i];
-    w += s.w[i];
+#pragma unroll
+  for (int i = 0; i < kRowThreads / 64 - 1; ++i) {
+    c += i < wave ? s.c[i] : 0;
+    w += i < wave ? s.w[i] : 0;
   }
   __syncthreads();
 }
@@ -547,12 +557,19 @@ __global__ __launch_bounds__(kRowThreads) void sample_plan_kernel(SampleParams p
   // XCD's cache.  (A greedy row has no histograms; its sums go nowhere.)
   uint32_t c = 0;
   uint64_t w = 0;
-#pragma unroll 8
-  for (int i = 0; i < p.slices; ++i) {
-    const int64_t at = (r * p.slices + i) * kBins + tid;
-    c += p.hist_c[at];
-    w += p.hist_w[at];
-  }
+  auto add = [&](auto most) {
+#pragma unroll
+    for (int i = 0; i < most; ++i) {
+      // No branch, so that no read waits for another.
+      const int64_t at = (r * p.slices + (i < p.slices ? i : p.slices - 1)) * kBins + tid;
+      const uint32_t ci = p.hist_c[at];
+      const uint64_t wi = p.hist_w[at];
+      c += i < p.slices ? ci : 0;
+      w += i < p.slices ? wi : 0;
+    }
+  };
+  if (p.slices <= 4) add(std::integral_constant<int, 4>());
+  else add(std::integral_constant<int, kMostSlices>());
   const float u = p.u[r], temperature = p.temperature[r], tp = top_p_of(p, r);
   const int64_t k = top_k_of(p, r);
   const bool has_min = p.min_p && p.min_p[r] > 0.f;
@@ -1042,7 +1059,7 @@ Layout layout_of(int64_t M, int64_t N) {
   // more still (256 rows: 28, 21, 19 us with 4, 8, 16 slices).
   auto cut = [&](int64_t groups, int& slices, int64_t& elems) {
     int64_t n = groups / M < 1 ? 1 : groups / M;
-    n = n > 16 ? 16 : n;
+    n = n > kMostSlices ? kMostSlices : n;
     const int64_t most = (N + 2047) / 2048;
     n = n > most ? most : n;
     elems = ((N + n - 1) / n + 7) / 8 * 8;
