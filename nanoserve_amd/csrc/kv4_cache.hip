@@ -12,7 +12,8 @@
 // infinity, or whose scale or offset leaves the dtype's range, is stored as
 // code 0, scale 0, offset NaN: whatever reads it gets NaN, and nothing else does.
 //
-// Bound: launches and memory.  A row is read once and leaves a quarter of its
+// Bound: launches and memory (with rotary, 32 tokens of 14 + 4 heads of 64 4.0 us,
+// 2048 of 28 + 8 heads of 128 10.3: 37 MB at 3.6 TB/s).  A row is read once and leaves a quarter of its
 // bytes behind; the only reduction is the row's minimum and maximum, over the
 // lanes that hold it (head_dim / 8 of them, so 8 rows of 64 in a wave).  A
 // lane holds four values of the row's first half and the four that
@@ -36,7 +37,8 @@ struct Kv4WriteParams {
   int slots64;
   int num_heads, num_kv_heads, head_dim, block_size;
   int64_t num_slots, record;
-  int64_t nq, nk;          // query rows (0 without rotary), key rows (value rows = nk)
+  int64_t nq, nk;          // groups of query rows (0 without rotary), key rows (value rows = nk)
+  int groups;              // of a token's query rows
   int lane_shift;          // a row has 1 << lane_shift lanes, head_dim / 8 of them with values
   int vec;                 // rows start on 8-byte boundaries
 };
@@ -75,7 +77,9 @@ __device__ __forceinline__ void store4(char* p, int vec, const float (&x)[4]) {
   }
 }
 
-template <class DT>
+// QROWS query rows of a token share one read of its cos and sin: a row is 16 bytes
+// a lane in and out, the tables 32.
+template <class DT, int QROWS>
 __global__ __launch_bounds__(256) void kv4_write_kernel(Kv4WriteParams p) {
   const int lanes = 1 << p.lane_shift;
   const int c = threadIdx.x & (lanes - 1);
@@ -83,7 +87,7 @@ __global__ __launch_bounds__(256) void kv4_write_kernel(Kv4WriteParams p) {
   if (r >= p.nq + 2 * p.nk) return;  // whole rows leave together: the shuffles below stay within one
   const int kind = r < p.nq ? 0 : r < p.nq + p.nk ? 1 : 2;
   r -= kind == 0 ? 0 : kind == 1 ? p.nq : p.nq + p.nk;
-  const int heads = kind == 0 ? p.num_heads : p.num_kv_heads;
+  const int heads = kind == 0 ? p.groups : p.num_kv_heads;
   const int64_t t = r / heads;
   const int h = static_cast<int>(r - t * heads);
   const int half = p.head_dim / 2;
@@ -94,37 +98,52 @@ __global__ __launch_bounds__(256) void kv4_write_kernel(Kv4WriteParams p) {
     slot = load_index(p.slots, t, p.slots64);
     if (slot < 0 || slot >= p.num_slots) return;  // padding / invalid slot: never written
   }
-  const char* src = kind == 0   ? p.q + (t * p.q_st + h * p.q_sh) * 2
-                    : kind == 1 ? p.key + (t * p.k_st + h * p.k_sh) * 2
-                                : p.value + (t * p.v_st + h * p.v_sh) * 2;
   const int e0 = 4 * c;
+  float c1[4], c2[4], s1[4], s2[4];
+  if (has && kind != 2 && p.cos) {
+    const char* cs = p.cos + t * p.cs_st * 2;
+    const char* sn = p.sin + t * p.cs_st * 2;
+    load4<DT>(cs + e0 * 2, p.vec, c1);
+    load4<DT>(cs + (half + e0) * 2, p.vec, c2);
+    load4<DT>(sn + e0 * 2, p.vec, s1);
+    load4<DT>(sn + (half + e0) * 2, p.vec, s2);
+  }
+  auto rotate = [&](float (&lo)[4], float (&hi)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float x1 = lo[e], x2 = hi[e];
+      lo[e] = x1 * c1[e] - x2 * s1[e];
+      hi[e] = x2 * c2[e] + x1 * s2[e];
+    }
+  };
+  if (kind == 0) {
+    if (!has) return;
+    const int h0 = h * QROWS;
+    float lo[QROWS][4], hi[QROWS][4];
+#pragma unroll
+    for (int j = 0; j < QROWS; ++j) {
+      // Past the last head the last one again, so that all are read at once.
+      const int hj = h0 + j < p.num_heads ? h0 + j : p.num_heads - 1;
+      const char* src = p.q + (t * p.q_st + hj * p.q_sh) * 2;
+      load4<DT>(src + e0 * 2, p.vec, lo[j]);
+      load4<DT>(src + (half + e0) * 2, p.vec, hi[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < QROWS; ++j) {
+      if (h0 + j >= p.num_heads) break;
+      rotate(lo[j], hi[j]);
+      char* d = p.q_out + (t * p.num_heads + h0 + j) * static_cast<int64_t>(p.head_dim) * 2;
+      store4<DT>(d + e0 * 2, p.vec, lo[j]);
+      store4<DT>(d + (half + e0) * 2, p.vec, hi[j]);
+    }
+    return;
+  }
+  const char* src = kind == 1 ? p.key + (t * p.k_st + h * p.k_sh) * 2 : p.value + (t * p.v_st + h * p.v_sh) * 2;
   float lo[4] = {0.f, 0.f, 0.f, 0.f}, hi[4] = {0.f, 0.f, 0.f, 0.f};
   if (has) {
     load4<DT>(src + e0 * 2, p.vec, lo);
     load4<DT>(src + (half + e0) * 2, p.vec, hi);
-    if (kind != 2 && p.cos) {
-      float c1[4], c2[4], s1[4], s2[4];
-      const char* cs = p.cos + t * p.cs_st * 2;
-      const char* sn = p.sin + t * p.cs_st * 2;
-      load4<DT>(cs + e0 * 2, p.vec, c1);
-      load4<DT>(cs + (half + e0) * 2, p.vec, c2);
-      load4<DT>(sn + e0 * 2, p.vec, s1);
-      load4<DT>(sn + (half + e0) * 2, p.vec, s2);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x1 = lo[e], x2 = hi[e];
-        lo[e] = x1 * c1[e] - x2 * s1[e];
-        hi[e] = x2 * c2[e] + x1 * s2[e];
-      }
-    }
-  }
-  if (kind == 0) {
-    if (has) {
-      char* d = p.q_out + (t * p.num_heads + h) * static_cast<int64_t>(p.head_dim) * 2;
-      store4<DT>(d + e0 * 2, p.vec, lo);
-      store4<DT>(d + (half + e0) * 2, p.vec, hi);
-    }
-    return;
+    if (kind == 1 && p.cos) rotate(lo, hi);
   }
 
   // The row's minimum and maximum; a lane with a NaN or an infinity makes the maximum infinite.
@@ -233,13 +252,24 @@ int launch_write(Kv4WriteParams& p, int dtype, hipStream_t stream) {
   int shift = 0;
   while ((8 << shift) < p.head_dim) ++shift;
   p.lane_shift = shift;
-  const int64_t rows = p.nq + 2 * p.nk;
   const int64_t per = 256 >> shift;
-  const int64_t blocks = (rows + per - 1) / per;
+  auto blocks_of = [&] { return (p.nq + 2 * p.nk + per - 1) / per; };
+  // Four query rows a thread where there are more than four workgroups for each
+  // compute unit without: 2048 tokens of 28 heads of 128 10.3 us, 12.3 singly; 32 of 14
+  // of 64 4.4 and 4.1.
+  const bool four = blocks_of() > 4 * 256 && p.nq > 0;
+  if (four) {
+    const int64_t tokens = p.nq / p.groups;
+    p.groups = (p.num_heads + 3) / 4;
+    p.nq = tokens * p.groups;
+  }
+  const int64_t blocks = blocks_of();
   if (blocks > 0x7FFFFFFF) return NS_ERR_INVALID_ARG;
   void* args[] = {&p};
-  const void* fn = dtype == NS_DTYPE_F16 ? reinterpret_cast<const void*>(&kv4_write_kernel<F16>)
-                                         : reinterpret_cast<const void*>(&kv4_write_kernel<BF16>);
+  const void* fn = dtype == NS_DTYPE_F16 ? (four ? reinterpret_cast<const void*>(&kv4_write_kernel<F16, 4>)
+                                                 : reinterpret_cast<const void*>(&kv4_write_kernel<F16, 1>))
+                                         : (four ? reinterpret_cast<const void*>(&kv4_write_kernel<BF16, 4>)
+                                                 : reinterpret_cast<const void*>(&kv4_write_kernel<BF16, 1>));
   const hipError_t e = hipLaunchKernel(fn, dim3(static_cast<unsigned>(blocks)), dim3(256), args, 0, stream);
   return e == hipSuccess ? NS_OK : NS_ERR_HIP;
 }
@@ -325,6 +355,7 @@ extern "C" int ns_rope_reshape_and_cache_int4(void* q_out, const void* query,
   p.sin = static_cast<const char*>(sin);
   p.cs_st = cos_sin_stride_token;
   p.num_heads = num_heads;
+  p.groups = num_heads;
   p.nq = num_tokens * num_heads;
   p.vec = p.vec && !misaligned(q_out, 8) && !misaligned(query, 8) && !misaligned(cos, 8) && !misaligned(sin, 8) &&
           q_stride_token % 4 == 0 && q_stride_head % 4 == 0 && cos_sin_stride_token % 4 == 0;

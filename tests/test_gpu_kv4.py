@@ -155,7 +155,8 @@ def _turn(x, cos, sin):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("T,hq,hkv,d,bs", [(1, 14, 2, 64, 16), (37, 28, 4, 128, 16), (5, 4, 4, 80, 8), (9, 3, 1, 8, 4)])
+@pytest.mark.parametrize("T,hq,hkv,d,bs", [(1, 14, 2, 64, 16), (37, 28, 4, 128, 16), (5, 4, 4, 80, 8), (9, 3, 1, 8, 4),
+                                            (2100, 14, 2, 64, 16), (701, 27, 3, 128, 16), (3500, 6, 2, 40, 8)])
 def test_rope_write_matches_float64(T, hq, hkv, d, bs, dtype):
     qkv, cos, sin = _rope_case(T, hq, hkv, d, dtype)
     nb = -(-T // bs) + 2
@@ -167,12 +168,14 @@ def test_rope_write_matches_float64(T, hq, hkv, d, bs, dtype):
     eps = torch.finfo(dtype).eps
     want = _turn(q, cos, sin)
     size = q.double().abs() + q.double().roll(d // 2, -1).abs()  # |x1| + |x2|: two float32 roundings of each product
-    assert ((out.double().cpu() - want).abs() <= want.abs() * eps / 2 + size * 2 ** -22).all()
+    # Half a step of a subnormal result is smallest_normal * eps / 2 whatever its size: the step below the smallest
+    # normal number is the one just above it, smallest_normal * eps.
+    tiny = torch.finfo(dtype).smallest_normal * eps
+    assert ((out.double().cpu() - want).abs() <= want.abs() * eps / 2 + size * 2 ** -22 + tiny / 2).all()
     # K: within half a step of the rotated row, plus what the roundings of scale and offset move.
     codes, s, b = kv4.get_rows(got[0].cpu(), slots, dtype, False)
     kr = _turn(k, cos, sin)
     err = (kv4.stored_values(codes, s, b) - kr).abs()
-    tiny = torch.finfo(dtype).smallest_normal * eps
     assert (err <= s.double() * (0.5 + 15 * eps / 2 + 1e-4) + kr.abs().amax(-1, keepdim=True) * eps + 16 * tiny).all()
     lo, hi = kr.amin(-1, keepdim=True), kr.amax(-1, keepdim=True)
     assert ((b.double() - lo).abs() <= lo.abs() * (eps / 2 + 2 ** -20) + 2 ** -20).all()
@@ -180,6 +183,10 @@ def test_rope_write_matches_float64(T, hq, hkv, d, bs, dtype):
     # V is not rotated: the oracle's bytes.
     kv4.put_rows(caches[1], slots.tolist(), *kv4.quantise_rows(v.float(), dtype), is_v=True)
     assert torch.equal(got[1].cpu(), caches[1])
+    # In place: the same.
+    q = q.contiguous().to(DEV)
+    rope_reshape_and_cache_int4(q, k.to(DEV), v.to(DEV), cos.to(DEV), sin.to(DEV), *got, slots.to(DEV), out=q)
+    assert torch.equal(q, out)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
