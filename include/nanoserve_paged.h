@@ -487,7 +487,7 @@ int ns_paged_attention_noalloc(void* out, const void* query,
  * dims 2i and 2i + 1 in the low and high nibble of byte i; V's in groups of
  * four tokens, the byte of dims 2i and 2i + 1 of token t being byte
  * 4 i + (0, 2, 1, 3)[t % 4] of group t / 4.  A row x becomes
- *     offset = R(min x), scale = R((max x - min x) / 15),
+ *     offset = R(min x), scale = R((max x - min x) * (1 / 15)),
  *     code = clamp(rint((x - offset) / scale), 0, 15), 0 where scale is 0,
  * in float32, R the rounding to the model's dtype.  A row with a NaN or an
  * infinity, or whose scale or offset overflows the dtype, is stored with

@@ -2,10 +2,11 @@
 // its reader by slot (record layout: kv4.h).
 //
 // A row x of head_dim values becomes
-//   offset = R(min x),  scale = R((max x - min x) / 15),
+//   offset = R(min x),  scale = R((max x - min x) * (1 / 15)),
 //   code   = clamp(rint((x - offset) / scale), 0, 15)      (0 where scale is 0)
-// with R the rounding to the model's dtype and everything else in float32, so
-// a stored value is within half a scale of the row's, plus the roundings of
+// with R the rounding to the model's dtype and everything else in float32 (the
+// factor 1 / 15 too, which moves the scale by a float32 step at most, where R drops
+// 13 or 16 of those bits), so a stored value is within half a scale of the row's, plus the roundings of
 // scale and offset.  The rotary embedding in front of it is evaluated in
 // float32 from the model-dtype cos and sin and not rounded before the codes
 // are taken; the rotated query is rounded once.  A row that holds a NaN or an
@@ -19,6 +20,10 @@
 // lane holds four values of the row's first half and the four that
 // rotate_half couples with them.
 #include "kv4.h"
+
+// Every product and sum is rounded by itself: a value next to the border of two
+// codes is stored as the formula above has it, however a compiler would fuse them.
+#pragma clang fp contract(off)
 
 namespace ns {
 namespace {
@@ -162,7 +167,9 @@ __global__ __launch_bounds__(256) void kv4_write_kernel(Kv4WriteParams p) {
     mn = fminf(mn, __shfl_xor(mn, off));
     mx = fmaxf(mx, __shfl_xor(mx, off));
   }
-  uint32_t sb = Half<DT>::from_f32((mx - mn) / 15.f), ob = Half<DT>::from_f32(mn);
+  float step = (mx - mn) * (1.f / 15.f);
+  asm("" : "+v"(step));  // rounded to float32 first: the compiler would round the product to float16 at once
+  uint32_t sb = Half<DT>::from_f32(step), ob = Half<DT>::from_f32(mn);
   float s = Half<DT>::to_f32(sb);
   const float b = Half<DT>::to_f32(ob);
   if (!(s < INFINITY) || !(fabsf(b) < INFINITY)) {

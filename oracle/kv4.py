@@ -18,7 +18,7 @@ def quantise_rows(x: torch.Tensor, dtype: torch.dtype):
     """float32 rows [..., D] -> (codes uint8 [..., D], scale, offset [..., 1] in dtype)."""
     x = x.float()
     lo, hi = x.amin(-1, keepdim=True), x.amax(-1, keepdim=True)
-    scale, offset = ((hi - lo) / torch.tensor(15.0)).to(dtype), lo.to(dtype)
+    scale, offset = ((hi - lo) * torch.tensor(1 / 15)).to(dtype), lo.to(dtype)
     fine = torch.isfinite(x).all(-1, keepdim=True) & torch.isfinite(scale) & torch.isfinite(offset)
     scale = torch.where(fine, scale, torch.zeros_like(scale))
     offset = torch.where(fine, offset, torch.full_like(offset, float("nan")))

@@ -180,7 +180,14 @@ def test_rope_write_matches_float64(T, hq, hkv, d, bs, dtype):
     lo, hi = kr.amin(-1, keepdim=True), kr.amax(-1, keepdim=True)
     assert ((b.double() - lo).abs() <= lo.abs() * (eps / 2 + 2 ** -20) + 2 ** -20).all()
     assert ((s.double() - (hi - lo) / 15).abs() <= (hi - lo) / 15 * (eps / 2 + 2 ** -20) + 2 ** -20).all()
-    # V is not rotated: the oracle's bytes.
+    # The same in float32, each product and sum rounded: the oracle's bytes.
+    x, c, n = k.float(), cos.float(), sin.float()
+    h = d // 2
+    k32 = torch.cat((x[..., :h] * c[..., :h] - x[..., h:] * n[..., :h], x[..., h:] * c[..., h:] + x[..., :h] * n[..., h:]),
+                    -1)
+    kv4.put_rows(caches[0], slots.tolist(), *kv4.quantise_rows(k32, dtype), is_v=False)
+    assert torch.equal(got[0].cpu(), caches[0])
+    # V is not rotated.
     kv4.put_rows(caches[1], slots.tolist(), *kv4.quantise_rows(v.float(), dtype), is_v=True)
     assert torch.equal(got[1].cpu(), caches[1])
     # In place: the same.
