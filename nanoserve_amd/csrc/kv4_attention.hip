@@ -71,6 +71,19 @@ __device__ __forceinline__ Rows rows_of(const Kv4AttnParams& p, int s) {
   return r;
 }
 
+// The sequence of query row t: the last s with query_start_loc[s] <= t, where there
+// are offsets (a decode-only batch has none: its rows are its sequences).
+__device__ __forceinline__ int sequence_of(const Kv4AttnParams& p, int64_t t) {
+  if (p.decode_only) return static_cast<int>(t);
+  int lo = 0, hi = p.num_seqs - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (load_index(p.qsl, mid, p.qsl64) <= t) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
 // ---- any shape: one wave per (token row, query head) ------------------------
 //
 // One key per lane: the lane's dot product of the query (in LDS, float32) with
@@ -87,17 +100,7 @@ __global__ __launch_bounds__(64) void kv4_attention_generic_kernel(Kv4AttnParams
   const int D = p.head_dim, half = D / 2, bs = p.block_size;
   const int kvh = h / p.group;
 
-  // The row's sequence: the last s with query_start_loc[s] <= t.
-  int s = static_cast<int>(t);
-  if (!p.decode_only) {
-    int lo = 0, hi = p.num_seqs - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (load_index(p.qsl, mid, p.qsl64) <= t) lo = mid;
-      else hi = mid - 1;
-    }
-    s = lo;
-  }
+  const int s = sequence_of(p, t);
   const Rows r = rows_of(p, s);
   if (t < r.row0 || t >= r.row0 + r.ql) return;  // a row of no sequence is left as it is
   const int64_t limit = r.len - r.ql + (t - r.row0);  // the row's last key
@@ -1137,19 +1140,8 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnParams p) {
   const int lane = threadIdx.x & 63;
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t r = at / p.num_heads;
-  int s = static_cast<int>(r);
-  if (DECODE) {
-    if (s >= p.num_seqs) return;
-  } else {
-    if (r >= p.num_tokens) return;
-    int lo = 0, hi = p.num_seqs - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (load_index(p.qsl, mid, p.qsl64) <= r) lo = mid;
-      else hi = mid - 1;
-    }
-    s = lo;
-  }
+  if (r >= (DECODE ? p.num_seqs : p.num_tokens)) return;
+  const int s = DECODE ? static_cast<int>(r) : sequence_of(p, r);
   const Rows rows = rows_of(p, s);
   if (rg.of(static_cast<int>(rows.len)) == 1) return;  // whole: there is its output already
   int64_t keys = rows.len;

@@ -28,6 +28,7 @@ from nanoserve_amd import (Int4PagedKVCache, gather_cache_int4, paged_attention_
 from nanoserve_amd.capture import graph_capture
 from oracle import kv4
 from tests._helpers import make_md, md_to
+from tests.test_oracle_kv4 import WIDE_GROUPS
 
 pytestmark = pytest.mark.gpu
 
@@ -674,3 +675,27 @@ def test_write_then_attend_and_write_again(dtype):
     _check(_run(c), c, what="whole")
     k, v = cache.read(0, torch.tensor(slots, device=DEV))
     assert np.allclose(k.double().cpu().numpy(), kv4.stored_values(*rows[0]).numpy(), atol=2e-2, rtol=1e-2)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,hkv,d,seqs", WIDE_GROUPS)
+def test_decode_of_wide_groups_over_split_keys(hq, hkv, d, seqs, dtype):
+    """More than 16 query heads per KV head, one row a sequence, no query offsets, keys in
+    ranges: eager calls and replays, with the host's lengths and without."""
+    c = _case(seqs, [1] * len(seqs), hq, hkv, d, 16, dtype)
+    q, kc, vc, md = _graph_case(c)
+    md = dataclasses.replace(md, query_start_loc=None, query_start_loc_cpu=None)
+    _check(paged_attention_int4(q, kc, vc, md, c.scale), c, what="host lengths")
+    md = dataclasses.replace(md, query_lens_cpu=None, seq_lens_cpu=None)
+    want = paged_attention_int4(q, kc, vc, md, c.scale)
+    _check(want, c, what="device lengths")
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with graph_capture(g, stream):
+        out = paged_attention_int4(q, kc, vc, md, c.scale)
+    for _ in range(3):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)

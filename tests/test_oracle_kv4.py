@@ -200,6 +200,20 @@ def test_workspace_is_needed_only_where_keys_are_split():
     assert size(2, 13, 2, 64, 16, 4000, 2, 1, 0, -1) == 0 and size(0, 14, 2, 64, 16, 4000, 2, 1, 0, -1) == 0
 
 
+WIDE_GROUPS = [(hq, 1, d, seqs) for hq in (20, 32) for d in (64, 128)
+               for seqs in ((1000, 900), (1000, 40, 2000, 1), (3000, 900, 1, 0, 1500, 2000, 960, 1100))]
+
+
+@pytest.mark.parametrize("hq,hkv,d,seqs", WIDE_GROUPS)
+def test_decode_rows_of_wide_groups_split_their_keys(hq, hkv, d, seqs):
+    """More than 16 query heads per KV head: these decode-only calls, which have no
+    query offsets, join ranges of keys (test_gpu_kv4 runs them)."""
+    for context in (0, sum(seqs)):
+        size = _lib.load().ns_paged_attention_int4_workspace_size(len(seqs), hq, hkv, d, 16, max(seqs), len(seqs), 1,
+                                                                  context, len(seqs))
+        assert size > 0
+
+
 def test_no_tokens_is_a_no_op():
     lib = _lib.load()
     assert lib.ns_reshape_and_cache_int4(*_write_args(T=0, key=None)) == OK
