@@ -550,7 +550,9 @@ int ns_gather_cache_int4(void* k_out, void* v_out, const void* k_cache, const vo
  * where the caller knows it, else -1; it decides only which kernel takes such
  * rows.  No context passes 2^30 tokens.  workspace: 256-byte aligned,
  * ns_paged_attention_int4_workspace_size bytes for the same sizes (0: none is
- * needed), not initialised, not read by later calls.  Calls that overlap in
+ * needed), not initialised, not read by later calls.  It holds the results of the
+ * key ranges of contexts that are split, which the device's size bounds (some tens
+ * of MB at most), and 16 bytes a sequence.  Calls that overlap in
  * time need their own.  Head sizes 64 and 128 with blocks of whole 16-token
  * tiles run on the matrix cores, every other shape a plain kernel.
  */

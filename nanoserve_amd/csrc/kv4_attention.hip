@@ -16,20 +16,34 @@
 namespace ns {
 namespace {
 
-// A row's keys are cut into n ranges of `tokens` (a multiple of 32).  With more
-// than one, range i of row r and head h leaves its maximum (log2 units), sum and
-// unnormalised output at index (r * num_heads + h) * n + i of the three.
+// A context's keys are cut into ranges of `tokens` (a multiple of 32), up to n of
+// them.  Where there is more than one, m, range i of row j and head h of the
+// sequence leaves its maximum (log2 units), sum and unnormalised output at index
+// first * num_heads + (j * num_heads + h) * m + i of the three: a sequence has
+// rows * m cells of num_heads results, and only sequences that are split have
+// any, from `first` on.  There are `cells` of them.  The lengths that were
+// expected need no more; where the device's would, every workgroup takes ranges
+// twice as long until they fit, and the join is told.
+struct Place {
+  int first, tokens;
+};
 struct Ranges {
-  int n, tokens;
+  int n, tokens, cells;
   float* maxima;
   float* sums;
   float* outputs;
+  Place* places;  // [num_seqs], of the sequences of the part; where n > 1
 
   // Ranges of a context: one where it is empty or nothing is split.
-  __device__ __forceinline__ int of(int len) const {
-    return n == 1 || len <= tokens ? 1 : (len + tokens - 1) / tokens;
+  __device__ __forceinline__ int of(int len, int each) const {
+    return n == 1 || len <= each ? 1 : (len + each - 1) / each;
   }
 };
+constexpr int kManyCells = 1 << 24;  // more than any workspace has; sums of 64 stay within 32 bits
+__device__ __forceinline__ int cells_of(int ql, int ranges) {
+  const int64_t n = static_cast<int64_t>(ql) * ranges;
+  return ranges == 1 ? 0 : n < kManyCells ? static_cast<int>(n) : kManyCells;
+}
 
 struct Kv4AttnParams {
   char* out;
@@ -743,24 +757,34 @@ __device__ __forceinline__ void store_row(char* dst, const float (&x)[D / 4]) {
   }
 }
 
-// One sequence's part of a launch: index of count(rows) work items.
+// One sequence's part of a launch: index of its work items, and its first cell.
 struct Part {
-  int seq, row, ql, len, index;
+  int seq, row, ql, len, index, cell;
 };
 
-// The work items of all sequences, count(rows) each, in order.  Every wave keeps
-// the list for itself: lane l the sequences from l * per on, and the items up to
-// and with theirs, so that an item costs one look at its lane's sequences (and,
-// up to 64 sequences, none).
+// The work items of all sequences, count(query rows, ranges) each, in order, and
+// the cells that those of more than one range take.  Every wave keeps the list for
+// itself: lane l the sequences from l * per on, and the items up to and with
+// theirs, so that an item costs one look at its lane's sequences (and, up to 64
+// sequences, none).
 template <class Count>
 struct PartList {
   const Kv4AttnParams& p;
+  const Ranges& rg;
   Count count;
+  int tokens;              // of a range
   int per, upto, mine;
-  int row, ql, len;  // of the lane's first sequence
+  int row, ql, len, cell;  // of the lane's first sequence
 
-  __device__ __forceinline__ PartList(const Kv4AttnParams& params, int lane, Count c)
-      : p(params), count(c), per((params.num_seqs + 63) >> 6), mine(0), row(0), ql(0), len(0) {
+  __device__ __forceinline__ PartList(const Kv4AttnParams& params, const Ranges& ranges, int lane, Count c)
+      : p(params), rg(ranges), count(c), tokens(ranges.tokens), per((params.num_seqs + 63) >> 6) {
+    while (list(lane) > rg.cells) tokens *= 2;  // ends at the latest where no context is split
+    upto = scan(mine, lane);
+  }
+  // Returns the cells of all sequences.
+  __device__ __forceinline__ int list(int lane) {
+    int cells = 0;
+    mine = row = ql = len = cell = 0;
     for (int i = per - 1; i >= 0; --i) {
       const int s = lane * per + i;
       Rows r = {0, 0, 0};
@@ -768,9 +792,15 @@ struct PartList {
       row = static_cast<int>(r.row0);
       ql = static_cast<int>(r.ql);
       len = static_cast<int>(r.len);
-      mine += s < p.num_seqs ? count(ql, len) : 0;
+      const int n = rg.of(len, tokens), items = s < p.num_seqs ? count(ql, n) : 0;
+      mine += items;
+      cells += items > 0 ? cells_of(ql, n) : 0;
+      cells = cells < kManyCells ? cells : kManyCells;
     }
-    upto = scan(mine, lane);
+    if (rg.n == 1) return 0;
+    const int sum = scan(cells, lane);
+    cell = sum - cells;
+    return lane_value(sum, 63);
   }
   static __device__ __forceinline__ int scan(int v, int lane) {
 #pragma unroll
@@ -785,24 +815,32 @@ struct PartList {
   __device__ __forceinline__ Part find(int index, int lane) const {
     const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > index));
     index -= lane_value(upto, at) - lane_value(mine, at);
-    if (per == 1) return {at, lane_value(row, at), lane_value(ql, at), lane_value(len, at), index};
+    int first = lane_value(cell, at);
+    if (per == 1) return {at, lane_value(row, at), lane_value(ql, at), lane_value(len, at), index, first};
     for (int i = 0;; i += 64) {
       const int s = at * per + i + lane;
       const bool one = i + lane < per && s < p.num_seqs;
       Rows r = {0, 0, 0};
       if (one) r = rows_of(p, s);
-      const int q = static_cast<int>(r.ql), n = static_cast<int>(r.len);
-      const int own = one ? count(q, n) : 0;
+      const int q = static_cast<int>(r.ql), n = static_cast<int>(r.len), ranges = rg.of(n, tokens);
+      const int own = one ? count(q, ranges) : 0;
       const int sum = scan(own, lane);
+      const int own_cells = own > 0 ? cells_of(q, ranges) : 0;
+      const int cells = rg.n == 1 ? 0 : scan(own_cells, lane);
       const uint64_t hit = __builtin_amdgcn_ballot_w64(sum > index);
       if (hit) {
         const int l = __builtin_ctzll(hit);
         return {at * per + i + l, lane_value(static_cast<int>(r.row0), l), lane_value(q, l), lane_value(n, l),
-                index - (lane_value(sum, l) - lane_value(own, l))};
+                index - (lane_value(sum, l) - lane_value(own, l)), first + lane_value(cells - own_cells, l)};
       }
-      if (i + 64 >= per) return {0, 0, 0, 0, 0};  // not reached: the lane has the item
+      if (i + 64 >= per) return {0, 0, 0, 0, 0, 0};  // not reached: the lane has the item
       index -= lane_value(sum, 63);
+      first += lane_value(cells, 63);
     }
+  }
+  // What the join has to know of a part, from one workgroup of its first item.
+  __device__ __forceinline__ void tell(const Part& part) const {
+    if (rg.n > 1 && part.index == 0 && threadIdx.x == 0) rg.places[part.seq] = Place{part.cell, tokens};
   }
 };
 
@@ -829,16 +867,17 @@ __device__ __forceinline__ void one_rows(const Kv4AttnParams& p, RowState<D, W, 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, col = lane & 15;
-  auto ranges = [&](int ql, int len) { return ql == 1 ? rg.of(len) : 0; };
-  const PartList<decltype(ranges)> parts(p, lane, ranges);
+  auto ranges = [](int ql, int n) { return ql == 1 ? n : 0; };
+  const PartList<decltype(ranges)> parts(p, rg, lane, ranges);
   const int items = parts.size() * p.num_kv_heads;  // the same for every wave
   for (int item = first; item < items; item += groups) {
     const int kvh = item % p.num_kv_heads;
     const Part found = parts.find(item / p.num_kv_heads, lane);
+    if (kvh == 0) parts.tell(found);
     const int s = found.seq, len = found.len, range = found.index;
     const int64_t row0 = found.row;
-    const int t0 = range * rg.tokens;
-    const int t1 = rg.n > 1 && len - t0 > rg.tokens ? t0 + rg.tokens : len;
+    const int t0 = range * parts.tokens;
+    const int t1 = rg.n > 1 && len - t0 > parts.tokens ? t0 + parts.tokens : len;
 
     Wave<DT, D, 1> w;
     w.init();
@@ -882,8 +921,9 @@ __device__ __forceinline__ void one_rows(const Kv4AttnParams& p, RowState<D, W, 
         for (int e = 0; e < E; ++e) o[e] = __builtin_fmaf(f, *so(v, c, d0 + e), o[e]);
       }
       const int64_t h = kvh * p.group + c;
-      if (rg.of(len) > 1) {
-        const int64_t at = (static_cast<int64_t>(s) * p.num_heads + h) * rg.n + range;
+      const int n = rg.of(len, parts.tokens);
+      if (n > 1) {
+        const int64_t at = static_cast<int64_t>(found.cell) * p.num_heads + h * n + range;
         if (d0 == 0) {
           rg.maxima[at] = m;
           rg.sums[at] = sum;
@@ -943,7 +983,7 @@ __device__ __forceinline__ int column_blocks(const Kv4AttnParams& p, int ql) {
 }
 template <class DT, bool LOOP, int D, int NT, int W>
 __device__ __forceinline__ void column_block(const Kv4AttnParams& p, ColumnState<D, NT, W>& lds, const Part& found,
-                                             int kvh) {
+                                             int tokens, int kvh) {
   const Ranges& rg = p.more;
   auto& buffers = lds.buffers;
   int thread = threadIdx.x;
@@ -955,14 +995,14 @@ __device__ __forceinline__ void column_block(const Kv4AttnParams& p, ColumnState
   const int64_t row0 = found.row;
   const int cols = ql * p.group;
   // The last columns, which see the most keys, first.
-  const int blocks = column_blocks<NT>(p, ql), ranges = rg.of(len);
+  const int blocks = column_blocks<NT>(p, ql), ranges = rg.of(len, tokens);
   const int block = found.index / ranges, range = found.index - block * ranges;
   const int block_base = (blocks - 1 - block) * (64 * NT);
   auto last_of = [&](int end_col) { return len - ql + ((end_col < cols ? end_col : cols) - 1) / p.group; };
-  const int t0 = range * rg.tokens;
+  const int t0 = range * tokens;
   const int block_last = last_of(block_base + 64 * NT);  // the workgroup's last key
   if (t0 > block_last && range > 0) return;              // the merge reads ranges that hold keys
-  auto end_of = [&](int last) { return rg.n > 1 && last + 1 - t0 > rg.tokens ? t0 + rg.tokens : last + 1; };
+  auto end_of = [&](int last) { return rg.n > 1 && last + 1 - t0 > tokens ? t0 + tokens : last + 1; };
   const int block_end = end_of(block_last);
   const int base = block_base + (wave & 3) * (16 * NT);
   const bool idle = base >= cols;  // brings keys for the others
@@ -1067,11 +1107,13 @@ __device__ __forceinline__ void column_block(const Kv4AttnParams& p, ColumnState
     if (base + 16 * n + col >= cols || (range > 0 && t0 >= end)) continue;
     const int64_t at = row[n] * p.num_heads + head[n];
     if (ranges > 1) {
+      const int64_t cell =
+          static_cast<int64_t>(found.cell) * p.num_heads + (at - row0 * p.num_heads) * ranges + range;
       if (g == 0) {
-        rg.maxima[at * rg.n + range] = w.m[n];
-        rg.sums[at * rg.n + range] = l[n];
+        rg.maxima[cell] = w.m[n];
+        rg.sums[cell] = l[n];
       }
-      float* dst = rg.outputs + (at * rg.n + range) * D + g * (D / 4);
+      float* dst = rg.outputs + cell * D + g * (D / 4);
 #pragma unroll
       for (int i = 0; i < D / 4; i += 4)
         *reinterpret_cast<floatx4*>(dst + i) = floatx4{x[n][i], x[n][i + 1], x[n][i + 2], x[n][i + 3]};
@@ -1090,22 +1132,22 @@ __device__ __forceinline__ void column_block(const Kv4AttnParams& p, ColumnState
 template <class DT, int D, int NT, int W, bool LOOP>
 __device__ __forceinline__ void columns(const Kv4AttnParams& p, ColumnState<D, NT, W>& lds, int first, int groups) {
   const int lane = threadIdx.x & 63;
-  auto blocks = [&](int ql, int len) {
-    return ql < (p.every_row ? 1 : 2) ? 0 : column_blocks<NT>(p, ql) * p.more.of(len);
-  };
+  auto blocks = [&](int ql, int n) { return ql < (p.every_row ? 1 : 2) ? 0 : column_blocks<NT>(p, ql) * n; };
   // Mostly one round: for another the list is made anew, and holds no registers meanwhile.
   int item = first;
 #pragma unroll 1
   for (;;) {
-    int items;  // the same for every wave
+    int items, tokens;  // the same for every wave
     Part found;
     {
-      const PartList<decltype(blocks)> parts(p, lane, blocks);
+      const PartList<decltype(blocks)> parts(p, p.more, lane, blocks);
       items = parts.size() * p.num_kv_heads;
       if (item >= items) return;
       found = parts.find(item / p.num_kv_heads, lane);
+      if (item % p.num_kv_heads == 0) parts.tell(found);
+      tokens = parts.tokens;
     }
-    column_block<DT, LOOP>(p, lds, found, item % p.num_kv_heads);
+    column_block<DT, LOOP>(p, lds, found, tokens, item % p.num_kv_heads);
     if (!LOOP) return;
     item += groups;
     if (item >= items) return;
@@ -1130,7 +1172,7 @@ __global__ __launch_bounds__(64 * W, D == 64 ? (NT == 1 ? 4 : W == 4 ? 3 : 2) : 
 }
 
 // Joins the ranges of a row, in order: one wave per (row, query head).  DECODE:
-// row r of the partials is sequence r's only row; else it is query row r.  About
+// row r is sequence r's only one; else it is query row r.  About
 // 2 us over an empty launch, a chain of the lengths, the maxima and the outputs;
 // reading ahead of the lengths, weights passed between lanes instead of read as
 // scalars, made it 6.7 us (32 rows of 14 heads; 4.5 so).
@@ -1142,8 +1184,8 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnParams p) {
   const int64_t r = at / p.num_heads;
   if (r >= (DECODE ? p.num_seqs : p.num_tokens)) return;
   const int s = DECODE ? static_cast<int>(r) : sequence_of(p, r);
+  const Place place = rg.places[s];  // of another part's sequence: not used
   const Rows rows = rows_of(p, s);
-  if (rg.of(static_cast<int>(rows.len)) == 1) return;  // whole: there is its output already
   int64_t keys = rows.len;
   int64_t row = rows.row0;
   if (DECODE) {
@@ -1153,10 +1195,14 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnParams p) {
     row = r;
     keys = rows.len - rows.ql + (r - rows.row0) + 1;
   }
-  const int n = keys <= 0 ? 0 : static_cast<int>((keys + rg.tokens - 1) / rg.tokens);
-  const float* pm = rg.maxima + at * rg.n;
-  const float* pl = rg.sums + at * rg.n;
-  const float* po = rg.outputs + at * rg.n * D;
+  const int ranges = rg.of(static_cast<int>(rows.len), place.tokens);
+  if (ranges == 1) return;  // whole: there is its output already
+  const int n = keys <= 0 ? 0 : static_cast<int>((keys + place.tokens - 1) / place.tokens);
+  const int64_t head = at - r * p.num_heads;
+  const int64_t cell = static_cast<int64_t>(place.first) * p.num_heads + ((row - rows.row0) * p.num_heads + head) * ranges;
+  const float* pm = rg.maxima + cell;
+  const float* pl = rg.sums + cell;
+  const float* po = rg.outputs + cell * D;
   float m = -INFINITY;
   for (int i = lane; i < n; i += 64) m = fmaxf(m, pm[i]);
 #pragma unroll
@@ -1173,7 +1219,7 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnParams p) {
     for (int e = 0; e < D / 64; ++e) o[e] = __builtin_fmaf(f, po[static_cast<int64_t>(i) * D + (D / 64) * lane + e], o[e]);
   }
   const float inv = sum > 0.f ? 1.f / sum : sum;
-  uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + (row * p.num_heads + (at - r * p.num_heads)) * D + (D / 64) * lane;
+  uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + (row * p.num_heads + head) * D + (D / 64) * lane;
   if constexpr (D == 64) {
     *dst = static_cast<uint16_t>(Half<DT>::from_f32(o[0] * inv));
   } else {
@@ -1192,7 +1238,8 @@ struct Cut {
   int col_split, col_n;         // the same of longer queries
   int col_waves, col_tiles;     // waves of a workgroup of the column kernel, column tiles of a wave
   int64_t col_blocks, col_most; // column blocks of all queries, expected and at most
-  size_t dec_bytes, col_bytes;  // partials
+  int dec_cells, col_cells;     // Ranges::cells
+  size_t dec_bytes, col_bytes;  // what they and the sequences' places take
 };
 
 int64_t round_up(int64_t x, int to) { return (x + to - 1) / to * to; }
@@ -1211,7 +1258,12 @@ Cut cut_of(int num_seqs, int64_t num_tokens, int max_seq_len, int64_t context, i
   const int64_t longest = max_seq_len > 0 ? max_seq_len : 1;
   const int64_t all = num_seqs * longest;
   const int64_t tokens = context > 0 && context < all ? context : all;  // of K, and of V, that a KV head reads
-  const size_t row_bytes = (head_dim + 2) * sizeof(float);
+  // Partial results: as many cells as the expected lengths can need, which is a
+  // number of ranges for the device, however many sequences and whatever the
+  // longest of them.
+  const size_t cell_bytes = num_heads * (head_dim + 2) * sizeof(float);
+  auto bytes_of = [&](int n, int cells) { return n > 1 ? cells * cell_bytes + num_seqs * sizeof(Place) : 0; };
+  auto least = [](int64_t a, int64_t b) { return static_cast<int>(a < b ? a : b > 1 ? b : 1); };
   if (c.decode) {
     // About one range for each workgroup that the device holds, but not under
     // 384 tokens: a range costs its workgroup ~7 us of its own (the search, three
@@ -1220,11 +1272,12 @@ Cut cut_of(int num_seqs, int64_t num_tokens, int max_seq_len, int64_t context, i
     // 11.7 us; 64 around 4K (four of 128): 512 / 1024 / 2048 tokens 70.5 / 64.6 /
     // 64.6 us.  Contexts of up to 1024 stay whole: one of 750 takes 9.7 us, in two
     // ranges 8.6 and 3.0 for the second launch.
-    c.dec_split = static_cast<int>(round_up(tokens * num_kv_heads / (4 * kCUs), 128));
-    c.dec_split = c.dec_split < 384 ? 384 : c.dec_split;
-    if (longest <= 1024) c.dec_split = 1024;
+    const int64_t split = round_up((tokens * num_kv_heads + 4 * kCUs - 1) / (4 * kCUs), 128);
+    c.dec_split = longest <= 1024 ? 1024 : split < 384 ? 384 : split < 1 << 30 ? static_cast<int>(split) : 1 << 30;
     c.dec_n = static_cast<int>((longest + c.dec_split - 1) / c.dec_split);
-    c.dec_bytes = c.dec_n > 1 ? static_cast<size_t>(num_seqs) * num_heads * c.dec_n * row_bytes : 0;
+    // A split context has under 2 len / dec_split ranges, all of them 2 tokens / dec_split.
+    c.dec_cells = least(static_cast<int64_t>(num_seqs) * c.dec_n, 8 * kCUs / num_kv_heads);
+    c.dec_bytes = bytes_of(c.dec_n, c.dec_cells);
     c.dec_items = (tokens / c.dec_split + num_seqs) * num_kv_heads;
   }
   if (c.columns) {
@@ -1258,7 +1311,9 @@ Cut cut_of(int num_seqs, int64_t num_tokens, int max_seq_len, int64_t context, i
     // A sequence's last block may hold a single column.
     c.col_blocks = rows * group / (64 * c.col_tiles) + (num_seqs - ones > 0 ? num_seqs - ones : 1);
     c.col_most = num_tokens * group / (64 * c.col_tiles) + num_seqs;
-    c.col_bytes = c.col_n > 1 ? static_cast<size_t>(num_tokens) * num_heads * c.col_n * row_bytes : 0;
+    // col_n is at most kCUs / blocks, and the rows have 64 col_tiles columns a block.
+    c.col_cells = least(num_tokens * c.col_n, 64 * c.col_tiles * kCUs / num_heads);
+    c.col_bytes = bytes_of(c.col_n, c.col_cells);
   }
   return c;
 }
@@ -1275,15 +1330,15 @@ hipError_t launch(const void* fn, int64_t blocks, Kv4AttnParams& p, hipStream_t 
 template <class DT, int D>
 hipError_t launch_fast(Kv4AttnParams p, const Cut& c, char* workspace, hipStream_t st) {
   const int64_t pairs = static_cast<int64_t>(p.num_seqs) * p.num_kv_heads;
-  auto ranges = [&](char* at, int64_t rows, int n, int tokens) {
-    const int64_t cells = rows * p.num_heads * n;
+  auto ranges = [&](char* at, int cells, int n, int tokens) {
+    const int64_t all = static_cast<int64_t>(cells) * p.num_heads;
     float* o = reinterpret_cast<float*>(at);
-    return Ranges{n, tokens, o + cells * D, o + cells * (D + 1), o};
+    return Ranges{n, tokens, cells, o + all * D, o + all * (D + 1), o, reinterpret_cast<Place*>(o + all * (D + 2))};
   };
   const int64_t held = static_cast<int64_t>(kCUs) * kDecodeGroups;
   int64_t row_groups = 0;
   if (c.decode) {
-    p.one = ranges(workspace, p.num_seqs, c.dec_n, c.dec_split);
+    p.one = ranges(workspace, c.dec_cells, c.dec_n, c.dec_split);
     const int64_t most = pairs * c.dec_n < c.dec_items ? pairs * c.dec_n : c.dec_items;
     row_groups = most < held ? most : held;
   }
@@ -1294,7 +1349,7 @@ hipError_t launch_fast(Kv4AttnParams p, const Cut& c, char* workspace, hipStream
   const bool together = c.columns && row_groups < held;
   hipError_t e = hipSuccess;
   if (c.columns) {
-    p.more = ranges(workspace + align256(c.dec_bytes), p.num_tokens, c.col_n, c.col_split);
+    p.more = ranges(workspace + align256(c.dec_bytes), c.col_cells, c.col_n, c.col_split);
     p.every_row = c.every_row ? 1 : 0;
     // Where the caller's count of one-row sequences leaves far fewer blocks than the
     // rows could make, as many workgroups as blocks are expected, and a loop.
@@ -1399,7 +1454,7 @@ extern "C" int ns_paged_attention_int4(void* out, const void* query,
   const int64_t table = block_table_width * static_cast<int64_t>(block_size);
   p.max_ctx = max_seq_len < table ? max_seq_len : table;
   p.scale = scale;
-  p.one = p.more = {1, 0, nullptr, nullptr, nullptr};
+  p.one = p.more = {1, 0, 0, nullptr, nullptr, nullptr, nullptr};
   p.every_row = 0;
   p.column_groups = 0;
   const hipStream_t st = static_cast<hipStream_t>(stream);

@@ -25,6 +25,7 @@ import torch
 
 from nanoserve_amd import (Int4PagedKVCache, gather_cache_int4, paged_attention_int4, reshape_and_cache_int4,
                            rope_reshape_and_cache_int4)
+from nanoserve_amd import _lib
 from nanoserve_amd.capture import graph_capture
 from oracle import kv4
 from tests._helpers import make_md, md_to
@@ -699,3 +700,53 @@ def test_decode_of_wide_groups_over_split_keys(hq, hkv, d, seqs, dtype):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+def _workspace(c: Case):
+    """The workspace of the call, as its wrapper asks for it."""
+    md, (_, hq, d), (_, hkv, bs, _) = c.md, c.q.shape, c.kc.shape
+    ones = md.num_seqs if md.is_decode_only else md.query_lens_cpu.count(1)
+    return _lib.load().ns_paged_attention_int4_workspace_size(md.num_seqs, hq, hkv, d, bs, md.max_seq_len, md.num_tokens,
+                                                              md.is_decode_only, sum(md.seq_lens_cpu), ones)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,hkv,d,n", [(14, 2, 64, 40), (28, 4, 128, 40), (4, 2, 64, 300), (20, 1, 128, 70)])
+@pytest.mark.parametrize("host", [True, False])
+def test_one_long_context_among_short_ones(hq, hkv, d, n, host, dtype):
+    """Only the long contexts have ranges, and cells for them; one is the last of all."""
+    rng = np.random.default_rng(n)
+    seqs = [int(x) for x in rng.integers(0, 30, n)]
+    seqs[n // 3], seqs[-1] = 5000, 1700
+    c = _case(seqs, [1] * n, hq, hkv, d, 16, dtype, host=host)
+    _check(_run(c), c)
+    ql = [1] * n
+    ql[n // 3], ql[n // 2], ql[-1] = 3, min(5, seqs[n // 2]), 2
+    c = _case(seqs, ql, hq, hkv, d, 16, dtype, host=host, seed=1)
+    _check(_run(c), c)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("short", [0, 70])
+def test_decode_ranges_that_outgrow_the_workspace(d, short):
+    """Lists of another step promise few keys: ranges get longer until their results fit."""
+    h, long = 64, 3000
+    seqs = [20] * short + [long] * 5
+    c = _case(seqs, [1] * len(seqs), h, h, d, 16, torch.float16)
+    c.md.seq_lens_cpu = [1] * len(seqs)
+    cells = 5 * -(-long // 384)
+    assert 0 < _workspace(c) < cells * h * (d + 2) * 4
+    _check(_run(c), c)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_column_ranges_that_outgrow_the_workspace(d):
+    hq, hkv = 64, 4
+    seqs = [2000] * 10 + [50] * 10 + [30] * 84
+    ql = [5] * 20 + [1] * 4 + [0] * 80
+    c = _case(seqs, ql, hq, hkv, d, 16, torch.bfloat16)
+    c.md.query_lens_cpu = [1] * 100 + [2] * 4
+    cells = 10 * 5 * -(-2000 // 256)
+    decode = 2048 // hkv
+    assert 0 < _workspace(c) < (cells + decode) * hq * (d + 2) * 4
+    _check(_run(c), c)

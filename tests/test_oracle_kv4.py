@@ -214,6 +214,29 @@ def test_decode_rows_of_wide_groups_split_their_keys(hq, hkv, d, seqs):
         assert size > 0
 
 
+@pytest.mark.parametrize("hq,hkv,d", [(28, 4, 128), (14, 2, 64), (64, 4, 128), (8, 8, 128), (64, 64, 64)])
+def test_partial_results_follow_the_ranges_not_the_longest_context(hq, hkv, d):
+    """A split context has at most twice its share of the about 1024 / hkv ranges that a
+    device's worth of keys is cut into, and longer queries at most 16384 / hq (row, range)s:
+    many short contexts beside a long one cost 8 bytes each."""
+    size = _lib.load().ns_paged_attention_int4_workspace_size
+    cell = hq * (d + 2) * 4
+    decode, chunk = 2048 // hkv * cell, 16384 // hq * cell
+    for short, count, long in ((400, 511, 131072), (1000, 63, 131072), (500, 255, 131072), (30, 20000, 32768)):
+        n = count + 1
+        total = short * count + long
+        for context in (total, 0, 1):
+            got = size(n, hq, hkv, d, 16, long, n, 1, context, n)
+            assert got <= decode + 8 * n + 256
+        # The same rows beside a chunk behind the long context, of which the host knows all, the rows or nothing.
+        for ql in (3, 16):
+            for context, ones in ((total, count), (0, count), (0, -1)):
+                got = size(n, hq, hkv, d, 16, long, count + ql, 0, context, ones)
+                assert got <= decode + chunk + 16 * n + 512
+    # No more than every row in every range, either.
+    assert size(2, hq, hkv, d, 16, 1500, 2, 1, 0, 2) <= 2 * 4 * cell + 16 + 256
+
+
 def test_no_tokens_is_a_no_op():
     lib = _lib.load()
     assert lib.ns_reshape_and_cache_int4(*_write_args(T=0, key=None)) == OK
