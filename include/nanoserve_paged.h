@@ -542,7 +542,8 @@ int ns_gather_cache_int4(void* k_out, void* v_out, const void* k_cache, const vo
  * aligned.  A row without keys is zero; a row of no sequence is left as it
  * is; no context is longer than max_seq_len (keys from there on are not seen).
  * A block id outside [0, num_blocks) is never dereferenced and
- * makes the rows that need it NaN.
+ * makes the rows that need it NaN.  Sums are float32 and weights up to 2^14 before
+ * they are divided: values of V need the largest times the context below 2^113.
  *
  * context_tokens is the sum of the context lengths where the caller knows it,
  * else 0; it decides only how long contexts are cut for the device (and so the

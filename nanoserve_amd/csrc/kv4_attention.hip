@@ -642,7 +642,8 @@ struct Wave {
   // Unnormalised output dim (D / 4) g + (D / 16) r + i of column n.
   __device__ __forceinline__ float value(int n, int r, int i, float b_sum) const {
     const float code = (i & 1) ? acc[n][i][r] * 0.0625f : acc[n][i][r];
-    return __builtin_fmaf(code - mid[n][r], sigma * kCodeUnit, b_sum);
+    // Two factors: sigma * kCodeUnit may pass float32's range where neither product does.
+    return __builtin_fmaf((code - mid[n][r]) * kCodeUnit, sigma, b_sum);
   }
 };
 

@@ -750,3 +750,20 @@ def test_column_ranges_that_outgrow_the_workspace(d):
     decode = 2048 // hkv
     assert 0 < _workspace(c) < (cells + decode) * hq * (d + 2) * 4
     _check(_run(c), c)
+
+
+@pytest.mark.parametrize("d", [64, 128, 24])
+@pytest.mark.parametrize("ql", [1, 40])
+def test_values_of_v_far_beyond_float16(d, ql):
+    """bfloat16 rows of V with a scale above 2^104: 2^24 times it is no float32.  The header's
+    bound holds here, 1.7e32 * 40 < 2^113."""
+    n, hkv = 40, 2
+    c = _case([n], [ql], 4, hkv, d, 16, torch.bfloat16)
+    x = torch.rand(n, hkv, d, generator=_g(3)) * 3.4e32 - 1.7e32
+    x[..., 0], x[..., 1] = -1.7e32, 1.7e32
+    rows = kv4.quantise_rows(x, torch.bfloat16)
+    assert (rows[1].float() > 2.0 ** 104).all()
+    slots = [int(c.md.block_tables[0, p // 16]) * 16 + p % 16 for p in range(n)]
+    kv4.put_rows(c.vc, slots, *rows, is_v=True)
+    c.kv[0] = (c.kv[0][0], rows)
+    _check(_run(c), c)
