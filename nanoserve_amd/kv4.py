@@ -141,8 +141,8 @@ def rope_reshape_and_cache_int4(q: torch.Tensor, k: torch.Tensor, v: torch.Tenso
     num_blocks, heads, block_size, head_dim = _caches(k_cache, v_cache, what)
     dtype, device = q.dtype, k_cache.device
     code = _model_dtype(dtype, what)
-    if q.dim() != 3:
-        raise ValueError(f"q must be [T, Hq, {head_dim}], got {tuple(q.shape)}")
+    if q.dim() != 3 or q.shape[1] == 0:
+        raise ValueError(f"q must be [T, Hq, {head_dim}] with a head at least, got {tuple(q.shape)}")
     T, Hq, _ = q.shape
     q, qs = _rows(q, (T, Hq, head_dim), dtype, device, "q")
     k, ks = _rows(k, (T, heads, head_dim), dtype, device, "k")
@@ -160,7 +160,7 @@ def rope_reshape_and_cache_int4(q: torch.Tensor, k: torch.Tensor, v: torch.Tenso
         raise ValueError(f"out must be a contiguous [{T}, {Hq}, {head_dim}] {dtype} tensor on {device}")
     elif out.data_ptr() == q.data_ptr() and not q.is_contiguous():
         raise ValueError("out may alias q only when q is contiguous")
-    if T == 0 or Hq == 0:
+    if T == 0:
         return out
     _lib.launch(device, what, _lib.load().ns_rope_reshape_and_cache_int4,
                 out.data_ptr(), q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],

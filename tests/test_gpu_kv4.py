@@ -767,3 +767,12 @@ def test_values_of_v_far_beyond_float16(d, ql):
     kv4.put_rows(c.vc, slots, *rows, is_v=True)
     c.kv[0] = (c.kv[0][0], rows)
     _check(_run(c), c)
+
+
+def test_rope_write_without_query_heads_is_refused():
+    """Its K and V would be left unwritten."""
+    c = Int4PagedKVCache(2, 16, 1, 2, 64, torch.float16, DEV)
+    x = torch.ones(3, 2, 64, dtype=torch.float16, device=DEV)
+    with pytest.raises(ValueError):
+        rope_reshape_and_cache_int4(x[:, :0], x, x, x[:, 0], x[:, 0], c.k_cache[0], c.v_cache[0],
+                                    torch.arange(3, device=DEV))
