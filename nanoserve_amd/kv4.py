@@ -192,7 +192,12 @@ def paged_attention_int4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: to
                          md: AttentionMetadata, scale: float) -> torch.Tensor:
     """Paged attention over a cache held in 4 bits: attn_fn's contract
     (attention.paged_attention_hip) with the caches of Int4PagedKVCache, in the
-    dtype they were written in.  Returns [num_tokens, num_heads, head_dim]."""
+    dtype they were written in.  Returns [num_tokens, num_heads, head_dim], with
+    zeros for rows without keys and rows behind the last sequence.
+
+    The device's lengths, offsets and tables decide what is computed; the host's
+    lists in `md`, where there are any, shape the launches and, outside of a
+    graph capture, tell whether every row belongs to a sequence."""
     what = "paged_attention_int4"
     num_blocks, heads, block_size, head_dim = _caches(k_cache, v_cache, what)
     code = _model_dtype(query.dtype, what)
@@ -232,9 +237,11 @@ def paged_attention_int4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: to
         qsl = _vector(md.query_start_loc, "query_start_loc", n + 1, device)
         qsl_ptr, qsl64 = qsl.data_ptr(), qsl.dtype is torch.int64
         # Rows behind the last sequence are not written: zero unless the host
-        # offsets show that there are none.
+        # offsets show that there are none, which they cannot for the replays
+        # of a capture.
         host = md.query_start_loc_cpu
-        full = host is not None and len(host) > n and host[0] == 0 and host[n] == T
+        full = (host is not None and len(host) > n and host[0] == 0 and host[n] == T
+                and not torch.cuda.is_current_stream_capturing())
         out = torch.empty_like(q) if full else torch.zeros_like(q)
     # The context lengths' sum and the number of decode rows, where the host
     # has them, shape the launches.  The partial results live in a tensor of

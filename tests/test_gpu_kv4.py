@@ -776,3 +776,24 @@ def test_rope_write_without_query_heads_is_refused():
     with pytest.raises(ValueError):
         rope_reshape_and_cache_int4(x[:, :0], x, x, x[:, 0], x[:, 0], c.k_cache[0], c.v_cache[0],
                                     torch.arange(3, device=DEV))
+
+
+@pytest.mark.parametrize("d", [64, 128, 24])
+def test_a_replay_of_a_shorter_batch_leaves_zeros_behind_its_last_row(d):
+    """The host's offsets at capture cover every row; those of a later replay need not."""
+    full = _case([40, 20], [30, 3], 4, 2, d, 16, torch.float16)
+    q, kc, vc, md = _graph_case(full)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        paged_attention_int4(q, kc, vc, md, full.scale)
+    stream.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with graph_capture(g, stream):
+        out = paged_attention_int4(q, kc, vc, md, full.scale)
+    for ql in ([30, 3], [20, 1], [30, 3], [0, 2], [1, 20]):
+        part = dataclasses.replace(full, q=full.q[:sum(ql)], query_lens=ql)
+        md.query_start_loc.copy_(torch.tensor([0, ql[0], sum(ql)], dtype=md.query_start_loc.dtype))
+        g.replay()
+        _check(out[:sum(ql)], part, what=str(ql))
+        assert (out[sum(ql):] == 0).all(), ql
