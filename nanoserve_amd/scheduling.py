@@ -28,6 +28,7 @@ from __future__ import annotations
 
 import enum
 import math
+import numbers
 import time
 from collections import deque
 from dataclasses import dataclass, field
@@ -57,14 +58,14 @@ class SamplingParams:
     def __post_init__(self) -> None:
         if not 0.0 <= self.temperature < math.inf:
             raise ValueError(f"temperature must be finite and not negative, got {self.temperature}")
-        if self.top_k < 0:
+        if not self.top_k >= 0:
             raise ValueError(f"top_k must not be negative, got {self.top_k}")
         if not 0.0 < self.top_p <= 1.0:
             raise ValueError(f"top_p must be in (0, 1], got {self.top_p}")
         if not 0.0 <= self.min_p <= 1.0:
             raise ValueError(f"min_p must be in [0, 1], got {self.min_p}")
-        if self.seed is not None and self.seed < 0:
-            raise ValueError(f"seed must not be negative, got {self.seed}")
+        if self.seed is not None and (not isinstance(self.seed, numbers.Integral) or self.seed < 0):
+            raise ValueError(f"seed must be an integer that is not negative, got {self.seed!r}")
 
     @property
     def draws(self) -> bool:

@@ -18,6 +18,13 @@ def test_settings_out_of_range_are_refused(bad):
         SamplingParams(**bad)
 
 
+@pytest.mark.parametrize("bad", [dict(seed=1.5), dict(seed=float("nan")), dict(seed="7"), dict(top_k=float("nan"))])
+def test_settings_that_would_fail_in_a_later_step_are_refused(bad):
+    with pytest.raises(ValueError):
+        SamplingParams(**bad)
+    assert SamplingParams(seed=np.int64(7), top_k=np.int32(5)).seed == 7
+
+
 def test_the_default_is_greedy():
     assert not SamplingParams().draws and SamplingParams(temperature=0.5).draws
 
