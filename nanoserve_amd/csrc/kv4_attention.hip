@@ -232,9 +232,12 @@ hipError_t launch_generic(const Kv4AttnParams& p, hipStream_t stream) {
 // another) or into chunks that a workgroup shares (longer queries).  A lane's part
 // of a tile is one LDS read (8 or 16 bytes), and a mask turns its words into
 // operands (kv4.h).  Both model dtypes run in float16: the codes are exact there, the query is brought
-// into its range by a power of two for the columns that share a workgroup (exact
-// but for elements below 2^-25 of the largest, whose error is below 2^-36 of it;
-// bfloat16 rows beyond 2^16 by a power of their own besides), and the
+// into its range by a power of two for the columns that share a workgroup: the
+// largest element becomes 2^14 at least (of 2^-86 and more), so all are exact but
+// those below 2^-24 of it in odd dims, which are stored as a sixteenth, and below
+// 2^-28 in even ones; their error is at most 2^-35 of it.  (bfloat16 rows beyond
+// 2^16 are divided by a power of their own besides, and the largest becomes 2^13
+// at least: 2^-23, 2^-27 and 2^-34 of a row's own largest.)  The
 // probabilities keep 11 bits where bfloat16 would keep 8.
 //
 // A score in log2 units is two fused multiply-adds, s_t (q.c_t) + (b_t sum(q) -
