@@ -573,6 +573,98 @@ int ns_paged_attention_int4(void* out, const void* query,
                             float scale, int dtype,
                             void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * A decode step that verifies drafted tokens.  A request's query rows are its
+ * last token (row 0) and drafted ones, at most 64; a row's parent is an earlier
+ * row of the request, or -1.  Row j's K and V take cache position c + j, c being
+ * the request's tokens with K and V before the step, whatever the row's depth.
+ * No counterpart in the reference, which computes one token per request and
+ * decode step (nanoserve/model_runner.py:85-147).
+ *
+ * ns_step_inputs -- the step's addresses, from what the requests are: the
+ * reference's ModelRunner.build_inputs (nanoserve/model_runner.py:85-147,
+ * block_manager.py:93-157) on the device.  `tables` [table_rows, table_width]
+ * (row stride in elements, int32 or int64) holds a request's block ids from step
+ * to step.  Request i has table row rows[i], computed[i] tokens with K and V and
+ * query_lens[i] rows in this step; new_blocks[new_start[i] .. new_start[i + 1])
+ * are appended to its table from column held[i] on (num_new entries in all; 0: no
+ * request has any).  With start the sum of the query lengths before:
+ *   query_start_loc [num_seqs + 1]  those sums;
+ *   seq_lens [num_seqs]             computed + query_lens;
+ *   slot_mapping [num_tokens]       of row j: table[(c + j) / bs] * bs + (c + j) % bs;
+ *   positions [num_tokens]          c + j, or c + the row's depth in its tree;
+ *   tree_mask [num_tokens]          bit i: row i of the request is row j or on its
+ *                                   way to the root (only with parents);
+ *   block_tables [num_seqs, max_blocks]  (as `tables`) the blocks up to seq_lens, then 0.
+ * A row outside the table has slot -1, and a block outside it id -1; so has every
+ * row of a request whose table row is outside [0, table_rows).  Rows behind the
+ * last request have position 0, slot -1 and mask 0.  A parent that is no earlier
+ * row makes its row a root; rows from the 64th on belong to no tree (position c +
+ * j, mask 0).  Negative lengths count as 0; no length passes 2^30.  The table rows
+ * of a call must differ where blocks are appended.  rows, computed, query_lens,
+ * new_blocks, new_start, held and parents are int32 or int64 alike.  At most 65535
+ * requests.
+ *
+ * ns_commit_drafts -- which drafted rows hold, and their K and V in place.
+ * chosen[t] is the token that the model takes after row t, input_ids[t] the token
+ * that row t was fed.  From row 0, the walk goes on to the first child (parent ==
+ * the current row) whose input id is the current row's choice, until there is
+ * none.  counts[i] is the number of rows of request i's walk (0 without rows),
+ * tokens [num_seqs, max_rows] their choices, then -1.  In every one of `caches`
+ * (host array of device pointers, [num_slots, row_bytes] bytes each) the row at
+ * the slot of the walk's row d moves to the slot of the request's row d.  The slots
+ * of a request's rows must differ; slots outside [0, num_slots) are left alone.
+ * Rows from max_rows (at most 64) on take no part.
+ *
+ * ns_paged_attention_tree -- ns_paged_attention for such rows: row j of a
+ * sequence with context length L (its q rows included) sees keys 0 .. L - q - 1
+ * and key L - q + i where bit i of tree_mask (int64 [num_tokens]) is set, i < 64.
+ * A row without keys is zero, a row of no sequence is left as it is.  K and V of a
+ * key that a row does not see do not reach it, whatever they hold.  Without
+ * query_start_loc (NULL) row s is sequence s.  max_query_len is the longest
+ * sequence's rows, at most 64; it shapes the launch, the device's offsets decide.
+ * A block id outside [0, num_blocks) is never dereferenced; the affected (sequence,
+ * KV head) outputs are NaN.  float16 and bfloat16 at head sizes 64 and 128 with
+ * blocks of whole 16-token tiles run on the matrix cores (pointers 16-byte
+ * aligned; out and query contiguous), every other shape with head_dim <= 256 a
+ * plain kernel that reads no workspace.  workspace: 16-byte aligned,
+ * ns_paged_attention_tree_workspace_size bytes (0: none is needed), not
+ * initialised.  counters: ns_paged_attention_tree_counters() int32, zero before
+ * the first call, zero again after every call.  Calls that overlap in time need
+ * their own of both.
+ */
+int ns_step_inputs(void* tables, int64_t table_rows, int64_t table_width, int64_t table_stride,
+                   int tables_is_int64,
+                   const void* rows, const void* computed, const void* query_lens,
+                   const void* new_blocks, const void* new_start, const void* held, int64_t num_new,
+                   const void* parents, int index_is_int64,
+                   int64_t num_seqs, int64_t num_tokens, int block_size, int64_t max_blocks,
+                   int64_t* query_start_loc, int64_t* seq_lens, int64_t* positions,
+                   int64_t* slot_mapping, void* block_tables, int64_t* tree_mask, void* stream);
+int ns_commit_drafts(int64_t* counts, int64_t* tokens,
+                     const void* chosen, const void* input_ids, const void* parents, int index_is_int64,
+                     const void* query_start_loc, int query_start_loc_is_int64,
+                     const void* slot_mapping, int slot_mapping_is_int64,
+                     int64_t num_seqs, int64_t num_tokens, int max_rows,
+                     void* const* caches, int num_caches, int64_t num_slots, int64_t row_bytes,
+                     void* stream);
+int ns_paged_attention_tree_counters(void);
+size_t ns_paged_attention_tree_workspace_size(int num_seqs, int num_heads, int num_kv_heads, int head_dim,
+                                              int block_size, int max_query_len, int64_t num_tokens,
+                                              int dtype);
+int ns_paged_attention_tree(void* out, const void* query,
+                            const void* k_cache, const void* v_cache,
+                            const void* block_tables, int64_t block_table_stride,
+                            int64_t block_table_width, int block_tables_is_int64,
+                            const void* seq_lens, int seq_lens_is_int64,
+                            const void* query_start_loc, int query_start_loc_is_int64,
+                            const int64_t* tree_mask,
+                            int num_seqs, int64_t num_tokens, int max_query_len, int max_seq_len,
+                            int num_heads, int num_kv_heads, int head_dim,
+                            int block_size, int64_t num_blocks,
+                            float scale, int dtype,
+                            int* counters, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

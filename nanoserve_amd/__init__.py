@@ -10,8 +10,9 @@ write with hand-written gfx950 HIP kernels behind a C ABI
   rotary.apply + PagedKVCache.write fused              (rope_reshape_and_cache)
 
 Beside the reference's: the same write and attention over a cache held in 4
-bits (kv4.py), and the draw of a token from given uniform numbers
-(sampling.sample_rows).
+bits (kv4.py), the draw of a token from given uniform numbers
+(sampling.sample_rows), and a decode step that verifies trees of drafted tokens
+(tree.py).
 """
 
 from .attention import AttentionMetadata, get_attention_backend, paged_attention_hip
@@ -21,6 +22,7 @@ from .kv4 import (Int4PagedKVCache, gather_cache_int4, paged_attention_int4, res
                   rope_reshape_and_cache_int4)
 from .rotary import RotaryEmbedding, rope_reshape_and_cache
 from .sampling import argmax_rows, sample_rows
+from .tree import StepInputs, commit_drafts, paged_attention_tree, step_inputs
 
 __version__ = "0.1.0"
 
@@ -29,16 +31,20 @@ __all__ = [
     "BlockSpaceManager",
     "Int4PagedKVCache",
     "PagedKVCache",
+    "StepInputs",
     "argmax_rows",
+    "commit_drafts",
     "gather_cache_int4",
     "get_attention_backend",
     "kv_bytes_per_token",
     "paged_attention_hip",
     "paged_attention_int4",
+    "paged_attention_tree",
     "reshape_and_cache",
     "reshape_and_cache_int4",
     "RotaryEmbedding",
     "rope_reshape_and_cache",
     "rope_reshape_and_cache_int4",
     "sample_rows",
+    "step_inputs",
 ]

@@ -24,7 +24,7 @@ LIB_NAME = "libnanoserve_paged.so"
 LIB_PATH = PKG_DIR / LIB_NAME
 SOURCES = ["paged_attention.hip", "decode_plan.hip", "reshape_and_cache.hip", "rope_cache.hip",
            "int4_linear.hip", "argmax.hip", "generic_attention.hip", "kv4_cache.hip", "kv4_attention.hip",
-           "sample.hip"]
+           "sample.hip", "tree_attention.hip", "draft_step.hip"]
 # The benchmark's measurement probe (an empty launch and a plain streaming
 # read) is a library of its own: nothing in the product loads or declares it.
 FLOORS_SOURCES = ["floors.hip"]

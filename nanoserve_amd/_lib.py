@@ -204,6 +204,40 @@ SIGNATURES = {
         c_float, c_int,                          # scale, dtype
         c_void_p, c_size_t, c_void_p,            # workspace, bytes, stream
     ]),
+    "ns_step_inputs": (c_int, [
+        c_void_p, c_int64, c_int64, c_int64, c_int,  # tables, rows, width, row stride, is_int64
+        c_void_p, c_void_p, c_void_p,            # rows, computed, query_lens
+        c_void_p, c_void_p, c_void_p, c_int64,   # new_blocks, new_start, held, num_new
+        c_void_p, c_int,                         # parents (or None), index is_int64
+        c_int64, c_int64, c_int, c_int64,        # S, T, block_size, max_blocks
+        c_void_p, c_void_p, c_void_p,            # query_start_loc, seq_lens, positions (out)
+        c_void_p, c_void_p, c_void_p, c_void_p,  # slot_mapping, block_tables, tree_mask (out), stream
+    ]),
+    "ns_commit_drafts": (c_int, [
+        c_void_p, c_void_p,                      # counts, tokens (out)
+        c_void_p, c_void_p, c_void_p, c_int,     # chosen, input_ids, parents, is_int64
+        c_void_p, c_int, c_void_p, c_int,        # query_start_loc, is_int64, slot_mapping, is_int64
+        c_int64, c_int64, c_int,                 # S, T, max_rows
+        c_void_p, c_int, c_int64, c_int64,       # cache pointers (host array), their number, num_slots, row_bytes
+        c_void_p,                                # stream
+    ]),
+    "ns_paged_attention_tree_counters": (c_int, []),
+    "ns_paged_attention_tree_workspace_size": (c_size_t, [
+        c_int, c_int, c_int, c_int, c_int,       # S, Hq, Hkv, D, block_size
+        c_int, c_int64, c_int,                   # max_query_len, T, dtype
+    ]),
+    "ns_paged_attention_tree": (c_int, [
+        c_void_p, c_void_p,                      # out, query
+        c_void_p, c_void_p,                      # k_cache, v_cache
+        c_void_p, c_int64, c_int64, c_int,       # block_tables, row stride, width, is_int64
+        c_void_p, c_int,                         # seq_lens, is_int64
+        c_void_p, c_int,                         # query_start_loc (or None), is_int64
+        c_void_p,                                # tree_mask
+        c_int, c_int64, c_int, c_int,            # S, T, max_query_len, max_seq_len
+        c_int, c_int, c_int, c_int, c_int64,     # Hq, Hkv, D, block_size, num_blocks
+        c_float, c_int,                          # scale, dtype
+        c_void_p, c_void_p, c_size_t, c_void_p,  # counters, workspace, bytes, stream
+    ]),
 }
 
 _lock = threading.Lock()

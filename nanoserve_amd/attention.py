@@ -62,6 +62,10 @@ class AttentionMetadata:
     # step's first attention call (or explicitly before it) and read by every
     # layer's call.
     decode_plan: "DecodePlan | None" = None
+    # [num_tokens] int64, for trees of drafted tokens (tree.py): bit i of a row
+    # says that it sees its sequence's row i; keys before the rows are seen by all.
+    # None: every row sees the keys up to its own, as the reference's.
+    tree_mask: torch.Tensor | None = None
 
 
 @dataclass(frozen=True)
@@ -173,8 +177,8 @@ def prepare_decode_plan(md: AttentionMetadata, cache: torch.Tensor) -> None:
     that calls this rebuilds it from the replayed step's lengths.  Calls whose
     sizes differ from the plan's build their own instead.
     """
-    if md.num_seqs == 0 or md.num_tokens == 0:
-        return
+    if md.num_seqs == 0 or md.num_tokens == 0 or md.tree_mask is not None:
+        return  # attention for trees cuts its work in the call itself
     lib = _lib.load()
     _, block_size, num_kv_heads, head_dim = cache.shape
     if takes_generic_kernel(cache.dtype, head_dim, block_size, 1):
@@ -234,7 +238,12 @@ def paged_attention_hip(
     """Unified paged attention on the GPU.  Returns [num_tokens, num_heads, head_dim].
 
     The reference's attn_fn contract (attention.py:99-151).  The decode plan
-    is shared by the calls of one md: built by the first, reused by the rest."""
+    is shared by the calls of one md: built by the first, reused by the rest.
+    An md with a tree_mask takes paged_attention_tree."""
+    if md.tree_mask is not None:
+        from .tree import paged_attention_tree
+
+        return paged_attention_tree(query, k_cache, v_cache, md, scale)
     return _attention(query, k_cache, v_cache, md, scale, share_plan=True)
 
 

@@ -211,6 +211,8 @@ def paged_attention_int4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     n, longest = md.num_seqs, md.max_seq_len
     if md.num_tokens != T:
         raise ValueError(f"metadata has {md.num_tokens} tokens, query has {T}")
+    if md.tree_mask is not None:
+        raise ValueError(f"{what} takes no tree_mask: trees of drafted tokens need a 16-bit cache")
     if Hq % heads:
         raise ValueError(f"{Hq} query heads over {heads} KV heads")
     q = query if query.is_contiguous() else query.contiguous()
