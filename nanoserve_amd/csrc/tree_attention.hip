@@ -34,10 +34,8 @@ struct TreeParams {
   int64_t max_ctx;         // keys a sequence may have: max_seq_len, within the table
   float scale;
   // Matrix-core kernel.
-  float* partials;         // kPartWords(columns, D) words per slot
-  int* counters;           // [slots], zero before and after
-  int slots;               // 2 * target
-  int target;              // items that the key ranges are cut for
+  float* partials;         // two slots a workgroup
+  int* counters;           // one a workgroup, zero before and after
 };
 
 struct SeqRows {
@@ -194,22 +192,30 @@ hipError_t launch_generic(const TreeParams& p, hipStream_t stream) {
 
 // ---- head sizes 64 and 128, blocks of whole 16-token tiles --------------------
 //
-// A sequence's rows times the heads of one KV head are columns, 16 a tile.  A work
-// item is up to NT tiles of columns and a range of keys; a wave takes the range's
-// chunks of 32 keys w, w + 4, ... for all of the item's columns, so that every row
-// of K and V is loaded once for up to 16 NT rows of the product, and the waves meet
-// once, at the item's end.  K and V come by LDS-DMA into a ring of each wave's own,
-// S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32.  The result layout of the
-// first product (keys 4 g + r of column lane % 16 in lane group g) is the operand
-// layout of the second.
+// A sequence's rows times the heads of one KV head are columns, 16 a tile.  A group
+// is up to NT tiles of columns of one (sequence, KV head); a workgroup takes a range
+// of a group's keys, and a wave the range's chunks of 32 keys w, w + 4, ... for all of
+// the group's columns, so that every row of K and V is loaded once for up to 16 NT
+// rows of the product, and the waves meet once, at the range's end.  K and V come by
+// LDS-DMA into a ring of each wave's own, S^T = K Q^T and O^T = V^T P^T on
+// v_mfma_f32_16x16x32.  The result layout of the first product (keys 4 g + r of
+// column lane % 16 in lane group g) is the operand layout of the second.
 //
 // The probabilities enter the second product in the model's dtype, and their sum
 // is taken by the same product with a tile of ones, so that a rounding acts on both.
+//
+// Work is cut evenly: the groups' chunks, and kGroupCost for what a group costs
+// beside them, are laid end to end, and workgroup k takes the k-th equal share of
+// that line, whatever it covers: parts of groups, whole ones, or both.  Cuts move to
+// whole rounds of the four waves.  A group that a cut falls into is joined by the last
+// of its workgroups to finish.  Every workgroup works its share out of the device's
+// lengths for itself.
 
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
-constexpr int kMostRanges = 16;  // of a sequence: what the last workgroup has to join
-constexpr int kLeastTokens = 128;
+constexpr int kMostRanges = 32;  // of a group: what the last workgroup has to join
+constexpr int kGroupCost = 4;    // in chunks
+constexpr int kLeastShare = 8;   // chunks
 
 template <int D, int NT>
 struct Cfg {
@@ -227,7 +233,9 @@ struct Cfg {
   static constexpr int PART = COLS * (D + 2);   // words of a slot: outputs, then (maximum, sum) of every column
   // The waves meet a group of column tiles at a time, as many as fit the ring.
   static constexpr int JOIN = RING / (kWaves * 16 * D * 4) < NT ? RING / (kWaves * 16 * D * 4) : NT;
+  static constexpr int OWN = COLS * (D / 4) / kThreads;  // float4 of the output per thread
   static_assert(JOIN >= 1, "a column tile of every wave fits the ring");
+  static_assert(2 * kMostRanges * COLS * 4 <= RING, "the ranges' maxima and sums fit the ring");
 };
 
 constexpr int kSc1 = 16;                  // cache-policy bit SC1 of gfx950 buffer operations: device scope
@@ -249,59 +257,153 @@ __device__ __forceinline__ int v_swizzle(int key) {
   return D == 64 ? ((key >> 1) & 3) << 1 : (key & 7) << 1;
 }
 
-// The sum of x over the workgroup's threads (scratch: kWaves words).
-__device__ __forceinline__ int64_t block_sum(int64_t x, int64_t* scratch) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off);
-  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = x;
-  __syncthreads();
-  x = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) x += scratch[w];
-  __syncthreads();
-  return x;
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x >> 32));
+  return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
 }
-// The sums of x over the threads before this one; the sum of all in `total`.
-__device__ __forceinline__ int block_scan(int x, int* scratch, int& total) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  int y = x;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int z = __shfl_up(y, off);
-    if (lane >= off) y += z;
-  }
-  if (lane == 63) scratch[w] = y;
-  __syncthreads();
-  int before = 0;
-  total = 0;
-#pragma unroll
-  for (int i = 0; i < kWaves; ++i) {
-    if (i < w) before += scratch[i];
-    total += scratch[i];
-  }
-  __syncthreads();
-  return before + y - x;
+__device__ __forceinline__ int64_t lane_value64(int64_t x, int lane) {
+  const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), lane));
+  const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x >> 32), lane));
+  return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
+}
+__device__ __forceinline__ int64_t shuffle_up64(int64_t x, int by) {
+  const uint32_t lo = static_cast<uint32_t>(__shfl_up(static_cast<int>(x), by));
+  const uint32_t hi = static_cast<uint32_t>(__shfl_up(static_cast<int>(x >> 32), by));
+  return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
+}
+// x / y for x >= 0, y > 0: the quotient in float32, put right.
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
+  int64_t q = static_cast<int64_t>(static_cast<float>(x) / static_cast<float>(y));
+  while (q * y > x) --q;
+  while ((q + 1) * y <= x) ++q;
+  return q;
 }
 
-// What the workgroups of a launch agree on: every sequence's first item and first
-// slot, from the device's lengths alone.
-struct Schedule {
-  int first[kSeqs + 1];
-  int slot[kSeqs + 1];
+// The sequences of a launch along the line of work, from the device's lengths.  Up to
+// 64 of them live in the lanes of every wave; more are held in LDS.
+struct Held {
+  int64_t start[kSeqs];
   int row0[kSeqs], ql[kSeqs], len[kSeqs];
   int64_t sums[kWaves];
-  int scans[kWaves];
-  int each;   // keys of a range
-  int found;  // the item's sequence
-  int last;   // whether this workgroup joins the ranges
+  int most[kWaves];
 };
 
-__device__ __forceinline__ int ranges_of(int len, int each) {
-  const int most = (len + kMostRanges - 1) / kMostRanges;
-  each = each > most ? each : (most + 31) / 32 * 32;
-  const int n = (len + each - 1) / each;
-  return n < 1 ? 1 : n;
-}
+template <int COLS>
+struct Line {
+  int64_t start;          // this lane's sequence (num_seqs <= 64)
+  int row0, ql, len;
+  Held* held;             // otherwise
+  int num_seqs, heads, group;
+  int64_t total;
+  int most;               // weight of the longest group
+
+  __device__ __forceinline__ int weight(int len_) const { return ((len_ + 31) >> 5) + kGroupCost; }
+  __device__ __forceinline__ int groups(int ql_) const { return (ql_ * group + COLS - 1) / COLS * heads; }
+
+  __device__ __forceinline__ void scan(int64_t x, int m, int lane, int64_t& before, int64_t& all, int& longest) {
+    int64_t y = x;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int64_t z = shuffle_up64(y, off);
+      if (lane >= off) y += z;
+      m = max(m, __shfl_xor(m, off));
+    }
+    before = y - x;
+    all = lane_value64(y, 63);
+    longest = __builtin_amdgcn_readfirstlane(m);
+  }
+
+  __device__ __forceinline__ void make(const TreeParams& p, Held& h) {
+    const int lane = threadIdx.x & 63;
+    held = &h;
+    num_seqs = p.num_seqs;
+    heads = p.num_kv_heads;
+    group = p.group;
+    row0 = ql = len = 0;
+    if (num_seqs <= 64) {
+      int64_t x = 0;
+      int m = 0;
+      if (lane < num_seqs) {
+        const SeqRows r = rows_of(p, lane);
+        row0 = static_cast<int>(r.row0);
+        ql = static_cast<int>(r.ql);
+        len = static_cast<int>(r.len);
+        m = ql > 0 ? weight(len) : 0;
+        x = static_cast<int64_t>(groups(ql)) * m;
+      }
+      scan(x, m, lane, start, total, most);
+      return;
+    }
+    constexpr int PER = kSeqs / kThreads;
+    const int w = threadIdx.x >> 6;
+    int64_t x[PER], sum = 0;
+    int m = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int s = PER * static_cast<int>(threadIdx.x) + i;
+      x[i] = 0;
+      if (s < num_seqs) {
+        const SeqRows r = rows_of(p, s);
+        h.row0[s] = static_cast<int>(r.row0);
+        h.ql[s] = static_cast<int>(r.ql);
+        h.len[s] = static_cast<int>(r.len);
+        const int wt = r.ql > 0 ? weight(static_cast<int>(r.len)) : 0;
+        m = max(m, wt);
+        x[i] = static_cast<int64_t>(groups(static_cast<int>(r.ql))) * wt;
+        sum += x[i];
+      }
+    }
+    int64_t before, all;
+    scan(sum, m, lane, before, all, most);
+    if (lane == 0) {
+      h.sums[w] = all;
+      h.most[w] = most;
+    }
+    __syncthreads();
+    total = 0;
+    most = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+      if (i < w) before += h.sums[i];
+      total += h.sums[i];
+      most = max(most, h.most[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int s = PER * static_cast<int>(threadIdx.x) + i;
+      if (s < num_seqs) h.start[s] = before;
+      before += x[i];
+    }
+    __syncthreads();
+    total = uniform64(total);
+    most = __builtin_amdgcn_readfirstlane(most);
+  }
+
+  __device__ __forceinline__ void get(int s, int64_t& start_, int& row0_, int& ql_, int& len_) const {
+    if (num_seqs <= 64) {
+      start_ = lane_value64(start, s);
+      row0_ = __builtin_amdgcn_readlane(row0, s);
+      ql_ = __builtin_amdgcn_readlane(ql, s);
+      len_ = __builtin_amdgcn_readlane(len, s);
+    } else {
+      start_ = uniform64(held->start[s]);
+      row0_ = __builtin_amdgcn_readfirstlane(held->row0[s]);
+      ql_ = __builtin_amdgcn_readfirstlane(held->ql[s]);
+      len_ = __builtin_amdgcn_readfirstlane(held->len[s]);
+    }
+  }
+
+  // The sequence that place `at` of the line lies in: the last that starts there or before.
+  __device__ __forceinline__ int find(int64_t at) const {
+    const int lane = threadIdx.x & 63;
+    if (num_seqs <= 64) return 63 - __builtin_clzll(__builtin_amdgcn_ballot_w64(lane < num_seqs && start <= at));
+    int n = -1;
+    for (int s0 = 0; s0 < num_seqs; s0 += 64)
+      n += __popcll(__builtin_amdgcn_ballot_w64(s0 + lane < num_seqs && held->start[s0 + lane < num_seqs ? s0 + lane : 0] <= at));
+    return n;
+  }
+};
 
 template <class DT, int D, int NT>
 __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void tree_attention_kernel(TreeParams p) {
@@ -310,59 +412,29 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void tree_attention_kern
   using V8 = typename DT::vec8;
   constexpr int NC = C::NC, NN = C::NN, LPT = C::LPT, KPI = C::KPI, CPR = C::CPR, NK = C::NK;
   __shared__ __attribute__((aligned(1024))) char smem[C::RING];
-  __shared__ Schedule sh;
+  __shared__ Held held;
   __shared__ float maxima[kWaves][C::COLS], sums[kWaves][C::COLS];
   __shared__ int bads[kWaves];
+  __shared__ int last;
 
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c16 = lane & 15;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int G = p.group, Hkv = p.num_kv_heads;
 
-  // The schedule: sequences tid and tid + 256 are this thread's.
-  constexpr int PER = kSeqs / kThreads;
-  int blocks[PER], lens[PER];
-  int64_t units = 0;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int s = PER * tid + i;
-    blocks[i] = lens[i] = 0;
-    if (s < p.num_seqs) {
-      const SeqRows r = rows_of(p, s);
-      blocks[i] = static_cast<int>((r.ql * G + C::COLS - 1) / C::COLS) * Hkv;
-      lens[i] = static_cast<int>(r.len);
-      sh.row0[s] = static_cast<int>(r.row0);
-      sh.ql[s] = static_cast<int>(r.ql);
-      sh.len[s] = lens[i];
-      units += static_cast<int64_t>(blocks[i]) * lens[i];
-    }
-  }
-  units = block_sum(units, sh.sums);
-  int64_t each64 = (units + p.target - 1) / p.target;
-  each64 = (each64 + 31) / 32 * 32;
-  const int each = static_cast<int>(each64 < kLeastTokens ? kLeastTokens : each64);
-  int items = 0, slots = 0;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int n = ranges_of(lens[i], each);
-    items += blocks[i] * n;
-    slots += n > 1 ? blocks[i] * n : 0;
-  }
-  int total, unused;
-  int item = block_scan(items, sh.scans, total);
-  int slot = block_scan(slots, sh.scans, unused);
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int s = PER * tid + i;
-    if (s < p.num_seqs) {
-      sh.first[s] = item;
-      sh.slot[s] = slot;
-    }
-    const int n = ranges_of(lens[i], each);
-    item += blocks[i] * n;
-    slot += n > 1 ? blocks[i] * n : 0;
-    if (s == p.num_seqs - 1) sh.first[p.num_seqs] = item;
-  }
-  __syncthreads();
+  Line<C::COLS> line;
+  line.make(p, held);
+  // Shares: one a workgroup, but none too small, and no group in more than kMostRanges of them.
+  const int grid = static_cast<int>(gridDim.x);
+  int64_t share = quotient(line.total + grid - 1, grid);
+  const int least = line.most / (kMostRanges - 2) + 1;
+  share = share > least ? share : least;
+  share = share > kLeastShare ? share : kLeastShare;
+  // Neighbouring shares, which read the same keys where a sequence has several
+  // groups of columns, go to one XCD (workgroups go to the eight in turn).
+  const int shares = static_cast<int>(quotient(line.total + share - 1, share));
+  const int per_xcd = (shares + 7) >> 3;
+  const int k = static_cast<int>(blockIdx.x & 7) * per_xcd + static_cast<int>(blockIdx.x >> 3);
+  if (static_cast<int>(blockIdx.x >> 3) >= per_xcd || k >= shares) return;
 
   const float scale = fabsf(p.scale) * 1.4426950408889634f;
   const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;  // a negative scale turns the query around, exactly
@@ -386,28 +458,34 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void tree_attention_kern
   const int vkey = 4 * g + (c16 >> 2);
   vread = vkey * (D * 2) + ((((c16 & 3) >> 1) ^ v_swizzle<D>(vkey)) << 4) + (c16 & 1) * 8;
 
-  for (int it = blockIdx.x; it < total; it += gridDim.x) {
-    for (int s = tid; s < p.num_seqs; s += kThreads)
-      if (sh.first[s] <= it && it < sh.first[s + 1]) sh.found = s;
-    __syncthreads();
-    const int s = __builtin_amdgcn_readfirstlane(sh.found);
-    const int row0 = sh.row0[s], ql = sh.ql[s], len = sh.len[s];
+  int s = line.find(k * share);
+  int64_t start;
+  int row0, ql, len;
+  line.get(s, start, row0, ql, len);
+  int64_t gi = quotient(k * share - start, line.weight(len));
+  for (;; ++gi) {
+    while (gi >= line.groups(ql)) {
+      if (++s >= p.num_seqs) return;
+      line.get(s, start, row0, ql, len);
+      gi = 0;
+    }
+    // The group's place on the line, the workgroups a .. b that it falls to, and
+    // the chunks c0 .. c1 of this one.
+    const int n = (len + 31) >> 5;
+    const int64_t gs = start + gi * line.weight(len);
+    const int a = static_cast<int>(quotient(gs + 1, share));
+    if (a > k) return;
+    const int e = (n + 3) / 4 * 4 - 3;
+    int b = e > 0 ? static_cast<int>(quotient(gs + e, share)) : a;
+    b = b > a ? b : a;
+    if (k > b) continue;
+    auto cut = [&](int kk) { return static_cast<int>(kk * share - gs + 2) >> 2 << 2; };
+    const int c0 = k == a ? 0 : cut(k), c1 = k == b ? n : cut(k + 1);
     const int base = len - ql;
-    const int n_ranges = ranges_of(len, each);
     const int cols = ql * G, cbs = (cols + C::COLS - 1) / C::COLS;
-    // A sequence's items: column blocks of one (KV head, range) are 8 apart, so that
-    // the workgroups that read the same keys run on one XCD.
-    const int j = it - sh.first[s];
-    const int pairs = Hkv * n_ranges;
-    const int grp = j / (8 * cbs), in = j % (8 * cbs);
-    const int wide = pairs - 8 * grp < 8 ? pairs - 8 * grp : 8;
-    const int cb = in / wide, pair = 8 * grp + in % wide;
-    const int kvh = pair / n_ranges, range = pair % n_ranges;
-    const int per = ((len + n_ranges - 1) / n_ranges + 31) / 32 * 32;
-    const int t0 = range * per;
-    const int t1 = t0 + per < len ? t0 + per : len;
-    const int chunks = t1 > t0 ? (t1 - t0 + 31) >> 5 : 0;
-    const int mine = chunks > w ? (chunks - w + kWaves - 1) / kWaves : 0;
+    const int kvh = static_cast<int>(gi) / cbs, cb = static_cast<int>(gi) % cbs;
+    const int t1 = 32 * c1 < len ? 32 * c1 : len;
+    const int mine = c1 - c0 > w ? (c1 - c0 - w + kWaves - 1) / kWaves : 0;
 
     // The columns' query rows and masks.
     V8 q[NT][NC];
@@ -423,11 +501,11 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void tree_attention_kern
       const char* qr = p.query + ((row * p.num_heads + kvh * G + c % G) * D + 8 * g) * 2;
       mask[n] = static_cast<uint64_t>(p.mask[row]);
 #pragma unroll
-      for (int k = 0; k < NC; ++k) {
-        u32x4 x = *reinterpret_cast<const u32x4*>(qr + 64 * k);
+      for (int i = 0; i < NC; ++i) {
+        u32x4 x = *reinterpret_cast<const u32x4*>(qr + 64 * i);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] ^= flip;
-        q[n][k] = __builtin_bit_cast(V8, x);
+        for (int e2 = 0; e2 < 4; ++e2) x[e2] ^= flip;
+        q[n][i] = __builtin_bit_cast(V8, x);
       }
       m[n] = -INFINITY;
       l[n] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -440,7 +518,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void tree_attention_kern
     uint32_t at_lo = 0, at_hi = 0;
     auto window = [&](int step) {
       const int64_t bt_row = static_cast<int64_t>(p.first_seq + s) * p.bt_stride;
-      int key = t0 + 32 * (w + kWaves * (step + (lane >> 1))) + 16 * (lane & 1);
+      int key = 32 * (c0 + w + kWaves * (step + (lane >> 1))) + 16 * (lane & 1);
       key = key < t1 ? key : (t1 - 1) & ~15;  // a tile past the range repeats the last
       int64_t blk = load_index(p.bt, bt_row + key / p.block_size, p.bt64);
       if (blk < 0 || blk >= p.num_blocks) {
@@ -471,7 +549,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void tree_attention_kern
     };
 
     auto step_of = [&](int step) {
-      const int tb = t0 + 32 * (w + kWaves * step);
+      const int tb = 32 * (c0 + w + kWaves * step);
       const char* kt = ring + (step % C::R) * C::SLOT_B;
       const char* vt = kt + C::TILE_B;
       u32x4 kraw[2][NC];
@@ -620,43 +698,43 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void tree_attention_kern
     // when every wave is here.
     if (g == 0) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        maxima[w][16 * n + c16] = m[n];
-        sums[w][16 * n + c16] = l[n][0];
+      for (int i = 0; i < NT; ++i) {
+        maxima[w][16 * i + c16] = m[i];
+        sums[w][16 * i + c16] = l[i][0];
       }
     }
     {
       const int wave_bad = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
       if (lane == 0) bads[w] = wave_bad;
     }
-    const int at_slot = n_ranges > 1 ? sh.slot[s] + (cb * Hkv + kvh) * n_ranges : 0;
-    const bool split = n_ranges > 1;
-    const bool fits = !split || at_slot + n_ranges <= p.slots;
+    const bool split = b > a;
+    // A workgroup has at most one cut group that it begins (its last: slot 2 k + 1)
+    // and one that it does not (its first: slot 2 k).
+    auto slot_of = [&](int kk) { return kk == a ? 2 * kk + 1 : 2 * kk; };
     const __amdgpu_buffer_rsrc_t pr = __builtin_amdgcn_make_buffer_rsrc(
-        p.partials + static_cast<int64_t>(at_slot) * C::PART, static_cast<short>(0),
-        fits && split ? n_ranges * C::PART * 4 : 0, kBufferWord3);
+        p.partials + static_cast<int64_t>(2) * a * C::PART, static_cast<short>(0),
+        split ? 2 * (b - a + 1) * C::PART * 4 : 0, kBufferWord3);
+    auto part_of = [&](int kk) { return (slot_of(kk) - 2 * a) * C::PART; };
     T* out = reinterpret_cast<T*>(p.out);
-    auto place_of = [&](int col) {  // element of the output where a column's row starts
+    auto write = [&](int col, int f, floatx4 o, float inv) {
       const int c = cb * C::COLS + col;
-      return ((static_cast<int64_t>(row0) + c / G) * p.num_heads + kvh * G + c % G) * D;
-    };
-    auto write = [&](int col, int f, floatx4 o, float sum) {
-      const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;  // no key: zero; a NaN stays one
+      const int64_t at = ((static_cast<int64_t>(row0) + c / G) * p.num_heads + kvh * G + c % G) * D + 4 * f;
       typename DT::vec4 v;
 #pragma unroll
       for (int r = 0; r < 4; ++r) v[r] = static_cast<T>(o[r] * inv);
-      *reinterpret_cast<u32x2*>(out + place_of(col) + 4 * f) = __builtin_bit_cast(u32x2, v);
+      *reinterpret_cast<u32x2*>(out + at) = __builtin_bit_cast(u32x2, v);
     };
-    const int here = cols - cb * C::COLS < C::COLS ? cols - cb * C::COLS : C::COLS;  // columns of the item
+    auto inverse = [&](float sum) { return sum > 0.f || sum != sum ? 1.f / sum : 0.f; };  // no key: zero; a NaN stays one
+    const int here = cols - cb * C::COLS < C::COLS ? cols - cb * C::COLS : C::COLS;  // columns of the group
 #pragma unroll
     for (int n0 = 0; n0 < NT; n0 += C::JOIN) {
       __syncthreads();
       float* mine_o = reinterpret_cast<float*>(smem) + w * (C::JOIN * 16 * D);
 #pragma unroll
-      for (int n = n0; n < n0 + C::JOIN && n < NT; ++n)
+      for (int i = n0; i < n0 + C::JOIN && i < NT; ++i)
 #pragma unroll
-        for (int i = 0; i < NN; ++i)
-          *reinterpret_cast<floatx4*>(mine_o + (16 * (n - n0) + c16) * D + 4 * ((4 * i + g) ^ c16)) = acc[n][i];
+        for (int j = 0; j < NN; ++j)
+          *reinterpret_cast<floatx4*>(mine_o + (16 * (i - n0) + c16) * D + 4 * ((4 * j + g) ^ c16)) = acc[i][j];
       __syncthreads();
       int bad_any = 0;
 #pragma unroll
@@ -679,81 +757,100 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void tree_attention_kern
         floatx4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int ww = 0; ww < kWaves; ++ww) {
-          const float a = fast_exp2(mw[ww] - ref);
-          sum = __builtin_fmaf(lw[ww], a, sum);
+          const float f2 = fast_exp2(mw[ww] - ref);
+          sum = __builtin_fmaf(lw[ww], f2, sum);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) o[r] = __builtin_fmaf(ow[ww][r], a, o[r]);
+          for (int r = 0; r < 4; ++r) o[r] = __builtin_fmaf(ow[ww][r], f2, o[r]);
         }
         if (bad_any) {
           sum = NAN;
           o = floatx4{NAN, NAN, NAN, NAN};
         }
         if (!split) {
-          write(col, f, o, sum);
+          write(col, f, o, inverse(sum));
         } else {
-          const int to = 4 * (range * C::PART + col * D + 4 * f);
+          const int to = 4 * (part_of(k) + col * D + 4 * f);
           __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), pr, to, 0, kSc1);
           if (f == 0)
             __builtin_amdgcn_raw_buffer_store_b64(
                 u32x2{__builtin_bit_cast(uint32_t, top), __builtin_bit_cast(uint32_t, sum)}, pr,
-                4 * (range * C::PART + C::COLS * D + 2 * col), 0, kSc1);
+                4 * (part_of(k) + C::COLS * D + 2 * col), 0, kSc1);
         }
       }
     }
     if (!split) {
-      __syncthreads();  // the ring, the maxima and the found sequence are the next item's
+      __syncthreads();  // the ring and the maxima are the next group's
       continue;
     }
 
-    // The last of the item's ranges to arrive joins them, in their order.  A partial
-    // is acknowledged (device scope) before its arrival is counted.
+    // The last of the group's workgroups to arrive joins its ranges, in their order.
+    // A partial is acknowledged (device scope) before its arrival is counted.
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
     __syncthreads();
-    if (tid == 0) {
-      sh.last = 0;
-      if (fits) {
-        const int before = __hip_atomic_fetch_add(&p.counters[at_slot], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        sh.last = before == n_ranges - 1;
-      }
-    }
+    if (tid == 0)
+      last = __hip_atomic_fetch_add(&p.counters[a], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == b - a;
     __syncthreads();
-    if (sh.last) {
-      for (int x = tid; x < here * (D / 4); x += kThreads) {
-        const int col = x / (D / 4), f = x % (D / 4);
-        float mr[kMostRanges], lr[kMostRanges], top = -INFINITY;
-        floatx4 o = {0.f, 0.f, 0.f, 0.f};
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < kMostRanges; ++i) {
-          const int r = i < n_ranges ? i : 0;
-          mr[i] = ld_sc1(pr, 4 * (r * C::PART + C::COLS * D + 2 * col));
-          lr[i] = ld_sc1(pr, 4 * (r * C::PART + C::COLS * D + 2 * col + 1));
+    if (last) {
+      const int ranges = b - a + 1;
+      // Every range's maximum and sum of every column, then its weight, in LDS.
+      float* ml = reinterpret_cast<float*>(smem);
+      for (int x = tid; x < ranges * C::COLS; x += kThreads) {
+        const int r = x / C::COLS, col = x % C::COLS;
+        if (col < here) {
+          const int from = 4 * (part_of(a + r) + C::COLS * D + 2 * col);
+          ml[x] = ld_sc1(pr, from);
+          ml[kMostRanges * C::COLS + x] = ld_sc1(pr, from + 4);
         }
-#pragma unroll
-        for (int i = 0; i < kMostRanges; ++i) top = i < n_ranges ? fmaxf(top, mr[i]) : top;
-        const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll
-        for (int i0 = 0; i0 < kMostRanges; i0 += 8) {
-          if (i0 >= n_ranges) break;
-          floatx4 part[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = i0 + i < n_ranges ? i0 + i : 0;
-            const int from = 4 * (r * C::PART + col * D + 4 * f);
-            part[i] = floatx4{ld_sc1(pr, from), ld_sc1(pr, from + 4), ld_sc1(pr, from + 8), ld_sc1(pr, from + 12)};
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (i0 + i >= n_ranges) break;
-            const float a = fast_exp2(mr[i0 + i] - ref);
-            sum = __builtin_fmaf(lr[i0 + i], a, sum);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] = __builtin_fmaf(part[i][r], a, o[r]);
-          }
-        }
-        write(col, f, o, sum);
       }
-      if (tid == 0) __hip_atomic_store(&p.counters[at_slot], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __syncthreads();
+      if (tid < here) {
+        float top = -INFINITY, sum = 0.f;
+        for (int r = 0; r < ranges; ++r) top = fmaxf(top, ml[r * C::COLS + tid]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        for (int r = 0; r < ranges; ++r) {
+          const float f2 = fast_exp2(ml[r * C::COLS + tid] - ref);
+          ml[r * C::COLS + tid] = f2;
+          sum = __builtin_fmaf(ml[kMostRanges * C::COLS + r * C::COLS + tid], f2, sum);
+        }
+        maxima[0][tid] = inverse(sum);
+      }
+      __syncthreads();
+      floatx4 o[C::OWN];
+#pragma unroll
+      for (int i = 0; i < C::OWN; ++i) o[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+      constexpr int AT_ONCE = 16 / C::OWN;  // ranges whose loads are in flight together
+      for (int r0 = 0; r0 < ranges; r0 += AT_ONCE) {
+        floatx4 part[AT_ONCE][C::OWN];
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+          const int r = r0 + j < ranges ? r0 + j : ranges - 1;
+#pragma unroll
+          for (int i = 0; i < C::OWN; ++i) {
+            const int from = 4 * (part_of(a + r) + 4 * (tid + i * kThreads));
+            part[j][i] = floatx4{ld_sc1(pr, from), ld_sc1(pr, from + 4), ld_sc1(pr, from + 8), ld_sc1(pr, from + 12)};
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+          if (r0 + j < ranges) {
+#pragma unroll
+            for (int i = 0; i < C::OWN; ++i) {
+              const int col = (tid + i * kThreads) / (D / 4);
+              if (col < here) {
+                const float f2 = ml[(r0 + j) * C::COLS + col];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[i][r] = __builtin_fmaf(part[j][i][r], f2, o[i][r]);
+              }
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < C::OWN; ++i) {
+        const int x = tid + i * kThreads, col = x / (D / 4);
+        if (col < here) write(col, x % (D / 4), o[i], maxima[0][col]);
+      }
+      if (tid == 0) __hip_atomic_store(&p.counters[a], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
   }
@@ -783,7 +880,8 @@ int tiles_of(int max_rows, int group) {
   return static_cast<int>((tiles + blocks - 1) / blocks);
 }
 
-int items_of(int head_dim) { return device_cus() * (head_dim == 64 ? 2 : 1); }
+// Workgroups that the device holds at once, in whole rounds of the XCDs.
+int places_of(int head_dim) { return (device_cus() + 7) / 8 * 8 * (head_dim == 64 ? 2 : 1); }
 
 size_t slot_bytes(int head_dim, int nt) { return static_cast<size_t>(16) * nt * (head_dim + 2) * 4; }
 
@@ -798,7 +896,7 @@ hipError_t launch_tiles(const TreeParams& p, int nt, hipStream_t stream) {
   for (int s = 0; s < p.num_seqs; s += kSeqs) {
     part.first_seq = s;
     part.num_seqs = p.num_seqs - s < kSeqs ? p.num_seqs - s : kSeqs;
-    const hipError_t e = hipLaunchKernel(fn, dim3(static_cast<unsigned>(p.target)), dim3(kThreads), args, 0, stream);
+    const hipError_t e = hipLaunchKernel(fn, dim3(static_cast<unsigned>(places_of(D))), dim3(kThreads), args, 0, stream);
     if (e != hipSuccess) return e;
   }
   return hipSuccess;
@@ -814,7 +912,7 @@ bool sizes_ok(int num_seqs, int64_t num_tokens, int num_heads, int num_kv_heads,
 }  // namespace
 }  // namespace ns
 
-extern "C" int ns_paged_attention_tree_counters(void) { return 4 * ns::device_cus(); }
+extern "C" int ns_paged_attention_tree_counters(void) { return ns::places_of(64); }
 
 extern "C" size_t ns_paged_attention_tree_workspace_size(int num_seqs, int num_heads, int num_kv_heads, int head_dim,
                                                          int block_size, int max_query_len, int64_t num_tokens,
@@ -823,7 +921,7 @@ extern "C" size_t ns_paged_attention_tree_workspace_size(int num_seqs, int num_h
   if (!sizes_ok(num_seqs, num_tokens, num_heads, num_kv_heads, head_dim, block_size) || num_seqs == 0 ||
       num_tokens == 0 || !takes_tiles(head_dim, block_size, num_heads / num_kv_heads, dtype))
     return 0;
-  return static_cast<size_t>(2) * items_of(head_dim) *
+  return static_cast<size_t>(2) * places_of(head_dim) *
          slot_bytes(head_dim, tiles_of(max_query_len, num_heads / num_kv_heads));
 }
 
@@ -887,8 +985,6 @@ extern "C" int ns_paged_attention_tree(void* out, const void* query,
   p.scale = scale;
   p.partials = static_cast<float*>(workspace);
   p.counters = counters;
-  p.target = items_of(head_dim);
-  p.slots = 2 * p.target;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   hipError_t e;
   if (!tiles) {
@@ -898,7 +994,7 @@ extern "C" int ns_paged_attention_tree(void* out, const void* query,
   } else {
     const int nt = tiles_of(max_query_len, group);
     if (!counters || misaligned(counters, 4) || !workspace || misaligned(workspace, 16) ||
-        workspace_bytes < static_cast<size_t>(p.slots) * slot_bytes(head_dim, nt))
+        workspace_bytes < static_cast<size_t>(2) * places_of(head_dim) * slot_bytes(head_dim, nt))
       return NS_ERR_WORKSPACE;
     e = dtype == NS_DTYPE_F16 ? (head_dim == 64 ? launch_tiles<F16, 64>(p, nt, st) : launch_tiles<F16, 128>(p, nt, st))
                               : (head_dim == 64 ? launch_tiles<BF16, 64>(p, nt, st) : launch_tiles<BF16, 128>(p, nt, st));
