@@ -103,7 +103,8 @@ __global__ __launch_bounds__(64) void tree_attention_generic_kernel(TreeParams p
     s = lo;
   }
   const SeqRows r = rows_of(p, s);
-  if (t < r.row0 || t >= r.row0 + r.ql) return;  // a row of no sequence is left as it is
+  // A row of no sequence, or past a sequence's 64th, is left as it is.
+  if (t < r.row0 || t >= r.row0 + (r.ql < kRows ? r.ql : kRows)) return;
   const int64_t base = r.len - r.ql;
   const uint64_t mask = static_cast<uint64_t>(p.mask[t]);
 
@@ -192,14 +193,16 @@ hipError_t launch_generic(const TreeParams& p, hipStream_t stream) {
 
 // ---- head sizes 64 and 128, blocks of whole 16-token tiles --------------------
 //
-// A sequence's rows times the heads of one KV head are columns, 16 a tile.  A group
-// is up to NT tiles of columns of one (sequence, KV head); a workgroup takes a range
-// of a group's keys, and a wave the range's chunks of 32 keys w, w + 4, ... for all of
-// the group's columns, so that every row of K and V is loaded once for up to 16 NT
-// rows of the product, and the waves meet once, at the range's end.  K and V come by
-// LDS-DMA into a ring of each wave's own, S^T = K Q^T and O^T = V^T P^T on
-// v_mfma_f32_16x16x32.  The result layout of the first product (keys 4 g + r of
-// column lane % 16 in lane group g) is the operand layout of the second.
+// A sequence's rows times the heads of one KV head are columns, 16 a tile.  A group is
+// up to WC * NT tiles of columns of one (sequence, KV head); a workgroup takes a range
+// of a group's keys.  Its waves are KG key groups of WC column waves: key group i
+// takes the range's chunks of 32 keys i, i + KG, ..., each column wave NT of the tiles
+// for all of them, so that every row of K and V is loaded once for up to 16 WC NT rows
+// of the product.  K and V come by LDS-DMA into a ring of the key group's, loaded by its
+// waves in equal parts (with more than one, a barrier a chunk hands them over); S^T = K
+// Q^T and O^T = V^T P^T run on v_mfma_f32_16x16x32.  The result layout of the first
+// product (keys 4 g + r of column lane % 16 in lane group g) is the operand layout of
+// the second.  The key groups meet once, at the range's end.
 //
 // The probabilities enter the second product in the model's dtype, and their sum
 // is taken by the same product with a tile of ones, so that a rounding acts on both.
@@ -207,43 +210,56 @@ hipError_t launch_generic(const TreeParams& p, hipStream_t stream) {
 // Work is cut evenly: the groups' chunks, and kGroupCost for what a group costs
 // beside them, are laid end to end, and workgroup k takes the k-th equal share of
 // that line, whatever it covers: parts of groups, whole ones, or both.  Cuts move to
-// whole rounds of the four waves.  A group that a cut falls into is joined by the last
+// whole rounds of the key groups.  A group that a cut falls into is joined by the last
 // of its workgroups to finish.  Every workgroup works its share out of the device's
 // lengths for itself.
 
-constexpr int kWaves = 4;
-constexpr int kThreads = kWaves * 64;
 constexpr int kMostRanges = 32;  // of a group: what the last workgroup has to join
-constexpr int kGroupCost = 4;    // in chunks
+constexpr int kGroupCost = 4;    // in chunks, at least half a round of the key groups
+constexpr float kNoScore = -3e38f;  // a column's reference before its first score
+constexpr float kSlack = 8.f;    // binades that a score may pass its column's reference by
 constexpr int kLeastShare = 8;   // chunks
 
-template <int D, int NT>
+template <int D_, int KG_, int WC_, int NT_>
 struct Cfg {
-  static constexpr int COLS = 16 * NT;
+  static constexpr int D = D_, KG = KG_, WC = WC_, NT = NT_;
+  static constexpr int W = KG * WC;             // waves
+  static constexpr int THREADS = 64 * W;
+  static constexpr int COLS = 16 * NT * WC;
   static constexpr int CPR = D / 8;             // 16-byte units of a row
   static constexpr int KPI = 64 / CPR;          // rows of a tile that one load brings
   static constexpr int LPT = 16 / KPI;          // loads of a tile
   static constexpr int NK = 8 / KPI;            // loads until K's swizzle repeats
   static constexpr int TILE_B = 32 * D * 2;     // K or V of a chunk
   static constexpr int SLOT_B = 2 * TILE_B;
-  static constexpr int R = 2;                   // chunks in the ring
-  static constexpr int PER_CHUNK = 4 * LPT;     // loads of a chunk
+  static constexpr int FIT = 131072 / (KG * SLOT_B);
+  static constexpr int R = WC == 1 ? 2 : FIT < 4 ? FIT : 4;  // chunks in a key group's ring
+  static constexpr int LOADS = 4 * LPT / WC;    // of a chunk, by one wave
   static constexpr int NC = D / 32, NN = D / 16;
-  static constexpr int RING = kWaves * R * SLOT_B;
-  static constexpr int PART = COLS * (D + 2);   // words of a slot: outputs, then (maximum, sum) of every column
-  // The waves meet a group of column tiles at a time, as many as fit the ring.
-  static constexpr int JOIN = RING / (kWaves * 16 * D * 4) < NT ? RING / (kWaves * 16 * D * 4) : NT;
-  static constexpr int OWN = COLS * (D / 4) / kThreads;  // float4 of the output per thread
-  static_assert(JOIN >= 1, "a column tile of every wave fits the ring");
+  static constexpr int RING = KG * R * SLOT_B;
+  static constexpr int UNIT = 256;              // floats of 16 dims of a tile: four a lane
+  static constexpr int PART = COLS * (D + 2);   // words of a slot: units, then (maximum, sum) of every column
+  // The key groups meet JOIN tiles of a wave at a time, as many as fit the ring.
+  static constexpr int JOIN = RING / (W * NN * UNIT * 4) < NT ? RING / (W * NN * UNIT * 4) : NT;
+  static constexpr int OWN = (NT * NN + KG - 1) / KG;  // units that a wave joins the ranges of
+  static_assert(R >= 2 && JOIN >= 1 && NT % JOIN == 0, "chunks in flight; a tile of every wave fits the ring");
   static_assert(2 * kMostRanges * COLS * 4 <= RING, "the ranges' maxima and sums fit the ring");
+  static_assert(kGroupCost >= KG / 2, "a group's workgroups begin within its stretch of the line");
+  static_assert(kLeastShare >= KG, "a group has one cut at most that moves to its start or end");
 };
 
 constexpr int kSc1 = 16;                  // cache-policy bit SC1 of gfx950 buffer operations: device scope
 constexpr int kBufferWord3 = 0x00020000;  // raw 32-bit buffer descriptor, word 3
 
+// Until at most N of the wave's vector memory operations are pending.
 template <int N>
 __device__ __forceinline__ void vector_wait() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// The same, then a barrier; the wave's LDS operations are done.
+template <int N>
+__device__ __forceinline__ void vector_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ float ld_sc1(__amdgpu_buffer_rsrc_t r, int off) {
   return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, kSc1));
@@ -256,189 +272,150 @@ template <int D>
 __device__ __forceinline__ int v_swizzle(int key) {
   return D == 64 ? ((key >> 1) & 3) << 1 : (key & 7) << 1;
 }
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-__device__ __forceinline__ int64_t uniform64(int64_t x) {
-  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x));
-  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x >> 32));
-  return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
-}
-__device__ __forceinline__ int64_t lane_value64(int64_t x, int lane) {
-  const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), lane));
-  const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x >> 32), lane));
-  return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
-}
-__device__ __forceinline__ int64_t shuffle_up64(int64_t x, int by) {
-  const uint32_t lo = static_cast<uint32_t>(__shfl_up(static_cast<int>(x), by));
-  const uint32_t hi = static_cast<uint32_t>(__shfl_up(static_cast<int>(x >> 32), by));
-  return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
-}
-// x / y for x >= 0, y > 0: the quotient in float32, put right.
-__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
-  int64_t q = static_cast<int64_t>(static_cast<float>(x) / static_cast<float>(y));
-  while (q * y > x) --q;
-  while ((q + 1) * y <= x) ++q;
+// x / y for uniform 0 <= x < 2^30, y > 0: in float32, put right.
+__device__ __forceinline__ int quotient(int x, int y) {
+  int q = uniform(static_cast<int>(static_cast<float>(x) * __builtin_amdgcn_rcpf(static_cast<float>(y))));
+  while (x - q * y < 0) --q;
+  while (x - q * y >= y) ++q;
   return q;
 }
 
-// The sequences of a launch along the line of work, from the device's lengths.  Up to
-// 64 of them live in the lanes of every wave; more are held in LDS.
+// The sequences of a launch along the line of work, from the device's lengths: where
+// each starts, and its rows, in LDS.
 struct Held {
-  int64_t start[kSeqs];
-  int row0[kSeqs], ql[kSeqs], len[kSeqs];
-  int64_t sums[kWaves];
-  int most[kWaves];
+  int start[kSeqs], row0[kSeqs], ql[kSeqs], len[kSeqs];
+  int sums[8], most[8];
 };
 
-template <int COLS>
+template <class C>
 struct Line {
-  int64_t start;          // this lane's sequence (num_seqs <= 64)
-  int row0, ql, len;
-  Held* held;             // otherwise
+  Held& h;
   int num_seqs, heads, group;
-  int64_t total;
+  int total;
   int most;               // weight of the longest group
 
-  __device__ __forceinline__ int weight(int len_) const { return ((len_ + 31) >> 5) + kGroupCost; }
-  __device__ __forceinline__ int groups(int ql_) const { return (ql_ * group + COLS - 1) / COLS * heads; }
-
-  __device__ __forceinline__ void scan(int64_t x, int m, int lane, int64_t& before, int64_t& all, int& longest) {
-    int64_t y = x;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int64_t z = shuffle_up64(y, off);
-      if (lane >= off) y += z;
-      m = max(m, __shfl_xor(m, off));
-    }
-    before = y - x;
-    all = lane_value64(y, 63);
-    longest = __builtin_amdgcn_readfirstlane(m);
+  __device__ __forceinline__ int weight(int len) const { return ((len + 31) >> 5) + kGroupCost; }
+  __device__ __forceinline__ int groups(int ql) const {
+    return ((ql < kRows ? ql : kRows) * group + C::COLS - 1) / C::COLS * heads;
   }
 
-  __device__ __forceinline__ void make(const TreeParams& p, Held& h) {
-    const int lane = threadIdx.x & 63;
-    held = &h;
-    num_seqs = p.num_seqs;
-    heads = p.num_kv_heads;
-    group = p.group;
-    row0 = ql = len = 0;
-    if (num_seqs <= 64) {
-      int64_t x = 0;
-      int m = 0;
-      if (lane < num_seqs) {
-        const SeqRows r = rows_of(p, lane);
-        row0 = static_cast<int>(r.row0);
-        ql = static_cast<int>(r.ql);
-        len = static_cast<int>(r.len);
-        m = ql > 0 ? weight(len) : 0;
-        x = static_cast<int64_t>(groups(ql)) * m;
-      }
-      scan(x, m, lane, start, total, most);
-      return;
-    }
-    constexpr int PER = kSeqs / kThreads;
-    const int w = threadIdx.x >> 6;
-    int64_t x[PER], sum = 0;
-    int m = 0;
+  __device__ __forceinline__ Line(const TreeParams& p, Held& held)
+      : h(held), num_seqs(p.num_seqs), heads(p.num_kv_heads), group(p.group) {
+    // Up to 64 sequences every wave lists for itself, one a lane: each writes what
+    // the others write, and reads it back without waiting for them.
+    constexpr int PER = kSeqs / C::THREADS;
+    const bool alone = num_seqs <= 64;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    int x[PER], sum = 0, m = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int s = PER * static_cast<int>(threadIdx.x) + i;
+      const int s = alone ? (i == 0 ? lane : kSeqs) : PER * static_cast<int>(threadIdx.x) + i;
       x[i] = 0;
       if (s < num_seqs) {
         const SeqRows r = rows_of(p, s);
+        const int ql = static_cast<int>(r.ql), len = static_cast<int>(r.len);
         h.row0[s] = static_cast<int>(r.row0);
-        h.ql[s] = static_cast<int>(r.ql);
-        h.len[s] = static_cast<int>(r.len);
-        const int wt = r.ql > 0 ? weight(static_cast<int>(r.len)) : 0;
+        h.ql[s] = ql;
+        h.len[s] = len;
+        const int wt = ql > 0 ? weight(len) : 0;
         m = max(m, wt);
-        x[i] = static_cast<int64_t>(groups(static_cast<int>(r.ql))) * wt;
+        x[i] = groups(ql) * wt;
         sum += x[i];
       }
     }
-    int64_t before, all;
-    scan(sum, m, lane, before, all, most);
-    if (lane == 0) {
-      h.sums[w] = all;
-      h.most[w] = most;
-    }
-    __syncthreads();
-    total = 0;
-    most = 0;
+    int y = sum;
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-      if (i < w) before += h.sums[i];
-      total += h.sums[i];
-      most = max(most, h.most[i]);
+    for (int off = 1; off < 64; off <<= 1) {
+      const int z = __shfl_up(y, off);
+      if (lane >= off) y += z;
+      m = max(m, __shfl_xor(m, off));
+    }
+    int before = y - sum;
+    total = __builtin_amdgcn_readlane(y, 63);
+    most = uniform(m);
+    if (!alone) {
+      if (lane == 0) {
+        h.sums[w] = total;
+        h.most[w] = most;
+      }
+      __syncthreads();
+      total = 0;
+      most = 0;
+#pragma unroll
+      for (int i = 0; i < C::W; ++i) {
+        if (i < w) before += h.sums[i];
+        total += h.sums[i];
+        most = max(most, h.most[i]);
+      }
+      total = uniform(total);
+      most = uniform(most);
     }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int s = PER * static_cast<int>(threadIdx.x) + i;
+      const int s = alone ? (i == 0 ? lane : kSeqs) : PER * static_cast<int>(threadIdx.x) + i;
       if (s < num_seqs) h.start[s] = before;
       before += x[i];
     }
-    __syncthreads();
-    total = uniform64(total);
-    most = __builtin_amdgcn_readfirstlane(most);
+    if (!alone) __syncthreads();
   }
 
-  __device__ __forceinline__ void get(int s, int64_t& start_, int& row0_, int& ql_, int& len_) const {
-    if (num_seqs <= 64) {
-      start_ = lane_value64(start, s);
-      row0_ = __builtin_amdgcn_readlane(row0, s);
-      ql_ = __builtin_amdgcn_readlane(ql, s);
-      len_ = __builtin_amdgcn_readlane(len, s);
-    } else {
-      start_ = uniform64(held->start[s]);
-      row0_ = __builtin_amdgcn_readfirstlane(held->row0[s]);
-      ql_ = __builtin_amdgcn_readfirstlane(held->ql[s]);
-      len_ = __builtin_amdgcn_readfirstlane(held->len[s]);
-    }
+  __device__ __forceinline__ void get(int s, int& start, int& row0, int& ql, int& len) const {
+    start = uniform(h.start[s]);
+    row0 = uniform(h.row0[s]);
+    ql = uniform(h.ql[s]);
+    len = uniform(h.len[s]);
   }
 
   // The sequence that place `at` of the line lies in: the last that starts there or before.
-  __device__ __forceinline__ int find(int64_t at) const {
+  __device__ __forceinline__ int find(int at) const {
     const int lane = threadIdx.x & 63;
-    if (num_seqs <= 64) return 63 - __builtin_clzll(__builtin_amdgcn_ballot_w64(lane < num_seqs && start <= at));
     int n = -1;
-    for (int s0 = 0; s0 < num_seqs; s0 += 64)
-      n += __popcll(__builtin_amdgcn_ballot_w64(s0 + lane < num_seqs && held->start[s0 + lane < num_seqs ? s0 + lane : 0] <= at));
+    for (int s0 = 0; s0 < num_seqs; s0 += 64) {
+      const int s = s0 + lane < num_seqs ? s0 + lane : 0;
+      n += __popcll(__builtin_amdgcn_ballot_w64(s0 + lane < num_seqs && h.start[s] <= at));
+    }
     return n;
   }
 };
 
-template <class DT, int D, int NT>
-__global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void tree_attention_kernel(TreeParams p) {
-  using C = Cfg<D, NT>;
+template <class DT, class C>
+__global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreeParams p) {
   using T = typename DT::T;
   using V8 = typename DT::vec8;
-  constexpr int NC = C::NC, NN = C::NN, LPT = C::LPT, KPI = C::KPI, CPR = C::CPR, NK = C::NK;
+  constexpr int D = C::D, KG = C::KG, WC = C::WC, NT = C::NT, W = C::W, COLS = C::COLS;
+  constexpr int NC = C::NC, NN = C::NN, LPT = C::LPT, KPI = C::KPI, CPR = C::CPR, NK = C::NK, R = C::R;
   __shared__ __attribute__((aligned(1024))) char smem[C::RING];
   __shared__ Held held;
-  __shared__ float maxima[kWaves][C::COLS], sums[kWaves][C::COLS];
-  __shared__ int bads[kWaves];
+  __shared__ float maxima[KG][COLS], sums[KG][COLS];
+  __shared__ int bads[W];
   __shared__ int last;
 
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c16 = lane & 15;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int w = uniform(tid >> 6);
+  const int kg = w / WC, cw = w % WC;
   const int G = p.group, Hkv = p.num_kv_heads;
 
-  Line<C::COLS> line;
-  line.make(p, held);
+  const Line<C> line(p, held);
   // Shares: one a workgroup, but none too small, and no group in more than kMostRanges of them.
   const int grid = static_cast<int>(gridDim.x);
-  int64_t share = quotient(line.total + grid - 1, grid);
+  int share = quotient(line.total + grid - 1, grid);
   const int least = line.most / (kMostRanges - 2) + 1;
   share = share > least ? share : least;
   share = share > kLeastShare ? share : kLeastShare;
   // Neighbouring shares, which read the same keys where a sequence has several
   // groups of columns, go to one XCD (workgroups go to the eight in turn).
-  const int shares = static_cast<int>(quotient(line.total + share - 1, share));
+  const int shares = quotient(line.total + share - 1, share);
   const int per_xcd = (shares + 7) >> 3;
   const int k = static_cast<int>(blockIdx.x & 7) * per_xcd + static_cast<int>(blockIdx.x >> 3);
   if (static_cast<int>(blockIdx.x >> 3) >= per_xcd || k >= shares) return;
 
-  const float scale = fabsf(p.scale) * 1.4426950408889634f;
+  // Log2 units per score unit; never zero, so that -inf, a key that is not seen, stays it.
+  const float scale = __uint_as_float(__builtin_amdgcn_readfirstlane(
+      __float_as_uint(fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1.1754944e-38f))));
   const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;  // a negative scale turns the query around, exactly
-  char* ring = smem + w * (C::R * C::SLOT_B);
+  char* ring = smem + kg * (R * C::SLOT_B);
   const uint32_t stride = static_cast<uint32_t>(Hkv) * D * 2;  // bytes between a block's token rows
 
   // A lane's part of a load: its unit of its row, where it lies in memory.
@@ -448,6 +425,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void tree_attention_kern
     const int key = u * KPI + lane / CPR, unit = lane % CPR;
     koff[u] = (lane / CPR) * stride + ((unit ^ k_swizzle(key)) << 4);
     voff[u] = (lane / CPR) * stride + ((unit ^ v_swizzle<D>(key)) << 4);
+    if (WC > 1) koff[u] = cw & 1 ? voff[u] : koff[u];  // a column wave loads of K or of V
   }
   // Operand reads within a chunk.  K: key 16 h + c16, unit 4 c + g.  V^T: keys
   // 16 h + 4 g + e of dims 16 n + c16 (ds_read_b64_tr_b16 gives lane i of a 16-lane
@@ -458,11 +436,12 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void tree_attention_kern
   const int vkey = 4 * g + (c16 >> 2);
   vread = vkey * (D * 2) + ((((c16 & 3) >> 1) ^ v_swizzle<D>(vkey)) << 4) + (c16 & 1) * 8;
 
-  int s = line.find(k * share);
-  int64_t start;
-  int row0, ql, len;
+  constexpr int kHalf = KG / 2;
+  const int place = k * share;
+  int s = line.find(place);
+  int start, row0, ql, len;
   line.get(s, start, row0, ql, len);
-  int64_t gi = quotient(k * share - start, line.weight(len));
+  int gi = quotient(place - start, line.weight(len));
   for (;; ++gi) {
     while (gi >= line.groups(ql)) {
       if (++s >= p.num_seqs) return;
@@ -472,55 +451,37 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void tree_attention_kern
     // The group's place on the line, the workgroups a .. b that it falls to, and
     // the chunks c0 .. c1 of this one.
     const int n = (len + 31) >> 5;
-    const int64_t gs = start + gi * line.weight(len);
-    const int a = static_cast<int>(quotient(gs + 1, share));
+    const int gs = start + gi * line.weight(len);
+    const int a = quotient(gs + kHalf - 1, share);
     if (a > k) return;
-    const int e = (n + 3) / 4 * 4 - 3;
-    int b = e > 0 ? static_cast<int>(quotient(gs + e, share)) : a;
+    const int e = (n + KG - 1) / KG * KG - kHalf - 1;
+    int b = e > 0 ? quotient(gs + e, share) : a;
     b = b > a ? b : a;
     if (k > b) continue;
-    auto cut = [&](int kk) { return static_cast<int>(kk * share - gs + 2) >> 2 << 2; };
+    auto cut = [&](int kk) { return (kk * share - gs + kHalf) / KG * KG; };
     const int c0 = k == a ? 0 : cut(k), c1 = k == b ? n : cut(k + 1);
     const int base = len - ql;
-    const int cols = ql * G, cbs = (cols + C::COLS - 1) / C::COLS;
-    const int kvh = static_cast<int>(gi) / cbs, cb = static_cast<int>(gi) % cbs;
+    const int cols = (ql < kRows ? ql : kRows) * G, cbs = (cols + COLS - 1) / COLS;
+    const int kvh = uniform(gi / cbs), cb = gi - kvh * cbs;
+    const int col0 = cb * COLS + cw * (16 * NT);  // this wave's first column
     const int t1 = 32 * c1 < len ? 32 * c1 : len;
-    const int mine = c1 - c0 > w ? (c1 - c0 - w + kWaves - 1) / kWaves : 0;
+    const int steps = (c1 - c0 + KG - 1) / KG;  // of the workgroup
+    const int mine = c1 - c0 > kg ? (c1 - c0 - kg + KG - 1) / KG : 0;
 
-    // The columns' query rows and masks.
-    V8 q[NT][NC];
-    uint64_t mask[NT];
+    // Where tile l & 1 of this wave's step l / 2 of a window of 32 steps lies, in lane
+    // l: its block, then bytes from the start of a cache.
     int bad = 0;
-    float m[NT];
-    floatx4 acc[NT][NN], l[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      int c = cb * C::COLS + 16 * n + c16;
-      c = c < cols ? c : cols - 1;
-      const int64_t row = row0 + c / G;
-      const char* qr = p.query + ((row * p.num_heads + kvh * G + c % G) * D + 8 * g) * 2;
-      mask[n] = static_cast<uint64_t>(p.mask[row]);
-#pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        u32x4 x = *reinterpret_cast<const u32x4*>(qr + 64 * i);
-#pragma unroll
-        for (int e2 = 0; e2 < 4; ++e2) x[e2] ^= flip;
-        q[n][i] = __builtin_bit_cast(V8, x);
-      }
-      m[n] = -INFINITY;
-      l[n] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < NN; ++i) acc[n][i] = floatx4{0.f, 0.f, 0.f, 0.f};
-    }
-
-    // Lane l: where tile l & 1 of this wave's step l / 2 of a window of 32 steps
-    // lies, as bytes from the start of a cache.
     uint32_t at_lo = 0, at_hi = 0;
-    auto window = [&](int step) {
-      const int64_t bt_row = static_cast<int64_t>(p.first_seq + s) * p.bt_stride;
-      int key = 32 * (c0 + w + kWaves * (step + (lane >> 1))) + 16 * (lane & 1);
-      key = key < t1 ? key : (t1 - 1) & ~15;  // a tile past the range repeats the last
-      int64_t blk = load_index(p.bt, bt_row + key / p.block_size, p.bt64);
+    auto key_of = [&](int step) {
+      int of = lane;
+      asm volatile("" : "+v"(of));
+      const int key = 32 * (c0 + kg + KG * (step + (of >> 1))) + 16 * (of & 1);
+      return key < t1 ? key : (t1 - 1) & ~15;  // a tile past the range repeats the last
+    };
+    auto block_of = [&](int key) {
+      return load_index(p.bt, static_cast<int64_t>(p.first_seq + s) * p.bt_stride + key / p.block_size, p.bt64);
+    };
+    auto set_window = [&](int key, int64_t blk) {
       if (blk < 0 || blk >= p.num_blocks) {
         bad = 1;
         blk = 0;
@@ -529,252 +490,353 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void tree_attention_kern
       at_lo = static_cast<uint32_t>(at);
       at_hi = static_cast<uint32_t>(at >> 32);
     };
+    const int first_key = mine > 0 ? key_of(0) : 0;
+    const int64_t first_block = mine > 0 ? block_of(first_key) : 0;
+
+    // The columns' query rows (a column past the last repeats it), on their way
+    // together with the block ids.
+    auto row_of = [&](int i, int& head) {
+      int c = c16;
+      asm volatile("" : "+v"(c));  // worked out where it is needed, not held in registers over the loop
+      c += col0 + 16 * i;
+      c = c < cols ? c : cols - 1;
+      head = kvh * G + c % G;
+      return static_cast<int64_t>(row0) + c / G;
+    };
+    V8 q[NT][NC];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      int head;
+      const int64_t row = row_of(i, head);
+      const char* qr = p.query + ((row * p.num_heads + head) * D + 8 * g) * 2;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) q[i][c] = load16<DT>(qr + 64 * c);
+    }
+    if (mine > 0) set_window(first_key, first_block);
+    float m[NT];  // a column's reference, log2 units
+    floatx4 acc[NT][NN], l[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        u32x4 x = __builtin_bit_cast(u32x4, q[i][c]);
+#pragma unroll
+        for (int e2 = 0; e2 < 4; ++e2) x[e2] ^= flip;
+        lds_ready(x);  // here, so that the loop's first product waits for no load of its own
+        q[i][c] = __builtin_bit_cast(V8, x);
+      }
+      m[i] = kNoScore;
+      l[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < NN; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+
     auto issue = [&](int step) {
-      if ((step & 31) == 0) window(step);
-      char* to = ring + (step % C::R) * C::SLOT_B;
+      if ((step & 31) == 0 && step > 0) {
+        const int key = key_of(step);
+        set_window(key, block_of(key));
+      }
+      char* to = ring + (step % R) * C::SLOT_B;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        if (WC == 4 && h != cw >> 1) continue;
         const int from = 2 * (step & 31) + h;
         const uint64_t at =
             (static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(at_hi), from))) << 32) |
             static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(at_lo), from));
-        const char* kp = p.k_cache + at;
-        const char* vp = p.v_cache + at;
+        if (WC == 1) {
+          const char* kp = p.k_cache + at;
+          const char* vp = p.v_cache + at;
 #pragma unroll
-        for (int u = 0; u < LPT; ++u) {
-          dma_lds16_off(kp + u * KPI * stride, koff[u % NK], to + (h * LPT + u) * 1024);
-          dma_lds16_off(vp + u * KPI * stride, voff[u % NK], to + C::TILE_B + (h * LPT + u) * 1024);
+          for (int u = 0; u < LPT; ++u) {
+            dma_lds16_off(kp + u * KPI * stride, koff[u % NK], to + (h * LPT + u) * 1024);
+            dma_lds16_off(vp + u * KPI * stride, voff[u % NK], to + C::TILE_B + (h * LPT + u) * 1024);
+          }
+        } else {
+          const char* from_cache = (cw & 1 ? p.v_cache : p.k_cache) + at;
+          char* part = to + (cw & 1) * C::TILE_B + h * LPT * 1024;
+#pragma unroll
+          for (int u = 0; u < LPT; ++u) dma_lds16_off(from_cache + u * KPI * stride, koff[u % NK], part + u * 1024);
         }
       }
     };
 
-    auto step_of = [&](int step) {
-      const int tb = 32 * (c0 + w + kWaves * step);
-      const char* kt = ring + (step % C::R) * C::SLOT_B;
-      const char* vt = kt + C::TILE_B;
-      u32x4 kraw[2][NC];
-      u32x2 vraw[NN][2];
-      const uint32_t ka = lds_addr(kt), va = lds_addr(vt) + vread;
+    V8 ones;
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        kraw[0][c] = ds_read_b128_at<0>(ka + kread[c]);
-        kraw[1][c] = ds_read_b128_at<16 * D * 2>(ka + kread[c]);
-      }
-      // Unit 2 n of a row: the swizzle touches bits above the lowest, and so is an exclusive or of the address.
+    for (int e2 = 0; e2 < 8; ++e2) ones[e2] = static_cast<T>(1.f);
+    constexpr int AHEAD = WC == 1 ? R : R - 1;  // chunks issued before the first is waited for
 #pragma unroll
-      for (int n = 0; n < NN; ++n) {
-        const uint32_t a = va ^ (n << 5);
-        vraw[n][0] = ds_read_tr16_b64_at<0>(a);
-        vraw[n][1] = ds_read_tr16_b64_at<16 * D * 2>(a);
-      }
-      lds_wait_all();
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int c = 0; c < NC; ++c) lds_ready(kraw[h][c]);
-#pragma unroll
-      for (int n = 0; n < NN; ++n) {
-        lds_ready(vraw[n][0]);
-        lds_ready(vraw[n][1]);
-      }
-      const bool tail = tb + 32 > base || tb + 32 > len;
-      // Keys that not every column sees: V of a key past the end is taken as zero, and
-      // a chunk with an element of V that is not finite is added one key at a time, so
-      // that it reaches only the rows that see it.
-      bool odd = false;
-      if (tail) {
-        const int left = len - tb;
-        int wild = 0;
-#pragma unroll
-        for (int n = 0; n < NN; ++n)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int key = 16 * h + 4 * g + 2 * e;
-              uint32_t x = vraw[n][h][e];
-              x = key + 1 < left ? x : key < left ? x & 0xFFFFu : 0u;
-              vraw[n][h][e] = x;
-              constexpr uint32_t top = DT::code == NS_DTYPE_F16 ? 0x7C00u : 0x7F80u;
-              wild |= (x & top) == top || (x & (top << 16)) == top << 16;
-            }
-        odd = __builtin_amdgcn_ballot_w64(wild != 0) != 0;
-      }
-      // The chunk is in registers (odd ones are read again): the next but one takes its place.
-      const int next = step + C::R;
-      if (!odd && next < mine) issue(next);
-      V8 ones;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ones[e] = static_cast<T>(1.f);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        floatx4 sacc[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          sacc[h] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < NC; ++c) sacc[h] = mfma16x16x32(DT{}, __builtin_bit_cast(V8, kraw[h][c]), q[n][c], sacc[h]);
+    for (int i = 0; i < AHEAD; ++i)
+      if (i < mine) issue(i);
+    // The inner loop holds the common chunk and nothing that changes the accumulators
+    // in another way (a branch that did would cost a second set of their registers):
+    // it is left before a chunk that moves a reference, which is then taken again.
+    const int count = WC == 1 ? mine : steps;
+    const bool idle = col0 >= cols;  // no columns: this wave loads for the others
+    int step = 0, there = 0;
+    uint32_t odd = 0;  // bit i: the chunk of step count - 1 - i is added one key at a time
+    while (step < count) {
+      float top[NT];
+      bool past = false;
+      for (; step < count; ++step) {
+        if (WC == 1) {
+          if (step + 1 < mine) vector_wait<C::LOADS>();
+          else vector_wait<0>();
+        } else if (there == step) {
+          // The key group's waves have all of chunk `step`, and none reads the one before.
+          const int younger = mine - 1 - step;
+          if (R > 3 && younger >= 2) vector_barrier<2 * C::LOADS>();
+          else if (R > 2 && younger >= 1) vector_barrier<C::LOADS>();
+          else vector_barrier<0>();
+          there = step + 1;
+          if (step + R - 1 < mine) issue(step + R - 1);
         }
-        uint32_t seen = ~0u;
+        if (WC > 1 && (step >= mine || idle)) continue;
+        const int tb = 32 * (c0 + kg + KG * step);
+        const char* kt = ring + (step % R) * C::SLOT_B;
+        u32x4 kraw[2][NC];
+        u32x2 vraw[NN][2];
+        const uint32_t ka = lds_addr(kt), va = ka + C::TILE_B + vread;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          kraw[0][c] = ds_read_b128_at<0>(ka + kread[c]);
+          kraw[1][c] = ds_read_b128_at<16 * D * 2>(ka + kread[c]);
+        }
+        lds_wait_all();
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int c = 0; c < NC; ++c) lds_ready(kraw[h][c]);
+        floatx4 sacc[NT][2];
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            sacc[i][h] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+              sacc[i][h] = mfma16x16x32(DT{}, __builtin_bit_cast(V8, kraw[h][c]), q[i][c], sacc[i][h]);
+          }
+        __builtin_amdgcn_sched_barrier(0);
+        // Unit 2 j of a row: the swizzle touches bits above the lowest, and so is an exclusive or of the address.
+#pragma unroll
+        for (int j = 0; j < NN; ++j) {
+          const uint32_t at = va ^ (j << 5);
+          vraw[j][0] = ds_read_tr16_b64_at<0>(at);
+          vraw[j][1] = ds_read_tr16_b64_at<16 * D * 2>(at);
+        }
+        const bool tail = tb + 32 > base;  // some keys are not seen by every column
         if (tail) {
-          seen = seen_of(mask[n], tb, base, len) >> (4 * g);
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            int head;
+            const uint32_t seen = seen_of(static_cast<uint64_t>(p.mask[row_of(i, head)]), tb, base, len) >> (4 * g);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) sacc[i][h][r] = (seen >> (16 * h + r)) & 1 ? sacc[i][h][r] : -INFINITY;
+          }
+        }
+        // A column's reference follows its maximum only when a score passes it by kSlack
+        // binades, which is seen without a trip between lanes.
+        past = false;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          top[i] = sacc[i][0][0];
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sacc[h][r] = (seen >> (16 * h + r)) & 1 ? sacc[h][r] : -INFINITY;
+            for (int r = 0; r < 4; ++r) top[i] = fmaxf(top[i], sacc[i][h][r]);
+          past |= top[i] * scale > m[i] + kSlack;
         }
-        float top = -INFINITY;
+        past = __builtin_amdgcn_ballot_w64(past) != 0;
+        lds_wait_all();
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) top = fmaxf(top, sacc[h][r]);
-        top = group4_max_swap(top);
-        top = top == -INFINITY ? top : top * scale;
-        if (__builtin_amdgcn_ballot_w64(top > m[n]) != 0) {
-          const float next_m = fmaxf(m[n], top);
-          const float alpha = next_m == -INFINITY ? 1.f : fast_exp2(m[n] - next_m);
-          m[n] = next_m;
-          l[n] *= alpha;
-#pragma unroll
-          for (int i = 0; i < NN; ++i) acc[n][i] *= alpha;
+        for (int j = 0; j < NN; ++j) {
+          lds_ready(vraw[j][0]);
+          lds_ready(vraw[j][1]);
         }
-        const float ref = m[n] == -INFINITY ? 0.f : m[n];
-        float pr[2][4];
-        V8 pt;
+        if (__builtin_expect(past, 0)) break;
+        if (tail) {
+          // V of a key past the end is taken as zero.  A chunk with an element of V that
+          // is not finite is left for later (add_keys), so that it reaches only the rows
+          // that see it.
+          const int left = len - tb;
+          int wild = 0;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+          for (int j = 0; j < NN; ++j)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float x = fast_exp2(__builtin_fmaf(sacc[h][r], scale, -ref));
-            if (tail) x = (seen >> (16 * h + r)) & 1 ? x : 0.f;
-            pr[h][r] = x;
-            pt[4 * h + r] = static_cast<T>(x);
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int e2 = 0; e2 < 2; ++e2) {
+                const int key = 16 * h + 4 * g + 2 * e2;
+                uint32_t x = vraw[j][h][e2];
+                x = key + 1 < left ? x : key < left ? x & 0xFFFFu : 0u;
+                vraw[j][h][e2] = x;
+                constexpr uint32_t inf = DT::code == NS_DTYPE_F16 ? 0x7C00u : 0x7F80u;
+                wild |= (x & inf) == inf || (x & (inf << 16)) == inf << 16;
+              }
+          if (__builtin_amdgcn_ballot_w64(wild != 0) != 0 && count - 1 - step < 32) {
+            odd |= 1u << (count - 1 - step);
+#pragma unroll
+            for (int j = 0; j < NN; ++j) vraw[j][0] = vraw[j][1] = u32x2{0u, 0u};
           }
-        l[n] = mfma16x16x32(DT{}, ones, pt, l[n]);
-        if (!odd) {
+        }
+        // The chunk is in registers: the next but one takes its place.
+        if (WC == 1 && step + R < mine) issue(step + R);
+        V8 pt[NT];
 #pragma unroll
-          for (int i = 0; i < NN; ++i) {
-            const V8 v = __builtin_bit_cast(V8, u32x4{vraw[i][0][0], vraw[i][0][1], vraw[i][1][0], vraw[i][1][1]});
-            acc[n][i] = mfma16x16x32(DT{}, v, pt, acc[n][i]);
-          }
-        } else {
+        for (int i = 0; i < NT; ++i)
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              for (int gk = 0; gk < 4; ++gk) {
-                const int key = 16 * h + 4 * gk + r;
-                const float x = __shfl(static_cast<float>(static_cast<T>(pr[h][r])), 16 * gk + c16);
-                const int sees = __shfl(static_cast<int>((seen >> (16 * h + r)) & 1), 16 * gk + c16);
-                if (sees) {
+              pt[i][4 * h + r] = static_cast<T>(fast_exp2(__builtin_fmaf(sacc[i][h][r], scale, -m[i])));
 #pragma unroll
-                  for (int i = 0; i < NN; ++i) {
-                    const int unit = 2 * i + (g >> 1);
-                    const typename DT::vec4 v = *reinterpret_cast<const typename DT::vec4*>(
-                        vt + key * (D * 2) + ((unit ^ v_swizzle<D>(key)) << 4) + (g & 1) * 8);
+        for (int i = 0; i < NT; ++i) l[i] = mfma16x16x32(DT{}, ones, pt[i], l[i]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                      acc[n][i][e] = __builtin_fmaf(x, static_cast<float>(v[e]), acc[n][i][e]);
-                  }
-                }
-              }
+        for (int j = 0; j < NN; ++j) {
+          const V8 v = __builtin_bit_cast(V8, u32x4{vraw[j][0][0], vraw[j][0][1], vraw[j][1][0], vraw[j][1][1]});
+#pragma unroll
+          for (int i = 0; i < NT; ++i) acc[i][j] = mfma16x16x32(DT{}, v, pt[i], acc[i][j]);
         }
       }
-      if (odd) {
-        lds_wait_all();
-        if (next < mine) issue(next);
+      if (past) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          const float x = group4_max_swap(top[i]);
+          const float next_m = x == -INFINITY ? m[i] : fmaxf(m[i], x * scale);
+          const float alpha = fast_exp2(m[i] - next_m);
+          m[i] = next_m;
+          l[i] *= alpha;
+#pragma unroll
+          for (int j = 0; j < NN; ++j) acc[i][j] *= alpha;
+        }
+      }
+    }
+
+    // What follows a range's chunks works its places out anew from here, or they would
+    // be held in registers over the loop.
+    int tid2 = tid;
+    asm volatile("" : "+v"(tid2));
+    const int lane2 = tid2 & 63, g2 = lane2 >> 4, c2 = lane2 & 15;
+
+    // Adds the rows of V of a chunk to this lane's outputs of column c2 of tile i, at `to`
+    // (a unit's floats apart), for the keys that the column sees; their weights, which
+    // the sum has, are worked out again.
+    auto add_keys = [&](int i, int tb, float reference, float factor, float* to) {
+      int head;
+      const int64_t row = row_of(i, head);
+      const uint32_t seen = seen_of(static_cast<uint64_t>(p.mask[row]), tb, base, len);
+      const T* qr = reinterpret_cast<const T*>(p.query) + (row * p.num_heads + head) * D + g2 * (D / 4);
+      for (int key = tb; key < tb + 32 && key < len; ++key) {
+        const int64_t blk = block_of(key);
+        if (blk < 0 || blk >= p.num_blocks) break;  // the outputs are NaN
+        const int64_t at = ((blk * p.block_size + key % p.block_size) * Hkv + kvh) * D;
+        const T* kr = reinterpret_cast<const T*>(p.k_cache) + at + g2 * (D / 4);
+        const T* vr = reinterpret_cast<const T*>(p.v_cache) + at + 4 * g2;
+        float x = 0.f;
+        for (int d = 0; d < D / 4; ++d) x = __builtin_fmaf(static_cast<float>(qr[d]), static_cast<float>(kr[d]), x);
+        x = group4_sum(x) * (p.scale < 0.f ? -scale : scale);
+        x = static_cast<float>(static_cast<T>(fast_exp2(x - reference))) * factor;
+        if ((seen >> (key - tb)) & 1) {
+          for (int j = 0; j < NN; ++j)
+            for (int e2 = 0; e2 < 4; ++e2) {
+              float& o = to[j * C::UNIT + e2];
+              o = __builtin_fmaf(x, static_cast<float>(vr[16 * j + e2]), o);
+            }
+        }
       }
     };
 
-    if (mine > 0) issue(0);
-    if (mine > 1) issue(1);
-    for (int step = 0; step < mine; ++step) {
-      if (step + 1 < mine) vector_wait<C::PER_CHUNK>();
-      else vector_wait<0>();
-      step_of(step);
-    }
-
-    // The waves' states meet in LDS, JOIN column tiles at a time.  The ring is free
-    // when every wave is here.
-    if (g == 0) {
+    // The key groups' states meet in LDS.  The ring is free when every wave is here.
+    if (g2 == 0) {
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        maxima[w][16 * i + c16] = m[i];
-        sums[w][16 * i + c16] = l[i][0];
+        maxima[kg][(cw * NT + i) * 16 + c2] = m[i];
+        sums[kg][(cw * NT + i) * 16 + c2] = l[i][0];
       }
     }
     {
       const int wave_bad = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
-      if (lane == 0) bads[w] = wave_bad;
+      if (lane2 == 0) bads[w] = wave_bad;
     }
+    __syncthreads();
+    int bad_any = 0;
+#pragma unroll
+    for (int ww = 0; ww < W; ++ww) bad_any |= bads[ww];
     const bool split = b > a;
     // A workgroup has at most one cut group that it begins (its last: slot 2 k + 1)
     // and one that it does not (its first: slot 2 k).
-    auto slot_of = [&](int kk) { return kk == a ? 2 * kk + 1 : 2 * kk; };
+    auto part_of = [&](int kk) { return (kk == a ? 1 : 2 * (kk - a)) * C::PART; };
     const __amdgpu_buffer_rsrc_t pr = __builtin_amdgcn_make_buffer_rsrc(
         p.partials + static_cast<int64_t>(2) * a * C::PART, static_cast<short>(0),
         split ? 2 * (b - a + 1) * C::PART * 4 : 0, kBufferWord3);
-    auto part_of = [&](int kk) { return (slot_of(kk) - 2 * a) * C::PART; };
     T* out = reinterpret_cast<T*>(p.out);
-    auto write = [&](int col, int f, floatx4 o, float inv) {
-      const int c = cb * C::COLS + col;
-      const int64_t at = ((static_cast<int64_t>(row0) + c / G) * p.num_heads + kvh * G + c % G) * D + 4 * f;
+    // Dims 16 j + 4 g .. + 3 of the columns of tile i of this wave.
+    auto write = [&](int i, int j, floatx4 o, float inv) {
+      const int c = col0 + 16 * i + c2;
+      if (c >= cols) return;
+      const int64_t at = ((static_cast<int64_t>(row0) + c / G) * p.num_heads + kvh * G + c % G) * D + 16 * j + 4 * g2;
       typename DT::vec4 v;
 #pragma unroll
       for (int r = 0; r < 4; ++r) v[r] = static_cast<T>(o[r] * inv);
       *reinterpret_cast<u32x2*>(out + at) = __builtin_bit_cast(u32x2, v);
     };
     auto inverse = [&](float sum) { return sum > 0.f || sum != sum ? 1.f / sum : 0.f; };  // no key: zero; a NaN stays one
-    const int here = cols - cb * C::COLS < C::COLS ? cols - cb * C::COLS : C::COLS;  // columns of the group
+    float* buf = reinterpret_cast<float*>(smem);
+    float join_top[NT], join_sum[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const int col = (cw * NT + i) * 16 + c2;
+      join_top[i] = kNoScore;
+#pragma unroll
+      for (int kk = 0; kk < KG; ++kk) join_top[i] = fmaxf(join_top[i], maxima[kk][col]);
+      join_sum[i] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < KG; ++kk)
+        join_sum[i] = __builtin_fmaf(sums[kk][col], fast_exp2(maxima[kk][col] - join_top[i]), join_sum[i]);
+      if (bad_any) join_sum[i] = NAN;
+      if (split && kg == 0 && g2 == 0)
+        __builtin_amdgcn_raw_buffer_store_b64(
+            u32x2{__builtin_bit_cast(uint32_t, join_top[i]), __builtin_bit_cast(uint32_t, join_sum[i])}, pr,
+            4 * (part_of(k) + COLS * D + 2 * col), 0, kSc1);
+    }
 #pragma unroll
     for (int n0 = 0; n0 < NT; n0 += C::JOIN) {
-      __syncthreads();
-      float* mine_o = reinterpret_cast<float*>(smem) + w * (C::JOIN * 16 * D);
+      if (n0 > 0) __syncthreads();
+      float* mine_o = buf + w * (C::JOIN * NN * C::UNIT) + 4 * lane2;
 #pragma unroll
-      for (int i = n0; i < n0 + C::JOIN && i < NT; ++i)
+      for (int i = n0; i < n0 + C::JOIN; ++i) {
+        const float f = fast_exp2(m[i] - join_top[i]);
 #pragma unroll
         for (int j = 0; j < NN; ++j)
-          *reinterpret_cast<floatx4*>(mine_o + (16 * (i - n0) + c16) * D + 4 * ((4 * j + g) ^ c16)) = acc[i][j];
+          *reinterpret_cast<floatx4*>(mine_o + ((i - n0) * NN + j) * C::UNIT) = acc[i][j] * f;
+        if (__builtin_expect(odd != 0, 0))
+          for (int left = static_cast<int>(odd); left != 0; left &= left - 1)
+            add_keys(i, 32 * (c0 + kg + KG * (count - 1 - __builtin_ctz(left))), m[i], f,
+                     mine_o + (i - n0) * NN * C::UNIT);
+      }
       __syncthreads();
-      int bad_any = 0;
+      // Unit u KG + kg of the tiles is this wave's to add up.
 #pragma unroll
-      for (int ww = 0; ww < kWaves; ++ww) bad_any |= bads[ww];
-      for (int x = tid; x < C::JOIN * 16 * (D / 4); x += kThreads) {
-        const int col = 16 * n0 + x / (D / 4), f = x % (D / 4);
-        if (col >= here) break;
-        float mw[kWaves], lw[kWaves], top = -INFINITY;
-        floatx4 ow[kWaves];
+      for (int u = 0; u < (C::JOIN * NN + KG - 1) / KG; ++u) {
+        const int unit = u * KG + kg;
+        if (unit < C::JOIN * NN) {
+          floatx4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int ww = 0; ww < kWaves; ++ww) {
-          mw[ww] = maxima[ww][col];
-          lw[ww] = sums[ww][col];
-          ow[ww] = *reinterpret_cast<const floatx4*>(reinterpret_cast<const float*>(smem) +
-                                                     ww * (C::JOIN * 16 * D) + (col - 16 * n0) * D + 4 * (f ^ (col & 15)));
-          top = fmaxf(top, mw[ww]);
-        }
-        const float ref = top == -INFINITY ? 0.f : top;
-        float sum = 0.f;
-        floatx4 o = {0.f, 0.f, 0.f, 0.f};
+          for (int kk = 0; kk < KG; ++kk)
+            o += *reinterpret_cast<const floatx4*>(buf + ((kk * WC + cw) * (C::JOIN * NN) + unit) * C::UNIT + 4 * lane2);
+          const int i = unit / NN, j = unit % NN;  // of the JOIN tiles
+          float sum = join_sum[n0];
 #pragma unroll
-        for (int ww = 0; ww < kWaves; ++ww) {
-          const float f2 = fast_exp2(mw[ww] - ref);
-          sum = __builtin_fmaf(lw[ww], f2, sum);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o[r] = __builtin_fmaf(ow[ww][r], f2, o[r]);
-        }
-        if (bad_any) {
-          sum = NAN;
-          o = floatx4{NAN, NAN, NAN, NAN};
-        }
-        if (!split) {
-          write(col, f, o, inverse(sum));
-        } else {
-          const int to = 4 * (part_of(k) + col * D + 4 * f);
-          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), pr, to, 0, kSc1);
-          if (f == 0)
-            __builtin_amdgcn_raw_buffer_store_b64(
-                u32x2{__builtin_bit_cast(uint32_t, top), __builtin_bit_cast(uint32_t, sum)}, pr,
-                4 * (part_of(k) + C::COLS * D + 2 * col), 0, kSc1);
+          for (int ii = 1; ii < C::JOIN; ++ii) sum = i == ii ? join_sum[n0 + ii] : sum;
+          if (!split)
+            write(n0 + i, j, o, inverse(sum));
+          else
+            __builtin_amdgcn_raw_buffer_store_b128(
+                __builtin_bit_cast(u32x4, o), pr,
+                4 * (part_of(k) + ((cw * NT + n0) * NN + unit) * C::UNIT + 4 * lane2), 0, kSc1);
         }
       }
     }
@@ -787,70 +849,63 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void tree_attention_kern
     // A partial is acknowledged (device scope) before its arrival is counted.
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
     __syncthreads();
-    if (tid == 0)
+    if (tid2 == 0)
       last = __hip_atomic_fetch_add(&p.counters[a], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == b - a;
     __syncthreads();
     if (last) {
       const int ranges = b - a + 1;
       // Every range's maximum and sum of every column, then its weight, in LDS.
-      float* ml = reinterpret_cast<float*>(smem);
-      for (int x = tid; x < ranges * C::COLS; x += kThreads) {
-        const int r = x / C::COLS, col = x % C::COLS;
-        if (col < here) {
-          const int from = 4 * (part_of(a + r) + C::COLS * D + 2 * col);
-          ml[x] = ld_sc1(pr, from);
-          ml[kMostRanges * C::COLS + x] = ld_sc1(pr, from + 4);
-        }
+      for (int x = tid2; x < ranges * COLS; x += C::THREADS) {
+        const int from = 4 * (part_of(a + x / COLS) + COLS * D + 2 * (x % COLS));
+        buf[x] = ld_sc1(pr, from);
+        buf[kMostRanges * COLS + x] = ld_sc1(pr, from + 4);
       }
       __syncthreads();
-      if (tid < here) {
-        float top = -INFINITY, sum = 0.f;
-        for (int r = 0; r < ranges; ++r) top = fmaxf(top, ml[r * C::COLS + tid]);
-        const float ref = top == -INFINITY ? 0.f : top;
+      if (tid2 < COLS) {
+        float top = kNoScore, sum = 0.f;
+        for (int r = 0; r < ranges; ++r) top = fmaxf(top, buf[r * COLS + tid2]);
         for (int r = 0; r < ranges; ++r) {
-          const float f2 = fast_exp2(ml[r * C::COLS + tid] - ref);
-          ml[r * C::COLS + tid] = f2;
-          sum = __builtin_fmaf(ml[kMostRanges * C::COLS + r * C::COLS + tid], f2, sum);
+          const float f = fast_exp2(buf[r * COLS + tid2] - top);
+          buf[r * COLS + tid2] = f;
+          sum = __builtin_fmaf(buf[kMostRanges * COLS + r * COLS + tid2], f, sum);
         }
-        maxima[0][tid] = inverse(sum);
+        maxima[0][tid2] = inverse(sum);
       }
       __syncthreads();
       floatx4 o[C::OWN];
 #pragma unroll
-      for (int i = 0; i < C::OWN; ++i) o[i] = floatx4{0.f, 0.f, 0.f, 0.f};
-      constexpr int AT_ONCE = 16 / C::OWN;  // ranges whose loads are in flight together
+      for (int u = 0; u < C::OWN; ++u) o[u] = floatx4{0.f, 0.f, 0.f, 0.f};
+      constexpr int AT_ONCE = C::OWN >= 8 ? 2 : 16 / C::OWN;  // ranges whose loads are in flight together
       for (int r0 = 0; r0 < ranges; r0 += AT_ONCE) {
         floatx4 part[AT_ONCE][C::OWN];
 #pragma unroll
         for (int j = 0; j < AT_ONCE; ++j) {
           const int r = r0 + j < ranges ? r0 + j : ranges - 1;
 #pragma unroll
-          for (int i = 0; i < C::OWN; ++i) {
-            const int from = 4 * (part_of(a + r) + 4 * (tid + i * kThreads));
-            part[j][i] = floatx4{ld_sc1(pr, from), ld_sc1(pr, from + 4), ld_sc1(pr, from + 8), ld_sc1(pr, from + 12)};
+          for (int u = 0; u < C::OWN; ++u) {
+            const int unit = u * KG + kg < NT * NN ? u * KG + kg : 0;
+            const int from = 4 * (part_of(a + r) + (cw * NT * NN + unit) * C::UNIT + 4 * lane2);
+            part[j][u] = floatx4{ld_sc1(pr, from), ld_sc1(pr, from + 4), ld_sc1(pr, from + 8), ld_sc1(pr, from + 12)};
           }
         }
 #pragma unroll
         for (int j = 0; j < AT_ONCE; ++j) {
           if (r0 + j < ranges) {
 #pragma unroll
-            for (int i = 0; i < C::OWN; ++i) {
-              const int col = (tid + i * kThreads) / (D / 4);
-              if (col < here) {
-                const float f2 = ml[(r0 + j) * C::COLS + col];
+            for (int u = 0; u < C::OWN; ++u) {
+              const float f = buf[(r0 + j) * COLS + (cw * NT + (u * KG + kg) / NN % NT) * 16 + c2];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) o[i][r] = __builtin_fmaf(part[j][i][r], f2, o[i][r]);
-              }
+              for (int r = 0; r < 4; ++r) o[u][r] = __builtin_fmaf(part[j][u][r], f, o[u][r]);
             }
           }
         }
       }
 #pragma unroll
-      for (int i = 0; i < C::OWN; ++i) {
-        const int x = tid + i * kThreads, col = x / (D / 4);
-        if (col < here) write(col, x % (D / 4), o[i], maxima[0][col]);
+      for (int u = 0; u < C::OWN; ++u) {
+        const int unit = u * KG + kg;
+        if (unit < NT * NN) write(unit / NN, unit % NN, o[u], maxima[0][(cw * NT + unit / NN) * 16 + c2]);
       }
-      if (tid == 0) __hip_atomic_store(&p.counters[a], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (tid2 == 0) __hip_atomic_store(&p.counters[a], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
   }
@@ -871,35 +926,61 @@ int device_cus() {
   return n;
 }
 
-// Column tiles of an item for sequences of up to max_rows rows: those of the widest
-// sequence, in equal blocks of at most four.
-int tiles_of(int max_rows, int group) {
+// Workgroups that the device holds at once, in whole rounds of the XCDs.
+int places() { return (device_cus() + 7) / 8 * 8; }
+
+// Column tiles of a group: those of the widest sequence, in equal blocks.
+int tiles_of(int max_rows, int group, int head_dim) {
+  const int most = head_dim == 64 ? 16 : 8;
   const int64_t rows = max_rows < 1 ? 1 : max_rows < kRows ? max_rows : kRows;
   const int64_t tiles = (rows * group + 15) / 16;
-  const int64_t blocks = (tiles + 3) / 4;
+  const int64_t blocks = (tiles + most - 1) / most;
   return static_cast<int>((tiles + blocks - 1) / blocks);
 }
 
-// Workgroups that the device holds at once, in whole rounds of the XCDs.
-int places_of(int head_dim) { return (device_cus() + 7) / 8 * 8 * (head_dim == 64 ? 2 : 1); }
+// The kernels, by head size and tiles: key groups, column waves and tiles of a wave.
+template <int D, class F>
+auto with_shape(int tiles, F&& f) {
+  if constexpr (D == 64) {
+    if (tiles <= 1) return f(Cfg<64, 8, 1, 1>{});
+    if (tiles <= 2) return f(Cfg<64, 8, 1, 2>{});
+    if (tiles <= 4) return f(Cfg<64, 4, 2, 2>{});
+    if (tiles <= 8) return f(Cfg<64, 2, 4, 2>{});
+    return f(Cfg<64, 2, 4, 4>{});
+  } else {
+    if (tiles <= 1) return f(Cfg<128, 4, 1, 1>{});
+    if (tiles <= 2) return f(Cfg<128, 4, 1, 2>{});
+    if (tiles <= 4) return f(Cfg<128, 4, 2, 2>{});
+    return f(Cfg<128, 2, 4, 2>{});
+  }
+}
 
-size_t slot_bytes(int head_dim, int nt) { return static_cast<size_t>(16) * nt * (head_dim + 2) * 4; }
+size_t workspace_bytes_of(int head_dim, int tiles) {
+  auto words = [](auto c) { return static_cast<size_t>(decltype(c)::PART); };
+  return static_cast<size_t>(2) * places() * 4 * (head_dim == 64 ? with_shape<64>(tiles, words) : with_shape<128>(tiles, words));
+}
 
 template <class DT, int D>
-hipError_t launch_tiles(const TreeParams& p, int nt, hipStream_t stream) {
-  const void* fn = nt == 1   ? reinterpret_cast<const void*>(&tree_attention_kernel<DT, D, 1>)
-                   : nt == 2 ? reinterpret_cast<const void*>(&tree_attention_kernel<DT, D, 2>)
-                   : nt == 3 ? reinterpret_cast<const void*>(&tree_attention_kernel<DT, D, 3>)
-                             : reinterpret_cast<const void*>(&tree_attention_kernel<DT, D, 4>);
-  TreeParams part = p;
-  void* args[] = {&part};
-  for (int s = 0; s < p.num_seqs; s += kSeqs) {
-    part.first_seq = s;
-    part.num_seqs = p.num_seqs - s < kSeqs ? p.num_seqs - s : kSeqs;
-    const hipError_t e = hipLaunchKernel(fn, dim3(static_cast<unsigned>(places_of(D))), dim3(kThreads), args, 0, stream);
-    if (e != hipSuccess) return e;
-  }
-  return hipSuccess;
+hipError_t launch_tiles(const TreeParams& p, int tiles, hipStream_t stream) {
+  return with_shape<D>(tiles, [&](auto c) {
+    using C = decltype(c);
+    // A launch's line of work is counted in 32 bits: as many sequences as it is sure to hold.
+    const int64_t groups = (static_cast<int64_t>(kRows) * p.group + C::COLS - 1) / C::COLS * p.num_kv_heads;
+    const int64_t line = groups * (p.max_ctx / 32 + 1 + kGroupCost);
+    const int64_t fits = (int64_t{1} << 30) / line;
+    if (fits < 1) return hipErrorInvalidValue;
+    const int most = static_cast<int>(fits < kSeqs ? fits : kSeqs);
+    TreeParams part = p;
+    void* args[] = {&part};
+    for (int s = 0; s < p.num_seqs; s += most) {
+      part.first_seq = s;
+      part.num_seqs = p.num_seqs - s < most ? p.num_seqs - s : most;
+      const hipError_t e = hipLaunchKernel(reinterpret_cast<const void*>(&tree_attention_kernel<DT, C>),
+                                           dim3(static_cast<unsigned>(places())), dim3(C::THREADS), args, 0, stream);
+      if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+  });
 }
 
 bool misaligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a != 0; }
@@ -912,7 +993,7 @@ bool sizes_ok(int num_seqs, int64_t num_tokens, int num_heads, int num_kv_heads,
 }  // namespace
 }  // namespace ns
 
-extern "C" int ns_paged_attention_tree_counters(void) { return ns::places_of(64); }
+extern "C" int ns_paged_attention_tree_counters(void) { return ns::places(); }
 
 extern "C" size_t ns_paged_attention_tree_workspace_size(int num_seqs, int num_heads, int num_kv_heads, int head_dim,
                                                          int block_size, int max_query_len, int64_t num_tokens,
@@ -921,8 +1002,7 @@ extern "C" size_t ns_paged_attention_tree_workspace_size(int num_seqs, int num_h
   if (!sizes_ok(num_seqs, num_tokens, num_heads, num_kv_heads, head_dim, block_size) || num_seqs == 0 ||
       num_tokens == 0 || !takes_tiles(head_dim, block_size, num_heads / num_kv_heads, dtype))
     return 0;
-  return static_cast<size_t>(2) * places_of(head_dim) *
-         slot_bytes(head_dim, tiles_of(max_query_len, num_heads / num_kv_heads));
+  return workspace_bytes_of(head_dim, tiles_of(max_query_len, num_heads / num_kv_heads, head_dim));
 }
 
 extern "C" int ns_paged_attention_tree(void* out, const void* query,
@@ -992,9 +1072,9 @@ extern "C" int ns_paged_attention_tree(void* out, const void* query,
         : dtype == NS_DTYPE_F16 ? launch_generic<_Float16>(p, st)
                                 : launch_generic<__bf16>(p, st);
   } else {
-    const int nt = tiles_of(max_query_len, group);
+    const int nt = tiles_of(max_query_len, group, head_dim);
     if (!counters || misaligned(counters, 4) || !workspace || misaligned(workspace, 16) ||
-        workspace_bytes < static_cast<size_t>(2) * places_of(head_dim) * slot_bytes(head_dim, nt))
+        workspace_bytes < workspace_bytes_of(head_dim, nt))
       return NS_ERR_WORKSPACE;
     e = dtype == NS_DTYPE_F16 ? (head_dim == 64 ? launch_tiles<F16, 64>(p, nt, st) : launch_tiles<F16, 128>(p, nt, st))
                               : (head_dim == 64 ? launch_tiles<BF16, 64>(p, nt, st) : launch_tiles<BF16, 128>(p, nt, st));
