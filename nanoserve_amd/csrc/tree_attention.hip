@@ -215,10 +215,10 @@ hipError_t launch_generic(const TreeParams& p, hipStream_t stream) {
 // lengths for itself.
 
 constexpr int kMostRanges = 32;  // of a group: what the last workgroup has to join
-constexpr int kGroupCost = 4;    // in chunks, at least half a round of the key groups
+constexpr int kGroupCost = 16;   // in chunks
 constexpr float kNoScore = -3e38f;  // a column's reference before its first score
 constexpr float kSlack = 8.f;    // binades that a score may pass its column's reference by
-constexpr int kLeastShare = 8;   // chunks
+constexpr int kLeastRounds = 2;  // of the key groups, in a share; groups of no more stay whole
 
 template <int D_, int KG_, int WC_, int NT_>
 struct Cfg {
@@ -245,7 +245,7 @@ struct Cfg {
   static_assert(R >= 2 && JOIN >= 1 && NT % JOIN == 0, "chunks in flight; a tile of every wave fits the ring");
   static_assert(2 * kMostRanges * COLS * 4 <= RING, "the ranges' maxima and sums fit the ring");
   static_assert(kGroupCost >= KG / 2, "a group's workgroups begin within its stretch of the line");
-  static_assert(kLeastShare >= KG, "a group has one cut at most that moves to its start or end");
+  static_assert(kLeastRounds >= 1, "a group has one cut at most that moves to its start or end");
 };
 
 constexpr int kSc1 = 16;                  // cache-policy bit SC1 of gfx950 buffer operations: device scope
@@ -403,7 +403,7 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
   int share = quotient(line.total + grid - 1, grid);
   const int least = line.most / (kMostRanges - 2) + 1;
   share = share > least ? share : least;
-  share = share > kLeastShare ? share : kLeastShare;
+  share = share > kLeastRounds * KG ? share : kLeastRounds * KG;
   // Neighbouring shares, which read the same keys where a sequence has several
   // groups of columns, go to one XCD (workgroups go to the eight in turn).
   const int shares = quotient(line.total + share - 1, share);
@@ -455,7 +455,7 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
     const int a = quotient(gs + kHalf - 1, share);
     if (a > k) return;
     const int e = (n + KG - 1) / KG * KG - kHalf - 1;
-    int b = e > 0 ? quotient(gs + e, share) : a;
+    int b = n > kLeastRounds * KG ? quotient(gs + e, share) : a;
     b = b > a ? b : a;
     if (k > b) continue;
     auto cut = [&](int kk) { return (kk * share - gs + kHalf) / KG * KG; };
@@ -929,12 +929,17 @@ int device_cus() {
 // Workgroups that the device holds at once, in whole rounds of the XCDs.
 int places() { return (device_cus() + 7) / 8 * 8; }
 
-// Column tiles of a group: those of the widest sequence, in equal blocks.
-int tiles_of(int max_rows, int group, int head_dim) {
-  const int most = head_dim == 64 ? 16 : 8;
+// Column tiles of a group: those of the widest sequence, in equal blocks.  Wide
+// blocks load K and V for more columns at once, narrow ones leave more groups to work on
+// at the same time: as wide as leaves a quarter of the device's workgroups a group.
+int tiles_of(int num_seqs, int num_kv_heads, int max_rows, int group, int head_dim) {
   const int64_t rows = max_rows < 1 ? 1 : max_rows < kRows ? max_rows : kRows;
   const int64_t tiles = (rows * group + 15) / 16;
-  const int64_t blocks = (tiles + most - 1) / most;
+  int64_t blocks = 0;
+  for (int most = head_dim == 64 ? 16 : 8; most >= 2; most /= 2) {
+    blocks = (tiles + most - 1) / most;
+    if (num_seqs * blocks * num_kv_heads * 4 >= places()) break;
+  }
   return static_cast<int>((tiles + blocks - 1) / blocks);
 }
 
@@ -1002,7 +1007,7 @@ extern "C" size_t ns_paged_attention_tree_workspace_size(int num_seqs, int num_h
   if (!sizes_ok(num_seqs, num_tokens, num_heads, num_kv_heads, head_dim, block_size) || num_seqs == 0 ||
       num_tokens == 0 || !takes_tiles(head_dim, block_size, num_heads / num_kv_heads, dtype))
     return 0;
-  return workspace_bytes_of(head_dim, tiles_of(max_query_len, num_heads / num_kv_heads, head_dim));
+  return workspace_bytes_of(head_dim, tiles_of(num_seqs, num_kv_heads, max_query_len, num_heads / num_kv_heads, head_dim));
 }
 
 extern "C" int ns_paged_attention_tree(void* out, const void* query,
@@ -1072,7 +1077,7 @@ extern "C" int ns_paged_attention_tree(void* out, const void* query,
         : dtype == NS_DTYPE_F16 ? launch_generic<_Float16>(p, st)
                                 : launch_generic<__bf16>(p, st);
   } else {
-    const int nt = tiles_of(max_query_len, group, head_dim);
+    const int nt = tiles_of(num_seqs, num_kv_heads, max_query_len, group, head_dim);
     if (!counters || misaligned(counters, 4) || !workspace || misaligned(workspace, 16) ||
         workspace_bytes < workspace_bytes_of(head_dim, nt))
       return NS_ERR_WORKSPACE;
