@@ -21,18 +21,29 @@ captured graph serves other lengths, trees and choices on every replay.
 
 from __future__ import annotations
 
-import ctypes
+import array
 from dataclasses import dataclass
+from operator import attrgetter
 
 import torch
 
 from . import _lib
 from .attention import AttentionMetadata
 
+_SIZE, _DEVICE, _CONTIGUOUS, _ADDRESS = (torch.Tensor.size, torch.Tensor.get_device, torch.Tensor.is_contiguous,
+                                         torch.Tensor.data_ptr)
+_DTYPE = attrgetter("dtype")
+
 MAX_TREE_ROWS = 64  # rows of a request that a 64-bit mask can name
 
 
-@dataclass(frozen=True)
+# These wrappers run in every step (paged_attention_tree in every layer) and hold a
+# launch back by a few microseconds each: every tensor attribute is read once, and
+# devices are compared by their index.  None of the ops is differentiable; what they
+# return has no history.
+
+
+@dataclass
 class StepInputs:
     """A step's addresses on the device, as AttentionMetadata takes them (int64;
     block_tables in the tables' dtype)."""
@@ -45,26 +56,23 @@ class StepInputs:
     tree_mask: torch.Tensor | None        # [T], with parents
 
 
-def _integers(tensors: dict, device: torch.device) -> tuple[dict, bool]:
-    """The tensors (name -> tensor or None, and its length) contiguous and of one integer dtype; whether that is int64."""
-    kinds = set()
-    for name, (t, n) in tensors.items():
-        if t is None:
-            continue
-        if t.device != device:
-            raise ValueError(f"{name} is on {t.device}, expected {device}")
-        if t.dim() != 1 or t.shape[0] != n:
-            raise ValueError(f"{name} must hold {n} entries, got {tuple(t.shape)}")
-        if t.dtype is not torch.int64 and t.dtype is not torch.int32:
-            raise TypeError(f"{name} must be int32 or int64, got {t.dtype}")
-        kinds.add(t.dtype)
-    wide = kinds != {torch.int32}
-    out = {}
-    for name, (t, _) in tensors.items():
-        if t is not None and wide and t.dtype is torch.int32:
-            t = t.to(torch.int64)
-        out[name] = t if t is None or t.is_contiguous() else t.contiguous()
-    return out, wide
+def _vector(t: torch.Tensor, name: str, n: int, index: int) -> torch.Tensor:
+    """t, contiguous, if it holds n int32 or int64 entries on GPU `index`."""
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{index}")
+    if t.shape != (n,):
+        raise ValueError(f"{name} must hold {n} entries, got {tuple(t.shape)}")
+    if t.dtype is not torch.int64 and t.dtype is not torch.int32:
+        raise TypeError(f"{name} must be int32 or int64, got {t.dtype}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _alike(tensors: list) -> tuple[list, bool]:
+    """The tensors (or None) of one integer dtype, and whether that is int64."""
+    wide = any(t is not None and t.dtype is torch.int64 for t in tensors)
+    if wide:
+        tensors = [t if t is None or t.dtype is torch.int64 else t.to(torch.int64) for t in tensors]
+    return tensors, wide
 
 
 def _pointer(t: torch.Tensor | None):
@@ -100,26 +108,31 @@ def step_inputs(tables: torch.Tensor, rows: torch.Tensor, computed: torch.Tensor
     given = [x is not None for x in (new_blocks, new_start, held)]
     if any(given) and not all(given):
         raise ValueError("new_blocks, new_start and held belong together")
-    device = tables.device
+    index = tables.get_device()
     B = rows.shape[0] if rows.dim() else 0
     N = 0 if new_blocks is None else new_blocks.numel()
-    x, wide = _integers({"rows": (rows, B), "computed": (computed, B), "query_lens": (query_lens, B),
-                         "new_blocks": (new_blocks, N), "new_start": (new_start, B + 1), "held": (held, B),
-                         "parents": (parents, num_tokens)}, device)
-    per_token = 2 if parents is None else 3
+    vectors = [_vector(rows, "rows", B, index), _vector(computed, "computed", B, index),
+               _vector(query_lens, "query_lens", B, index),
+               None if new_blocks is None else _vector(new_blocks, "new_blocks", N, index),
+               None if new_start is None else _vector(new_start, "new_start", B + 1, index),
+               None if held is None else _vector(held, "held", B, index),
+               None if parents is None else _vector(parents, "parents", num_tokens, index)]
+    vectors, wide = _alike(vectors)
+    device = tables.device
     # One allocation for every int64 output.
-    flat = torch.empty(2 * B + 1 + per_token * num_tokens, dtype=torch.int64, device=device)
-    qsl, lens, positions, slots, *mask = flat.split([B + 1, B] + [num_tokens] * per_token)
+    T = num_tokens
+    sizes = [B + 1, B, T, T] if parents is None else [B + 1, B, T, T, T]
+    flat = torch.empty(sum(sizes), dtype=torch.int64, device=device)
+    qsl, lens, positions, slots, *mask = flat.split_with_sizes(sizes)
     packed = torch.empty((B, max_blocks), dtype=tables.dtype, device=device)
-    out = StepInputs(qsl, lens, positions, slots, packed, mask[0] if mask else None)
+    at = flat.data_ptr()
+    pointers = [None if t is None else t.data_ptr() for t in vectors]
     _lib.launch(device, what, _lib.load().ns_step_inputs,
                 tables.data_ptr(), R, W, max(tables.stride(0), W), tables.dtype is torch.int64,
-                _pointer(x["rows"]), _pointer(x["computed"]), _pointer(x["query_lens"]),
-                _pointer(x["new_blocks"]), _pointer(x["new_start"]), _pointer(x["held"]), N,
-                _pointer(x["parents"]), wide, B, num_tokens, block_size, max_blocks,
-                qsl.data_ptr(), lens.data_ptr(), positions.data_ptr(), slots.data_ptr(), packed.data_ptr(),
-                _pointer(out.tree_mask))
-    return out
+                *pointers[:6], N, pointers[6], wide, B, T, block_size, max_blocks,
+                at, at + 8 * (B + 1), at + 8 * (2 * B + 1), at + 8 * (2 * B + 1 + T), packed.data_ptr(),
+                at + 8 * (2 * B + 1 + 2 * T) if mask else None)
+    return StepInputs(qsl, lens, positions, slots, packed, mask[0] if mask else None)
 
 
 # Arrival counters of the key ranges, zero before and after every call, one
@@ -129,14 +142,15 @@ def step_inputs(tables: torch.Tensor, rows: torch.Tensor, computed: torch.Tensor
 _counters: dict[tuple[int, int], torch.Tensor] = {}
 
 
-def _arrivals(device: torch.device) -> torch.Tensor:
-    n = _lib.load().ns_paged_attention_tree_counters()
-    if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(n, dtype=torch.int32, device=device)
-    key = (device.index, torch._C._cuda_getCurrentRawStream(device.index))
-    c = _counters.get(key)
-    if c is None:
-        c = _counters[key] = torch.zeros(n, dtype=torch.int32, device=device)
+def _arrivals(device: torch.device, capturing: bool) -> torch.Tensor:
+    index = device.index
+    if not capturing:
+        c = _counters.get((index, torch._C._cuda_getCurrentRawStream(index)))
+        if c is not None:
+            return c
+    c = torch.zeros(_lib.load().ns_paged_attention_tree_counters(), dtype=torch.int32, device=device)
+    if not capturing:
+        _counters[index, torch._C._cuda_getCurrentRawStream(index)] = c
     return c
 
 
@@ -153,18 +167,19 @@ def paged_attention_tree(query: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     max_query_len, max_seq_len and query_start_loc_cpu are read, and shape the
     launch."""
     what = "paged_attention_tree"
-    if query.dim() != 3 or k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
-        raise ValueError(
-            f"expected query [T,Hq,D] and caches [NB,BS,Hkv,D], got "
-            f"{tuple(query.shape)}, {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
-    T, Hq, D = query.shape
-    num_blocks, block_size, heads, cache_dim = k_cache.shape
-    device, dtype, n = query.device, query.dtype, md.num_seqs
+    shape, cache = query.shape, k_cache.shape
+    if len(shape) != 3 or len(cache) != 4 or v_cache.shape != cache:
+        raise ValueError(f"expected query [T,Hq,D] and caches [NB,BS,Hkv,D], got {tuple(shape)}, {tuple(cache)}, "
+                         f"{tuple(v_cache.shape)}")
+    T, Hq, D = shape
+    num_blocks, block_size, heads, cache_dim = cache
+    index, dtype, n, longest = query.get_device(), query.dtype, md.num_seqs, md.max_seq_len
     if cache_dim != D:
         raise ValueError(f"head_dim mismatch: query {D}, cache {cache_dim}")
-    if not query.is_cuda or k_cache.device != device or v_cache.device != device:
+    if index < 0 or k_cache.get_device() != index or v_cache.get_device() != index:
         raise ValueError(f"{what} needs GPU tensors on one device (the HIP path has no CPU fallback)")
-    if dtype not in _lib.DTYPE_CODES or k_cache.dtype is not dtype or v_cache.dtype is not dtype:
+    code = _lib.DTYPE_CODES.get(dtype)
+    if code is None or k_cache.dtype is not dtype or v_cache.dtype is not dtype:
         raise TypeError(f"{what} takes float32, float16 or bfloat16 alike, got {dtype}, {k_cache.dtype}, {v_cache.dtype}")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("caches must be contiguous [num_blocks, block_size, num_kv_heads, head_dim]")
@@ -176,64 +191,67 @@ def paged_attention_tree(query: torch.Tensor, k_cache: torch.Tensor, v_cache: to
         raise ValueError(f"a sequence of a tree has at most {MAX_TREE_ROWS} rows, got max_query_len {md.max_query_len}")
     if md.tree_mask is None:
         raise ValueError(f"{what} needs md.tree_mask")
-    x, _ = _integers({"tree_mask": (md.tree_mask, T)}, device)
-    mask = x["tree_mask"]
+    mask = _vector(md.tree_mask, "tree_mask", T, index)
     if mask.dtype is not torch.int64:
         raise TypeError(f"tree_mask must be int64, got {mask.dtype}")
     q = query if query.is_contiguous() else query.contiguous()
     if T == 0 or n == 0:
         return torch.zeros_like(q)
-    bt = _index(md.block_tables, "block_tables", device)
+    bt = _index(md.block_tables, "block_tables", index)
     if bt.dim() != 2 or bt.shape[0] < n:
         raise ValueError(f"block_tables must be [num_seqs, max_blocks], got {tuple(bt.shape)}")
     width = bt.shape[1]
-    if width * block_size < md.max_seq_len:
-        raise ValueError(f"block_tables has {width} columns but max_seq_len={md.max_seq_len} needs "
-                         f"{-(-md.max_seq_len // block_size)}")
+    if width * block_size < longest:
+        raise ValueError(f"block_tables has {width} columns but max_seq_len={longest} needs {-(-longest // block_size)}")
     if width == 0:
         return torch.zeros_like(q)
-    if bt.stride(1) != 1 or bt.stride(0) < width:
+    stride = bt.stride()
+    if stride[1] != 1 or stride[0] < width:
         bt = bt.contiguous()
-    sl = _index(md.seq_lens, "seq_lens", device)
-    if sl.dim() != 1 or sl.shape[0] < n:
-        raise ValueError(f"seq_lens must hold at least {n} entries, got {tuple(sl.shape)}")
-    sl = sl.contiguous()
+        stride = bt.stride()
+    sl = _prefix(md.seq_lens, "seq_lens", n, index)
+    capturing = torch._C._cuda_isCurrentStreamCapturing()
     qsl_ptr, qsl64 = None, 0
     if md.query_start_loc is None:
         if T != n:
             raise ValueError("without query_start_loc there is one row per sequence")
-        out = torch.empty_like(q)
+        full = True
     else:
-        qsl = _index(md.query_start_loc, "query_start_loc", device)
-        if qsl.dim() != 1 or qsl.shape[0] < n + 1:
-            raise ValueError(f"query_start_loc must hold at least {n + 1} entries, got {tuple(qsl.shape)}")
-        qsl = qsl.contiguous()
+        qsl = _prefix(md.query_start_loc, "query_start_loc", n + 1, index)
         qsl_ptr, qsl64 = qsl.data_ptr(), qsl.dtype is torch.int64
         # Rows behind the last sequence are not written: zero unless the host's
         # offsets show that there are none, which they cannot for the replays of a
         # capture.
         host = md.query_start_loc_cpu
-        full = (host is not None and len(host) > n and host[0] == 0 and host[n] == T
-                and not torch.cuda.is_current_stream_capturing())
-        out = torch.empty_like(q) if full else torch.zeros_like(q)
+        full = host is not None and len(host) > n and host[0] == 0 and host[n] == T and not capturing
+    out = torch.empty_like(q) if full else torch.zeros_like(q)
     lib = _lib.load()
-    code = _lib.DTYPE_CODES[dtype]
     nbytes = lib.ns_paged_attention_tree_workspace_size(n, Hq, heads, D, block_size, md.max_query_len, T, code)
-    # The partial results live in a tensor of this call's.
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    counters = _arrivals(device) if nbytes else None
+    ws = counters = None
+    device = q.device
+    if nbytes:
+        # The partial results live in a tensor of this call's.
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        counters = _arrivals(device, capturing)
     _lib.launch(device, what, lib.ns_paged_attention_tree,
                 out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-                bt.data_ptr(), bt.stride(0), width, bt.dtype is torch.int64, sl.data_ptr(), sl.dtype is torch.int64,
-                qsl_ptr, qsl64, mask.data_ptr(), n, T, md.max_query_len, md.max_seq_len, Hq, heads, D, block_size,
+                bt.data_ptr(), stride[0], width, bt.dtype is torch.int64, sl.data_ptr(), sl.dtype is torch.int64,
+                qsl_ptr, qsl64, mask.data_ptr(), n, T, md.max_query_len, longest, Hq, heads, D, block_size,
                 num_blocks, float(scale), code, _pointer(counters), _pointer(ws), nbytes)
     return out
 
 
-def _index(t: torch.Tensor, name: str, device: torch.device) -> torch.Tensor:
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
+def _index(t: torch.Tensor, name: str, index: int) -> torch.Tensor:
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{index}")
     return t if t.dtype is torch.int64 or t.dtype is torch.int32 else t.to(torch.int64)
+
+
+def _prefix(t: torch.Tensor, name: str, least: int, index: int) -> torch.Tensor:
+    t = _index(t, name, index)
+    if t.dim() != 1 or t.shape[0] < least:
+        raise ValueError(f"{name} must hold at least {least} entries, got {tuple(t.shape)}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def commit_drafts(chosen: torch.Tensor, input_ids: torch.Tensor, parents: torch.Tensor,
@@ -251,20 +269,19 @@ def commit_drafts(chosen: torch.Tensor, input_ids: torch.Tensor, parents: torch.
     of a request's rows must differ; slots outside the cache are left alone.
     max_rows (at most 64): the most rows of a request; later ones take no part."""
     what = "commit_drafts"
-    device = chosen.device
-    if not chosen.is_cuda:
+    index = chosen.get_device()
+    if index < 0:
         raise ValueError(f"{what} needs GPU tensors (the HIP path has no CPU fallback)")
     if not 0 <= max_rows <= MAX_TREE_ROWS:
         raise ValueError(f"max_rows must be between 0 and {MAX_TREE_ROWS}, got {max_rows}")
     T = chosen.shape[0] if chosen.dim() else 0
-    x, wide = _integers({"chosen": (chosen, T), "input_ids": (input_ids, T), "parents": (parents, T)}, device)
-    one, _ = _integers({"slot_mapping": (slot_mapping, T)}, device)
-    slots = one["slot_mapping"]
     B = query_start_loc.shape[0] - 1 if query_start_loc.dim() else -1
     if B < 0:
         raise ValueError(f"query_start_loc must be [requests + 1], got {tuple(query_start_loc.shape)}")
-    one, _ = _integers({"query_start_loc": (query_start_loc, B + 1)}, device)
-    qsl = one["query_start_loc"]
+    rows, wide = _alike([_vector(chosen, "chosen", T, index), _vector(input_ids, "input_ids", T, index),
+                         _vector(parents, "parents", T, index)])
+    slots = _vector(slot_mapping, "slot_mapping", T, index)
+    qsl = _vector(query_start_loc, "query_start_loc", B + 1, index)
     caches = [*k_caches, *v_caches]
     num_slots = row_bytes = 0
     if caches:
@@ -272,17 +289,20 @@ def commit_drafts(chosen: torch.Tensor, input_ids: torch.Tensor, parents: torch.
         shape, dtype = first.shape, first.dtype
         if len(shape) != 4:
             raise ValueError(f"caches must be [num_blocks, block_size, kv_heads, head_dim], got {tuple(shape)}")
-        for c in caches:
-            if c.shape != shape or c.dtype is not dtype or c.device != device or not c.is_contiguous():
-                raise ValueError(f"caches must be contiguous tensors of one shape and dtype on {device}, got "
-                                 f"{c.dtype} {tuple(c.shape)} on {c.device} beside {dtype} {tuple(shape)}")
+        # Some tens of tensors in every call: checked without a Python loop.
+        if ([*map(_SIZE, caches)].count(shape) != len(caches) or {*map(_DTYPE, caches)} != {dtype}
+                or {*map(_DEVICE, caches)} != {index} or not all(map(_CONTIGUOUS, caches))):
+            raise ValueError(f"caches must be contiguous tensors of one shape and dtype on cuda:{index}, got "
+                             f"{sorted({(str(c.dtype), tuple(c.shape), str(c.device)) for c in caches})}")
         num_slots, row_bytes = shape[0] * shape[1], shape[2] * shape[3] * first.element_size()
+    device = chosen.device
     out = torch.empty(B * (1 + max_rows), dtype=torch.int64, device=device)
-    counts, tokens = out[:B], out[B:].view(B, max_rows)
-    pointers = (ctypes.c_void_p * len(caches))(*[c.data_ptr() for c in caches]) if num_slots and row_bytes else None
+    counts, tokens = out.split_with_sizes([B, B * max_rows])
+    held = len(caches) if num_slots and row_bytes else 0
+    pointers = array.array("Q", map(_ADDRESS, caches)) if held else None
+    at = out.data_ptr()
     _lib.launch(device, what, _lib.load().ns_commit_drafts,
-                counts.data_ptr(), tokens.data_ptr(), _pointer(x["chosen"]), _pointer(x["input_ids"]),
-                _pointer(x["parents"]), wide, qsl.data_ptr(), qsl.dtype is torch.int64, slots.data_ptr(),
-                slots.dtype is torch.int64, B, T, max_rows, pointers, 0 if pointers is None else len(caches),
-                num_slots, row_bytes)
-    return counts, tokens
+                at, at + 8 * B, rows[0].data_ptr(), rows[1].data_ptr(), rows[2].data_ptr(), wide,
+                qsl.data_ptr(), qsl.dtype is torch.int64, slots.data_ptr(), slots.dtype is torch.int64, B, T, max_rows,
+                pointers.buffer_info()[0] if held else None, held, num_slots, row_bytes)
+    return counts, tokens.view(B, max_rows)
