@@ -23,7 +23,7 @@ class BlockSpaceManager:
 
     A sequence is any object with a `block_table` list (and, for error
     messages, a `seq_id`).  Tables only grow in place; `free` gives the
-    sequence a new empty list.  `watermark` holds a fraction of the blocks
+    sequence a new empty list and `trim` a new shorter one.  `watermark` holds a fraction of the blocks
     back from `can_allocate` (admission of new requests), never from
     `allocate` (growth of admitted ones), so running sequences can still
     grow when admission stops (reference block_manager.py:64-86).
@@ -63,6 +63,19 @@ class BlockSpaceManager:
             self._held[b] = 1
             seq.block_table.append(b)
         return True
+
+    def trim(self, seq, num_tokens: int) -> None:
+        """Return the blocks of `seq` past those that hold [0, num_tokens), as after a
+        step whose drafted tokens were not all kept.  The shorter table is a new list:
+        who follows a table's growth (engine.DecodeGraphs) takes it for another."""
+        keep = self.blocks_for(num_tokens)
+        table = seq.block_table
+        if len(table) <= keep:
+            return
+        for b in reversed(table[keep:]):
+            self._held[b] = 0
+            self._free_stack.append(b)
+        seq.block_table = table[:keep]
 
     def free(self, seq) -> None:
         """Return every block of `seq` and give it an empty table."""

@@ -10,6 +10,9 @@ drawn as each request's SamplingParams say; the cache is 16 bits wide or held
 in 4 (`kv_bits`).  A step's metadata is built in scheduler order with int64 indices
 in one host-to-device copy (model_runner.py:52-147); a sequence yields a
 token only in the step that computes its last uncomputed token.
+
+With `draft_tokens` a decode step verifies drafted tokens (drafting.py, tree.py)
+and yields as many tokens of a request as the model confirms, and one.
 """
 
 from __future__ import annotations
@@ -23,10 +26,12 @@ import torch
 from .attention import AttentionMetadata, get_attention_backend
 from .block_manager import BlockSpaceManager
 from .capture import no_cycle_collection
+from .drafting import NgramDrafter, check_draft
 from .kv4 import Int4PagedKVCache
 from .kv_cache import PagedKVCache
 from .sampling import SamplerInputs, argmax_rows, sample_rows
 from .scheduling import RequestMetrics, SamplingParams, Scheduler, SchedulerConfig, Sequence, SeqState
+from .tree import MAX_TREE_ROWS, BlockTables, commit_drafts, step_inputs
 
 __all__ = ["DecodeGraphs", "LLMEngine", "ModelRunner", "RequestMetrics", "SamplingParams", "Scheduler",
            "SchedulerConfig", "Sequence", "SeqState", "summarize"]
@@ -52,6 +57,8 @@ class ModelRunner:
         self._host: torch.Tensor | None = None
         self._dev: torch.Tensor | None = None
         self._draw: SamplerInputs | None = None
+        self.max_model_len = max_model_len
+        self._tables: BlockTables | None = None
         self.graphs = DecodeGraphs(self, graph_batch_sizes, max_model_len) if use_graphs else None
 
     def _stage(self, chunks: list[list[int]]) -> list[torch.Tensor]:
@@ -124,6 +131,58 @@ class ModelRunner:
             chosen = argmax_rows(logits)
         tokens = chosen.tolist()  # the step's one device-to-host sync
         return list(zip(sample_seqs, tokens))
+
+    @torch.inference_mode()
+    def execute_drafted(self, seqs: list[Sequence], drafts: list[tuple[list[int], list[int]]]) -> list[list[int]]:
+        """One decode step of `seqs`, each with its last token and the (tokens, parents)
+        drafted behind it; returns every sequence's confirmed tokens, one at least.
+        The K and V of all but the last are in place; the sequences are left as
+        they are, with blocks for every row."""
+        if self._tables is None:
+            width = -(-(self.max_model_len + MAX_TREE_ROWS) // self.block_size)
+            self._tables = BlockTables(width, self.device)
+        ids, up, rows_of, ahead, lens = [], [], [], [], []
+        for seq, (tokens, parents) in zip(seqs, drafts):
+            depth = [0]
+            for p in parents:
+                depth.append(depth[p] + 1)
+            ids += [*seq.token_slice(seq.num_computed_tokens, seq.num_tokens), *tokens]
+            up += [-1, *parents]
+            rows_of += [seq] * len(depth)
+            ahead += depth
+            lens.append(len(depth))
+        computed = [s.num_computed_tokens for s in seqs]
+        longest = max(c + q for c, q in zip(computed, lens))
+        place, held, start, blocks = self._tables.place(seqs)
+        ids_t, up_t, place_t, computed_t, lens_t, held_t, start_t, blocks_t = self._stage(
+            [ids, up, place, computed, lens, held, start, blocks])
+        T = len(ids)
+        x = step_inputs(self._tables.tensor, place_t, computed_t, lens_t, T, self.block_size,
+                        -(-longest // self.block_size), blocks_t, start_t, held_t, up_t)
+        qsl = [0, *np.cumsum(lens).tolist()]
+        md = AttentionMetadata(
+            slot_mapping=x.slot_mapping, query_start_loc=x.query_start_loc, seq_lens=x.seq_lens,
+            block_tables=x.block_tables, max_query_len=max(lens), max_seq_len=longest, num_seqs=len(seqs),
+            num_tokens=T, is_decode_only=False, query_lens_cpu=lens,
+            seq_lens_cpu=[c + q for c, q in zip(computed, lens)], query_start_loc_cpu=qsl, tree_mask=x.tree_mask)
+        logits = self.model.compute_logits(self.model(ids_t, x.positions, self.kv_cache, md, self.attn_fn))
+        if any(s.sampling.draws for s in seqs):
+            if self._draw is None:
+                self._draw = SamplerInputs(self.device)
+            chosen = sample_rows(logits, **self._draw.stage(rows_of, ahead=ahead))
+        else:
+            chosen = argmax_rows(logits)
+        _, kept = commit_drafts(chosen, ids_t, up_t, x.query_start_loc, x.slot_mapping, self.kv_cache.k_cache,
+                                self.kv_cache.v_cache, max(lens))
+        return [[t for t in row if t >= 0] for row in kept.tolist()]
+
+    def trimmed(self, seq: Sequence) -> None:
+        if self._tables is not None:
+            self._tables.trimmed(seq)
+
+    def forget(self, seq: Sequence) -> None:
+        if self._tables is not None:
+            self._tables.forget(seq)
 
 
 class DecodeGraphs:
@@ -380,9 +439,17 @@ class LLMEngine:
     def __init__(self, model, num_blocks: int, block_size: int = 16, device="cuda",
                  scheduler_config: SchedulerConfig | None = None, eos_token_id: int | None = None,
                  max_model_len: int = 4096, use_graphs: bool = False, pipeline_decode: bool = True,
-                 kv_bits: int = 16) -> None:
+                 kv_bits: int = 16, draft_tokens: int = 0, drafter=None) -> None:
+        """draft_tokens: drafted tokens that a request's decode step verifies at most (0:
+        none), from `drafter` (drafting.NgramDrafter unless given).  A step in which some
+        prompt is computed, or nobody has a draft, runs as without; drafting steps run
+        eagerly, and no step is launched ahead of the tokens of the one before."""
         if kv_bits not in (4, 16):
             raise ValueError(f"kv_bits must be 16 or 4, got {kv_bits}")
+        if not 0 <= draft_tokens < MAX_TREE_ROWS:
+            raise ValueError(f"draft_tokens must be between 0 and {MAX_TREE_ROWS - 1}, got {draft_tokens}")
+        if draft_tokens and kv_bits == 4:
+            raise ValueError("draft_tokens need a 16-bit cache: attention over 4 bits takes no drafted trees")
         self.model = model.eval().requires_grad_(False)
         self.device = torch.device(device)
         dtype = model.model.embed_tokens.weight.dtype
@@ -399,7 +466,10 @@ class LLMEngine:
         self.finished: list[Sequence] = []
         # A graph-replayed decode step whose tokens have not been read back.
         self._inflight: GraphLaunch | None = None
-        self.pipeline_decode = pipeline_decode
+        self.pipeline_decode = pipeline_decode and not draft_tokens
+        self.draft_tokens = draft_tokens
+        self.drafter = drafter if drafter is not None or not draft_tokens else NgramDrafter()
+        self.num_drafted = self.num_accepted = 0  # drafted tokens verified, and kept
 
     def add_request(self, prompt_token_ids: list[int], sampling: SamplingParams | None = None) -> int:
         sampling = sampling or SamplingParams()
@@ -430,16 +500,66 @@ class LLMEngine:
         m.output_tokens = len(seq.output_token_ids)
         m.end = now
 
+    def _drafts(self, scheduled) -> list[tuple[list[int], list[int]]] | None:
+        """Every sequence's draft, with blocks for its rows; None without any."""
+        if not self.draft_tokens or any(q != 1 or s.pending_tokens != 1 for s, q in scheduled):
+            return None
+        # The step's token budget in equal parts.
+        limit = min(self.draft_tokens, self.scheduler.cfg.max_num_batched_tokens // len(scheduled) - 1)
+        drafts, some = [], False
+        for seq, _ in scheduled:
+            # The last token of a chain and the model's choice after it are the most that a request may add.
+            depth = seq.sampling.max_new_tokens - len(seq.output_token_ids) - 1
+            tokens, parents = self.drafter.draft(seq, limit, depth) if limit > 0 and depth > 0 else ([], [])
+            check_draft(tokens, parents, limit, depth, self.model.config.vocab_size)
+            rows = seq.num_tokens + len(tokens)
+            if tokens and not self.block_manager.allocate(seq, rows):
+                # The blocks it has; rows that name a parent come after it.
+                fit = len(seq.block_table) * self.block_manager.block_size - seq.num_tokens
+                tokens, parents = tokens[:fit], parents[:fit]
+            some = some or bool(tokens)
+            drafts.append((tokens, parents))
+        return drafts if some else None
+
+    def _run_drafted(self, scheduled, drafts) -> list[Sequence]:
+        seqs = [s for s, _ in scheduled]
+        kept = self.runner.execute_drafted(seqs, drafts)
+        now = time.perf_counter()
+        for seq, tokens, (draft, _) in zip(seqs, kept, drafts):
+            self.num_drafted += len(draft)
+            self.num_accepted += len(tokens) - 1
+            for t in tokens:
+                seq.mark_computed(1)
+                seq.output_token_ids.append(t)
+                if seq.check_done(self.eos_token_id):
+                    break
+            self._record(seq, now)
+            self.block_manager.trim(seq, seq.num_tokens)
+            self.runner.trimmed(seq)
+        return self._finish()
+
+    def _finish(self) -> list[Sequence]:
+        done = self.scheduler.free_finished()
+        if self.draft_tokens:
+            for seq in done:
+                self.runner.forget(seq)
+                forget = getattr(self.drafter, "forget", None)
+                if forget is not None:
+                    forget(seq)
+        self.finished.extend(done)
+        return done
+
     def _run(self, scheduled) -> list[Sequence]:
+        drafts = self._drafts(scheduled)
+        if drafts is not None:
+            return self._run_drafted(scheduled, drafts)
         results = self.runner.execute(scheduled)
         now = time.perf_counter()
         for seq, tok in results:
             seq.output_token_ids.append(tok)
             self._record(seq, now)
             seq.check_done(self.eos_token_id)
-        done = self.scheduler.free_finished()
-        self.finished.extend(done)
-        return done
+        return self._finish()
 
     def step(self) -> list[Sequence]:
         """One scheduling step.  Decode steps that replay a graph are pipelined:

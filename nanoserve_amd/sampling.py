@@ -150,9 +150,10 @@ class SamplerInputs:
         self._np = self._host.numpy()
         self._dev = torch.zeros(5, rows, dtype=torch.float32, device=self.device)
 
-    def stage(self, seqs, non_blocking: bool = False) -> dict:
+    def stage(self, seqs, non_blocking: bool = False, ahead: list[int] | None = None) -> dict:
         """sample_rows' arguments for the next token of each sequence
-        (scheduling.Sequence).  With non_blocking the host buffer is still being
+        (scheduling.Sequence), or for the one `ahead` tokens behind it (a row of a
+        drafted tree, by its depth).  With non_blocking the host buffer is still being
         read on return: a caller that stages again before the copy is done
         needs another object."""
         n = len(seqs)
@@ -160,7 +161,7 @@ class SamplerInputs:
             self._reserve(2 * n)
         h = self._np
         p = [s.sampling for s in seqs]
-        h[0, :n] = [s.uniform(len(s.output_token_ids)) for s in seqs]
+        h[0, :n] = [s.uniform(len(s.output_token_ids) + a) for s, a in zip(seqs, ahead or [0] * n)]
         h[1, :n] = [x.temperature for x in p]
         h[2, :n] = [x.top_p for x in p]
         h[3, :n] = [x.min_p for x in p]

@@ -14,6 +14,7 @@ its depth.
                            an md with a tree_mask)
     commit_drafts          the rows that the model's choices confirm, and their K
                            and V moved to the places of the tokens they became
+    BlockTables            the tables that step_inputs reads and extends
 
 Each is one launch on the current stream and reads the device's lengths, so a
 captured graph serves other lengths, trees and choices on every replay.
@@ -133,6 +134,60 @@ def step_inputs(tables: torch.Tensor, rows: torch.Tensor, computed: torch.Tensor
                 at, at + 8 * (B + 1), at + 8 * (2 * B + 1), at + 8 * (2 * B + 1 + T), packed.data_ptr(),
                 at + 8 * (2 * B + 1 + 2 * T) if mask else None)
     return StepInputs(qsl, lens, positions, slots, packed, mask[0] if mask else None)
+
+
+class BlockTables:
+    """The requests' block ids on the device, one row each, for step_inputs.
+
+    `place` names a batch's rows and what the step has to append to them: a
+    request's table grows in place (BlockSpaceManager.allocate), so a row that
+    holds the same list needs only the blocks added since.  A request that has no
+    row gets a free one, or that of a request outside the batch."""
+
+    def __init__(self, width: int, device, rows: int = 64) -> None:
+        self.width = width
+        self.device = device
+        self.tensor = torch.zeros(rows, width, dtype=torch.int64, device=device)
+        # Per request: its row, the list written there (held, so that its identity is
+        # its own) and how many of its entries.
+        self._rows: dict[int, tuple[int, list[int], int]] = {}
+        self._free = list(range(rows - 1, -1, -1))
+
+    def forget(self, seq) -> None:
+        held = self._rows.pop(seq.seq_id, None)
+        if held is not None:
+            self._free.append(held[0])
+
+    def trimmed(self, seq) -> None:
+        """`seq` has a shorter table of the same blocks (BlockSpaceManager.trim)."""
+        held = self._rows.get(seq.seq_id)
+        if held is not None:
+            self._rows[seq.seq_id] = (held[0], seq.block_table, min(held[2], len(seq.block_table)))
+
+    def place(self, seqs) -> tuple[list[int], list[int], list[int], list[int]]:
+        """(rows, held, new_start, new_blocks) of the batch, as step_inputs takes them.  Counts on that call."""
+        missing = sum(s.seq_id not in self._rows for s in seqs)
+        if missing > len(self._free):
+            here = {s.seq_id for s in seqs}
+            for i in [i for i in self._rows if i not in here][:missing - len(self._free)]:
+                self._free.append(self._rows.pop(i)[0])
+        if missing > len(self._free):
+            have = self.tensor.shape[0]
+            more = max(have, missing)
+            self.tensor = torch.cat((self.tensor, torch.zeros(more, self.width, dtype=torch.int64, device=self.device)))
+            self._free += range(have + more - 1, have - 1, -1)
+        rows, held, start, blocks = [], [], [0], []
+        for s in seqs:
+            table = s.block_table
+            row, old, n = self._rows.get(s.seq_id) or (self._free.pop(), None, 0)
+            if old is not table:
+                n = 0
+            rows.append(row)
+            held.append(n)
+            blocks += table[n:]
+            start.append(len(blocks))
+            self._rows[s.seq_id] = (row, table, len(table))
+        return rows, held, start, blocks
 
 
 # Arrival counters of the key ranges, zero before and after every call, one
