@@ -33,7 +33,11 @@ struct TreeParams {
   int64_t num_tokens, num_blocks;
   int64_t max_ctx;         // keys a sequence may have: max_seq_len, within the table
   float scale;
-  // Matrix-core kernel.
+  // Matrix-core kernel.  key / block_size is mulhi(key, block_mul) >> block_shift, c / group
+  // is c times by_group.
+  uint32_t block_mul;
+  int block_shift;
+  float by_group;
   float* partials;         // two slots a workgroup
   int* counters;           // one a workgroup, zero before and after
 };
@@ -274,12 +278,33 @@ __device__ __forceinline__ int v_swizzle(int key) {
 }
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// x / y for uniform 0 <= x < 2^30, y > 0: in float32, put right.
-__device__ __forceinline__ int quotient(int x, int y) {
-  int q = uniform(static_cast<int>(static_cast<float>(x) * __builtin_amdgcn_rcpf(static_cast<float>(y))));
-  while (x - q * y < 0) --q;
-  while (x - q * y >= y) ++q;
-  return q;
+// Division by a uniform y > 0 of uniform 0 <= x < 2^30 with quotients below 2^20: by the
+// reciprocal in float32, which is one off at most, and put right.
+struct Divisor {
+  int y;
+  float r;
+  __device__ __forceinline__ explicit Divisor(int y_) : y(y_), r(__builtin_amdgcn_rcpf(static_cast<float>(y_))) {}
+  __device__ __forceinline__ int of(int x) const {
+    int q = uniform(static_cast<int>(static_cast<float>(x) * r));
+    const int rest = x - q * y;
+    q -= rest < 0;
+    q += rest >= y;
+    return q;
+  }
+};
+
+// f over the lanes up to each, for values that f leaves as they are with a zero: shifts
+// within the rows of 16 lanes, then a row's last lane to the row behind it and lane 31
+// to the upper half.
+template <class F>
+__device__ __forceinline__ int wave_scan(int x, F f) {
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false));  // row_shr:1
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false));
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false));
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false));
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false));  // row_bcast:15 into rows 1 and 3
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false));  // row_bcast:31 into rows 2 and 3
+  return x;
 }
 
 // The sequences of a launch along the line of work, from the device's lengths: where
@@ -325,16 +350,10 @@ struct Line {
         sum += x[i];
       }
     }
-    int y = sum;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int z = __shfl_up(y, off);
-      if (lane >= off) y += z;
-      m = max(m, __shfl_xor(m, off));
-    }
+    const int y = wave_scan(sum, [](int a, int b) { return a + b; });
     int before = y - sum;
     total = __builtin_amdgcn_readlane(y, 63);
-    most = uniform(m);
+    most = __builtin_amdgcn_readlane(wave_scan(m, [](int a, int b) { return max(a, b); }), 63);
     if (!alone) {
       if (lane == 0) {
         h.sums[w] = total;
@@ -400,13 +419,15 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
   const Line<C> line(p, held);
   // Shares: one a workgroup, but none too small, and no group in more than kMostRanges of them.
   const int grid = static_cast<int>(gridDim.x);
-  int share = quotient(line.total + grid - 1, grid);
+  int share = Divisor(grid).of(line.total + grid - 1);
+  if (static_cast<uint32_t>(share) * grid < static_cast<uint32_t>(line.total)) ++share;
   const int least = line.most / (kMostRanges - 2) + 1;
   share = share > least ? share : least;
   share = share > kLeastRounds * KG ? share : kLeastRounds * KG;
   // Neighbouring shares, which read the same keys where a sequence has several
   // groups of columns, go to one XCD (workgroups go to the eight in turn).
-  const int shares = quotient(line.total + share - 1, share);
+  const Divisor by_share(share);
+  const int shares = by_share.of(line.total + share - 1);
   const int per_xcd = (shares + 7) >> 3;
   const int k = static_cast<int>(blockIdx.x & 7) * per_xcd + static_cast<int>(blockIdx.x >> 3);
   if (static_cast<int>(blockIdx.x >> 3) >= per_xcd || k >= shares) return;
@@ -441,7 +462,7 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
   int s = line.find(place);
   int start, row0, ql, len;
   line.get(s, start, row0, ql, len);
-  int gi = quotient(place - start, line.weight(len));
+  int gi = Divisor(line.weight(len)).of(place - start);
   for (;; ++gi) {
     while (gi >= line.groups(ql)) {
       if (++s >= p.num_seqs) return;
@@ -452,19 +473,20 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
     // the chunks c0 .. c1 of this one.
     const int n = (len + 31) >> 5;
     const int gs = start + gi * line.weight(len);
-    const int a = quotient(gs + kHalf - 1, share);
+    const int a = by_share.of(gs + kHalf - 1);
     if (a > k) return;
     const int e = (n + KG - 1) / KG * KG - kHalf - 1;
-    int b = n > kLeastRounds * KG ? quotient(gs + e, share) : a;
+    int b = n > kLeastRounds * KG ? by_share.of(gs + e) : a;
     b = b > a ? b : a;
     if (k > b) continue;
     auto cut = [&](int kk) { return (kk * share - gs + kHalf) / KG * KG; };
     const int c0 = k == a ? 0 : cut(k), c1 = k == b ? n : cut(k + 1);
     const int base = len - ql;
     const int cols = (ql < kRows ? ql : kRows) * G, cbs = (cols + COLS - 1) / COLS;
-    const int kvh = uniform(gi / cbs), cb = gi - kvh * cbs;
+    const int kvh = Divisor(cbs).of(gi), cb = gi - kvh * cbs;
     const int col0 = cb * COLS + cw * (16 * NT);  // this wave's first column
     const int t1 = 32 * c1 < len ? 32 * c1 : len;
+    const int whole = base < t1 ? base : t1;   // keys below are seen by every column
     const int steps = (c1 - c0 + KG - 1) / KG;  // of the workgroup
     const int mine = c1 - c0 > kg ? (c1 - c0 - kg + KG - 1) / KG : 0;
 
@@ -478,21 +500,28 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
       const int key = 32 * (c0 + kg + KG * (step + (of >> 1))) + 16 * (of & 1);
       return key < t1 ? key : (t1 - 1) & ~15;  // a tile past the range repeats the last
     };
+    auto entry_of = [&](int key) {
+      return static_cast<int>(__umulhi(static_cast<uint32_t>(key), p.block_mul) >> p.block_shift);
+    };
     auto block_of = [&](int key) {
-      return load_index(p.bt, static_cast<int64_t>(p.first_seq + s) * p.bt_stride + key / p.block_size, p.bt64);
+      return load_index(p.bt, static_cast<int64_t>(p.first_seq + s) * p.bt_stride + entry_of(key), p.bt64);
     };
     auto set_window = [&](int key, int64_t blk) {
       if (blk < 0 || blk >= p.num_blocks) {
         bad = 1;
         blk = 0;
       }
-      const uint64_t at = ((static_cast<uint64_t>(blk) * p.block_size + key % p.block_size) * Hkv + kvh) * (D * 2);
+      const int in = key - entry_of(key) * p.block_size;
+      const uint64_t at = ((static_cast<uint64_t>(blk) * p.block_size + in) * Hkv + kvh) * (D * 2);
       at_lo = static_cast<uint32_t>(at);
       at_hi = static_cast<uint32_t>(at >> 32);
     };
     const int first_key = mine > 0 ? key_of(0) : 0;
     const int64_t first_block = mine > 0 ? block_of(first_key) : 0;
 
+    // Column c is query head c % G of row c / G (c < 2^16: the quotient's error in
+    // float32 is far below half of 1 / G).
+    auto row_in = [&](int c) { return static_cast<int>((static_cast<float>(c) + 0.5f) * p.by_group); };
     // The columns' query rows (a column past the last repeats it), on their way
     // together with the block ids.
     auto row_of = [&](int i, int& head) {
@@ -500,8 +529,9 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
       asm volatile("" : "+v"(c));  // worked out where it is needed, not held in registers over the loop
       c += col0 + 16 * i;
       c = c < cols ? c : cols - 1;
-      head = kvh * G + c % G;
-      return static_cast<int64_t>(row0) + c / G;
+      const int j = row_in(c);
+      head = kvh * G + c - j * G;
+      return static_cast<int64_t>(row0) + j;
     };
     V8 q[NT][NC];
 #pragma unroll
@@ -568,40 +598,46 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i)
       if (i < mine) issue(i);
+    const int count = WC == 1 ? mine : steps;
+    const bool idle = WC > 1 && col0 >= cols;  // no columns: this wave loads for the others
+    // Chunk `step` has come (to all of the key group's waves, and none reads the one before it).
+    auto advance = [&](int step) {
+      const int younger = mine - 1 - step;
+      if (WC == 1) {
+        if (younger >= 1) vector_wait<C::LOADS>();
+        else vector_wait<0>();
+      } else {
+        if (R > 3 && younger >= 2) vector_barrier<2 * C::LOADS>();
+        else if (R > 2 && younger >= 1) vector_barrier<C::LOADS>();
+        else vector_barrier<0>();
+        if (step + R - 1 < mine) issue(step + R - 1);
+      }
+    };
+    u32x4 kraw[2][NC];
+    auto read_keys = [&](int step) {
+      const uint32_t ka = lds_addr(ring + (step % R) * C::SLOT_B);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        kraw[0][c] = ds_read_b128_at<0>(ka + kread[c]);
+        kraw[1][c] = ds_read_b128_at<16 * D * 2>(ka + kread[c]);
+      }
+    };
+    int step = 0;
+    const int work = idle ? 0 : count;  // a key group without a chunk in the last step sees none of its keys
+    if (count > 0) advance(0);
+    if (work > 0) read_keys(0);
     // The inner loop holds the common chunk and nothing that changes the accumulators
     // in another way (a branch that did would cost a second set of their registers):
-    // it is left before a chunk that moves a reference, which is then taken again.
-    const int count = WC == 1 ? mine : steps;
-    const bool idle = col0 >= cols;  // no columns: this wave loads for the others
-    int step = 0, there = 0;
+    // it is left at a chunk that moves a reference, whose scores are then taken again.
+    // K of the next chunk is read beside the products of V, V beside the softmax.
     uint32_t odd = 0;  // bit i: the chunk of step count - 1 - i is added one key at a time
-    while (step < count) {
+    while (step < work) {
       float top[NT];
       bool past = false;
-      for (; step < count; ++step) {
-        if (WC == 1) {
-          if (step + 1 < mine) vector_wait<C::LOADS>();
-          else vector_wait<0>();
-        } else if (there == step) {
-          // The key group's waves have all of chunk `step`, and none reads the one before.
-          const int younger = mine - 1 - step;
-          if (R > 3 && younger >= 2) vector_barrier<2 * C::LOADS>();
-          else if (R > 2 && younger >= 1) vector_barrier<C::LOADS>();
-          else vector_barrier<0>();
-          there = step + 1;
-          if (step + R - 1 < mine) issue(step + R - 1);
-        }
-        if (WC > 1 && (step >= mine || idle)) continue;
+      for (; step < work; ++step) {
         const int tb = 32 * (c0 + kg + KG * step);
-        const char* kt = ring + (step % R) * C::SLOT_B;
-        u32x4 kraw[2][NC];
         u32x2 vraw[NN][2];
-        const uint32_t ka = lds_addr(kt), va = ka + C::TILE_B + vread;
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          kraw[0][c] = ds_read_b128_at<0>(ka + kread[c]);
-          kraw[1][c] = ds_read_b128_at<16 * D * 2>(ka + kread[c]);
-        }
+        const uint32_t va = lds_addr(ring + (step % R) * C::SLOT_B) + C::TILE_B + vread;
         lds_wait_all();
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -625,12 +661,12 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
           vraw[j][0] = ds_read_tr16_b64_at<0>(at);
           vraw[j][1] = ds_read_tr16_b64_at<16 * D * 2>(at);
         }
-        const bool tail = tb + 32 > base;  // some keys are not seen by every column
+        const bool tail = tb + 32 > whole;  // some keys are not seen by every column
         if (tail) {
 #pragma unroll
           for (int i = 0; i < NT; ++i) {
             int head;
-            const uint32_t seen = seen_of(static_cast<uint64_t>(p.mask[row_of(i, head)]), tb, base, len) >> (4 * g);
+            const uint32_t seen = seen_of(static_cast<uint64_t>(p.mask[row_of(i, head)]), tb, base, t1) >> (4 * g);
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -658,10 +694,10 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
         }
         if (__builtin_expect(past, 0)) break;
         if (tail) {
-          // V of a key past the end is taken as zero.  A chunk with an element of V that
+          // V of a key past the range is taken as zero.  A chunk with an element of V that
           // is not finite is left for later (add_keys), so that it reaches only the rows
           // that see it.
-          const int left = len - tb;
+          const int left = t1 - tb;
           int wild = 0;
 #pragma unroll
           for (int j = 0; j < NN; ++j)
@@ -684,6 +720,10 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
         }
         // The chunk is in registers: the next but one takes its place.
         if (WC == 1 && step + R < mine) issue(step + R);
+        if (step + 1 < work) {
+          advance(step + 1);
+          read_keys(step + 1);
+        }
         V8 pt[NT];
 #pragma unroll
         for (int i = 0; i < NT; ++i)
@@ -715,6 +755,9 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
       }
     }
 
+    if (WC > 1)
+      while (++step < count) advance(step);  // idle: all chunks but the first
+
     // What follows a range's chunks works its places out anew from here, or they would
     // be held in registers over the loop.
     int tid2 = tid;
@@ -727,12 +770,12 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
     auto add_keys = [&](int i, int tb, float reference, float factor, float* to) {
       int head;
       const int64_t row = row_of(i, head);
-      const uint32_t seen = seen_of(static_cast<uint64_t>(p.mask[row]), tb, base, len);
+      const uint32_t seen = seen_of(static_cast<uint64_t>(p.mask[row]), tb, base, t1);
       const T* qr = reinterpret_cast<const T*>(p.query) + (row * p.num_heads + head) * D + g2 * (D / 4);
-      for (int key = tb; key < tb + 32 && key < len; ++key) {
+      for (int key = tb; key < tb + 32 && key < t1; ++key) {
         const int64_t blk = block_of(key);
         if (blk < 0 || blk >= p.num_blocks) break;  // the outputs are NaN
-        const int64_t at = ((blk * p.block_size + key % p.block_size) * Hkv + kvh) * D;
+        const int64_t at = ((blk * p.block_size + key - entry_of(key) * p.block_size) * Hkv + kvh) * D;
         const T* kr = reinterpret_cast<const T*>(p.k_cache) + at + g2 * (D / 4);
         const T* vr = reinterpret_cast<const T*>(p.v_cache) + at + 4 * g2;
         float x = 0.f;
@@ -777,7 +820,8 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
     auto write = [&](int i, int j, floatx4 o, float inv) {
       const int c = col0 + 16 * i + c2;
       if (c >= cols) return;
-      const int64_t at = ((static_cast<int64_t>(row0) + c / G) * p.num_heads + kvh * G + c % G) * D + 16 * j + 4 * g2;
+      const int r0 = row_in(c);
+      const int64_t at = ((static_cast<int64_t>(row0) + r0) * p.num_heads + kvh * G + c - r0 * G) * D + 16 * j + 4 * g2;
       typename DT::vec4 v;
 #pragma unroll
       for (int r = 0; r < 4; ++r) v[r] = static_cast<T>(o[r] * inv);
@@ -1068,6 +1112,12 @@ extern "C" int ns_paged_attention_tree(void* out, const void* query,
   const int64_t held = block_table_width > (int64_t{1} << 30) ? max_seq_len : block_table_width * block_size;
   p.max_ctx = max_seq_len < held ? max_seq_len : held;
   p.scale = scale;
+  // For keys below 2^31 and 2^(l - 1) < block_size <= 2^l: 2^(31 + l) / block_size, rounded up.
+  int l = 1;
+  while ((int64_t{1} << l) < block_size) ++l;
+  p.block_mul = static_cast<uint32_t>(((uint64_t{1} << (31 + l)) + block_size - 1) / block_size);
+  p.block_shift = l - 1;
+  p.by_group = 1.f / static_cast<float>(group);
   p.partials = static_cast<float*>(workspace);
   p.counters = counters;
   const hipStream_t st = static_cast<hipStream_t>(stream);
