@@ -643,16 +643,16 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int c = 0; c < NC; ++c) lds_ready(kraw[h][c]);
+        // Products that follow one another add to different sums.
         floatx4 sacc[NT][2];
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
+        for (int c = 0; c < NC; ++c)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            sacc[i][h] = floatx4{0.f, 0.f, 0.f, 0.f};
+          for (int i = 0; i < NT; ++i)
 #pragma unroll
-            for (int c = 0; c < NC; ++c)
-              sacc[i][h] = mfma16x16x32(DT{}, __builtin_bit_cast(V8, kraw[h][c]), q[i][c], sacc[i][h]);
-          }
+            for (int h = 0; h < 2; ++h)
+              sacc[i][h] = mfma16x16x32(DT{}, __builtin_bit_cast(V8, kraw[h][c]), q[i][c],
+                                        c == 0 ? floatx4{0.f, 0.f, 0.f, 0.f} : sacc[i][h]);
         __builtin_amdgcn_sched_barrier(0);
         // Unit 2 j of a row: the swizzle touches bits above the lowest, and so is an exclusive or of the address.
 #pragma unroll
