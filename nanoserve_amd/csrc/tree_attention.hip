@@ -245,8 +245,10 @@ struct Cfg {
   static constexpr int PART = COLS * (D + 2);   // words of a slot: units, then (maximum, sum) of every column
   // The key groups meet JOIN tiles of a wave at a time, as many as fit the ring.
   static constexpr int JOIN = RING / (W * NN * UNIT * 4) < NT ? RING / (W * NN * UNIT * 4) : NT;
+  static constexpr bool KEEP = NT <= 2;         // a range's units stay in registers for the join of the ranges
   static constexpr int OWN = (NT * NN + KG - 1) / KG;  // units that a wave joins the ranges of
   static_assert(R >= 2 && JOIN >= 1 && NT % JOIN == 0, "chunks in flight; a tile of every wave fits the ring");
+  static_assert(JOIN == NT || JOIN * NN % KG == 0, "a wave's units of the joins are its units of all");
   static_assert(2 * kMostRanges * COLS * 4 <= RING, "the ranges' maxima and sums fit the ring");
   static_assert(kGroupCost >= KG / 2, "a group's workgroups begin within its stretch of the line");
   static_assert(kLeastRounds >= 1, "a group has one cut at most that moves to its start or end");
@@ -265,6 +267,14 @@ template <int N>
 __device__ __forceinline__ void vector_barrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
+// 16 bytes of each lane from base + off (base uniform) to LDS address to + 16 lane.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void load_lds16(const void* base, uint32_t off, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(to)
+               : "memory", "m0");
+}
+#pragma clang diagnostic pop
 __device__ __forceinline__ float ld_sc1(__amdgpu_buffer_rsrc_t r, int off) {
   return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, kSc1));
 }
@@ -436,7 +446,7 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
   const float scale = __uint_as_float(__builtin_amdgcn_readfirstlane(
       __float_as_uint(fmaxf(fabsf(p.scale) * 1.4426950408889634f, 1.1754944e-38f))));
   const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;  // a negative scale turns the query around, exactly
-  char* ring = smem + kg * (R * C::SLOT_B);
+  const uint32_t ring = lds_addr(smem) + kg * (R * C::SLOT_B);
   const uint32_t stride = static_cast<uint32_t>(Hkv) * D * 2;  // bytes between a block's token rows
 
   // A lane's part of a load: its unit of its row, where it lies in memory.
@@ -566,7 +576,7 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
         const int key = key_of(step);
         set_window(key, block_of(key));
       }
-      char* to = ring + (step % R) * C::SLOT_B;
+      const uint32_t to = ring + (static_cast<uint32_t>(step) % R) * C::SLOT_B;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         if (WC == 4 && h != cw >> 1) continue;
@@ -579,14 +589,14 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
           const char* vp = p.v_cache + at;
 #pragma unroll
           for (int u = 0; u < LPT; ++u) {
-            dma_lds16_off(kp + u * KPI * stride, koff[u % NK], to + (h * LPT + u) * 1024);
-            dma_lds16_off(vp + u * KPI * stride, voff[u % NK], to + C::TILE_B + (h * LPT + u) * 1024);
+            load_lds16(kp + u * KPI * stride, koff[u % NK], to + (h * LPT + u) * 1024);
+            load_lds16(vp + u * KPI * stride, voff[u % NK], to + C::TILE_B + (h * LPT + u) * 1024);
           }
         } else {
           const char* from_cache = (cw & 1 ? p.v_cache : p.k_cache) + at;
-          char* part = to + (cw & 1) * C::TILE_B + h * LPT * 1024;
+          const uint32_t part = to + (cw & 1) * C::TILE_B + h * LPT * 1024;
 #pragma unroll
-          for (int u = 0; u < LPT; ++u) dma_lds16_off(from_cache + u * KPI * stride, koff[u % NK], part + u * 1024);
+          for (int u = 0; u < LPT; ++u) load_lds16(from_cache + u * KPI * stride, koff[u % NK], part + u * 1024);
         }
       }
     };
@@ -615,7 +625,7 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
     };
     u32x4 kraw[2][NC];
     auto read_keys = [&](int step) {
-      const uint32_t ka = lds_addr(ring + (step % R) * C::SLOT_B);
+      const uint32_t ka = ring + (static_cast<uint32_t>(step) % R) * C::SLOT_B;
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         kraw[0][c] = ds_read_b128_at<0>(ka + kread[c]);
@@ -637,7 +647,7 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
       for (; step < work; ++step) {
         const int tb = 32 * (c0 + kg + KG * step);
         u32x2 vraw[NN][2];
-        const uint32_t va = lds_addr(ring + (step % R) * C::SLOT_B) + C::TILE_B + vread;
+        const uint32_t va = ring + (static_cast<uint32_t>(step) % R) * C::SLOT_B + C::TILE_B + vread;
         lds_wait_all();
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -732,6 +742,8 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
 #pragma unroll
             for (int r = 0; r < 4; ++r)
               pt[i][4 * h + r] = static_cast<T>(fast_exp2(__builtin_fmaf(sacc[i][h][r], scale, -m[i])));
+        // Two waves share a SIMD: the one whose products are due goes before the other's softmax.
+        if (WC > 1) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int i = 0; i < NT; ++i) l[i] = mfma16x16x32(DT{}, ones, pt[i], l[i]);
 #pragma unroll
@@ -740,6 +752,7 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
 #pragma unroll
           for (int i = 0; i < NT; ++i) acc[i][j] = mfma16x16x32(DT{}, v, pt[i], acc[i][j]);
         }
+        if (WC > 1) __builtin_amdgcn_s_setprio(0);
       }
       if (past) {
 #pragma unroll
@@ -760,9 +773,9 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
 
     // What follows a range's chunks works its places out anew from here, or they would
     // be held in registers over the loop.
-    int tid2 = tid;
-    asm volatile("" : "+v"(tid2));
-    const int lane2 = tid2 & 63, g2 = lane2 >> 4, c2 = lane2 & 15;
+    int tid2 = tid, w2 = w;
+    asm volatile("" : "+v"(tid2), "+s"(w2));
+    const int lane2 = tid2 & 63, g2 = lane2 >> 4, c2 = lane2 & 15, kg2 = w2 / WC, cw2 = w2 % WC;
 
     // Adds the rows of V of a chunk to this lane's outputs of column c2 of tile i, at `to`
     // (a unit's floats apart), for the keys that the column sees; their weights, which
@@ -796,13 +809,13 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
     if (g2 == 0) {
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        maxima[kg][(cw * NT + i) * 16 + c2] = m[i];
-        sums[kg][(cw * NT + i) * 16 + c2] = l[i][0];
+        maxima[kg2][(cw2 * NT + i) * 16 + c2] = m[i];
+        sums[kg2][(cw2 * NT + i) * 16 + c2] = l[i][0];
       }
     }
     {
       const int wave_bad = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
-      if (lane2 == 0) bads[w] = wave_bad;
+      if (lane2 == 0) bads[w2] = wave_bad;
     }
     __syncthreads();
     int bad_any = 0;
@@ -830,9 +843,10 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
     auto inverse = [&](float sum) { return sum > 0.f || sum != sum ? 1.f / sum : 0.f; };  // no key: zero; a NaN stays one
     float* buf = reinterpret_cast<float*>(smem);
     float join_top[NT], join_sum[NT];
+    floatx4 own[C::OWN] = {};  // this range's units, for the join of the ranges
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      const int col = (cw * NT + i) * 16 + c2;
+      const int col = (cw2 * NT + i) * 16 + c2;
       join_top[i] = kNoScore;
 #pragma unroll
       for (int kk = 0; kk < KG; ++kk) join_top[i] = fmaxf(join_top[i], maxima[kk][col]);
@@ -841,7 +855,7 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
       for (int kk = 0; kk < KG; ++kk)
         join_sum[i] = __builtin_fmaf(sums[kk][col], fast_exp2(maxima[kk][col] - join_top[i]), join_sum[i]);
       if (bad_any) join_sum[i] = NAN;
-      if (split && kg == 0 && g2 == 0)
+      if (split && kg2 == 0 && g2 == 0)
         __builtin_amdgcn_raw_buffer_store_b64(
             u32x2{__builtin_bit_cast(uint32_t, join_top[i]), __builtin_bit_cast(uint32_t, join_sum[i])}, pr,
             4 * (part_of(k) + COLS * D + 2 * col), 0, kSc1);
@@ -849,7 +863,7 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
 #pragma unroll
     for (int n0 = 0; n0 < NT; n0 += C::JOIN) {
       if (n0 > 0) __syncthreads();
-      float* mine_o = buf + w * (C::JOIN * NN * C::UNIT) + 4 * lane2;
+      float* mine_o = buf + w2 * (C::JOIN * NN * C::UNIT) + 4 * lane2;
 #pragma unroll
       for (int i = n0; i < n0 + C::JOIN; ++i) {
         const float f = fast_exp2(m[i] - join_top[i]);
@@ -858,29 +872,30 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
           *reinterpret_cast<floatx4*>(mine_o + ((i - n0) * NN + j) * C::UNIT) = acc[i][j] * f;
         if (__builtin_expect(odd != 0, 0))
           for (int left = static_cast<int>(odd); left != 0; left &= left - 1)
-            add_keys(i, 32 * (c0 + kg + KG * (count - 1 - __builtin_ctz(left))), m[i], f,
+            add_keys(i, 32 * (c0 + kg2 + KG * (count - 1 - __builtin_ctz(left))), m[i], f,
                      mine_o + (i - n0) * NN * C::UNIT);
       }
       __syncthreads();
       // Unit u KG + kg of the tiles is this wave's to add up.
 #pragma unroll
       for (int u = 0; u < (C::JOIN * NN + KG - 1) / KG; ++u) {
-        const int unit = u * KG + kg;
+        const int unit = u * KG + kg2;
         if (unit < C::JOIN * NN) {
           floatx4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int kk = 0; kk < KG; ++kk)
-            o += *reinterpret_cast<const floatx4*>(buf + ((kk * WC + cw) * (C::JOIN * NN) + unit) * C::UNIT + 4 * lane2);
+            o += *reinterpret_cast<const floatx4*>(buf + ((kk * WC + cw2) * (C::JOIN * NN) + unit) * C::UNIT + 4 * lane2);
           const int i = unit / NN, j = unit % NN;  // of the JOIN tiles
           float sum = join_sum[n0];
 #pragma unroll
           for (int ii = 1; ii < C::JOIN; ++ii) sum = i == ii ? join_sum[n0 + ii] : sum;
+          if (C::KEEP) own[n0 * NN / KG + u] = o;
           if (!split)
             write(n0 + i, j, o, inverse(sum));
           else
             __builtin_amdgcn_raw_buffer_store_b128(
                 __builtin_bit_cast(u32x4, o), pr,
-                4 * (part_of(k) + ((cw * NT + n0) * NN + unit) * C::UNIT + 4 * lane2), 0, kSc1);
+                4 * (part_of(k) + ((cw2 * NT + n0) * NN + unit) * C::UNIT + 4 * lane2), 0, kSc1);
         }
       }
     }
@@ -898,12 +913,32 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
     __syncthreads();
     if (last) {
       const int ranges = b - a + 1;
+      // AT_ONCE ranges' loads are in flight together, the first beside the work on the weights.
+      constexpr int AT_ONCE = NT > 2 ? 1 : C::OWN >= 8 ? 2 : 16 / C::OWN;
+      floatx4 first[AT_ONCE][C::OWN];
+      auto load_parts = [&](int r0, floatx4 (&part)[AT_ONCE][C::OWN]) {
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+          if (r0 + j < ranges && !(C::KEEP && r0 + j == k - a)) {
+#pragma unroll
+            for (int u = 0; u < C::OWN; ++u) {
+              const int unit = u * KG + kg2 < NT * NN ? u * KG + kg2 : 0;
+              const int from = 4 * (part_of(a + r0 + j) + (cw2 * NT * NN + unit) * C::UNIT + 4 * lane2);
+              part[j][u] = floatx4{ld_sc1(pr, from), ld_sc1(pr, from + 4), ld_sc1(pr, from + 8), ld_sc1(pr, from + 12)};
+            }
+          } else if (C::KEEP) {
+#pragma unroll
+            for (int u = 0; u < C::OWN; ++u) part[j][u] = own[u];
+          }
+        }
+      };
       // Every range's maximum and sum of every column, then its weight, in LDS.
       for (int x = tid2; x < ranges * COLS; x += C::THREADS) {
         const int from = 4 * (part_of(a + x / COLS) + COLS * D + 2 * (x % COLS));
         buf[x] = ld_sc1(pr, from);
         buf[kMostRanges * COLS + x] = ld_sc1(pr, from + 4);
       }
+      load_parts(0, first);
       __syncthreads();
       if (tid2 < COLS) {
         float top = kNoScore, sum = 0.f;
@@ -919,35 +954,29 @@ __global__ __launch_bounds__((C::THREADS), 1) void tree_attention_kernel(TreePar
       floatx4 o[C::OWN];
 #pragma unroll
       for (int u = 0; u < C::OWN; ++u) o[u] = floatx4{0.f, 0.f, 0.f, 0.f};
-      constexpr int AT_ONCE = C::OWN >= 8 ? 2 : 16 / C::OWN;  // ranges whose loads are in flight together
-      for (int r0 = 0; r0 < ranges; r0 += AT_ONCE) {
-        floatx4 part[AT_ONCE][C::OWN];
-#pragma unroll
-        for (int j = 0; j < AT_ONCE; ++j) {
-          const int r = r0 + j < ranges ? r0 + j : ranges - 1;
-#pragma unroll
-          for (int u = 0; u < C::OWN; ++u) {
-            const int unit = u * KG + kg < NT * NN ? u * KG + kg : 0;
-            const int from = 4 * (part_of(a + r) + (cw * NT * NN + unit) * C::UNIT + 4 * lane2);
-            part[j][u] = floatx4{ld_sc1(pr, from), ld_sc1(pr, from + 4), ld_sc1(pr, from + 8), ld_sc1(pr, from + 12)};
-          }
-        }
+      auto add_parts = [&](int r0, const floatx4 (&part)[AT_ONCE][C::OWN]) {
 #pragma unroll
         for (int j = 0; j < AT_ONCE; ++j) {
           if (r0 + j < ranges) {
 #pragma unroll
             for (int u = 0; u < C::OWN; ++u) {
-              const float f = buf[(r0 + j) * COLS + (cw * NT + (u * KG + kg) / NN % NT) * 16 + c2];
+              const float f = buf[(r0 + j) * COLS + (cw2 * NT + (u * KG + kg2) / NN % NT) * 16 + c2];
 #pragma unroll
               for (int r = 0; r < 4; ++r) o[u][r] = __builtin_fmaf(part[j][u][r], f, o[u][r]);
             }
           }
         }
+      };
+      add_parts(0, first);
+      for (int r0 = AT_ONCE; r0 < ranges; r0 += AT_ONCE) {
+        floatx4 part[AT_ONCE][C::OWN];
+        load_parts(r0, part);
+        add_parts(r0, part);
       }
 #pragma unroll
       for (int u = 0; u < C::OWN; ++u) {
-        const int unit = u * KG + kg;
-        if (unit < NT * NN) write(unit / NN, unit % NN, o[u], maxima[0][(cw * NT + unit / NN) * 16 + c2]);
+        const int unit = u * KG + kg2;
+        if (unit < NT * NN) write(unit / NN, unit % NN, o[u], maxima[0][(cw2 * NT + unit / NN) * 16 + c2]);
       }
       if (tid2 == 0) __hip_atomic_store(&p.counters[a], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
