@@ -1046,7 +1046,7 @@ hipError_t launch_tiles(const TreeParams& p, int tiles, hipStream_t stream) {
     const int64_t groups = (static_cast<int64_t>(kRows) * p.group + C::COLS - 1) / C::COLS * p.num_kv_heads;
     const int64_t line = groups * (p.max_ctx / 32 + 1 + kGroupCost);
     const int64_t fits = (int64_t{1} << 30) / line;
-    if (fits < 1) return hipErrorInvalidValue;
+    if (fits < 1) return hipErrorNotSupported;
     const int most = static_cast<int>(fits < kSeqs ? fits : kSeqs);
     TreeParams part = p;
     void* args[] = {&part};
@@ -1163,5 +1163,5 @@ extern "C" int ns_paged_attention_tree(void* out, const void* query,
     e = dtype == NS_DTYPE_F16 ? (head_dim == 64 ? launch_tiles<F16, 64>(p, nt, st) : launch_tiles<F16, 128>(p, nt, st))
                               : (head_dim == 64 ? launch_tiles<BF16, 64>(p, nt, st) : launch_tiles<BF16, 128>(p, nt, st));
   }
-  return e == hipSuccess ? NS_OK : NS_ERR_HIP;
+  return e == hipSuccess ? NS_OK : e == hipErrorNotSupported ? NS_ERR_UNSUPPORTED : NS_ERR_HIP;
 }
