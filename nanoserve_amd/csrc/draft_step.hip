@@ -81,7 +81,7 @@ __global__ __launch_bounds__(kThreads) void step_inputs_kernel(StepParams p) {
     held = load_index(p.held, i, p.index64);
     n0 = clamp_to(load_index(p.new_start, i, p.index64), p.num_new);
     fresh = clamp_to(load_index(p.new_start, i + 1, p.index64), p.num_new) - n0;
-    if (held < 0 || fresh < 0 || !has_table) fresh = 0;
+    if (held < 0 || held >= p.width || fresh < 0 || !has_table) fresh = 0;
   }
   auto block = [&](int64_t col) -> int64_t {
     if (!has_table || col >= p.width) return -1;

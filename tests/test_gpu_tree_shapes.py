@@ -7,8 +7,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from nanoserve_amd import paged_attention_tree
-from oracle.tree import ancestors, signed, tree_attention_ref
+from nanoserve_amd import paged_attention_tree, step_inputs
+from oracle.tree import ancestors, signed, step_inputs_ref, tree_attention_ref
 
 from tests.test_gpu_tree import DEV, Case, close
 
@@ -160,3 +160,19 @@ def test_one_device_batch_of_each_kind_in_one_graph():
         torch.cuda.synchronize()
         for c, o in zip(cases, outs):
             c.check(o, tree_attention_ref(c.query, c.kc, c.vc, c.starts, c.lens, c.tables, c.masks, c.scale))
+
+
+def test_columns_and_rows_at_the_ends_of_64_bits():
+    """New blocks named for columns and table rows that no table has are not written anywhere."""
+    to = lambda v: torch.tensor(v, dtype=torch.int64, device=DEV)  # noqa: E731
+    far = 2 ** 63 - 1
+    tables = to([[10, 11, 12, 13], [20, 21, 22, 23], [30, 31, 32, 33], [40, 41, 42, 43]])
+    plain = tables.tolist()
+    rows, held, new = [0, 1, far, -far, 3], [far, far - 1, 0, 0, 4], [[1, 2], [3, 4, 5], [6], [7], [8]]
+    start = [0, 2, 5, 6, 7, 8]
+    computed, lens = [17, 3, 5, 0, 33], [2, 1, 4, 2, 3]
+    x = step_inputs(tables, to(rows), to(computed), to(lens), 12, 16, 4, to([b for n in new for b in n]), to(start), to(held))
+    want = step_inputs_ref(plain, rows, computed, lens, 12, 16, 4, new, held)
+    got = [v.tolist() for v in (x.query_start_loc, x.seq_lens, x.positions, x.slot_mapping, x.block_tables)]
+    assert got == list(want[:5])
+    assert tables.tolist() == plain
