@@ -70,10 +70,10 @@ def _vector(t: torch.Tensor, name: str, n: int, index: int) -> torch.Tensor:
 
 def _alike(tensors: list) -> tuple[list, bool]:
     """The tensors (or None) of one integer dtype, and whether that is int64."""
-    wide = any(t is not None and t.dtype is torch.int64 for t in tensors)
-    if wide:
-        tensors = [t if t is None or t.dtype is torch.int64 else t.to(torch.int64) for t in tensors]
-    return tensors, wide
+    kinds = {t.dtype for t in tensors if t is not None}
+    if len(kinds) > 1:
+        tensors = [t if t is None else t.to(torch.int64) for t in tensors]
+    return tensors, torch.int64 in kinds
 
 
 def _pointer(t: torch.Tensor | None):
@@ -106,8 +106,7 @@ def step_inputs(tables: torch.Tensor, rows: torch.Tensor, computed: torch.Tensor
         raise ValueError("tables must have contiguous rows that do not overlap")
     if num_tokens < 0 or block_size <= 0 or max_blocks < 0:
         raise ValueError(f"num_tokens {num_tokens}, block_size {block_size} and max_blocks {max_blocks} are no sizes")
-    given = [x is not None for x in (new_blocks, new_start, held)]
-    if any(given) and not all(given):
+    if (new_blocks is None) != (new_start is None) or (new_blocks is None) != (held is None):
         raise ValueError("new_blocks, new_start and held belong together")
     index = tables.get_device()
     B = rows.shape[0] if rows.dim() else 0
@@ -120,11 +119,12 @@ def step_inputs(tables: torch.Tensor, rows: torch.Tensor, computed: torch.Tensor
                None if parents is None else _vector(parents, "parents", num_tokens, index)]
     vectors, wide = _alike(vectors)
     device = tables.device
-    # One allocation for every int64 output.
+    # One allocation for every int64 output (no two overlap, and none has a history:
+    # the split that keeps no record of the parts being views).
     T = num_tokens
     sizes = [B + 1, B, T, T] if parents is None else [B + 1, B, T, T, T]
     flat = torch.empty(sum(sizes), dtype=torch.int64, device=device)
-    qsl, lens, positions, slots, *mask = flat.split_with_sizes(sizes)
+    qsl, lens, positions, slots, *mask = torch.unsafe_split_with_sizes(flat, sizes)
     packed = torch.empty((B, max_blocks), dtype=tables.dtype, device=device)
     at = flat.data_ptr()
     pointers = [None if t is None else t.data_ptr() for t in vectors]
@@ -351,13 +351,12 @@ def commit_drafts(chosen: torch.Tensor, input_ids: torch.Tensor, parents: torch.
                              f"{sorted({(str(c.dtype), tuple(c.shape), str(c.device)) for c in caches})}")
         num_slots, row_bytes = shape[0] * shape[1], shape[2] * shape[3] * first.element_size()
     device = chosen.device
-    out = torch.empty(B * (1 + max_rows), dtype=torch.int64, device=device)
-    counts, tokens = out.split_with_sizes([B, B * max_rows])
+    counts = torch.empty(B, dtype=torch.int64, device=device)
+    tokens = torch.empty((B, max_rows), dtype=torch.int64, device=device)
     held = len(caches) if num_slots and row_bytes else 0
     pointers = array.array("Q", map(_ADDRESS, caches)) if held else None
-    at = out.data_ptr()
     _lib.launch(device, what, _lib.load().ns_commit_drafts,
-                at, at + 8 * B, rows[0].data_ptr(), rows[1].data_ptr(), rows[2].data_ptr(), wide,
+                counts.data_ptr(), tokens.data_ptr(), rows[0].data_ptr(), rows[1].data_ptr(), rows[2].data_ptr(), wide,
                 qsl.data_ptr(), qsl.dtype is torch.int64, slots.data_ptr(), slots.dtype is torch.int64, B, T, max_rows,
                 pointers.buffer_info()[0] if held else None, held, num_slots, row_bytes)
-    return counts, tokens.view(B, max_rows)
+    return counts, tokens
