@@ -24,6 +24,7 @@ from __future__ import annotations
 
 import array
 from dataclasses import dataclass
+from functools import lru_cache
 from operator import attrgetter
 
 import torch
@@ -209,6 +210,13 @@ def _arrivals(device: torch.device, capturing: bool) -> torch.Tensor:
     return c
 
 
+@lru_cache(maxsize=4096)
+def _workspace_bytes(index: int, *sizes: int) -> int:
+    """ns_paged_attention_tree_workspace_size, a function of sizes alone, which the layers of a step share."""
+    with torch.cuda.device(index):
+        return _lib.load().ns_paged_attention_tree_workspace_size(*sizes)
+
+
 def paged_attention_tree(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                          md: AttentionMetadata, scale: float) -> torch.Tensor:
     """Paged attention for trees of drafted tokens: attn_fn's contract
@@ -280,15 +288,14 @@ def paged_attention_tree(query: torch.Tensor, k_cache: torch.Tensor, v_cache: to
         host = md.query_start_loc_cpu
         full = host is not None and len(host) > n and host[0] == 0 and host[n] == T and not capturing
     out = torch.empty_like(q) if full else torch.zeros_like(q)
-    lib = _lib.load()
-    nbytes = lib.ns_paged_attention_tree_workspace_size(n, Hq, heads, D, block_size, md.max_query_len, T, code)
+    nbytes = _workspace_bytes(index, n, Hq, heads, D, block_size, md.max_query_len, T, code)
     ws = counters = None
     device = q.device
     if nbytes:
         # The partial results live in a tensor of this call's.
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
         counters = _arrivals(device, capturing)
-    _lib.launch(device, what, lib.ns_paged_attention_tree,
+    _lib.launch(device, what, _lib.load().ns_paged_attention_tree,
                 out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                 bt.data_ptr(), stride[0], width, bt.dtype is torch.int64, sl.data_ptr(), sl.dtype is torch.int64,
                 qsl_ptr, qsl64, mask.data_ptr(), n, T, md.max_query_len, longest, Hq, heads, D, block_size,
