@@ -204,7 +204,9 @@ def _arrivals(device: torch.device, capturing: bool) -> torch.Tensor:
         c = _counters.get((index, torch._C._cuda_getCurrentRawStream(index)))
         if c is not None:
             return c
-    c = torch.zeros(_lib.load().ns_paged_attention_tree_counters(), dtype=torch.int32, device=device)
+    with torch.cuda.device(index):  # as many as that device, not the current one, has workgroups
+        n = _lib.load().ns_paged_attention_tree_counters()
+    c = torch.zeros(n, dtype=torch.int32, device=device)
     if not capturing:
         _counters[index, torch._C._cuda_getCurrentRawStream(index)] = c
     return c

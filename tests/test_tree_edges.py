@@ -1,0 +1,45 @@
+"""A drafted step at its edges, as far as the host decides them (no GPU)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from nanoserve_amd import tree
+
+
+class Devices:
+    """torch's current device and a library on two devices of different sizes, stood in for on the CPU."""
+
+    current = 0
+
+    def __init__(self, index):
+        self.index = getattr(index, "index", index)
+
+    def __enter__(self):
+        self.before, Devices.current = Devices.current, self.index
+
+    def __exit__(self, *_):
+        Devices.current = self.before
+
+    @staticmethod
+    def ns_paged_attention_tree_counters():
+        return (64, 256)[Devices.current]
+
+
+@pytest.fixture
+def devices(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "device", Devices)
+    monkeypatch.setattr(tree._lib, "load", lambda: Devices)
+    monkeypatch.setattr(tree, "_counters", {})
+    monkeypatch.setattr(torch, "zeros", lambda n, **_: n)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 0, raising=False)
+
+
+@pytest.mark.parametrize("capturing", [False, True])
+def test_counters_are_those_of_the_tensors_device(devices, capturing):
+    """One a workgroup of the device that the call runs on, whichever is current."""
+    assert tree._arrivals(torch.device("cuda:1"), capturing) == 256
+    assert tree._arrivals(torch.device("cuda:0"), capturing) == 64
+    with Devices(1):
+        assert tree._arrivals(torch.device("cuda:0"), capturing) == 64
