@@ -212,6 +212,14 @@ def _arrivals(device: torch.device, capturing: bool) -> torch.Tensor:
     return c
 
 
+def _capturing(index: int) -> bool:
+    """Whether the current stream of GPU `index`, which a call on its tensors takes, is recording a graph."""
+    if index == torch._C._cuda_getDevice():
+        return torch._C._cuda_isCurrentStreamCapturing()
+    with torch.cuda.device(index):
+        return torch._C._cuda_isCurrentStreamCapturing()
+
+
 @lru_cache(maxsize=4096)
 def _workspace_bytes(index: int, *sizes: int) -> int:
     """ns_paged_attention_tree_workspace_size, a function of sizes alone, which the layers of a step share."""
@@ -275,7 +283,7 @@ def paged_attention_tree(query: torch.Tensor, k_cache: torch.Tensor, v_cache: to
         bt = bt.contiguous()
         stride = bt.stride()
     sl = _prefix(md.seq_lens, "seq_lens", n, index)
-    capturing = torch._C._cuda_isCurrentStreamCapturing()
+    capturing = _capturing(index)
     qsl_ptr, qsl64 = None, 0
     if md.query_start_loc is None:
         if T != n:

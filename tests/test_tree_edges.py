@@ -43,3 +43,12 @@ def test_counters_are_those_of_the_tensors_device(devices, capturing):
     assert tree._arrivals(torch.device("cuda:0"), capturing) == 64
     with Devices(1):
         assert tree._arrivals(torch.device("cuda:0"), capturing) == 64
+
+
+def test_a_capture_is_looked_for_on_the_tensors_device(devices, monkeypatch):
+    """Device 1 records a graph while device 0 is current, and the other way round."""
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: Devices.current, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: Devices.current == 1, raising=False)
+    assert tree._capturing(1) and not tree._capturing(0)
+    with Devices(1):
+        assert tree._capturing(1) and not tree._capturing(0)
