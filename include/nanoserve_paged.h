@@ -621,19 +621,19 @@ int ns_paged_attention_int4(void* out, const void* query,
  * and key L - q + i where bit i of tree_mask (int64 [num_tokens]) is set, i < 64.
  * A row without keys is zero; a row of no sequence, and a sequence's rows from the
  * 64th on, are left as they are.  K and V of a key that a row does not see do not
- * reach it, whatever they hold.  Without
- * query_start_loc (NULL) row s is sequence s.  max_query_len is the longest
- * sequence's rows, at most 64; it shapes the launch, the device's offsets decide.
- * A block id outside [0, num_blocks) is never dereferenced; the affected (sequence,
- * KV head) outputs are NaN.  float16 and bfloat16 at head sizes 64 and 128 with
- * blocks of whole 16-token tiles run on the matrix cores (pointers 16-byte
- * aligned; out and query contiguous), every other shape with head_dim <= 256 a
- * plain kernel that reads no workspace.  workspace: 16-byte aligned,
- * ns_paged_attention_tree_workspace_size bytes (0: none is needed), not
- * initialised.  counters: ns_paged_attention_tree_counters() int32, zero before
- * the first call, zero again after every call.  Both sizes are those of the current
- * device, which has to be the one that the call runs on.  Calls that overlap in time
- * need their own of both.  NS_ERR_UNSUPPORTED past 2^30 keys of a sequence, 2^30 rows
+ * reach it, whatever they hold.  Without query_start_loc (NULL) row s is sequence s.
+ * max_query_len is the longest sequence's rows, at most 64; it shapes the launch,
+ * the device's offsets decide.  A block id outside [0, num_blocks) is never
+ * dereferenced; where a sequence's keys lie in one, all of its rows are NaN, those
+ * that do not see these keys too.  float16 and bfloat16 at head sizes 64 and 128 with
+ * blocks of whole 16-token tiles run on the matrix cores (pointers 16-byte aligned;
+ * out and query contiguous), every other shape with head_dim <= 256 a plain kernel
+ * that reads no workspace.  workspace: 16-byte aligned,
+ * ns_paged_attention_tree_workspace_size bytes (0: none is needed), not initialised.
+ * counters: ns_paged_attention_tree_counters() int32, zero before the first call,
+ * zero again after every call.  Both sizes are those of the current device, which has
+ * to be the one that the call runs on.  Calls that overlap in time need their own of
+ * both.  NS_ERR_UNSUPPORTED past 2^30 keys of a sequence, 2^30 rows
  * times heads, or 2^30 chunks of 32 keys times column blocks times KV heads.
  */
 int ns_step_inputs(void* tables, int64_t table_rows, int64_t table_width, int64_t table_stride,

@@ -127,18 +127,16 @@ __global__ __launch_bounds__(64) void tree_attention_generic_kernel(TreeParams p
     const int64_t key = c0 + lane;
     int64_t row = 0;  // element offset of this lane's key (its K and V rows)
     bool ok = key < r.len;
+    if (ok) {
+      // A block outside the cache is every row's, seen or not, as in the kernel below.
+      const int64_t blk = load_index(p.bt, bt_row + key / bs, p.bt64);
+      ok = blk >= 0 && blk < p.num_blocks;
+      if (!ok) bad = 1;
+      else row = ((blk * bs + key % bs) * p.num_kv_heads + kvh) * D;
+    }
     if (ok && key >= base) {
       const int64_t i = key - base;
       ok = i < kRows && ((mask >> i) & 1);
-    }
-    if (ok) {
-      const int64_t blk = load_index(p.bt, bt_row + key / bs, p.bt64);
-      if (blk < 0 || blk >= p.num_blocks) {
-        bad = 1;
-        ok = false;
-      } else {
-        row = ((blk * bs + key % bs) * p.num_kv_heads + kvh) * D;
-      }
     }
     float sc = -INFINITY;
     if (ok) {
