@@ -145,7 +145,9 @@ __global__ __launch_bounds__(kThreads) void step_inputs_kernel(StepParams p) {
 // rows of the caches: a path's rows lie at or behind their new places, in order, so
 // that a thread that goes along the path never overwrites what it has still to read.
 
-constexpr int kCaches = 128;  // of a launch
+constexpr int kCaches = 128;              // of a launch, at most
+constexpr int kGridY = 65535;             // workgroups of a launch along y
+constexpr int kMostSeqs = (1 << 24) - 1;  // along x: a grid has less than 2^32 threads in a direction
 
 struct CommitParams {
   const void* chosen;
@@ -229,7 +231,6 @@ __global__ __launch_bounds__(kThreads) void commit_drafts_kernel(CommitParams p)
 
 template <class U>
 hipError_t launch_commit(CommitParams& p, int64_t num_seqs, hipStream_t stream) {
-  p.units = static_cast<int>(p.row_bytes / static_cast<int64_t>(sizeof(U)));
   const int64_t units = static_cast<int64_t>(p.num_caches) * p.units;
   const unsigned y = static_cast<unsigned>(units > 0 ? (units + kThreads - 1) / kThreads : 1);
   void* args[] = {&p};
@@ -317,7 +318,7 @@ extern "C" int ns_commit_drafts(int64_t* counts, int64_t* tokens,
   using namespace ns;
   if (num_seqs < 0 || num_tokens < 0 || max_rows < 0 || num_caches < 0 || num_slots < 0 || row_bytes < 0)
     return NS_ERR_INVALID_ARG;
-  if (max_rows > kTreeRows || num_seqs > 0x7FFFFFFF || row_bytes > 1 << 20) return NS_ERR_UNSUPPORTED;
+  if (max_rows > kTreeRows || num_seqs > kMostSeqs || row_bytes > 1 << 20) return NS_ERR_UNSUPPORTED;
   if (num_seqs == 0) return NS_OK;
   if (!counts || (max_rows > 0 && !tokens) || !query_start_loc) return NS_ERR_INVALID_ARG;
   if (num_tokens > 0 && (!chosen || !input_ids || !parents || !slot_mapping)) return NS_ERR_INVALID_ARG;
@@ -347,14 +348,19 @@ extern "C" int ns_commit_drafts(int64_t* counts, int64_t* tokens,
   p.index64 = index_is_int64;
   p.qsl64 = query_start_loc_is_int64;
   p.slots64 = slot_mapping_is_int64;
-  for (int c0 = 0; c0 == 0 || c0 < num_caches; c0 += kCaches) {
-    p.num_caches = num_caches - c0 < kCaches ? num_caches - c0 : kCaches;
+  const int unit = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : all % 2 == 0 ? 2 : 1;
+  p.units = static_cast<int>(row_bytes / unit);
+  // As many caches a launch as its grid holds: 15 or more, of rows of 2^20 units.
+  const int fits = p.units > 0 ? kGridY * kThreads / p.units : kCaches;
+  const int most = fits < kCaches ? fits : kCaches;
+  for (int c0 = 0; c0 == 0 || c0 < num_caches; c0 += most) {
+    p.num_caches = num_caches - c0 < most ? num_caches - c0 : most;
     for (int c = 0; c < kCaches; ++c) p.caches[c] = c < p.num_caches ? static_cast<char*>(caches[c0 + c]) : nullptr;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const hipError_t e = all % 16 == 0  ? launch_commit<u32x4>(p, num_seqs, st)
-                         : all % 4 == 0 ? launch_commit<uint32_t>(p, num_seqs, st)
-                         : all % 2 == 0 ? launch_commit<uint16_t>(p, num_seqs, st)
-                                        : launch_commit<uint8_t>(p, num_seqs, st);
+    const hipError_t e = unit == 16  ? launch_commit<u32x4>(p, num_seqs, st)
+                         : unit == 4 ? launch_commit<uint32_t>(p, num_seqs, st)
+                         : unit == 2 ? launch_commit<uint16_t>(p, num_seqs, st)
+                                     : launch_commit<uint8_t>(p, num_seqs, st);
     if (e != hipSuccess) return NS_ERR_HIP;
   }
   return NS_OK;

@@ -6,6 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from nanoserve_amd import commit_drafts
 from tests.test_gpu_tree import DEV, Case, close
 
 pytestmark = pytest.mark.gpu
@@ -28,3 +29,20 @@ def test_a_block_outside_the_cache_under_drafted_rows(dtype, heads, block_size, 
         assert torch.isnan(out[5:25]).all()
         keep = [*range(5), 25, 26, 27]
         close(out[keep], ref[keep], mag[keep], dtype, c.d, base + q)
+
+
+@pytest.mark.parametrize("row_bytes,caches", [((1 << 20) - 1, 34), ((1 << 20) - 2, 70), ((1 << 20) - 4, 130),
+                                              (1 << 20, 5), (6, 300)])
+def test_commit_of_rows_of_a_mebibyte(row_bytes, caches):
+    """More units of rows than one launch's grid holds."""
+    to = lambda v: torch.tensor(v, dtype=torch.int64, device=DEV)  # noqa: E731
+    held = [torch.zeros(3, 1, 1, row_bytes, dtype=torch.uint8, device=DEV) for _ in range(caches)]
+    g = torch.Generator(device=DEV).manual_seed(row_bytes)
+    row = torch.randint(0, 256, (row_bytes,), dtype=torch.uint8, device=DEV, generator=g)
+    for i, c in enumerate(held):
+        c[2, 0, 0] = row + i
+    counts, tokens = commit_drafts(to([7, 0, 3]), to([1, 5, 7]), to([-1, 0, 0]), to([0, 3]), to([0, 1, 2]),
+                                   held[:caches // 2], held[caches // 2:], 3)
+    assert counts.tolist() == [2] and tokens.tolist() == [[7, 3, -1]]
+    for i, c in enumerate(held):
+        assert torch.equal(c[1, 0, 0], row + i) and torch.equal(c[2], c[1]) and not c[0].any()

@@ -2,10 +2,12 @@
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
-from nanoserve_amd import tree
+from nanoserve_amd import _lib, tree
 
 
 class Devices:
@@ -52,3 +54,20 @@ def test_a_capture_is_looked_for_on_the_tensors_device(devices, monkeypatch):
     assert tree._capturing(1) and not tree._capturing(0)
     with Devices(1):
         assert tree._capturing(1) and not tree._capturing(0)
+
+
+# ---- the C entry points' limits: refused before any launch ------------------------
+
+BIG = 1 << 40  # aligned, never read
+UNSUPPORTED = _lib.NS_ERR_UNSUPPORTED
+
+
+def _commit(S=2, T=16, maxr=8, caches=(BIG, 2 * BIG), num_slots=512, row_bytes=256):
+    array = (ctypes.c_void_p * max(len(caches), 1))(*caches)
+    return _lib.load().ns_commit_drafts(BIG, BIG, BIG, BIG, BIG, 1, BIG, 1, BIG, 1, S, T, maxr, ctypes.addressof(array),
+                                        len(caches), num_slots, row_bytes, None)
+
+
+@pytest.mark.parametrize("over", [dict(S=1 << 24), dict(S=1 << 31), dict(row_bytes=(1 << 20) + 1), dict(maxr=65)])
+def test_commit_refuses_what_no_grid_holds(over):
+    assert _commit(**over) == UNSUPPORTED
