@@ -634,8 +634,9 @@ int ns_paged_attention_int4(void* out, const void* query,
  * counters: ns_paged_attention_tree_counters() int32, zero before the first call,
  * zero again after every call.  Both sizes are those of the current device, which has
  * to be the one that the call runs on.  Calls that overlap in time need their own of
- * both.  NS_ERR_UNSUPPORTED past 2^30 keys of a sequence, 2^30 rows
- * times heads, or 2^30 chunks of 32 keys times column blocks times KV heads.
+ * both.  NS_ERR_UNSUPPORTED past 2^30 keys of a sequence, 2^30 rows times heads,
+ * 2^26 - 1 rows of the plain kernel, or 2^30 chunks of 32 keys times column blocks
+ * times KV heads.
  */
 int ns_step_inputs(void* tables, int64_t table_rows, int64_t table_width, int64_t table_stride,
                    int tables_is_int64,

@@ -15,6 +15,7 @@ namespace {
 constexpr int kRows = 64;        // rows of a sequence that a mask can name
 constexpr int kSeqs = 512;       // sequences of a launch (their schedule is held in LDS)
 constexpr int kMaxHeadDim = 256;
+constexpr int kMostPlainRows = (1 << 26) - 1;  // of 64 threads each: a grid has less than 2^32 in a direction
 
 struct TreeParams {
   char* out;
@@ -1122,6 +1123,7 @@ extern "C" int ns_paged_attention_tree(void* out, const void* query,
   if (max_seq_len > 1 << 30 || num_heads > 65535 || num_tokens > 0x3FFFFFFF / num_heads ||
       num_seqs > 0x3FFFFFFF / num_heads || static_cast<int64_t>(num_kv_heads) * head_dim * 2 * 16 > 0x7FFFFFFF)
     return NS_ERR_UNSUPPORTED;
+  if (!tiles && num_tokens > kMostPlainRows) return NS_ERR_UNSUPPORTED;
   TreeParams p;
   p.out = static_cast<char*>(out);
   p.query = static_cast<const char*>(query);

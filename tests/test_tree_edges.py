@@ -71,3 +71,11 @@ def _commit(S=2, T=16, maxr=8, caches=(BIG, 2 * BIG), num_slots=512, row_bytes=2
 @pytest.mark.parametrize("over", [dict(S=1 << 24), dict(S=1 << 31), dict(row_bytes=(1 << 20) + 1), dict(maxr=65)])
 def test_commit_refuses_what_no_grid_holds(over):
     assert _commit(**over) == UNSUPPORTED
+
+
+@pytest.mark.parametrize("dtype,D,bs", [(_lib.NS_DTYPE_F32, 64, 16), (_lib.NS_DTYPE_F16, 8, 16), (_lib.NS_DTYPE_F16, 64, 4)])
+def test_attention_refuses_what_no_grid_holds(dtype, D, bs):
+    T = 1 << 26
+    assert _lib.load().ns_paged_attention_tree(
+        BIG, BIG, BIG, BIG, BIG, 64, 64, 1, BIG, 1, BIG, 1, BIG, 2, T, 8, 64, 1, 1, D, bs, 128, 0.125, dtype, None, None, 0,
+        None) == UNSUPPORTED
