@@ -611,11 +611,12 @@ int ns_paged_attention_int4(void* out, const void* query,
  * the current row) whose input id is the current row's choice, until there is
  * none.  counts[i] is the number of rows of request i's walk (0 without rows),
  * tokens [num_seqs, max_rows] their choices, then -1.  In every one of `caches`
- * (host array of device pointers, [num_slots, row_bytes] bytes each) the row at
- * the slot of the walk's row d moves to the slot of the request's row d.  The slots
- * of a request's rows must differ; slots outside [0, num_slots) are left alone.
- * Rows from max_rows (at most 64) on take no part.  At most 2^24 - 1 requests and
- * rows of 2^20 bytes.
+ * (host array of device pointers, [num_slots, row_bytes] bytes each, none of which
+ * overlap) the row at the slot of the walk's row d moves to the slot of the request's
+ * row d.  The slots of a request's rows must differ, and one that a row moves to must
+ * be no other request's; slots outside [0, num_slots) are left alone.
+ * Rows from max_rows (at most 64) on take no part.  At most 2^24 - 1 requests,
+ * 2^40 slots and rows of 2^20 bytes.
  *
  * ns_paged_attention_tree -- ns_paged_attention for such rows: row j of a
  * sequence with context length L (its q rows included) sees keys 0 .. L - q - 1

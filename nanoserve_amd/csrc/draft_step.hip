@@ -318,7 +318,8 @@ extern "C" int ns_commit_drafts(int64_t* counts, int64_t* tokens,
   using namespace ns;
   if (num_seqs < 0 || num_tokens < 0 || max_rows < 0 || num_caches < 0 || num_slots < 0 || row_bytes < 0)
     return NS_ERR_INVALID_ARG;
-  if (max_rows > kTreeRows || num_seqs > kMostSeqs || row_bytes > 1 << 20) return NS_ERR_UNSUPPORTED;
+  if (max_rows > kTreeRows || num_seqs > kMostSeqs || row_bytes > 1 << 20 || num_slots > int64_t{1} << 40)
+    return NS_ERR_UNSUPPORTED;
   if (num_seqs == 0) return NS_OK;
   if (!counts || (max_rows > 0 && !tokens) || !query_start_loc) return NS_ERR_INVALID_ARG;
   if (num_tokens > 0 && (!chosen || !input_ids || !parents || !slot_mapping)) return NS_ERR_INVALID_ARG;
@@ -328,10 +329,18 @@ extern "C" int ns_commit_drafts(int64_t* counts, int64_t* tokens,
       misaligned(parents, index) || misaligned(query_start_loc, query_start_loc_is_int64 ? 8 : 4) ||
       misaligned(slot_mapping, slot_mapping_is_int64 ? 8 : 4))
     return NS_ERR_INVALID_ARG;
+  // A row of two caches in one place would be moved twice, the second time perhaps from
+  // where the first move has written already.
   uintptr_t all = static_cast<uintptr_t>(row_bytes);
+  const uint64_t bytes = static_cast<uint64_t>(num_slots) * static_cast<uint64_t>(row_bytes);
   for (int c = 0; c < num_caches; ++c) {
-    if (!caches[c]) return NS_ERR_INVALID_ARG;
-    all |= reinterpret_cast<uintptr_t>(caches[c]);
+    const uint64_t at = reinterpret_cast<uintptr_t>(caches[c]);
+    if (!at) return NS_ERR_INVALID_ARG;
+    for (int b = 0; b < c; ++b) {
+      const uint64_t before = reinterpret_cast<uintptr_t>(caches[b]);
+      if ((at < before ? before - at : at - before) < bytes) return NS_ERR_INVALID_ARG;
+    }
+    all |= at;
   }
   CommitParams p;
   p.chosen = chosen;

@@ -337,8 +337,9 @@ def commit_drafts(chosen: torch.Tensor, input_ids: torch.Tensor, parents: torch.
     that was fed the current row's choice; its rows' choices are the request's next
     tokens (counts of them, then -1), and the rows' K and V move in every cache
     ([num_blocks, block_size, kv_heads, head_dim], one shape and dtype) from their
-    slots to those of the request's first rows, where the tokens belong.  The slots
-    of a request's rows must differ; slots outside the cache are left alone.
+    slots to those of the request's first rows, where the tokens belong.  No cache may
+    be listed twice.  The slots of a request's rows must differ, and one that a row
+    moves to must be no other request's; slots outside the cache are left alone.
     max_rows (at most 64): the most rows of a request; later ones take no part."""
     what = "commit_drafts"
     index = chosen.get_device()
@@ -372,6 +373,8 @@ def commit_drafts(chosen: torch.Tensor, input_ids: torch.Tensor, parents: torch.
     tokens = torch.empty((B, max_rows), dtype=torch.int64, device=device)
     held = len(caches) if num_slots and row_bytes else 0
     pointers = array.array("Q", map(_ADDRESS, caches)) if held else None
+    if held and len({*pointers}) != held:
+        raise ValueError("a cache is listed twice")
     _lib.launch(device, what, _lib.load().ns_commit_drafts,
                 counts.data_ptr(), tokens.data_ptr(), rows[0].data_ptr(), rows[1].data_ptr(), rows[2].data_ptr(), wide,
                 qsl.data_ptr(), qsl.dtype is torch.int64, slots.data_ptr(), slots.dtype is torch.int64, B, T, max_rows,

@@ -46,3 +46,19 @@ def test_commit_of_rows_of_a_mebibyte(row_bytes, caches):
     assert counts.tolist() == [2] and tokens.tolist() == [[7, 3, -1]]
     for i, c in enumerate(held):
         assert torch.equal(c[1, 0, 0], row + i) and torch.equal(c[2], c[1]) and not c[0].any()
+
+
+def test_commit_refuses_a_cache_that_is_listed_twice():
+    to = lambda v: torch.tensor(v, dtype=torch.int64, device=DEV)  # noqa: E731
+    both = torch.arange(2 * 3 * 16 * 8, device=DEV).half().view(2, 3, 16, 1, 8)
+    before = both.clone()
+    k, v = both.unbind()
+    args = to([7, 0, 3]), to([1, 5, 7]), to([-1, 0, 0]), to([0, 3]), to([0, 1, 2])
+    for caches in (([k, v], [k]), ([k], [k.view(3, 16, 1, 8)])):
+        with pytest.raises(ValueError, match="twice"):
+            commit_drafts(*args, *caches, 3)
+    with pytest.raises(RuntimeError, match="invalid"):
+        commit_drafts(*args, [both[0]], [both.view(6, 16, 1, 8)[1:4]], 3)
+    assert torch.equal(both, before)
+    commit_drafts(*args, [k], [v], 3)  # neighbours do not overlap
+    assert torch.equal(both[:, 0, 1], before[:, 0, 2]) and torch.equal(both[:, 0, 2:], before[:, 0, 2:])

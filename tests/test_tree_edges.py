@@ -62,15 +62,34 @@ BIG = 1 << 40  # aligned, never read
 UNSUPPORTED = _lib.NS_ERR_UNSUPPORTED
 
 
-def _commit(S=2, T=16, maxr=8, caches=(BIG, 2 * BIG), num_slots=512, row_bytes=256):
+def _commit(caches=(BIG, 2 * BIG), **over):
     array = (ctypes.c_void_p * max(len(caches), 1))(*caches)
-    return _lib.load().ns_commit_drafts(BIG, BIG, BIG, BIG, BIG, 1, BIG, 1, BIG, 1, S, T, maxr, ctypes.addressof(array),
-                                        len(caches), num_slots, row_bytes, None)
+    a = dict(counts=BIG, tokens=BIG, chosen=BIG, ids=BIG, parents=BIG, i64=1, qsl=BIG, qsl64=1, slots=BIG, slots64=1, S=2, T=16,
+             maxr=8, array=ctypes.addressof(array), n=len(caches), num_slots=512, row_bytes=256, stream=None)
+    a.update(over)
+    return _lib.load().ns_commit_drafts(*a.values())
 
 
 @pytest.mark.parametrize("over", [dict(S=1 << 24), dict(S=1 << 31), dict(row_bytes=(1 << 20) + 1), dict(maxr=65)])
 def test_commit_refuses_what_no_grid_holds(over):
     assert _commit(**over) == UNSUPPORTED
+
+
+@pytest.mark.parametrize("over", [
+    dict(counts=None), dict(tokens=None), dict(chosen=None), dict(ids=None), dict(parents=None), dict(qsl=None),
+    dict(slots=None), dict(S=-1), dict(T=-1), dict(maxr=-1), dict(array=None), dict(n=-1), dict(num_slots=-1),
+    dict(row_bytes=-1), dict(row_bytes=0), dict(caches=(BIG, 0)), dict(counts=BIG + 4), dict(chosen=BIG + 4),
+    dict(qsl=BIG + 4), dict(slots=BIG + 4), dict(chosen=BIG + 2, i64=0),
+])
+def test_commit_refuses_with_caches_beside_one_another(over):
+    assert _commit(**over) == _lib.NS_ERR_INVALID_ARG
+
+
+def test_commit_refuses_caches_that_overlap():
+    """A row in two caches would be moved twice: the second move may read what the first has written."""
+    size = 512 * 256
+    for caches in ((BIG, BIG), (BIG, BIG + size - 16), (BIG + 256, 2 * BIG, BIG), (3 * BIG, 2 * BIG, 3 * BIG - size + 1)):
+        assert _commit(caches=caches) == _lib.NS_ERR_INVALID_ARG
 
 
 @pytest.mark.parametrize("dtype,D,bs", [(_lib.NS_DTYPE_F32, 64, 16), (_lib.NS_DTYPE_F16, 8, 16), (_lib.NS_DTYPE_F16, 64, 4)])
