@@ -469,7 +469,7 @@ class LLMEngine:
         self.pipeline_decode = pipeline_decode and not draft_tokens
         self.draft_tokens = draft_tokens
         self.drafter = drafter if drafter is not None or not draft_tokens else NgramDrafter()
-        self.num_drafted = self.num_accepted = 0  # drafted tokens verified, and kept
+        self.num_drafted = self.num_accepted = 0  # drafted tokens verified, and kept in the output
 
     def add_request(self, prompt_token_ids: list[int], sampling: SamplingParams | None = None) -> int:
         sampling = sampling or SamplingParams()
@@ -527,12 +527,12 @@ class LLMEngine:
         now = time.perf_counter()
         for seq, tokens, (draft, _) in zip(seqs, kept, drafts):
             self.num_drafted += len(draft)
-            self.num_accepted += len(tokens) - 1
-            for t in tokens:
+            for n, t in enumerate(tokens, 1):
                 seq.mark_computed(1)
                 seq.output_token_ids.append(t)
                 if seq.check_done(self.eos_token_id):
                     break
+            self.num_accepted += min(n, len(tokens) - 1)  # the last one was not drafted
             self._record(seq, now)
             self.block_manager.trim(seq, seq.num_tokens)
             self.runner.trimmed(seq)

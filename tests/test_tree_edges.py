@@ -8,6 +8,9 @@ import pytest
 import torch
 
 from nanoserve_amd import _lib, tree
+from nanoserve_amd.engine import LLMEngine
+from nanoserve_amd.model import Qwen2Config, Qwen2ForCausalLM
+from nanoserve_amd.scheduling import SamplingParams
 
 
 class Devices:
@@ -98,3 +101,49 @@ def test_attention_refuses_what_no_grid_holds(dtype, D, bs):
     assert _lib.load().ns_paged_attention_tree(
         BIG, BIG, BIG, BIG, BIG, 64, 64, 1, BIG, 1, BIG, 1, BIG, 2, T, 8, 64, 1, 1, D, bs, 128, 0.125, dtype, None, None, 0,
         None) == UNSUPPORTED
+
+
+# ---- the engine, its model stood in for --------------------------------------------
+
+
+class Drafter:
+    """Three drafted tokens in a chain, or what room there is for them."""
+
+    def draft(self, seq, limit, depth):
+        n = min(3, limit, depth)
+        return [7, 8, 9][:n], list(range(n))
+
+
+def _engine(kept, **kw):
+    """An engine past its request's prompt, whose drafted steps give the lists of `kept` in turn."""
+    model = Qwen2ForCausalLM(Qwen2Config(vocab_size=16, hidden_size=16, intermediate_size=16, num_hidden_layers=1,
+                                         num_attention_heads=2, num_key_value_heads=1, tie_word_embeddings=False))
+    e = LLMEngine(model, 16, 4, "cpu", max_model_len=64, draft_tokens=3, drafter=Drafter(), **kw)
+
+    def prompt(scheduled):
+        for seq, q in scheduled:
+            seq.mark_computed(q)
+        return [(seq, 1) for seq, _ in scheduled]
+
+    e.runner.execute = prompt
+    e.add_request([1, 2, 3, 4, 5], SamplingParams(max_new_tokens=12))
+    e.step()
+    if kept is not None:
+        kept = iter(kept)
+        e.runner.execute_drafted = lambda seqs, drafts: [next(kept) for _ in seqs]
+    return e
+
+
+@pytest.mark.parametrize("kept,text,accepted", [
+    ([[5]], [5], 0), ([[7, 5]], [7, 5], 1), ([[7, 8, 9, 5]], [7, 8, 9, 5], 3),
+    # the end of the text: at the model's own token, at a drafted one, with more of them behind
+    ([[7, 0]], [7, 0], 1), ([[7, 8, 9, 0]], [7, 8, 9, 0], 3), ([[0]], [0], 0), ([[0, 8]], [0], 1),
+    ([[7, 0, 9, 5]], [7, 0], 2), ([[0, 8, 9, 5]], [0], 1), ([[7, 5], [7, 0, 9]], [7, 5, 7, 0], 3),
+])
+def test_accepted_tokens_are_those_that_the_text_keeps(kept, text, accepted):
+    e = _engine(kept, eos_token_id=0)
+    seq = e.scheduler.running[0]
+    for _ in kept:
+        e.step()
+    assert seq.output_token_ids == [1, *text]
+    assert (e.num_drafted, e.num_accepted) == (3 * len(kept), accepted)
