@@ -154,11 +154,17 @@ class ModelRunner:
         computed = [s.num_computed_tokens for s in seqs]
         longest = max(c + q for c, q in zip(computed, lens))
         place, held, start, blocks = self._tables.place(seqs)
-        ids_t, up_t, place_t, computed_t, lens_t, held_t, start_t, blocks_t = self._stage(
-            [ids, up, place, computed, lens, held, start, blocks])
         T = len(ids)
-        x = step_inputs(self._tables.tensor, place_t, computed_t, lens_t, T, self.block_size,
-                        -(-longest // self.block_size), blocks_t, start_t, held_t, up_t)
+        try:
+            ids_t, up_t, place_t, computed_t, lens_t, held_t, start_t, blocks_t = self._stage(
+                [ids, up, place, computed, lens, held, start, blocks])
+            x = step_inputs(self._tables.tensor, place_t, computed_t, lens_t, T, self.block_size,
+                            -(-longest // self.block_size), blocks_t, start_t, held_t, up_t)
+        except BaseException:
+            # The tables on the device lack what `place` has named for this step.
+            for seq in seqs:
+                self._tables.forget(seq)
+            raise
         qsl = [0, *np.cumsum(lens).tolist()]
         md = AttentionMetadata(
             slot_mapping=x.slot_mapping, query_start_loc=x.query_start_loc, seq_lens=x.seq_lens,

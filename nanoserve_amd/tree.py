@@ -166,7 +166,8 @@ class BlockTables:
             self._rows[seq.seq_id] = (held[0], seq.block_table, min(held[2], len(seq.block_table)))
 
     def place(self, seqs) -> tuple[list[int], list[int], list[int], list[int]]:
-        """(rows, held, new_start, new_blocks) of the batch, as step_inputs takes them.  Counts on that call."""
+        """(rows, held, new_start, new_blocks) of the batch, as step_inputs takes them.  Counts on
+        that call: `forget` the requests where it fails."""
         missing = sum(s.seq_id not in self._rows for s in seqs)
         if missing > len(self._free):
             here = {s.seq_id for s in seqs}

@@ -147,3 +147,24 @@ def test_accepted_tokens_are_those_that_the_text_keeps(kept, text, accepted):
         e.step()
     assert seq.output_token_ids == [1, *text]
     assert (e.num_drafted, e.num_accepted) == (3 * len(kept), accepted)
+
+
+@pytest.mark.parametrize("what", ["_stage", "step_inputs"])
+def test_a_step_that_never_reached_the_device_leaves_no_blocks_named(what, monkeypatch):
+    """The device's tables lack the blocks of a step that failed before its launch: the next one names them again."""
+    e = _engine(None)
+    seq = e.scheduler.running[0]
+
+    def fails(*a, **kw):
+        raise RuntimeError("out of memory")
+
+    with monkeypatch.context() as m:
+        if what == "_stage":
+            m.setattr(e.runner, what, fails)
+        else:
+            m.setattr("nanoserve_amd.engine.step_inputs", fails)
+        for _ in range(2):
+            with pytest.raises(RuntimeError, match="memory"):
+                e.step()
+    rows, held, start, blocks = e.runner._tables.place([seq])
+    assert held == [0] and blocks == seq.block_table and start == [0, len(blocks)]
