@@ -621,8 +621,9 @@ int ns_paged_attention_int4(void* out, const void* query,
  * ns_paged_attention_tree -- ns_paged_attention for such rows: row j of a
  * sequence with context length L (its q rows included) sees keys 0 .. L - q - 1
  * and key L - q + i where bit i of tree_mask (int64 [num_tokens]) is set, i < 64.
- * A row without keys is zero; a row of no sequence, and a sequence's rows from the
- * 64th on, are left as they are.  K and V of a key that a row does not see do not
+ * A row without keys is zero, and so is one whose scores are all -infinity, as in
+ * ns_paged_attention; a row of no sequence, and a sequence's rows from the 64th on,
+ * are left as they are.  K and V of a key that a row does not see do not
  * reach it, whatever they hold.  Without query_start_loc (NULL) row s is sequence s.
  * max_query_len is the longest sequence's rows, at most 64; it shapes the launch,
  * the device's offsets decide.  A block id outside [0, num_blocks) is never

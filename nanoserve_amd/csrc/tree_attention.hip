@@ -4,7 +4,7 @@
 // length L (its rows included) and q rows sees every key before the rows,
 // 0 .. L - q - 1, and key L - q + i where bit i of its mask is set.  KV head of
 // query head h is h / (Hq / Hkv); softmax and sums are float32; a row without keys
-// is zero.
+// is zero, and so is one whose scores are all -inf.
 #include <math.h>
 
 #include "ns_common.h"
@@ -227,7 +227,7 @@ hipError_t launch_generic(const TreeParams& p, hipStream_t stream) {
 
 constexpr int kMostRanges = 32;  // of a group: what the last workgroup has to join
 constexpr int kGroupCost = 16;   // in chunks
-constexpr float kNoScore = -3e38f;  // a column's reference before its first score
+constexpr float kNoScore = -3e38f;  // a column's reference before its first score; scores below it are as -inf
 constexpr float kSlack = 8.f;    // binades that a score may pass its column's reference by
 constexpr int kLeastRounds = 2;  // of the key groups, in a share; groups of no more stay whole
 

@@ -234,7 +234,8 @@ def paged_attention_tree(query: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     (attention.paged_attention_hip) with md.tree_mask.  Row j of a sequence with
     context length L and q <= 64 rows sees keys 0 .. L - q - 1, and key L - q + i
     where bit i of its mask is set.  Returns [num_tokens, num_heads, head_dim],
-    with zeros for rows without keys and rows behind the last sequence.
+    with zeros for rows without keys, rows whose scores are all -inf (as in
+    paged_attention_hip) and rows behind the last sequence.
 
     float32, float16 and bfloat16, head sizes up to 256.  The device's lengths,
     offsets, masks and tables decide what is computed; of the host's only

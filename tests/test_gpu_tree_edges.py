@@ -6,7 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from nanoserve_amd import commit_drafts
+from nanoserve_amd import commit_drafts, paged_attention_hip
 from tests.test_gpu_tree import DEV, Case, close
 
 pytestmark = pytest.mark.gpu
@@ -62,3 +62,24 @@ def test_commit_refuses_a_cache_that_is_listed_twice():
     assert torch.equal(both, before)
     commit_drafts(*args, [k], [v], 3)  # neighbours do not overlap
     assert torch.equal(both[:, 0, 1], before[:, 0, 2]) and torch.equal(both[:, 0, 2:], before[:, 0, 2:])
+
+
+@pytest.mark.parametrize("dtype,heads,block_size", KERNELS)
+def test_rows_whose_scores_are_all_minus_infinity(dtype, heads, block_size):
+    """Count as rows without keys, in one range and in many, and as paged_attention_hip has them;
+    one finite score among them takes all of the weight."""
+    c = Case([40, 3000, 40, 0], [1, 1, 1, 1], heads, dtype, block_size, fill=0.0)
+    c.query = c.query.abs() + 0.5
+    for i in (0, 1, 3):
+        c.kc[c.tables[i]] = -float("inf")
+    md = c.md()
+    out = c.run(md).cpu()
+    ref, mag = c.reference()  # NaN in these rows
+    zero = [0, 1, 3]
+    assert (out[zero] == 0).all()
+    close(out[2:3], ref[2:3], mag[2:3], dtype, c.d, 41)
+    md.tree_mask, md.is_decode_only, md.query_start_loc = None, True, None
+    assert (c.run(md, paged_attention_hip).cpu()[zero] == 0).all()
+    for i, at in ((0, 40), (1, 1700), (3, 0)):  # a row of the tree, one of the prefix
+        c.kc[c.tables[i][at // block_size], at % block_size] = 0.25
+    c.check(c.run())
