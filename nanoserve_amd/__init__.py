@@ -17,19 +17,22 @@ bits (kv4.py), the draw of a token from given uniform numbers
 
 from .attention import AttentionMetadata, get_attention_backend, paged_attention_hip
 from .block_manager import BlockSpaceManager
+from .drafting import NgramDrafter
 from .kv_cache import PagedKVCache, kv_bytes_per_token, reshape_and_cache
 from .kv4 import (Int4PagedKVCache, gather_cache_int4, paged_attention_int4, reshape_and_cache_int4,
                   rope_reshape_and_cache_int4)
 from .rotary import RotaryEmbedding, rope_reshape_and_cache
 from .sampling import argmax_rows, sample_rows
-from .tree import StepInputs, commit_drafts, paged_attention_tree, step_inputs
+from .tree import BlockTables, StepInputs, commit_drafts, paged_attention_tree, step_inputs
 
 __version__ = "0.1.0"
 
 __all__ = [
     "AttentionMetadata",
     "BlockSpaceManager",
+    "BlockTables",
     "Int4PagedKVCache",
+    "NgramDrafter",
     "PagedKVCache",
     "StepInputs",
     "argmax_rows",

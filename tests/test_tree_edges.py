@@ -7,6 +7,7 @@ import ctypes
 import pytest
 import torch
 
+import nanoserve_amd
 from nanoserve_amd import _lib, tree
 from nanoserve_amd.engine import LLMEngine
 from nanoserve_amd.model import Qwen2Config, Qwen2ForCausalLM
@@ -168,3 +169,11 @@ def test_a_step_that_never_reached_the_device_leaves_no_blocks_named(what, monke
                 e.step()
     rows, held, start, blocks = e.runner._tables.place([seq])
     assert held == [0] and blocks == seq.block_table and start == [0, len(blocks)]
+
+
+# ---- what a user imports ------------------------------------------------------------
+
+
+def test_what_goes_with_a_drafted_step_is_exported():
+    for name in ("AttentionMetadata", "BlockTables", "NgramDrafter", "commit_drafts", "paged_attention_tree", "step_inputs"):
+        assert name in nanoserve_amd.__all__ and hasattr(nanoserve_amd, name)
