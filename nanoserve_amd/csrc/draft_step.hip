@@ -333,13 +333,16 @@ extern "C" int ns_commit_drafts(int64_t* counts, int64_t* tokens,
   // where the first move has written already.
   uintptr_t all = static_cast<uintptr_t>(row_bytes);
   const uint64_t bytes = static_cast<uint64_t>(num_slots) * static_cast<uint64_t>(row_bytes);
+  uint64_t low = ~uint64_t{0}, high = 0;  // the caches so far lie in between
   for (int c = 0; c < num_caches; ++c) {
     const uint64_t at = reinterpret_cast<uintptr_t>(caches[c]);
     if (!at) return NS_ERR_INVALID_ARG;
-    for (int b = 0; b < c; ++b) {
+    for (int b = 0; b < c && at < high && at + bytes > low; ++b) {
       const uint64_t before = reinterpret_cast<uintptr_t>(caches[b]);
       if ((at < before ? before - at : at - before) < bytes) return NS_ERR_INVALID_ARG;
     }
+    low = at < low ? at : low;
+    high = at + bytes > high ? at + bytes : high;
     all |= at;
   }
   CommitParams p;

@@ -375,10 +375,14 @@ def commit_drafts(chosen: torch.Tensor, input_ids: torch.Tensor, parents: torch.
     tokens = torch.empty((B, max_rows), dtype=torch.int64, device=device)
     held = len(caches) if num_slots and row_bytes else 0
     pointers = array.array("Q", map(_ADDRESS, caches)) if held else None
-    if held and len({*pointers}) != held:
-        raise ValueError("a cache is listed twice")
-    _lib.launch(device, what, _lib.load().ns_commit_drafts,
-                counts.data_ptr(), tokens.data_ptr(), rows[0].data_ptr(), rows[1].data_ptr(), rows[2].data_ptr(), wide,
-                qsl.data_ptr(), qsl.dtype is torch.int64, slots.data_ptr(), slots.dtype is torch.int64, B, T, max_rows,
-                pointers.buffer_info()[0] if held else None, held, num_slots, row_bytes)
+    try:
+        _lib.launch(device, what, _lib.load().ns_commit_drafts,
+                    counts.data_ptr(), tokens.data_ptr(), rows[0].data_ptr(), rows[1].data_ptr(), rows[2].data_ptr(), wide,
+                    qsl.data_ptr(), qsl.dtype is torch.int64, slots.data_ptr(), slots.dtype is torch.int64, B, T, max_rows,
+                    pointers.buffer_info()[0] if held else None, held, num_slots, row_bytes)
+    except RuntimeError:
+        # The library refuses caches that overlap.
+        if held and len({*pointers}) != held:
+            raise ValueError("a cache is listed twice") from None
+        raise
     return counts, tokens
