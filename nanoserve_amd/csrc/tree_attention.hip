@@ -84,8 +84,10 @@ __device__ __forceinline__ uint32_t seen_of(uint64_t mask, int key, int base, in
 //
 // One key per lane: the lane's dot product of the query (in LDS, float32) with its
 // key joins the wave's running maximum and sum; then every lane adds the chunk's
-// weighted values into the output dims it owns, one key at a time.  Plain: the
-// serving shapes run the matrix-core kernel.
+// weighted values into the output dims it owns, one key at a time.  Plain, for shapes
+// that no serving configuration here has: every wave reads its K and V for itself, lanes a
+// row apart, and waits for each (32 requests of 8 rows around 1K keys: 2.0 to 2.5 ms by type
+// and head size, one of 24 rows 144 us; the matrix-core kernel takes 18 and 11 us).
 // DL: output dims per lane (head_dim <= 64 * DL).
 template <class T, int DL>
 __global__ __launch_bounds__(64) void tree_attention_generic_kernel(TreeParams p) {
@@ -222,7 +224,7 @@ hipError_t launch_generic(const TreeParams& p, hipStream_t stream) {
 // queries 2, first keys 2, loop, the join of the ranges 2 to 3).  32 requests of 8
 // rows around 1K keys: 18 us for 22 MB, the same chain.  64 x 12 rows around 4K keys,
 // head size 128: 169 us, K and V once at 4.3 TB/s (a copy moves 4.7).  8 x 64 rows
-// around 4K keys: 60 us, 550 TFLOP/s: a step of a compute unit takes 2600 cycles, of
+// around 4K keys: 60 us, 550 TFLOP/s: a step of a compute unit's loop takes 2630 cycles, of
 // which the matrix cores need 1090, the vector units 1110 and the LDS reads 1020.
 
 constexpr int kMostRanges = 32;  // of a group: what the last workgroup has to join
@@ -295,8 +297,9 @@ __device__ __forceinline__ int v_swizzle(int key) {
 }
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// Division by a uniform y > 0 of uniform 0 <= x < 2^30 with quotients below 2^20: by the
-// reciprocal in float32, which is one off at most, and put right.
+// Division by a uniform y > 0 of uniform 0 <= x < 2^30: by the reciprocal in float32, which
+// with quotients below 2^20 is one off at most, and put right.  (The kernel's first share of
+// a line can pass that, and is put right there.)
 struct Divisor {
   int y;
   float r;
@@ -1009,9 +1012,11 @@ int device_cus() {
 // Workgroups that the device holds at once, in whole rounds of the XCDs.
 int places() { return (device_cus() + 7) / 8 * 8; }
 
-// Column tiles of a group: those of the widest sequence, in equal blocks.  Wide
-// blocks load K and V for more columns at once, narrow ones leave more groups to work on
-// at the same time: as wide as leaves a quarter of the device's workgroups a group.
+// Column tiles that a kernel's blocks should hold at least: those of the widest sequence
+// over the number of its blocks.  Wide blocks load K and V for more columns at once, narrow
+// ones leave more groups to work on at the same time: as wide as leaves a quarter of the
+// device's workgroups a group.  The kernels come in a few widths, so that a sequence's last
+// block may hold fewer columns than the others (28 tiles in blocks of 8: 8, 8, 8 and 4).
 int tiles_of(int num_seqs, int num_kv_heads, int max_rows, int group, int head_dim) {
   const int64_t rows = max_rows < 1 ? 1 : max_rows < kRows ? max_rows : kRows;
   const int64_t tiles = (rows * group + 15) / 16;

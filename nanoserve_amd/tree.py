@@ -16,8 +16,11 @@ its depth.
                            and V moved to the places of the tokens they became
     BlockTables            the tables that step_inputs reads and extends
 
-Each is one launch on the current stream and reads the device's lengths, so a
-captured graph serves other lengths, trees and choices on every replay.
+Each runs on the current stream and reads the device's lengths, so a captured graph
+serves other lengths, trees and choices on every replay.  Each is one launch, but
+paged_attention_tree takes one per 512 sequences, after a fill of the output where
+rows may lie behind the last sequence (with query_start_loc in a capture: always) and,
+in a capture, one of its arrival counters; commit_drafts takes one per 128 caches.
 """
 
 from __future__ import annotations
